@@ -449,6 +449,116 @@ int oi_moe_ffn(const oi_moe_dims *d, int32_t router_type, const void *router_blo
                const void *gate_blocks, const void *up_blocks, const void *down_blocks, const float *x, float *y,
                int32_t *ids_out, float *w_out);
 
+/* ------------------------------------------- rotation by several axes --- */
+
+/* Shape of a layer's q and k heads: the first rotary_dim dimensions turn, in
+ * pairs (i, i + rotary_dim/2).  Each pair belongs to one of three axes (time,
+ * height, width): section after section (sections[0] pairs of axis 0, then
+ * sections[1] of axis 1, ...), or interleaved, pair i of axis i % 3 while
+ * i < 3 * sections[i % 3] and of axis 0 past that.  The sections sum to
+ * rotary_dim/2; {rotary_dim/2, 0, 0} is one axis. */
+typedef struct {
+    int32_t n_heads, n_kv_heads, head_dim, rotary_dim;
+    int32_t sections[3], interleaved;
+    float eps;
+} oi_rope_axes_dims;
+
+/* RMSNorm of every q and k head (q_norm, k_norm [head_dim]; NULL: no norm of
+ * that one) and its rotation by pos[axis][token] * inv_freq[pair] (the
+ * reference rotates text alone, one number per token: qwen3_5/ops.odin:77-89).
+ * pos is [3][n]; text has the same number on the three axes, image and video
+ * tokens their frame, row and column.  Angles are formed in 64 bits.  Device
+ * pointers.  q: head h of token t at t * q_stride + h * q_head_stride (in
+ * elements; a q projection with a gate beside each head has head stride
+ * 2 * head_dim); k, q_out and k_out: heads one after the other.  Types F32 or
+ * F16 each way; q_out may be q and k_out k where type and strides are the same.
+ * Pointers 16-byte aligned, strides multiples of 16 bytes; OI_E_ARG otherwise.
+ * head_dim 128 or 256.  Enqueued on `stream`. */
+int oi_rope_axes_launch(const oi_rope_axes_dims *d, int32_t n, const int32_t *pos, const float *inv_freq,
+                        const float *q_norm, const float *k_norm, int32_t in_type, const void *q, int64_t q_stride,
+                        int64_t q_head_stride, const void *k, int64_t k_stride, int32_t out_type, void *q_out,
+                        int64_t q_out_stride, void *k_out, int64_t k_out_stride, void *stream);
+
+/* ------------------------------------------------------ 8-bit K/V cache --- */
+
+/* A layer's cache in half the bytes of the f16 one (no counterpart in the
+ * reference).  A value is code * 2^exponent: a signed byte in [-127, 127] and an
+ * exponent in [-24, 10] (the range of f16; a byte outside counts as the nearest
+ * in it) per kv head and block of slots, apart for K and V.  One buffer of oi_kv8_bytes, 256-byte aligned:
+ *   K codes     int8 [n_kv_heads][capacity][head_dim]
+ *   V codes     int8 [n_kv_heads][capacity / 64][head_dim][64]
+ *   K exponents int8 [n_kv_heads][capacity / block]
+ *   V exponents int8 [n_kv_heads][capacity / block]
+ * head_dim 128 or 256, capacity a multiple of 64 (at most 2^28), block 16, 32
+ * or 64.  The memory needs no initialization: a call reads only slots below the
+ * length that it is given.  Lengths: n_past slots are in use before the call, or
+ * *n_past_dev where that pointer is set (a token loop that keeps its position on
+ * the device and replays one captured graph; clamped to 0 .. capacity - n).
+ * Slots are places in the cache, not positions: after an eviction they differ,
+ * and the caller rotates q and k by positions before they get here.
+ * The launches allocate nothing and may be captured.  `stream` must belong to
+ * the current device (OI_E_ARG otherwise).  Calls on one cache, mass or
+ * workspace that overlap in time race. */
+typedef struct {
+    int32_t n_kv_heads, head_dim, capacity, block;
+} oi_kv8_dims;
+
+/* Bytes of a cache buffer; 0 for bad dims. */
+int64_t oi_kv8_bytes(const oi_kv8_dims *d);
+
+/* Store n tokens' K and V behind the slots in use: k and v [n][n_kv_heads]
+ * [head_dim] with k_stride and v_stride elements from a token to the next, type
+ * OI_TYPE_F32 or OI_TYPE_F16, 16-byte aligned, strides multiples of 16 bytes.  A
+ * block's exponent is the least that holds its largest finite value (the
+ * largest, 10, saturates beyond 130048; +-infinity is stored as +-127 codes, NaN
+ * as 0).  A block that already holds slots keeps at least its exponent; where the
+ * new tokens raise it, the earlier codes are rounded again to the larger step,
+ * which moves each value by less than one final step in all, however many
+ * appends it takes.  Other slots' bytes stay as they are.  Appending at a smaller
+ * n_past than before (a rejected draft) overwrites. */
+int oi_kv8_append_launch(const oi_kv8_dims *d, void *cache, int32_t type, const void *k, int64_t k_stride,
+                         const void *v, int64_t v_stride, int32_t n, int32_t n_past, const int32_t *n_past_dev,
+                         void *stream);
+
+/* Slots slot0 .. slot0+n-1 as values, k and v [n_kv_heads][n][head_dim] of
+ * `type` (the layout of oi_engine_kv_fill's one layer), 16-byte aligned. */
+int oi_kv8_read_launch(const oi_kv8_dims *d, const void *cache, int32_t slot0, int32_t n, int32_t type, void *k,
+                       void *v, void *stream);
+
+/* Workspace that oi_kv8_attn_launch needs for n tokens at any length up to the
+ * capacity; 0 for bad arguments. */
+int64_t oi_kv8_attn_workspace_bytes(const oi_kv8_dims *d, int32_t n_heads, int32_t n);
+
+/* Causal attention of n tokens over the cache, which already holds them (append
+ * first): token i sees slots 0 .. n_past+i.  q and out [n][n_heads][head_dim]
+ * with q_stride and out_stride elements from a token to the next, both of
+ * `type`, 16-byte aligned, strides multiples of 16 bytes; query head h reads kv
+ * head h / (n_heads / n_kv_heads).  out = softmax(scale * q K) V with 32-bit
+ * sums.  mass (NULL: none), f32 [n_kv_heads][capacity]: what each slot receives,
+ * the softmax weight summed over the call's tokens and the query heads of its kv
+ * head, is added to slots below n_past and stored in slots n_past ..
+ * n_past+n-1 (a new slot starts at nothing); slots past those stay as they are.
+ * Every sum is in a fixed order.  `out` may be `q` where the strides are the
+ * same and mass is NULL. */
+int oi_kv8_attn_launch(const oi_kv8_dims *d, const void *cache, int32_t n_heads, int32_t type, const void *q,
+                       int64_t q_stride, float scale, int32_t n, int32_t n_past, const int32_t *n_past_dev,
+                       float *mass, void *out, int64_t out_stride, void *workspace, int64_t workspace_bytes,
+                       void *stream);
+
+/* Eviction: of slots 0 .. n-1 each kv head keeps the first n_first, the last
+ * n_last, and of those between the keep - n_first - n_last with the largest mass
+ * (equal masses: the lower slot; NaN counts as the least), in their order, and
+ * writes them to slots 0 .. keep-1 of another cache: codes brought to the
+ * exponents of their new blocks (exact where that does not rise, otherwise
+ * rounded to half to even once), masses, positions (src_pos and dst_pos int32
+ * [n_kv_heads][capacity], both NULL or neither) and, in kept [n_kv_heads][keep],
+ * the slots they came from.  dst may differ from src in capacity and block.  The
+ * buffers of the two caches must not overlap (OI_E_ARG): a program keeps one
+ * spare and exchanges them. */
+int oi_kv8_evict_launch(const oi_kv8_dims *src_dims, const void *src, const float *src_mass, const int32_t *src_pos,
+                        int32_t n, int32_t keep, int32_t n_first, int32_t n_last, const oi_kv8_dims *dst_dims,
+                        void *dst, float *dst_mass, int32_t *dst_pos, int32_t *kept, void *stream);
+
 #ifdef __cplusplus
 }
 #endif

@@ -6,4 +6,4 @@ engine_destroy, engine_config; dequant_row, row_byte_size) through ctypes on
 the C ABI of include/oi.h.  Nothing here computes: every call goes to
 liboi_hip.so, and importing a compute entry point without that library raises.
 """
-from . import ggml, infer, synth  # noqa: F401
+from . import ggml, infer, kv8, rope, synth  # noqa: F401

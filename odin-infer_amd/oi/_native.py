@@ -32,6 +32,15 @@ class MoeDims(ctypes.Structure):
     _fields_ = [("n_experts", c_i32), ("top_k", c_i32), ("dim", c_i32), ("inter", c_i32), ("norm_topk_prob", c_i32)]
 
 
+class RopeAxesDims(ctypes.Structure):
+    _fields_ = [("n_heads", c_i32), ("n_kv_heads", c_i32), ("head_dim", c_i32), ("rotary_dim", c_i32),
+                ("sections", c_i32 * 3), ("interleaved", c_i32), ("eps", c_f)]
+
+
+class KV8Dims(ctypes.Structure):
+    _fields_ = [("n_kv_heads", c_i32), ("head_dim", c_i32), ("capacity", c_i32), ("block", c_i32)]
+
+
 class Opts(ctypes.Structure):
     _fields_ = [("max_ctx", c_i32), ("use_hip", c_i32), ("num_threads", c_i32), ("device", c_i32)]
 
@@ -104,6 +113,15 @@ HIP_SYMBOLS = {
     "oi_moe_ffn_launch": (c_i32, [c_vp] * 9),
     "oi_moe_ffn_launch_noalloc": (c_i32, [c_vp] * 8),
     "oi_moe_ffn": (c_i32, [c_vp, c_i32, c_vp, c_i32] + [c_vp] * 7),
+    "oi_rope_axes_launch": (c_i32, [c_vp, c_i32, c_vp, c_vp, c_vp, c_vp, c_i32, c_vp, c_i64, c_i64, c_vp, c_i64, c_i32,
+                                    c_vp, c_i64, c_vp, c_i64, c_vp]),
+    "oi_kv8_bytes": (c_i64, [c_vp]),
+    "oi_kv8_append_launch": (c_i32, [c_vp, c_vp, c_i32, c_vp, c_i64, c_vp, c_i64, c_i32, c_i32, c_vp, c_vp]),
+    "oi_kv8_read_launch": (c_i32, [c_vp, c_vp, c_i32, c_i32, c_i32, c_vp, c_vp, c_vp]),
+    "oi_kv8_attn_workspace_bytes": (c_i64, [c_vp, c_i32, c_i32]),
+    "oi_kv8_attn_launch": (c_i32, [c_vp, c_vp, c_i32, c_i32, c_vp, c_i64, c_f, c_i32, c_i32, c_vp, c_vp, c_vp, c_i64,
+                                   c_vp, c_i64, c_vp]),
+    "oi_kv8_evict_launch": (c_i32, [c_vp, c_vp, c_vp, c_vp] + [c_i32] * 4 + [c_vp] * 6),
 }
 
 
