@@ -4,6 +4,7 @@
 // every launch can be captured into a graph.
 #include "kv8.h"
 
+#include <algorithm>
 #include <cmath>
 #include <string>
 
@@ -152,7 +153,9 @@ int oi_kv8_read_launch(const oi_kv8_dims *d, const void *cache, int32_t slot0, i
 
 int64_t oi_kv8_attn_workspace_bytes(const oi_kv8_dims *d, int32_t n_heads, int32_t n) {
     if (!dims_ok(d) || n_heads <= 0 || n_heads > 4096 || n_heads % d->n_kv_heads || n <= 0 || n > d->capacity) return 0;
-    const int s = kv8_attn_splits(d->n_kv_heads, n_heads / d->n_kv_heads, n, d->capacity);
+    const int group = n_heads / d->n_kv_heads;
+    const int s = std::max(kv8_attn_splits(d->n_kv_heads, group, n, d->capacity, d->head_dim, false),
+                           kv8_attn_splits(d->n_kv_heads, group, n, d->capacity, d->head_dim, true));
     return (int64_t)kv8_attn_workspace(n_heads, n, d->head_dim, s);
 }
 
@@ -175,7 +178,8 @@ int oi_kv8_attn_launch(const oi_kv8_dims *d, const void *cache, int32_t n_heads,
         if (!rows_ok(q, type, q_stride, row) || !rows_ok(out, type, out_stride, row)) return err(OI_E_ARG, W, BAD_ROWS);
         const int group = n_heads / d->n_kv_heads;
         if ((int64_t)n * group > 65535 * 16) return err(OI_E_RANGE, W, "too many rows in one call");
-        const int splits = kv8_attn_splits(d->n_kv_heads, group, n, n_past_dev ? d->capacity : n_past + n);
+        const int splits = kv8_attn_splits(d->n_kv_heads, group, n, n_past_dev ? d->capacity : n_past + n, d->head_dim,
+                                           type == OI_TYPE_F16);
         const int64_t need = (int64_t)kv8_attn_workspace(n_heads, n, d->head_dim, splits);
         if (workspace_bytes < need)
             return err(OI_E_ARG, W, "workspace of " + std::to_string(workspace_bytes) + " bytes, " +
@@ -192,11 +196,14 @@ int oi_kv8_attn_launch(const oi_kv8_dims *d, const void *cache, int32_t n_heads,
         a.n = n;
         a.n_heads = n_heads;
         a.group = group;
+        a.magic = group > 1 ? (uint32_t)((((uint64_t)1 << 32) + group - 1) / group) : 0u;
         a.past = {n_past, n_past_dev};
         a.mass = mass;
         a.splits = splits;
         a.part = (float *)workspace;
-        a.lse = mass ? a.part + (size_t)splits * n * n_heads * (d->head_dim + 2) : nullptr;
+        const size_t rows = (size_t)n * n_heads, parts = splits > 1 ? rows * splits : 0;
+        a.ml = (float2 *)(a.part + parts * d->head_dim);
+        a.lse = mass ? (float *)(a.ml + parts) : nullptr;
         return launched(launch_kv8_attn(a, (hipStream_t)stream), W);
     });
 }

@@ -50,14 +50,16 @@ struct Kv8AttnArgs {
     void *out;
     float scale;          // of q . k, times log2(e)
     int32_t f16, n, n_heads, group;
+    uint32_t magic;       // ceil(2^32 / group), 0 for a group of 1
     Kv8Past past;
     float *mass;          // [n_kv][cap] or null
-    float *part;          // [splits][n * n_heads][hd + 2]: o, m, l of a split
+    float *part;          // [n * n_heads][splits][hd], where splits > 1: the splits' o
+    float2 *ml;           // [n * n_heads][splits]: their m and l
     float *lse;           // [n * n_heads], where mass is set
     int32_t splits;
 };
 // splits over the slots for a call that sees at most `end` of them, and the workspace that they take
-int kv8_attn_splits(int n_kv, int group, int n, int end);
+int kv8_attn_splits(int n_kv, int group, int n, int end, int hd, bool f16);
 size_t kv8_attn_workspace(int n_heads, int n, int hd, int splits);
 hipError_t launch_kv8_attn(const Kv8AttnArgs &a, hipStream_t st);
 

@@ -14,6 +14,10 @@
 // own rounding).  2^15 is where the largest weight sits in f16: a weight keeps
 // all its bits down to 2^-29 of it and is lost below 2^-40.
 
+#include <algorithm>
+#include <cfloat>
+#include <type_traits>
+
 #include "kv8_common.h"
 
 namespace oi {
@@ -43,64 +47,129 @@ __device__ __forceinline__ f32x4 mfma(f16x8 a, f16x8 b, f32x4 c) {
     return __builtin_amdgcn_mfma_f32_16x16x32_f16(a, b, c, 0, 0, 0);
 }
 
-// over the four lanes of a column (xor 16 and 32)
+// v of the lanes 16 and 32 away, by register swaps between halves and rows of 16
+template <class F>
+__device__ __forceinline__ float col_reduce(float v, F f) {
+    const auto a = __builtin_amdgcn_permlane16_swap(__float_as_uint(v), __float_as_uint(v), false, false);
+    v = f(__uint_as_float(a[0]), __uint_as_float(a[1]));
+    const auto b = __builtin_amdgcn_permlane32_swap(__float_as_uint(v), __float_as_uint(v), false, false);
+    return f(__uint_as_float(b[0]), __uint_as_float(b[1]));
+}
+// over the four lanes of a column (16 and 32 apart)
 __device__ __forceinline__ float col_max(float v) {
-    v = fmaxf(v, __shfl_xor(v, 16, WAVE));
-    return fmaxf(v, __shfl_xor(v, 32, WAVE));
+    return col_reduce(v, [](float a, float b) { return fmaxf(a, b); });
 }
 __device__ __forceinline__ float col_sum(float v) {
-    v += __shfl_xor(v, 16, WAVE);
-    return v + __shfl_xor(v, 32, WAVE);
+    return col_reduce(v, [](float a, float b) { return a + b; });
 }
+// v and that of the column 8 away.  By value: __builtin_bit_cast of a vector's
+// element (inside OI_DPP) takes the vector's first one.
+__device__ __forceinline__ float half_sum(float v) { return v + OI_DPP(v, 0x128); }
+// 2^x; results below the normal numbers are 0
+__device__ __forceinline__ float ex2(float x) { return __builtin_amdgcn_exp2f(x); }
 
-// 16 rows of q as the products' second operand: lane (column c, group g) holds
-// dimensions 64 k + 16 g + 8 h + 0..7 of row c, the order in which its 16-byte
-// loads of K fall.  f32 rows: two halves of q 2^-e, e the row's exponent.
-template <int HD, bool F16>
+// How a tile of rows lies in the 16 columns of the products' second operand.
+enum {
+    ROWS_F16 = 0,   // 16 rows of an f16 q
+    ROWS_F32 = 1,   // 16 rows of an f32 q, two operands each (upper and lower half)
+    ROWS_PACK = 2,  // 8 rows of an f32 q: upper halves in columns 0..7, lower halves in 8..15, one product for both
+};
+constexpr int tile_rows(int mode) { return mode == ROWS_PACK ? 8 : 16; }
+
+// A tile of q as that operand: lane (column c, group g) holds dimensions
+// 64 k + 16 g + 8 h + 0..7 of its row, the order in which its 16-byte loads of K
+// fall.  f32 rows: two halves of q 2^-e, e the row's exponent.  A negative scale
+// turns q's sign, so that the largest score is that of the largest product.
+template <int HD, int MODE>
 struct QTile {
     static constexpr int NF = HD / 32;
-    f16x8 hi[NF], lo[F16 ? 1 : NF];
+    static constexpr bool F16 = MODE == ROWS_F16, TWO = MODE == ROWS_F32;
+    f16x8 hi[NF], lo[TWO ? NF : 1];
     int e = 0;
 
-    __device__ __forceinline__ void load(const void *q, int64_t at, int g, bool ok) {
+    // the row's loads (row `at` exists), then the operands (zero with ok = false)
+    struct Raw {
+        u32x4 w[F16 ? NF : 2 * NF];
+    };
+    static __device__ __forceinline__ void fetch(Raw &r, const void *q, int64_t at, int g) {
+#pragma unroll
+        for (int f = 0; f < NF; f++) {
+            const int64_t d = at + 64 * (f / 2) + 16 * g + 8 * (f & 1);
+            if constexpr (F16) {
+                r.w[f] = *(const u32x4 *)((const uint16_t *)q + d);
+            } else {
+                r.w[2 * f] = *(const u32x4 *)((const float *)q + d);
+                r.w[2 * f + 1] = *(const u32x4 *)((const float *)q + d + 4);
+            }
+        }
+    }
+    __device__ __forceinline__ void make(const Raw &r, bool ok, bool neg, bool lower) {
         if constexpr (F16) {
-            const u32x4 z = {0u, 0u, 0u, 0u};
+            const uint32_t sign = neg ? 0x80008000u : 0u;
 #pragma unroll
             for (int f = 0; f < NF; f++) {
-                const int d = 64 * (f / 2) + 16 * g + 8 * (f & 1);
-                hi[f] = __builtin_bit_cast(f16x8, ok ? *(const u32x4 *)((const uint16_t *)q + at + d) : z);
+                u32x4 w;
+#pragma unroll
+                for (int i = 0; i < 4; i++) w[i] = ok ? r.w[f][i] ^ sign : 0u;
+                hi[f] = __builtin_bit_cast(f16x8, w);
             }
         } else {
-            float x[NF][8];
             float amax = 0.f;
 #pragma unroll
-            for (int f = 0; f < NF; f++) {
-                const int d = 64 * (f / 2) + 16 * g + 8 * (f & 1);
-                const float4 *p = (const float4 *)((const float *)q + at + d), z = make_float4(0.f, 0.f, 0.f, 0.f);
-                const float4 u = ok ? p[0] : z, w = ok ? p[1] : z;
-                x[f][0] = u.x; x[f][1] = u.y; x[f][2] = u.z; x[f][3] = u.w;
-                x[f][4] = w.x; x[f][5] = w.y; x[f][6] = w.z; x[f][7] = w.w;
+            for (int f = 0; f < 2 * NF; f++)
 #pragma unroll
-                for (int i = 0; i < 8; i++) amax = fmaxf(amax, fabsf(x[f][i]));
-            }
-            amax = col_max(amax);
+                for (int i = 0; i < 4; i++) amax = fmaxf(amax, fabsf(__uint_as_float(r.w[f][i])));
+            amax = ok ? col_max(amax) : 0.f;
             e = amax > 0.f ? (int)(__float_as_uint(amax) >> 23) - 127 - 14 : 0;
 #pragma unroll
             for (int f = 0; f < NF; f++)
 #pragma unroll
                 for (int i = 0; i < 8; i++) {
-                    const float y = ldexpf(x[f][i], -e);
-                    const _Float16 h = (_Float16)y;
-                    hi[f][i] = h;
-                    lo[f][i] = (_Float16)(y - (float)h);
+                    const float x = __uint_as_float(r.w[2 * f + i / 4][i & 3]);
+                    const float y = ok ? ldexpf(neg ? -x : x, -e) : 0.f;
+                    const _Float16 h = (_Float16)y, l = (_Float16)(y - (float)h);
+                    if constexpr (TWO) {
+                        hi[f][i] = h;
+                        lo[f][i] = l;
+                    } else {
+                        hi[f][i] = lower ? l : h;
+                    }
                 }
         }
     }
 };
 
-// Where row r (of a kv head's n * group rows, token-major) has its head in q or out
-__device__ __forceinline__ int64_t row_at(int r, int group, int kvh, int64_t stride, int hd) {
-    return (int64_t)(r / group) * stride + (int64_t)(kvh * group + r % group) * hd;
+// One tile of 16 slots of raw K times the rows
+template <int HD, int MODE>
+__device__ __forceinline__ f32x4 scores(const u32x4 (&kr)[HD / 64], const QTile<HD, MODE> &q) {
+    f32x4 s = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+    for (int k = 0; k < HD / 64; k++)
+#pragma unroll
+        for (int h = 0; h < 2; h++) {
+            const f16x8 w = bytes_h(kr[k][2 * h], kr[k][2 * h + 1]);
+            s = mfma(w, q.hi[2 * k + h], s);
+            if constexpr (MODE == ROWS_F32) s = mfma(w, q.lo[2 * k + h], s);
+        }
+    if constexpr (MODE == ROWS_PACK)
+#pragma unroll
+        for (int i = 0; i < 4; i++) s[i] = half_sum(s[i]);
+    return s;
+}
+
+// The token of row r of a kv head's n * group rows (token-major): r / group by a
+// multiplication (magic = ceil(2^32 / group), exact while r * group < 2^32)
+__device__ __forceinline__ int row_token(const Kv8AttnArgs &a, int r) {
+    return a.magic ? (int)__umulhi((uint32_t)r, a.magic) : r;
+}
+// where the row's head lies in q or out, and its place among the n * n_heads rows
+__device__ __forceinline__ int64_t row_at(const Kv8AttnArgs &a, int r, int kvh, int64_t stride, int hd) {
+    const int t = row_token(a, r);
+    return t * stride + (int64_t)(kvh * a.group + r - t * a.group) * hd;
+}
+__device__ __forceinline__ size_t row_id(const Kv8AttnArgs &a, int r, int kvh) {
+    const int t = row_token(a, r);
+    return (size_t)t * a.n_heads + kvh * a.group + r - t * a.group;
 }
 
 // A wave takes a unit of 64 slots at a time for 16 rows of one kv head (the
@@ -113,47 +182,48 @@ __device__ __forceinline__ int64_t row_at(int r, int group, int kvh, int64_t str
 // the row maximum.  K and V go from memory to the operand registers without
 // LDS, 16 bytes a lane; K of the next unit is requested when this unit's scores
 // are done, V when its product is.  The waves' results meet in LDS.
-template <int HD, bool F16>
+template <int HD, int MODE>
 __global__ __launch_bounds__(WG) void kv8_rows_kernel(Kv8AttnArgs a) {
-    constexpr int NK = HD / 64, ND = HD / 16, PD = HD + 4;
-    __shared__ __attribute__((aligned(16))) float so[4][16][PD];
-    __shared__ float sm[4][16], sl[4][16];
+    constexpr int NK = HD / 64, ND = HD / 16, PD = HD + 4, R = tile_rows(MODE);
+    constexpr bool F16 = MODE == ROWS_F16;
+    __shared__ __attribute__((aligned(16))) float so[4][R][PD];
+    __shared__ float sm[4][R], sl[4][R];
     const int tid = threadIdx.x, lane = tid & (WAVE - 1), wave = tid / WAVE;
     const int c = lane & 15, g = lane >> 4;
     const int kvh = blockIdx.x, rt = blockIdx.y, split = blockIdx.z;
     const int rows = a.n * a.group, past = kv8_past(a.past, a.n, a.c.cap);
-    const int row = rt * 16 + c;
-    const bool ok = row < rows;
+    const int row = rt * R + c % R;
+    const bool ok = row < rows, lower = c >= R;
     const int rr = min(row, rows - 1);
-    const int limit = past + rr / a.group + 1;  // slots that this row sees
-    const int first_limit = past + (rt * 16) / a.group + 1;
-    const int last_limit = past + min(rt * 16 + 15, rows - 1) / a.group + 1;
+    const int limit = past + row_token(a, rr) + 1;  // slots that this row sees
+    const int first_limit = past + row_token(a, rt * R) + 1;
+    const int last_limit = past + row_token(a, min(rt * R + R - 1, rows - 1)) + 1;
     const int units = (last_limit + T - 1) / T;
-    const int per = (units + a.splits * 4 - 1) / (a.splits * 4) * 4;
-    const int u0 = split * per, u1 = min(u0 + per, units);
-    QTile<HD, F16> q;
-    q.load(a.q, row_at(rr, a.group, kvh, a.q_stride, HD), g, ok);
+    const int u0 = (int)((int64_t)split * units / a.splits), u1 = (int)((int64_t)(split + 1) * units / a.splits);
+    QTile<HD, MODE> q;
+    typename QTile<HD, MODE>::Raw qraw;
+    QTile<HD, MODE>::fetch(qraw, a.q, row_at(a, rr, kvh, a.q_stride, HD), g);
 
-    const int8_t *kb = a.c.kc + (size_t)kvh * a.c.cap * HD;
-    const int8_t *vb = a.c.vc + (size_t)kvh * a.c.cap * HD;
+    const int krow = 16 * (c >> 2) + (c & 3);
+    const int8_t *kb = a.c.kc + (size_t)kvh * a.c.cap * HD + krow * HD + 16 * g;
+    const int8_t *vb = a.c.vc + (size_t)kvh * a.c.cap * HD + c * T + 16 * g;
     const int8_t *ke = a.c.ke + (size_t)kvh * (a.c.cap >> a.c.lb);
     const int8_t *ve = a.c.ve + (size_t)kvh * (a.c.cap >> a.c.lb);
-    const int krow = 16 * (c >> 2) + (c & 3);
     u32x4 kr[4][NK], vr[ND];
     int kexp = 0, vexp = 0;
     auto load_k = [&](int u) {
+        const int8_t *p = kb + (size_t)u * (T * HD);
 #pragma unroll
         for (int t = 0; t < 4; t++)
 #pragma unroll
-            for (int k = 0; k < NK; k++)
-                kr[t][k] = ldg_nt((const u32x4 *)(kb + (size_t)(u * T + krow + 4 * t) * HD + 64 * k + 16 * g));
+            for (int k = 0; k < NK; k++) kr[t][k] = *(const u32x4 *)(p + 4 * t * HD + 64 * k);
         kexp = ke[(u * T + 16 * g) >> a.c.lb];
         vexp = ve[(u * T + 16 * g) >> a.c.lb];
     };
     auto load_v = [&](int u) {
+        const int8_t *p = vb + (size_t)u * (T * HD);
 #pragma unroll
-        for (int d = 0; d < ND; d++)
-            vr[d] = ldg_nt((const u32x4 *)(vb + ((size_t)u * HD + 16 * d + c) * T + 16 * g));
+        for (int d = 0; d < ND; d++) vr[d] = *(const u32x4 *)(p + 16 * d * T);
     };
     float m = NEG, l = 0.f;
     f32x4 o[ND];
@@ -164,229 +234,746 @@ __global__ __launch_bounds__(WG) void kv8_rows_kernel(Kv8AttnArgs a) {
         load_k(u);
         load_v(u);
     }
+    q.make(qraw, ok, a.scale < 0.f, lower);
+    const float scale = fabsf(a.scale);
     for (; u < u1; u += 4) {
         f32x4 s[4];
 #pragma unroll
-        for (int t = 0; t < 4; t++) {
-            s[t] = f32x4{0.f, 0.f, 0.f, 0.f};
-#pragma unroll
-            for (int k = 0; k < NK; k++)
-#pragma unroll
-                for (int h = 0; h < 2; h++) {
-                    const f16x8 w = bytes_h(kr[t][k][2 * h], kr[t][k][2 * h + 1]);
-                    s[t] = mfma(w, q.hi[2 * k + h], s[t]);
-                    if constexpr (!F16) s[t] = mfma(w, q.lo[2 * k + h], s[t]);
-                }
-        }
-        const float mul = ldexpf(a.scale, kv8_exp((int8_t)kexp) + q.e);
+        for (int t = 0; t < 4; t++) s[t] = scores<HD, MODE>(kr[t], q);
+        const float mul = fmaxf(ldexpf(scale, kv8_exp((int8_t)kexp) + q.e), FLT_MIN);  // above 0: -inf stays -inf
         const int ev = kv8_exp((int8_t)vexp);
         if (u + 4 < u1) load_k(u + 4);
-        const int p0 = u * T + 16 * g;  // the lane's first slot
-        const bool edge = u * T + T > first_limit;
-        float top = NEG;
+        if (u * T + T > first_limit) {  // some row does not see all of the unit
+            const int p0 = u * T + 16 * g;
+#pragma unroll
+            for (int t = 0; t < 4; t++)
+#pragma unroll
+                for (int i = 0; i < 4; i++)
+                    if (p0 + 4 * t + i >= limit) s[t][i] = -INFINITY;
+        }
+        float top = s[0][0];
 #pragma unroll
         for (int t = 0; t < 4; t++)
 #pragma unroll
-            for (int i = 0; i < 4; i++) {
-                s[t][i] = fmaf(s[t][i], mul, (float)ev);
-                if (edge && p0 + 4 * t + i >= limit) s[t][i] = -INFINITY;
-                top = fmaxf(top, s[t][i]);
-            }
-        top = col_max(top);
-        const float m1 = fmaxf(m, top), alpha = exp2f(m - m1);
+            for (int i = 0; i < 4; i++) top = fmaxf(top, s[t][i]);
+        top = col_max(fmaf(top, mul, (float)ev));
+        const float m1 = fmaxf(m, top), bias = (float)ev - m1 + PSCALE;
         float sum = 0.f;
         f16x8 ph[2], pl[2];
 #pragma unroll
         for (int t = 0; t < 4; t++)
 #pragma unroll
             for (int i = 0; i < 4; i++) {
-                const float p = exp2f(s[t][i] - m1 + PSCALE);
+                const float p = ex2(fmaf(s[t][i], mul, bias));
                 sum += p;
                 const _Float16 h = (_Float16)p;
                 ph[t / 2][4 * (t & 1) + i] = h;
                 if constexpr (!F16) pl[t / 2][4 * (t & 1) + i] = (_Float16)(p - (float)h);
             }
-        m = m1;
-        l = l * alpha + sum * pow2i(-ev);
+        if constexpr (MODE == ROWS_PACK) {
+            ph[0] = lower ? pl[0] : ph[0];
+            ph[1] = lower ? pl[1] : ph[1];
+        }
+        if (__any(m1 != m)) {  // a row's maximum rose
+            const float alpha = ex2(m - m1);
+            l *= alpha;
 #pragma unroll
-        for (int d = 0; d < ND; d++) {
-            o[d] *= alpha;
+            for (int d = 0; d < ND; d++) o[d] *= alpha;
+            m = m1;
+        }
+        l += sum * pow2i(-ev);
+#pragma unroll
+        for (int d = 0; d < ND; d++)
 #pragma unroll
             for (int h = 0; h < 2; h++) {
                 const f16x8 w = bytes_h(vr[d][2 * h], vr[d][2 * h + 1]);
                 o[d] = mfma(w, ph[h], o[d]);
-                if constexpr (!F16) o[d] = mfma(w, pl[h], o[d]);
+                if constexpr (MODE == ROWS_F32) o[d] = mfma(w, pl[h], o[d]);
             }
-        }
         if (u + 4 < u1) load_v(u + 4);
     }
+    // the four waves' results in LDS; their weights once per row, then the sum
     l = col_sum(l);
+    if constexpr (MODE == ROWS_PACK)
 #pragma unroll
-    for (int d = 0; d < ND; d++) *(f32x4 *)&so[wave][c][16 * d + 4 * g] = o[d];
-    if (g == 0) {
-        sm[wave][c] = m;
-        sl[wave][c] = l;
+        for (int d = 0; d < ND; d++)
+#pragma unroll
+            for (int i = 0; i < 4; i++) o[d][i] = half_sum(o[d][i]);
+    if (!lower) {
+#pragma unroll
+        for (int d = 0; d < ND; d++) *(f32x4 *)&so[wave][c][16 * d + 4 * g] = o[d];
+        if (g == 0) {
+            sm[wave][c] = m;
+            sl[wave][c] = l;
+        }
     }
     __syncthreads();
-    const int n_rows = min(16, rows - rt * 16);
-    for (int i = tid; i < n_rows * HD; i += WG) {
-        const int r = i / HD, d = i % HD;
-        const float M = fmaxf(fmaxf(sm[0][r], sm[1][r]), fmaxf(sm[2][r], sm[3][r]));
-        float O = 0.f, L = 0.f;
+    if (tid >= 16 * R) return;
+    float M = NEG, W[4], L = 0.f;
+    {
+        const int r = tid / 16;  // 16 threads a row from here on
+#pragma unroll
+        for (int w = 0; w < 4; w++) M = fmaxf(M, sm[w][r]);
 #pragma unroll
         for (int w = 0; w < 4; w++) {
-            const float f = exp2f(sm[w][r] - M);
-            O += so[w][r][d] * f;
-            L += sl[w][r] * f;
+            W[w] = ex2(sm[w][r] - M);
+            L += sl[w][r] * W[w];
         }
-        const int gr = rt * 16 + r, head = kvh * a.group + gr % a.group;
-        const size_t id = (size_t)(gr / a.group) * a.n_heads + head;
-        float *pt = a.part + ((size_t)split * a.n * a.n_heads + id) * (HD + 2);
-        pt[d] = O;
-        if (d == 0) {
-            pt[HD] = M;
-            pt[HD + 1] = L;
+    }
+    const int r = tid / 16, gr = rt * R + r;
+    if (gr >= rows) return;
+    const size_t id = row_id(a, gr, kvh);
+    const bool last = a.splits == 1;
+    const float inv = last ? 1.f / L : 1.f;
+#pragma unroll
+    for (int k = 0; k < HD / 64; k++) {
+        const int d = 64 * k + 4 * (tid & 15);
+        f32x4 y = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+        for (int w = 0; w < 4; w++) y += *(const f32x4 *)&so[w][r][d] * W[w];
+        y *= inv;
+        if (!last) {
+            *(f32x4 *)(a.part + (id * a.splits + split) * HD + d) = y;
+        } else {
+            const int64_t at = row_at(a, gr, kvh, a.out_stride, HD) + d;
+            if constexpr (F16)
+                *(u32x2 *)((uint16_t *)a.out + at) =
+                    u32x2{f2h(y[0]) | (uint32_t)f2h(y[1]) << 16, f2h(y[2]) | (uint32_t)f2h(y[3]) << 16};
+            else
+                *(f32x4 *)((float *)a.out + at) = y;
         }
+    }
+    if ((tid & 15) == 0) {
+        if (!last) a.ml[id * a.splits + split] = make_float2(M, L);
+        else if (a.lse) a.lse[id] = M + log2f(L) - PSCALE;
     }
 }
 
-// One wave-multiple of threads per (token, query head): the splits' weights,
-// their sum, out = o / l; and the row's base-2 log of the sum of weights.
+// Merge of the splits of one (token, query head): the first values of every
+// thread are requested together with the (m, l) pairs, one memory round trip for
+// up to MS * 8 splits; the weights 2^(m - M) are formed once, in LDS.
+constexpr int MW = 512, MPRE = 8;  // threads; splits per thread in the first round trip
+constexpr int KV8_MAX_SPLITS = 1024;
 template <int HD, bool F16>
-__global__ __launch_bounds__(HD) void kv8_merge_kernel(Kv8AttnArgs a) {
-    const int id = blockIdx.x, d = threadIdx.x;
-    const size_t step = (size_t)a.n * a.n_heads * (HD + 2);
-    const float *pt = a.part + (size_t)id * (HD + 2);
-    float M = NEG;
-    for (int s = 0; s < a.splits; s++) M = fmaxf(M, pt[s * step + HD]);
-    float O = 0.f, L = 0.f;
-    for (int s = 0; s < a.splits; s++) {
-        const float f = exp2f(pt[s * step + HD] - M);
-        O += pt[s * step + d] * f;
-        L += pt[s * step + HD + 1] * f;
+__global__ __launch_bounds__(MW) void kv8_merge_kernel(Kv8AttnArgs a) {
+    constexpr int LPR = HD / 4, MS = MW / LPR;  // lanes of a row, splits at a time
+    __shared__ float wt[KV8_MAX_SPLITS];
+    __shared__ __attribute__((aligned(16))) float red[MS][HD];
+    __shared__ float wmax[MW / WAVE], wsum[MW / WAVE];
+    const int tid = threadIdx.x, lane = tid & (WAVE - 1), wave = tid / WAVE, S = a.splits;
+    const size_t id = (size_t)blockIdx.y * a.n_heads + blockIdx.x;
+    const int col = tid % LPR, s0 = tid / LPR;
+    const float *pt = a.part + id * S * HD + 4 * col;
+    const float2 *ml = a.ml + id * S;
+    f32x4 pre[MPRE];
+    float2 mine[2];
+#pragma unroll
+    for (int k = 0; k < 2; k++) mine[k] = tid + k * MW < S ? ml[tid + k * MW] : make_float2(NEG, 0.f);
+#pragma unroll
+    for (int k = 0; k < MPRE; k++) {
+        const int s = s0 + k * MS;
+        pre[k] = s < S ? *(const f32x4 *)(pt + (size_t)s * HD) : f32x4{0.f, 0.f, 0.f, 0.f};
     }
-    const float y = O / L;
-    const int64_t at = (int64_t)(id / a.n_heads) * a.out_stride + (int64_t)(id % a.n_heads) * HD + d;
-    if constexpr (F16) ((uint16_t *)a.out)[at] = f2h(y);
-    else ((float *)a.out)[at] = y;
-    if (d == 0 && a.lse) a.lse[id] = M + log2f(L) - PSCALE;
+    const float m = wave_max_all(fmaxf(mine[0].x, mine[1].x));
+    if (lane == 0) wmax[wave] = m;
+    __syncthreads();
+    float M = wmax[0];
+#pragma unroll
+    for (int w = 1; w < MW / WAVE; w++) M = fmaxf(M, wmax[w]);
+    float L = 0.f;
+#pragma unroll
+    for (int k = 0; k < 2; k++) {
+        const float f = ex2(mine[k].x - M);
+        if (tid + k * MW < S) wt[tid + k * MW] = f;
+        L += mine[k].y * f;
+    }
+    L = wave_sum(L);
+    if (lane == 0) wsum[wave] = L;
+    __syncthreads();
+    L = 0.f;
+#pragma unroll
+    for (int w = 0; w < MW / WAVE; w++) L += wsum[w];
+    f32x4 y = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+    for (int k = 0; k < MPRE; k++)
+        if (s0 + k * MS < S) y += pre[k] * wt[s0 + k * MS];
+#pragma unroll 4
+    for (int s = s0 + MPRE * MS; s < S; s += MS) y += *(const f32x4 *)(pt + (size_t)s * HD) * wt[s];
+    *(f32x4 *)&red[s0][4 * col] = y;
+    __syncthreads();
+    if (tid < HD) {
+        float v = 0.f;
+#pragma unroll
+        for (int k = 0; k < MS; k++) v += red[k][tid];
+        v /= L;
+        const int64_t at = (int64_t)blockIdx.y * a.out_stride + (int64_t)blockIdx.x * HD + tid;
+        if constexpr (F16) ((uint16_t *)a.out)[at] = f2h(v);
+        else ((float *)a.out)[at] = v;
+    }
+    if (tid == 0 && a.lse) a.lse[id] = M + log2f(L) - PSCALE;
+}
+
+// ------------------------------------------------------------- prompts --
+
+typedef float f32x16 __attribute__((ext_vector_type(16)));
+
+__device__ __forceinline__ f32x16 mfma32(f16x8 a, f16x8 b, f32x16 c) {
+    return __builtin_amdgcn_mfma_f32_32x32x16_f16(a, b, c, 0, 0, 0);
+}
+// v of the lane 32 away
+template <class F>
+__device__ __forceinline__ float half_reduce(float v, F f) {
+    const auto b = __builtin_amdgcn_permlane32_swap(__float_as_uint(v), __float_as_uint(v), false, false);
+    return f(__uint_as_float(b[0]), __uint_as_float(b[1]));
+}
+
+// 32 rows of q in the second operand of 32x32x16 products, lane (column c, half
+// h): dimensions 16 f + 8 h + 0..7 of row c; an f32 row as two halves of q 2^-e.
+template <int HD, bool F16>
+struct QRows {
+    static constexpr int NF = HD / 16;
+    f16x8 hi[NF], lo[F16 ? 1 : NF];
+    int e = 0;
+
+    __device__ __forceinline__ void load(const void *q, int64_t at, int h, bool ok, bool neg) {
+        if constexpr (F16) {
+            const uint32_t sign = neg ? 0x80008000u : 0u;
+#pragma unroll
+            for (int f = 0; f < NF; f++) {
+                u32x4 w = *(const u32x4 *)((const uint16_t *)q + at + 16 * f + 8 * h);
+#pragma unroll
+                for (int i = 0; i < 4; i++) w[i] = ok ? w[i] ^ sign : 0u;
+                hi[f] = __builtin_bit_cast(f16x8, w);
+            }
+        } else {
+            const float *p = (const float *)q + at + 8 * h;
+            float amax = 0.f;
+#pragma unroll
+            for (int f = 0; f < NF; f++) {
+                const f32x4 u = *(const f32x4 *)(p + 16 * f), w = *(const f32x4 *)(p + 16 * f + 4);
+#pragma unroll
+                for (int i = 0; i < 4; i++) amax = fmaxf(amax, fmaxf(fabsf(u[i]), fabsf(w[i])));
+            }
+            amax = half_reduce(amax, [](float a, float b) { return fmaxf(a, b); });
+            e = ok && amax > 0.f ? (int)(__float_as_uint(amax) >> 23) - 127 - 14 : 0;
+#pragma unroll
+            for (int f = 0; f < NF; f++) {  // read again: the row is in cache, its registers are not free
+                const f32x4 u = *(const f32x4 *)(p + 16 * f), w = *(const f32x4 *)(p + 16 * f + 4);
+#pragma unroll
+                for (int i = 0; i < 8; i++) {
+                    const float x = i < 4 ? u[i & 3] : w[i & 3];
+                    const float y = ok ? ldexpf(neg ? -x : x, -e) : 0.f;
+                    const _Float16 t = (_Float16)y;
+                    hi[f][i] = t;
+                    lo[f][i] = (_Float16)(y - (float)t);
+                }
+            }
+        }
+    }
+};
+
+// A unit of 64 slots, K and V as halves in LDS, 16-byte pieces (8 values)
+// placed so that 8 neighbouring rows' equal pieces fall on different banks:
+// piece j of row r at j ^ (r & 7).  K row r holds the slot with bits 2 and 3 of r
+// exchanged: the products then leave a lane the scores of slots 8 h + 0..7 of
+// each 16, those whose weights it supplies to the product with V.
+template <int HD, int NT>
+struct Stage {
+    static constexpr int N = T * HD / 16 / NT;  // 16-byte pieces of codes per thread
+    u32x4 k[N], v[N];
+    int8_t e;  // thread 4 w + b: of K (w = 0) or V (w = 1), slots 16 b ..
+    __device__ __forceinline__ void load(const int8_t *kb, const int8_t *vb, const int8_t *ke, const int8_t *ve, int lb,
+                                         int u, int tid) {
+        if (tid < 8) e = (tid < 4 ? ke : ve)[(u * T + 16 * (tid & 3)) >> lb];
+        const u32x4 *kp = (const u32x4 *)(kb + (size_t)u * (T * HD)), *vp = (const u32x4 *)(vb + (size_t)u * (T * HD));
+#pragma unroll
+        for (int i = 0; i < N; i++) {
+            k[i] = kp[tid + i * NT];
+            v[i] = vp[tid + i * NT];
+        }
+    }
+    __device__ __forceinline__ void store(f16x8 *ks, f16x8 *vs, float *es, int tid) const {
+        if (tid < 8) es[tid] = tid < 4 ? pow2i(kv8_exp(e)) : (float)kv8_exp(e);
+#pragma unroll
+        for (int i = 0; i < N; i++) {
+            const int at = tid + i * NT;
+            const int s = at / (HD / 16), j = at % (HD / 16) * 2;
+            const int r = (s & ~12) | (s & 4) << 1 | (s & 8) >> 1;
+            ks[r * (HD / 8) + (j ^ (r & 7))] = bytes_h(k[i][0], k[i][1]);
+            ks[r * (HD / 8) + ((j + 1) ^ (r & 7))] = bytes_h(k[i][2], k[i][3]);
+            const int d = at / 4, m = at % 4 * 2;
+            vs[d * 8 + (m ^ (d & 7))] = bytes_h(v[i][0], v[i][1]);
+            vs[d * 8 + ((m + 1) ^ (d & 7))] = bytes_h(v[i][2], v[i][3]);
+        }
+    }
+};
+
+// Many rows: a workgroup of NW waves takes 32 NW / DS rows of one kv head, a wave
+// 32 of them (all their dimensions, or half of them beside another wave with DS =
+// 2, both of which form the scores), and the units one after another, turned into
+// halves in LDS once for all its rows (two buffers: the next unit is requested
+// before and stored after this one's products).  Scores transposed as above, on
+// 32x32x16 products, for half a unit at a time.  f16 rows rescale o only when a
+// maximum rises by more than 2^7: their weights then reach 2^15 at most, from 2^8
+// (a weight keeps its bits down to 2^-22 of the largest and is lost below 2^-33,
+// 2^17 of which are below the output's rounding).
+template <int HD, bool F16, int NW, int DS>
+__global__ __launch_bounds__(NW *WAVE, HD == 128 ? 2 : 1) void kv8_prompt_kernel(Kv8AttnArgs a) {
+    constexpr int NF = HD / 16, DT = HD / 32 / DS, R = 32 * NW / DS;
+    constexpr bool AHEAD = HD == 128;  // registers left to request operands from LDS ahead of their use
+    constexpr float PS = F16 ? 8.f : PSCALE, LAZY = F16 ? 7.f : 0.f;
+    __shared__ __attribute__((aligned(16))) f16x8 lds[2][2][T * HD / 8];  // [buffer][K, V]
+    __shared__ __attribute__((aligned(16))) float es[2][8];  // K's steps and V's exponents, per 16 slots
+    const int tid = threadIdx.x, lane = tid & (WAVE - 1), wave = tid / WAVE;
+    const int c = lane & 31, h = lane >> 5;
+    const int kvh = blockIdx.x, rt = gridDim.y - 1 - blockIdx.y, split = blockIdx.z;  // the longest first
+    const int rows = a.n * a.group, past = kv8_past(a.past, a.n, a.c.cap);
+    const int row0 = rt * R + wave / DS * 32, d0 = wave % DS * DT;  // my rows, my first tile of 32 dimensions
+    const int units = (past + row_token(a, min(rt * R + R - 1, rows - 1)) + T) / T;
+    const int u0 = (int)((int64_t)split * units / a.splits), u1 = (int)((int64_t)(split + 1) * units / a.splits);
+    const int mine = row0 < rows ? past + row_token(a, min(row0 + 31, rows - 1)) + 1 : 0;  // slots my rows see
+    const int first_limit = past + row_token(a, row0) + 1;
+    const int r = row0 + c, rr = min(r, rows - 1), limit = past + row_token(a, rr) + 1;
+    QRows<HD, F16> q;
+    q.load(a.q, row_at(a, rr, kvh, a.q_stride, HD), h, r < rows, a.scale < 0.f);
+    const int8_t *kb = a.c.kc + (size_t)kvh * a.c.cap * HD, *vb = a.c.vc + (size_t)kvh * a.c.cap * HD;
+    const int8_t *ke = a.c.ke + (size_t)kvh * (a.c.cap >> a.c.lb);
+    const int8_t *ve = a.c.ve + (size_t)kvh * (a.c.cap >> a.c.lb);
+    const float scale = fabsf(a.scale);
+    float m = NEG, l = 0.f;
+    f32x16 o[DT];
+#pragma unroll
+    for (int d = 0; d < DT; d++)
+#pragma unroll
+        for (int i = 0; i < 16; i++) o[d][i] = 0.f;
+    Stage<HD, NW * WAVE> st;
+    if (u0 < u1) {
+        st.load(kb, vb, ke, ve, a.c.lb, u0, tid);
+        st.store(lds[0][0], lds[0][1], es[0], tid);
+    }
+    __syncthreads();
+    for (int u = u0; u < u1; u++) {
+        const int buf = (u - u0) & 1;
+        const f16x8 *kt = lds[buf][0], *vt = lds[buf][1];
+        if (u + 1 < u1) st.load(kb, vb, ke, ve, a.c.lb, u + 1, tid);
+        if (u * T < mine) {
+            const f32x4 kmul = *(const f32x4 *)&es[buf][0] * scale, ev = *(const f32x4 *)&es[buf][4];
+            auto k_at = [&](int x, int f) { return kt[(32 * x + c) * (HD / 8) + ((2 * f + h) ^ (c & 7))]; };
+            auto v_at = [&](int x, int b, int d) {
+                return vt[(32 * (d0 + d) + c) * 8 + ((4 * x + 2 * b + h) ^ (c & 7))];
+            };
+            f16x8 kf[AHEAD ? NF : 1], vf[AHEAD ? DT : 1][2];
+            if constexpr (AHEAD)
+#pragma unroll
+                for (int f = 0; f < NF; f++) kf[f] = k_at(0, f);
+            // 32 slots: two groups of 16 with an exponent each
+#pragma unroll
+            for (int x = 0; x < 2; x++) {
+                f32x16 s;
+#pragma unroll
+                for (int i = 0; i < 16; i++) s[i] = 0.f;
+#pragma unroll
+                for (int f = 0; f < NF; f++) {
+                    const f16x8 w = AHEAD ? kf[AHEAD ? f : 0] : k_at(x, f);
+                    s = mfma32(w, q.hi[f], s);
+                    if constexpr (!F16) s = mfma32(w, q.lo[f], s);
+                }
+                // V of this half is requested before the softmax, K of the next half before V's products
+                if constexpr (AHEAD) {
+#pragma unroll
+                    for (int d = 0; d < DT; d++)
+#pragma unroll
+                        for (int b = 0; b < 2; b++) vf[d][b] = v_at(x, b, d);
+                    __builtin_amdgcn_sched_barrier(0);
+                }
+                if (u * T + 32 * x + 32 > first_limit) {
+#pragma unroll
+                    for (int i = 0; i < 16; i++)
+                        if (u * T + 32 * x + 16 * (i / 8) + 8 * h + i % 8 >= limit) s[i] = -INFINITY;
+                }
+                f16x8 ph[2], pl[2];
+                float mul[2], top = -INFINITY;
+#pragma unroll
+                for (int b = 0; b < 2; b++) {
+                    mul[b] = fmaxf(F16 ? kmul[2 * x + b] : ldexpf(kmul[2 * x + b], q.e), FLT_MIN);
+                    float t8 = s[8 * b];
+#pragma unroll
+                    for (int i = 1; i < 8; i++) t8 = fmaxf(t8, s[8 * b + i]);
+                    top = fmaxf(top, fmaf(t8, mul[b], ev[2 * x + b]));
+                }
+                top = half_reduce(top, [](float y, float z) { return fmaxf(y, z); });
+                if (__any(top > m + LAZY)) {
+                    const float m1 = fmaxf(m, top), alpha = ex2(m - m1);
+                    m = m1;
+                    l *= alpha;
+#pragma unroll
+                    for (int d = 0; d < DT; d++)
+#pragma unroll
+                        for (int i = 0; i < 16; i++) o[d][i] *= alpha;
+                }
+#pragma unroll
+                for (int b = 0; b < 2; b++) {
+                    const float bias = ev[2 * x + b] - m + PS;
+                    float sum = 0.f;
+#pragma unroll
+                    for (int i = 0; i < 8; i++) {
+                        const float p = ex2(fmaf(s[8 * b + i], mul[b], bias));
+                        sum += p;
+                        const _Float16 t = (_Float16)p;
+                        ph[b][i] = t;
+                        if constexpr (!F16) pl[b][i] = (_Float16)(p - (float)t);
+                    }
+                    l = fmaf(sum, pow2i(-(int)ev[2 * x + b]), l);
+                }
+                if constexpr (AHEAD)
+                    if (x == 0) {
+#pragma unroll
+                        for (int f = 0; f < NF; f++) kf[f] = k_at(1, f);
+                    }
+#pragma unroll
+                for (int b = 0; b < 2; b++)
+#pragma unroll
+                    for (int d = 0; d < DT; d++) {
+                        const f16x8 w = AHEAD ? vf[AHEAD ? d : 0][b] : v_at(x, b, d);
+                        o[d] = mfma32(w, ph[b], o[d]);
+                        if constexpr (!F16) o[d] = mfma32(w, pl[b], o[d]);
+                    }
+            }
+        }
+        if (u + 1 < u1) st.store(lds[buf ^ 1][0], lds[buf ^ 1][1], es[buf ^ 1], tid);
+        __syncthreads();
+    }
+    l = half_reduce(l, [](float x, float y) { return x + y; });
+    if (r >= rows) return;
+    const size_t id = row_id(a, r, kvh);
+    const bool last = a.splits == 1;
+    const float inv = last ? 1.f / l : 1.f;
+    const int64_t to = row_at(a, r, kvh, a.out_stride, HD);
+#pragma unroll
+    for (int d = 0; d < DT; d++)
+#pragma unroll
+        for (int i = 0; i < 4; i++) {
+            const int dim = 32 * (d0 + d) + 8 * i + 4 * h;
+            const f32x4 y = {o[d][4 * i] * inv, o[d][4 * i + 1] * inv, o[d][4 * i + 2] * inv, o[d][4 * i + 3] * inv};
+            if (!last)
+                *(f32x4 *)(a.part + (id * a.splits + split) * HD + dim) = y;
+            else if constexpr (F16)
+                *(u32x2 *)((uint16_t *)a.out + to + dim) =
+                    u32x2{f2h(y[0]) | (uint32_t)f2h(y[1]) << 16, f2h(y[2]) | (uint32_t)f2h(y[3]) << 16};
+            else
+                *(f32x4 *)((float *)a.out + to + dim) = y;
+        }
+    if (h == 0 && d0 == 0) {
+        if (!last) a.ml[id * a.splits + split] = make_float2(m + (PSCALE - PS), l);
+        else if (a.lse) a.lse[id] = m + log2f(l) - PS;
+    }
 }
 
 // The weight that every slot receives from the call's rows, summed in f32 over
 // all of them: scores formed again from K (half of the cache) and each row's
-// log-sum.  A workgroup owns a unit of 64 slots, or four where one tile of rows
-// is all there is; its waves take alternate row tiles and meet in LDS, so every
-// sum is in a fixed order.
-template <int HD, bool F16>
-__global__ __launch_bounds__(WG) void kv8_mass_kernel(Kv8AttnArgs a, int upw) {
-    constexpr int NK = HD / 64;
-    __shared__ float sum[4][T];
+// log-sum.  Every sum is in a fixed order.
+//
+// One tile of rows (decode): q stays in registers and a wave takes unit after
+// unit, K of the next one requested before this one's products.
+template <int HD, int MODE>
+__global__ __launch_bounds__(WG) void kv8_mass_few_kernel(Kv8AttnArgs a) {
+    constexpr int NK = HD / 64, R = tile_rows(MODE);
     const int tid = threadIdx.x, lane = tid & (WAVE - 1), wave = tid / WAVE;
     const int c = lane & 15, g = lane >> 4, kvh = blockIdx.x;
     const int rows = a.n * a.group, past = kv8_past(a.past, a.n, a.c.cap), end = past + a.n;
-    const int u = blockIdx.y * upw + (upw > 1 ? wave : 0);
-    const bool have = u * T < end;
+    const int units = (end + T - 1) / T, step = gridDim.y * 4;
+    const int rr = min(c % R, rows - 1);
+    const int limit = c < min(R, rows) ? past + row_token(a, rr) + 1 : 0;  // each row once
+    QTile<HD, MODE> q;
+    typename QTile<HD, MODE>::Raw raw;
+    QTile<HD, MODE>::fetch(raw, a.q, row_at(a, rr, kvh, a.q_stride, HD), g);
+    const float lse = a.lse[row_id(a, rr, kvh)];
     const int8_t *kb = a.c.kc + (size_t)kvh * a.c.cap * HD;
+    const int8_t *ke = a.c.ke + (size_t)kvh * (a.c.cap >> a.c.lb);
+    float *mass = a.mass + (size_t)kvh * a.c.cap;
     const int krow = 16 * (c >> 2) + (c & 3);
-    float acc[4][4];
-#pragma unroll
-    for (int t = 0; t < 4; t++)
-#pragma unroll
-        for (int i = 0; i < 4; i++) acc[t][i] = 0.f;
-    if (have) {
-        u32x4 kr[4][NK];
+    u32x4 kr[4][NK];
+    int kexp = 0;
+    float was = 0.f;
+    auto load = [&](int u) {
 #pragma unroll
         for (int t = 0; t < 4; t++)
 #pragma unroll
             for (int k = 0; k < NK; k++)
                 kr[t][k] = *(const u32x4 *)(kb + (size_t)(u * T + krow + 4 * t) * HD + 64 * k + 16 * g);
-        const int kexp = kv8_exp(a.c.ke[(size_t)kvh * (a.c.cap >> a.c.lb) + ((u * T + 16 * g) >> a.c.lb)]);
-        // the first row that sees a slot of this unit
-        const int tok0 = max(0, u * T - past), rt0 = tok0 * a.group / 16;
-        for (int rt = rt0 + (upw > 1 ? 0 : wave); rt * 16 < rows; rt += upw > 1 ? 1 : 4) {
-            const int row = rt * 16 + c, rr = min(row, rows - 1);
-            const bool ok = row < rows;
-            const int limit = ok ? past + rr / a.group + 1 : 0;
-            QTile<HD, F16> q;
-            q.load(a.q, row_at(rr, a.group, kvh, a.q_stride, HD), g, ok);
-            const float lse = a.lse[(size_t)(rr / a.group) * a.n_heads + kvh * a.group + rr % a.group];
-            const float mul = ldexpf(a.scale, kexp + q.e);
+        kexp = ke[(u * T + 16 * g) >> a.c.lb];
+        was = u * T + lane < past ? mass[u * T + lane] : 0.f;
+    };
+    int u = blockIdx.y * 4 + wave;
+    if (u < units) load(u);
+    q.make(raw, c % R < rows, a.scale < 0.f, c >= R);
+    const float scale = fabsf(a.scale);
+    for (; u < units; u += step) {
+        f32x4 s[4];
 #pragma unroll
-            for (int t = 0; t < 4; t++) {
-                f32x4 s = {0.f, 0.f, 0.f, 0.f};
+        for (int t = 0; t < 4; t++) s[t] = scores<HD, MODE>(kr[t], q);
+        const float mul = ldexpf(scale, kv8_exp((int8_t)kexp) + q.e), had = was;
+        if (u + step < units) load(u + step);
+        const int p0 = u * T + 16 * g;
+        // slot 16 g + 4 t + i summed over the 16 rows, kept by lane c = 4 t + i
+        float sum = 0.f;
 #pragma unroll
-                for (int k = 0; k < NK; k++)
+        for (int t = 0; t < 4; t++)
 #pragma unroll
-                    for (int h = 0; h < 2; h++) {
-                        const f16x8 w = bytes_h(kr[t][k][2 * h], kr[t][k][2 * h + 1]);
-                        s = mfma(w, q.hi[2 * k + h], s);
-                        if constexpr (!F16) s = mfma(w, q.lo[2 * k + h], s);
-                    }
+            for (int i = 0; i < 4; i++) {
+                const float p = p0 + 4 * t + i < limit ? ex2(fmaf(s[t][i], mul, -lse)) : 0.f;
+                const float v = lane_group_sum(p, 16);
+                sum = c == 4 * t + i ? v : sum;
+            }
+        if (u * T + lane < end) mass[u * T + lane] = had + sum;
+    }
+}
+
+// Many rows: a workgroup owns 64 X slots, a wave 32 X of them (K in its operand
+// registers, converted once) and every other 32 rows of the tiles of 64 rows of q
+// that pass through LDS (two buffers).  The sums over rows stay in registers; at
+// the end they cross the lanes and meet, two waves a slot, in LDS.
+template <int HD, bool F16, int X>
+__global__ __launch_bounds__(WG, 2) void kv8_mass_kernel(Kv8AttnArgs a) {
+    constexpr int NF = HD / 16, QR = 64, PC = F16 ? 1 : 2, TPR = WG / QR, EL = HD / TPR, WS = 32 * X, GS = 2 * WS;
+    __shared__ __attribute__((aligned(16))) f16x8 qs[2][PC][QR * HD / 8];
+    __shared__ float qmul[2][QR], qlse[2][QR], sum[2][GS];
+    const int tid = threadIdx.x, lane = tid & (WAVE - 1), wave = tid / WAVE;
+    const int c = lane & 31, h = lane >> 5, kvh = blockIdx.x, s0 = blockIdx.y * GS + (wave & 1) * WS;
+    const int rows = a.n * a.group, past = kv8_past(a.past, a.n, a.c.cap), end = past + a.n;
+    if ((int)blockIdx.y * GS >= end) return;
+    const float scale = fabsf(a.scale);
+    const bool neg = a.scale < 0.f;
+    // the tile's rows into registers, four threads a row, then as halves into LDS
+    const int qr = tid / TPR, qj = tid % TPR;
+    u32x4 raw[F16 ? EL / 8 : EL / 4];
+    float raw_lse = 0.f;
+    auto fetch = [&](int t0) {
+        const int r = min(t0 + qr, rows - 1);
+        const int64_t at = row_at(a, r, kvh, a.q_stride, HD) + qj * EL;
 #pragma unroll
-                for (int i = 0; i < 4; i++)
-                    if (u * T + 16 * g + 4 * t + i < limit) acc[t][i] += exp2f(fmaf(s[i], mul, -lse));
+        for (int i = 0; i < (F16 ? EL / 8 : EL / 4); i++)
+            raw[i] = F16 ? *(const u32x4 *)((const uint16_t *)a.q + at + 8 * i)
+                         : *(const u32x4 *)((const float *)a.q + at + 4 * i);
+        raw_lse = a.lse[row_id(a, r, kvh)];
+    };
+    auto store = [&](int b) {
+        int e = 0;
+        if constexpr (F16) {
+            const uint32_t sign = neg ? 0x80008000u : 0u;
+#pragma unroll
+            for (int i = 0; i < EL / 8; i++) {
+                u32x4 w = raw[i];
+#pragma unroll
+                for (int k = 0; k < 4; k++) w[k] ^= sign;
+                qs[b][0][qr * (HD / 8) + ((qj * (EL / 8) + i) ^ (qr & 7))] = __builtin_bit_cast(f16x8, w);
+            }
+        } else {
+            float amax = 0.f;
+#pragma unroll
+            for (int i = 0; i < EL / 4; i++)
+#pragma unroll
+                for (int k = 0; k < 4; k++) {
+                    const float x = __uint_as_float(raw[i][k]);
+                    amax = fmaxf(amax, fabsf(x));
+                }
+            amax = fmaxf(amax, OI_DPP(amax, 0xB1));
+            amax = fmaxf(amax, OI_DPP(amax, 0x4E));
+            e = amax > 0.f ? (int)(__float_as_uint(amax) >> 23) - 127 - 14 : 0;
+#pragma unroll
+            for (int i = 0; i < EL / 8; i++) {
+                f16x8 hi, lo;
+#pragma unroll
+                for (int k = 0; k < 8; k++) {
+                    const uint32_t bits = raw[2 * i + k / 4][k & 3];
+                    const float x = __uint_as_float(bits), y = ldexpf(neg ? -x : x, -e);
+                    const _Float16 t = (_Float16)y;
+                    hi[k] = t;
+                    lo[k] = (_Float16)(y - (float)t);
+                }
+                const int at = qr * (HD / 8) + ((qj * (EL / 8) + i) ^ (qr & 7));
+                qs[b][0][at] = hi;
+                qs[b][PC - 1][at] = lo;
             }
         }
+        if (qj == 0) {
+            qmul[b][qr] = ldexpf(scale, e);
+            qlse[b][qr] = raw_lse;
+        }
+    };
+    // K: row c of each half unit; its 16-byte loads supply two operands, dimensions 32 m + 16 h + 0..7 and + 8..15
+    f16x8 kf[X][NF];
+    const int8_t *kb = a.c.kc + (size_t)kvh * a.c.cap * HD;
+    const bool have = s0 < a.c.cap;
+    const int s_at = have ? s0 : 0;
+#pragma unroll
+    for (int x = 0; x < X; x++)
+#pragma unroll
+        for (int m = 0; m < NF / 2; m++) {
+            const u32x4 w = *(const u32x4 *)(kb + (size_t)(s_at + 32 * x + c) * HD + 32 * m + 16 * h);
+            kf[x][2 * m] = bytes_h(w[0], w[1]);
+            kf[x][2 * m + 1] = bytes_h(w[2], w[3]);
+        }
+    float step[2 * X];
+    const int8_t *ke = a.c.ke + (size_t)kvh * (a.c.cap >> a.c.lb);
+#pragma unroll
+    for (int b = 0; b < 2 * X; b++) step[b] = pow2i(kv8_exp(ke[(s_at + 16 * b) >> a.c.lb]));
+    float acc[X][16];
+#pragma unroll
+    for (int x = 0; x < X; x++)
+#pragma unroll
+        for (int i = 0; i < 16; i++) acc[x][i] = 0.f;
+    // from the tile of rows that first sees one of the slots
+    const int first = max(0, (int)blockIdx.y * GS - past) * a.group / QR * QR;
+    fetch(first);
+    store(0);
+    __syncthreads();
+    for (int t0 = first, b = 0; t0 < rows; t0 += QR, b ^= 1) {
+        if (t0 + QR < rows) fetch(t0 + QR);
+        const int lr = 32 * (wave >> 1) + c, r = t0 + lr;  // my column's row
+        const int r_last = min(t0 + 32 * (wave >> 1) + 31, rows - 1);
+        if (s0 < past + row_token(a, r_last) + 1 && t0 + 32 * (wave >> 1) < rows) {
+            const int limit = r < rows ? past + row_token(a, r) + 1 : 0;
+            const float qm = qmul[b][lr], lse = qlse[b][lr];
+            const bool edge = s0 + WS > past + row_token(a, t0 + 32 * (wave >> 1)) + 1 || t0 + QR > rows;
+#pragma unroll
+            for (int x = 0; x < X; x++) {
+                f32x16 s;
+#pragma unroll
+                for (int i = 0; i < 16; i++) s[i] = 0.f;
+#pragma unroll
+                for (int f = 0; f < NF; f++) {
+                    const int at = lr * (HD / 8) + ((4 * (f / 2) + 2 * h + (f & 1)) ^ (lr & 7));
+                    s = mfma32(kf[x][f], qs[b][0][at], s);
+                    if constexpr (!F16) s = mfma32(kf[x][f], qs[b][PC - 1][at], s);
+                }
+                if (edge) {
+#pragma unroll
+                    for (int i = 0; i < 16; i++) {
+                        const float p = ex2(fmaf(s[i], step[2 * x + i / 8] * qm, -lse));
+                        acc[x][i] += s0 + 32 * x + 8 * (i / 4) + 4 * h + i % 4 < limit ? p : 0.f;
+                    }
+                } else {
+#pragma unroll
+                    for (int i = 0; i < 16; i++) acc[x][i] += ex2(fmaf(s[i], step[2 * x + i / 8] * qm, -lse));
+                }
+            }
+        }
+        if (t0 + QR < rows) store(b ^ 1);
+        __syncthreads();
     }
 #pragma unroll
-    for (int t = 0; t < 4; t++)
+    for (int x = 0; x < X; x++)
 #pragma unroll
-        for (int i = 0; i < 4; i++) {
-            const float v = lane_group_sum(acc[t][i], 16);
-            if (c == 0) sum[wave][16 * g + 4 * t + i] = v;
+        for (int i = 0; i < 16; i++) {
+            float v = lane_group_sum(acc[x][i], 16);
+            const auto w = __builtin_amdgcn_permlane16_swap(__float_as_uint(v), __float_as_uint(v), false, false);
+            v = __uint_as_float(w[0]) + __uint_as_float(w[1]);
+            if (c == 0) sum[wave >> 1][(wave & 1) * WS + 32 * x + 8 * (i / 4) + 4 * h + i % 4] = v;
         }
     __syncthreads();
-    if (upw > 1) {
-        const int s = u * T + lane;
-        if (s < end) {
-            float *m = a.mass + (size_t)kvh * a.c.cap + s;
-            *m = s < past ? *m + sum[wave][lane] : sum[wave][lane];
-        }
-    } else if (tid < T) {
-        const int s = u * T + tid;
-        if (s < end) {
-            const float v = (sum[0][tid] + sum[1][tid]) + (sum[2][tid] + sum[3][tid]);
-            float *m = a.mass + (size_t)kvh * a.c.cap + s;
-            *m = s < past ? *m + v : v;
-        }
+    const int s = blockIdx.y * GS + tid;
+    if (tid < GS && s < end) {
+        float *m = a.mass + (size_t)kvh * a.c.cap + s;
+        const float v = sum[0][tid] + sum[1][tid];
+        *m = s < past ? *m + v : v;
     }
 }
 
 }  // namespace
 
-int kv8_attn_splits(int n_kv, int group, int n, int end) {
-    const int64_t units = (end + T - 1) / T, tiles = ((int64_t)n * group + 15) / 16 * n_kv;
-    int64_t s = (units + 3) / 4;  // a unit per wave
-    const int64_t want = (768 + tiles - 1) / tiles;
-    if (s > want) s = want;
-    return s < 1 ? 1 : (int)s;
+// Up to FEW_ROWS rows of a kv head go by 16 (kv8_rows_kernel), more to the prompt
+// kernel: workgroups of 8 waves where they fill the card's 256 CUs (a unit is
+// converted for 256 rows at a time), of 4 waves, two to a CU, otherwise; for
+// head_dim 256 the registers of f16 rows allow 8 waves in pairs that share 32 rows
+// and hold half of the dimensions each, those of f32 rows 4 waves.
+constexpr int FEW_ROWS = 64, CUS = 256;
+
+struct PromptPlan {
+    int waves, rows, resident;  // of a workgroup; workgroups at a time
+};
+static PromptPlan prompt_plan(int hd, bool f16, int n_kv, int64_t rows) {
+    if (hd == 256) return {f16 ? 8 : 4, 128, CUS};
+    if ((rows + 255) / 256 * n_kv >= CUS) return {8, 256, CUS};
+    return {4, 128, 2 * CUS};
+}
+
+int kv8_attn_splits(int n_kv, int group, int n, int end, int hd, bool f16) {
+    const int64_t units = (end + T - 1) / T, rows = (int64_t)n * group;
+    if (rows <= FEW_ROWS) {
+        // a unit per wave, up to two workgroups a CU
+        const int64_t tiles = (rows + 15) / 16 * n_kv, most = (2 * CUS + tiles - 1) / tiles;
+        return (int)std::max<int64_t>(1, std::min((units + 3) / 4, most));
+    }
+    // The least of rounds * (units of a split + 3 for its beginning and end) + the
+    // merge (a launch, and the splits' f32 results out and in), in units of one
+    // tile's step (about 2.7 us)
+    const PromptPlan p = prompt_plan(hd, f16, n_kv, rows);
+    const int64_t tiles = (rows + p.rows - 1) / p.rows * n_kv;
+    const double merge = (double)rows * n_kv * hd * 8 / 5e6 / 2.7;
+    int best = 1;
+    double least = 1e30;
+    for (int64_t s = 1; s <= 64 && s <= (units + 1) / 2; s++) {
+        const double c = (double)((tiles * s + p.resident - 1) / p.resident) * ((double)units / s + 3) +
+                         (s > 1 ? 2 + merge * s : 0);
+        if (c < least) {
+            least = c;
+            best = (int)s;
+        }
+    }
+    return best;
 }
 
 size_t kv8_attn_workspace(int n_heads, int n, int hd, int splits) {
-    return (size_t)n * n_heads * ((size_t)splits * (hd + 2) + 1) * 4;
+    return (size_t)n * n_heads * ((splits > 1 ? (size_t)splits * (hd + 2) : 0) + 1) * 4;
 }
 
-hipError_t launch_kv8_attn(const Kv8AttnArgs &a, hipStream_t st) {
+namespace {
+
+template <int HD, int MODE>
+void launch(const Kv8AttnArgs &a, hipStream_t st) {
+    constexpr int R = tile_rows(MODE);
+    constexpr bool F16 = MODE == ROWS_F16;
     const int rows = a.n * a.group;
-    const dim3 g1((unsigned)a.c.n_kv, (unsigned)((rows + 15) / 16), (unsigned)a.splits);
-    const dim3 g2((unsigned)(a.n * a.n_heads));
     const int end = a.past.dev ? a.c.cap : a.past.past + a.n, units = (end + T - 1) / T;
-    const int upw = rows <= 16 ? 4 : 1;
-    const dim3 g3((unsigned)a.c.n_kv, (unsigned)((units + upw - 1) / upw));
-    auto go = [&](auto k1, auto k2, auto k3) {
-        hipLaunchKernelGGL(k1, g1, dim3(WG), 0, st, a);
-        hipLaunchKernelGGL(k2, g2, dim3((unsigned)a.c.hd), 0, st, a);
-        if (a.mass) hipLaunchKernelGGL(k3, g3, dim3(WG), 0, st, a, upw);
-    };
-    if (a.c.hd == 128) {
-        if (a.f16) go(kv8_rows_kernel<128, true>, kv8_merge_kernel<128, true>, kv8_mass_kernel<128, true>);
-        else go(kv8_rows_kernel<128, false>, kv8_merge_kernel<128, false>, kv8_mass_kernel<128, false>);
-    } else if (a.c.hd == 256) {
-        if (a.f16) go(kv8_rows_kernel<256, true>, kv8_merge_kernel<256, true>, kv8_mass_kernel<256, true>);
-        else go(kv8_rows_kernel<256, false>, kv8_merge_kernel<256, false>, kv8_mass_kernel<256, false>);
-    } else {
-        return hipErrorInvalidValue;
+    if (rows <= FEW_ROWS) {
+        hipLaunchKernelGGL((kv8_rows_kernel<HD, MODE>),
+                           dim3((unsigned)a.c.n_kv, (unsigned)((rows + R - 1) / R), (unsigned)a.splits), dim3(WG), 0, st,
+                           a);
+    } else if constexpr (MODE != ROWS_PACK) {
+        const PromptPlan p = prompt_plan(HD, F16, a.c.n_kv, rows);
+        const dim3 grid((unsigned)a.c.n_kv, (unsigned)((rows + p.rows - 1) / p.rows), (unsigned)a.splits);
+        auto go = [&](auto kernel) { hipLaunchKernelGGL(kernel, grid, dim3((unsigned)(p.waves * WAVE)), 0, st, a); };
+        if constexpr (HD == 128) p.waves == 8 ? go(kv8_prompt_kernel<HD, F16, 8, 1>) : go(kv8_prompt_kernel<HD, F16, 4, 1>);
+        else if constexpr (F16) go(kv8_prompt_kernel<HD, F16, 8, 2>);
+        else go(kv8_prompt_kernel<HD, F16, 4, 1>);
     }
+    if (a.splits > 1)
+        hipLaunchKernelGGL((kv8_merge_kernel<HD, F16>), dim3((unsigned)a.n_heads, (unsigned)a.n), dim3(MW), 0, st, a);
+    if (!a.mass) return;
+    if (rows <= R) {
+        const int wgs = std::max(1, std::min((units + 3) / 4, 512 / a.c.n_kv));
+        hipLaunchKernelGGL((kv8_mass_few_kernel<HD, MODE>), dim3((unsigned)a.c.n_kv, (unsigned)wgs), dim3(WG), 0, st, a);
+    } else if constexpr (MODE != ROWS_PACK) {
+        constexpr int X = HD == 128 ? 2 : 1;  // 64 slots of K a wave, 32 where a row is twice as long
+        hipLaunchKernelGGL((kv8_mass_kernel<HD, F16, X>),
+                           dim3((unsigned)a.c.n_kv, (unsigned)((end + 64 * X - 1) / (64 * X))), dim3(WG), 0, st, a);
+    }
+}
+
+}  // namespace
+
+hipError_t launch_kv8_attn(const Kv8AttnArgs &a, hipStream_t st) {
+    const int mode = a.f16 ? ROWS_F16 : a.n * a.group <= 8 ? ROWS_PACK : ROWS_F32;
+    auto by_mode = [&](auto hd) {
+        constexpr int HD = decltype(hd)::value;
+        if (mode == ROWS_F16) launch<HD, ROWS_F16>(a, st);
+        else if (mode == ROWS_PACK) launch<HD, ROWS_PACK>(a, st);
+        else launch<HD, ROWS_F32>(a, st);
+    };
+    if (a.c.hd == 128) by_mode(std::integral_constant<int, 128>{});
+    else if (a.c.hd == 256) by_mode(std::integral_constant<int, 256>{});
+    else return hipErrorInvalidValue;
     return hipGetLastError();
 }
 
