@@ -219,6 +219,9 @@ int oi_kv8_evict_launch(const oi_kv8_dims *src_dims, const void *src, const floa
         if (!src || !src_mass || !dst || !dst_mass || !kept || !src_pos != !dst_pos)
             return err(OI_E_ARG, W, "null argument (positions come and go together)");
         if (!aligned(src, 256) || !aligned(dst, 256)) return err(OI_E_ARG, W, "a cache must be 256-byte aligned");
+        if (!aligned(src_mass, 16) || !aligned(dst_mass, 4) || !aligned(src_pos, 4) || !aligned(dst_pos, 4) ||
+            !aligned(kept, 4))
+            return err(OI_E_ARG, W, "src_mass must be 16-byte aligned, the others 4");
         if (n <= 0 || n > src_dims->capacity || keep <= 0 || keep > n || keep > dst_dims->capacity)
             return err(OI_E_RANGE, W, "n=" + std::to_string(n) + " keep=" + std::to_string(keep) + " out of range");
         if (n_first < 0 || n_last < 0 || (int64_t)n_first + n_last > keep)

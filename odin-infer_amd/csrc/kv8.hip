@@ -11,6 +11,8 @@
 // V lies transposed in tiles of 64 slots, [hd][64], the order in which the
 // matrix product P V takes it (kv8_attn.hip).
 
+#include <type_traits>
+
 #include "kv8_common.h"
 
 namespace oi {
@@ -195,122 +197,231 @@ __global__ __launch_bounds__(WG) void kv8_read_kernel(Kv8ReadArgs a) {
 
 constexpr int EV = 1024;  // threads of the selection
 
-// a mass as an unsigned key of the same order; NaN below everything, -0 as 0
-__device__ __forceinline__ uint32_t mass_key(float m) {
-    if (!(m == m)) return 0u;
+// Slot s's mass as an unsigned key of the same order, -0 as 0: infinities are
+// 0x007FFFFF and 0xFF800000, NaN is 1.  A slot that stays in any case (the first,
+// the last) has a key above them all, one past the end the key 0.
+__device__ __forceinline__ uint32_t slot_key(float m, int s, const Kv8EvictArgs &a) {
     const uint32_t b = __float_as_uint(m == 0.f ? 0.f : m);
-    return b & 0x80000000u ? ~b : b | 0x80000000u;
+    uint32_t k = b & 0x80000000u ? ~b : b | 0x80000000u;
+    k = m == m ? k : 1u;
+    k = s < a.first || s >= a.n - a.last ? 0xFFFFFFFFu : k;
+    return s < a.n ? k : 0u;
 }
 
-// inclusive scan of one value per thread over the workgroup; total in *sum
-__device__ __forceinline__ uint32_t block_scan(uint32_t v, uint32_t *ws, uint32_t *sum) {
-    const int tid = threadIdx.x, lane = tid & (WAVE - 1), wave = tid / WAVE;
+// Sum of v over the threads before this one; the total in *all.  ws: EV / 64 words.
+__device__ __forceinline__ uint32_t block_before(uint32_t v, uint32_t *ws, uint32_t *all) {
+    const int lane = threadIdx.x & (WAVE - 1), wave = threadIdx.x / WAVE;
+    uint32_t s = v;
 #pragma unroll
     for (int o = 1; o < WAVE; o <<= 1) {
-        const uint32_t u = __shfl_up(v, o, WAVE);
-        if (lane >= o) v += u;
+        const uint32_t u = __shfl_up(s, o, WAVE);
+        if (lane >= o) s += u;
     }
     __syncthreads();  // ws is free
-    if (lane == WAVE - 1) ws[wave] = v;
+    if (lane == WAVE - 1) ws[wave] = s;
     __syncthreads();
-    uint32_t before = 0, all = 0;
+    uint32_t before = 0, total = 0;
+#pragma unroll
     for (int w = 0; w < EV / WAVE; w++) {
         const uint32_t t = ws[w];
-        if (w < wave) before += t;
-        all += t;
+        before += w < wave ? t : 0u;
+        total += t;
     }
-    *sum = all;
-    return v + before;
+    *all = total;
+    return s - v + before;
 }
 
-// One workgroup per kv head.  The m-th largest key of the middle slots is found
-// digit by digit (8 bits, from the top) with a histogram in LDS; then every
-// thread walks a run of slots of its own, and two scans give the ties before it
-// (the lowest slots of them are kept) and its first place in the list.
+// One workgroup per kv head, a thread four neighbouring slots of every 4096.  The
+// keep-th largest key is found digit by digit (11, 11 and 10 bits from the top; a
+// first digit of the exponent and two more bits spreads the masses over many
+// counters) with counts in LDS.  Keys of the first digit's border go to a list in
+// LDS, so the other digits need no pass over the slots; only where too many share
+// it (more than EV_LIST) they take one each.  Then the slots that stay are counted
+// per wave, the counts summed up, and each finds its place; of equal keys at the
+// border the lowest slots stay.  Bound by its instructions on one CU: 25 a slot
+// and wave, three passes.
+constexpr int EV_TILE = 4 * EV, EV_CH = 64, EV_LIST = 8192;  // slots of a chunk; chunks counted at a time; the list
 __global__ __launch_bounds__(EV) void kv8_select_kernel(Kv8EvictArgs a) {
-    __shared__ uint32_t hist[256], ws[EV / WAVE];
-    __shared__ uint32_t s_prefix, s_need;
-    const int tid = threadIdx.x, kvh = blockIdx.x;
+    constexpr int NW = EV / WAVE;
+    __shared__ uint32_t hist[2048], cnt[EV_CH * NW], tcnt[EV_CH * NW], list[EV_LIST], ws[NW];
+    __shared__ uint32_t s_bin, s_left, s_ties, s_listed;
+    const int tid = threadIdx.x, lane = tid & (WAVE - 1), wave = tid / WAVE, kvh = blockIdx.x;
     const float *mass = a.mass + (size_t)kvh * a.src.cap;
-    const int lo = a.first, hi = a.n - a.last;  // the middle
-    const uint32_t m = (uint32_t)(a.keep - a.first - a.last);
-    uint32_t prefix = 0, need = m;
-    if (m > 0 && (uint32_t)(hi - lo) > m) {
-        for (int digit = 3; digit >= 0; digit--) {
-            const int sh = 8 * digit;
-            for (int i = tid; i < 256; i += EV) hist[i] = 0;
-            __syncthreads();
-            for (int s = lo + tid; s < hi; s += EV) {
-                const uint32_t k = mass_key(mass[s]);
-                if (digit == 3 || (k >> (sh + 8)) == (prefix >> (sh + 8))) atomicAdd(&hist[(k >> sh) & 255u], 1u);
+    int32_t *kept = a.kept + (size_t)kvh * a.keep;
+    const int chunks = (a.n + EV_TILE - 1) / EV_TILE;
+    // f(chunk - ch0, first slot, keys) for the thread's four slots of chunks ch0 .. ch0 + nch - 1
+    auto each = [&](int ch0, int nch, auto f) {
+        constexpr int B = 4;
+        for (int i0 = 0; i0 < nch; i0 += B) {
+            f32x4 x[B];
+#pragma unroll
+            for (int i = 0; i < B; i++)
+                x[i] = *(const f32x4 *)(mass + min((ch0 + i0 + i) * EV_TILE + 4 * tid, a.src.cap - 4));
+#pragma unroll
+            for (int i = 0; i < B; i++) {
+                if (i0 + i >= nch) continue;
+                const int s = (ch0 + i0 + i) * EV_TILE + 4 * tid;
+                uint32_t k[4];
+#pragma unroll
+                for (int j = 0; j < 4; j++) k[j] = slot_key(x[i][j], s + j, a);
+                f(i0 + i, s, k);
             }
-            __syncthreads();
-            if (tid == 0) {
-                uint32_t left = need;
-                int b = 255;
-                while (b > 0 && hist[b] < left) left -= hist[b--];
-                s_prefix = prefix | (uint32_t)b << sh;
-                s_need = left;
-            }
-            __syncthreads();
-            prefix = s_prefix;
-            need = s_need;  // of the keys equal to the prefix so far, how many
         }
-    } else if (m > 0) {  // all of the middle
-        prefix = 0;
-        need = 0xFFFFFFFFu;
+    };
+    // kept: keys above `border`, and `need` of the `ties` equal to it
+    uint32_t border = 0, need = (uint32_t)a.keep, ties = 0, all;
+    // the digit of `bits` bits at `sh`: the largest counter with at least `need` keys in it and above
+    auto digit = [&](int sh, int bits) {
+        __syncthreads();
+        const int top = (1 << bits) - 1 - 2 * tid;  // counters in falling order, two a thread
+        const uint32_t c0 = top >= 0 ? hist[top] : 0, c1 = top >= 0 ? hist[top - 1] : 0;
+        const uint32_t before = block_before(c0 + c1, ws, &all);
+        if (before < need && before + c0 >= need) {
+            s_bin = (uint32_t)top;
+            s_left = need - before;
+            s_ties = c0;
+        } else if (before + c0 < need && before + c0 + c1 >= need) {
+            s_bin = (uint32_t)(top - 1);
+            s_left = need - before - c0;
+            s_ties = c1;
+        }
+        __syncthreads();
+        border |= s_bin << sh;
+        need = s_left;
+        ties = s_ties;
+        hist[tid] = 0;
+        hist[tid + EV] = 0;
+        __syncthreads();
+    };
+    hist[tid] = 0;
+    hist[tid + EV] = 0;
+    cnt[tid] = 0;
+    if (tid == 0) s_listed = 0;
+    __syncthreads();
+    each(0, chunks, [&](int, int, const uint32_t (&k)[4]) {
+#pragma unroll
+        for (int j = 0; j < 4; j++) atomicAdd(&hist[k[j] >> 21], 1u);
+    });
+    digit(21, 11);
+    bool counted = false;
+    if (chunks <= EV_CH && ties <= EV_LIST) {
+        const uint32_t head = border >> 21;
+        each(0, chunks, [&](int i, int, const uint32_t (&k)[4]) {
+            uint32_t above = 0;
+#pragma unroll
+            for (int j = 0; j < 4; j++) {
+                above += (uint32_t)__popcll(__ballot(k[j] >> 21 > head));
+                if (k[j] >> 21 == head) list[atomicAdd(&s_listed, 1u)] = (k[j] & 0x1FFFFFu) << 10 | (uint32_t)(i * NW + wave);
+            }
+            if (lane == 0) cnt[i * NW + wave] = above;
+        });
+        __syncthreads();
+        const uint32_t listed = s_listed;
+        for (uint32_t i = tid; i < listed; i += EV) atomicAdd(&hist[list[i] >> 20], 1u);
+        digit(10, 11);
+        for (uint32_t i = tid; i < listed; i += EV)
+            if (list[i] >> 20 == ((border >> 10) & 0x7FFu)) atomicAdd(&hist[(list[i] >> 10) & 0x3FFu], 1u);
+        digit(0, 10);
+        counted = ties <= need;
+        if (counted)
+            for (uint32_t i = tid; i < listed; i += EV)
+                if (list[i] >> 10 >= (border & 0x1FFFFFu)) atomicAdd(&cnt[list[i] & 0x3FFu], 1u);
+        __syncthreads();
     } else {
-        prefix = 0xFFFFFFFFu;
-        need = 0;
-    }
-    // a key above the prefix is kept, `need` of those equal to it
-    const int per = (a.n + EV - 1) / EV, b0 = min(tid * per, a.n), b1 = min(b0 + per, a.n);
-    uint32_t above = 0, ties = 0;
-    for (int s = b0; s < b1; s++) {
-        if (s < lo || s >= hi) {
-            above++;
-            continue;
+        for (int pass = 1; pass < 3; pass++) {
+            const int sh = pass == 1 ? 10 : 0, bits = pass == 1 ? 11 : 10;
+            const uint32_t head = border >> (sh + bits), mask = (1u << bits) - 1;
+            each(0, chunks, [&](int, int, const uint32_t (&k)[4]) {
+#pragma unroll
+                for (int j = 0; j < 4; j++)
+                    if (k[j] >> (sh + bits) == head) atomicAdd(&hist[(k[j] >> sh) & mask], 1u);
+            });
+            digit(sh, bits);
         }
-        const uint32_t k = mass_key(mass[s]);
-        if (k > prefix) above++;
-        else if (k == prefix) ties++;
     }
-    uint32_t sum;
-    uint32_t before = block_scan(ties, ws, &sum) - ties;
-    const uint32_t mine = before >= need ? 0u : min(ties, need - before);
-    uint32_t at = block_scan(above + mine, ws, &sum) - (above + mine);
-    uint32_t left = mine;
-    for (int s = b0; s < b1; s++) {
-        bool keep = s < lo || s >= hi;
-        if (!keep) {
-            const uint32_t k = mass_key(mass[s]);
-            if (k > prefix) keep = true;
-            else if (k == prefix && left > 0) {
-                keep = true;
-                left--;
+    uint32_t base = 0, tie_base = 0;
+    auto before_me = [&](unsigned long long b, uint32_t from) {
+        return __builtin_amdgcn_mbcnt_hi((uint32_t)(b >> 32), __builtin_amdgcn_mbcnt_lo((uint32_t)b, from));
+    };
+    auto place = [&](auto ranked) {  // ranked: some of the ties go
+        constexpr bool RANK = decltype(ranked)::value;
+        for (int ch0 = 0; ch0 < chunks; ch0 += EV_CH) {
+            const int nch = min(EV_CH, chunks - ch0);
+            if (!counted) {
+                each(ch0, nch, [&](int i, int, const uint32_t (&k)[4]) {
+                    uint32_t n = 0, t = 0;
+#pragma unroll
+                    for (int j = 0; j < 4; j++) {
+                        n += (uint32_t)__popcll(__ballot(RANK ? k[j] > border : k[j] >= border));
+                        if constexpr (RANK) t += (uint32_t)__popcll(__ballot(k[j] == border));
+                    }
+                    if (lane == 0) {
+                        cnt[i * NW + wave] = n;
+                        if constexpr (RANK) tcnt[i * NW + wave] = t;
+                    }
+                });
+                __syncthreads();
             }
+            uint32_t mine = tid < nch * NW ? cnt[tid] : 0, tie_all = 0;
+            if constexpr (RANK) {
+                const uint32_t t = tid < nch * NW ? tcnt[tid] : 0, ranks = tie_base + block_before(t, ws, &tie_all);
+                mine += ranks >= need ? 0u : min(t, need - ranks);
+                tcnt[tid] = ranks;
+            }
+            const uint32_t before = base + block_before(mine, ws, &all);
+            cnt[tid] = before;
+            __syncthreads();
+            each(ch0, nch, [&](int i, int s, const uint32_t (&k)[4]) {
+                bool on[4];
+                if constexpr (RANK) {
+                    uint32_t r = tcnt[i * NW + wave];
+#pragma unroll
+                    for (int j = 0; j < 4; j++) r = before_me(__ballot(k[j] == border), r);
+#pragma unroll
+                    for (int j = 0; j < 4; j++) {
+                        on[j] = k[j] > border || (k[j] == border && r < need);
+                        r += k[j] == border;
+                    }
+                } else {
+#pragma unroll
+                    for (int j = 0; j < 4; j++) on[j] = k[j] >= border;
+                }
+                uint32_t at = cnt[i * NW + wave];
+#pragma unroll
+                for (int j = 0; j < 4; j++) at = before_me(__ballot(on[j]), at);
+#pragma unroll
+                for (int j = 0; j < 4; j++)
+                    if (on[j] && at < (uint32_t)a.keep) kept[at++] = s + j;
+            });
+            base += all;
+            tie_base += tie_all;
+            __syncthreads();  // the counts are free
         }
-        if (keep && at < (uint32_t)a.keep) a.kept[(size_t)kvh * a.keep + at++] = s;
-    }
+    };
+    if (ties <= need) place(std::integral_constant<bool, false>{});
+    else place(std::integral_constant<bool, true>{});
 }
 
-// One workgroup per (64 kept slots, kv head, K or V): codes of the slots in
+// One workgroup per (64 kept slots, kv head, K or V): the codes of the slots in
 // `kept`, brought to the exponent that their new block needs (a left shift is
-// exact, a right shift rounds half to even).  K rows are read where they lie; of
-// V the source tiles between the first and the last slot come through LDS, since
-// a slot is a byte column of its tile.
+// exact, a right shift rounds half to even; most need none), from registers to
+// registers.  K rows are read where they lie, 16 bytes a thread.  Of V a slot is a
+// byte column: a thread reads four slots' bytes of a dimension, a workgroup 64
+// slots of it, which lie in a few neighbouring 64-byte rows (tiles brought through
+// LDS whole took 49 us against 20 for 8192 of 40960 slots: 45 KB a workgroup).
+// Bound by memory: K reads what is kept, V every row that holds a kept slot.
 template <int HD>
 __global__ __launch_bounds__(WG) void kv8_gather_kernel(Kv8EvictArgs a) {
-    constexpr int PR = T + 4;
-    __shared__ __attribute__((aligned(16))) int8_t in[HD * PR];   // a source V tile
-    __shared__ __attribute__((aligned(16))) int8_t out[HD * PR];  // gathered codes [dim][slot]
-    __shared__ int slot[T], need[T];
-    const int tid = threadIdx.x, lane = tid & (WAVE - 1), wave = tid / WAVE;
+    constexpr int PPR = HD / 16, NP = T * PPR / WG, NV = HD / 16;  // K: 16-byte pieces of a row, of a thread; V: words
+    __shared__ int slot[T], es[T], mx[T], be[4], up[T];
+    const int tid = threadIdx.x;
     const int unit = blockIdx.x, kvh = blockIdx.y, which = blockIdx.z, n = min(T, a.keep - unit * T);
-    const int32_t *kept = a.kept + (size_t)kvh * a.keep + unit * T;
+    const int8_t *ep = (which ? a.src.ve : a.src.ke) + (size_t)kvh * (a.src.cap >> a.src.lb);
     if (tid < T) {
-        const int s = kept[min(tid, n - 1)];
+        const int s = a.kept[(size_t)kvh * a.keep + unit * T + min(tid, n - 1)];
         slot[tid] = s;
+        mx[tid] = 0;
+        es[tid] = kv8_exp(ep[s >> a.src.lb]);
         if (tid < n && which == 0) {
             const size_t to = (size_t)kvh * a.dst.cap + unit * T + tid, from = (size_t)kvh * a.src.cap + s;
             a.dst_mass[to] = a.mass[from];
@@ -318,69 +429,90 @@ __global__ __launch_bounds__(WG) void kv8_gather_kernel(Kv8EvictArgs a) {
         }
     }
     __syncthreads();
-    const int8_t *ep = (which ? a.src.ve : a.src.ke) + (size_t)kvh * (a.src.cap >> a.src.lb);
+    u32x4 w[NP];
+    uint32_t v[NV];
+    const int vr = 4 * (tid % 16), vd = tid / 16;  // V: my four slots, my first dimension
     if (which == 0) {
-        // a wave per row
-        constexpr int CPL = HD / WAVE;  // codes per lane
-        for (int r = wave; r < n; r += WG / WAVE) {
-            const int8_t *row = a.src.kc + ((size_t)kvh * a.src.cap + slot[r]) * HD + CPL * lane;
-            int mx = 0;
 #pragma unroll
-            for (int i = 0; i < CPL; i++) {
-                const int c = row[i];
-                out[r * HD + CPL * lane + i] = (int8_t)c;
-                mx = max(mx, c < 0 ? -c : c);
-            }
-            mx = (int)wave_max_all((float)mx);
-            if (lane == 0) need[r] = mx ? kv8_exp(ep[slot[r] >> a.src.lb]) + (31 - __clz(mx)) - 6 : KV8_EMIN;
+        for (int k = 0; k < NP; k++) {
+            const int i = tid + k * WG;
+            w[k] = *((const u32x4 *)(a.src.kc + ((size_t)kvh * a.src.cap + slot[i / PPR]) * HD) + i % PPR);
+        }
+#pragma unroll
+        for (int k = 0; k < NP; k++) {
+            int x = 0;
+#pragma unroll
+            for (int c = 0; c < 4; c++)
+#pragma unroll
+                for (int j = 0; j < 4; j++) x = max(x, abs(byte_of(w[k][c], j)));
+            atomicMax(&mx[(tid + k * WG) / PPR], x);
         }
     } else {
-        const int t0 = slot[0] / T, t1 = slot[n - 1] / T;
-        for (int t = t0; t <= t1; t++) {
-            const u32x4 *src = (const u32x4 *)(a.src.vc + ((size_t)kvh * (a.src.cap / T) + t) * HD * T);
-            __syncthreads();  // the previous tile has been read
-            for (int i = tid; i < HD * T / 16; i += WG) {
-                const u32x4 w = src[i];
-                uint32_t *p = (uint32_t *)(in + (i / 4) * PR + (i % 4) * 16);
+        const int8_t *from[4];
 #pragma unroll
-                for (int c = 0; c < 4; c++) p[c] = w[c];
-            }
-            __syncthreads();
-            for (int i = tid; i < HD * T; i += WG) {
-                const int d = i / T, r = i % T, s = slot[r];
-                if (r < n && s / T == t) out[d * PR + r] = in[d * PR + s % T];
-            }
+        for (int j = 0; j < 4; j++) {
+            const int s = slot[vr + j];
+            from[j] = a.src.vc + ((size_t)kvh * a.src.cap + (s & ~(T - 1))) * HD + vd * T + (s & (T - 1));
         }
-        __syncthreads();
-        if (tid < n) {
-            int mx = 0;
-            for (int d = 0; d < HD; d++) {
-                const int c = out[d * PR + tid];
-                mx = max(mx, c < 0 ? -c : c);
-            }
-            need[tid] = mx ? kv8_exp(ep[slot[tid] >> a.src.lb]) + (31 - __clz(mx)) - 6 : KV8_EMIN;
+        int8_t b[NV][4];
+#pragma unroll
+        for (int k = 0; k < NV; k++)
+#pragma unroll
+            for (int j = 0; j < 4; j++) b[k][j] = from[j][k * 16 * T];
+        int big[4] = {0, 0, 0, 0};
+#pragma unroll
+        for (int k = 0; k < NV; k++) {
+            v[k] = pack4(b[k][0], b[k][1], b[k][2], b[k][3]);
+#pragma unroll
+            for (int j = 0; j < 4; j++) big[j] = max(big[j], abs((int)b[k][j]));
         }
+#pragma unroll
+        for (int j = 0; j < 4; j++)
+            if (vr + j < n) atomicMax(&mx[vr + j], big[j]);
     }
     __syncthreads();
-    __shared__ int be[4];
     const int B = 1 << a.dst.lb;
-    if (tid < T / B) {
+    if (tid < T / B && tid * B < n) {
         int e = KV8_EMIN;
-        for (int r = tid * B; r < min((tid + 1) * B, n); r++) e = max(e, need[r]);
+        for (int r = tid * B; r < min((tid + 1) * B, n); r++)
+            if (mx[r]) e = max(e, es[r] + (31 - __clz(mx[r])) - 6);
         be[tid] = e;
-        if (tid * B < n)
-            (which ? a.dst.ve : a.dst.ke)[(size_t)kvh * (a.dst.cap >> a.dst.lb) + ((unit * T) >> a.dst.lb) + tid] =
-                (int8_t)e;
+        (which ? a.dst.ve : a.dst.ke)[(size_t)kvh * (a.dst.cap >> a.dst.lb) + ((unit * T) >> a.dst.lb) + tid] = (int8_t)e;
     }
     __syncthreads();
-    for (int i = tid; i < HD * T; i += WG) {
-        const int r = which ? i % T : i / HD, d = which ? i / T : i % HD;
-        if (r >= n) continue;
-        const int c = which ? out[d * PR + r] : out[i];
-        const int up = kv8_exp(ep[slot[r] >> a.src.lb]) - be[r >> a.dst.lb];
-        const int8_t v = (int8_t)rintf(ldexpf((float)c, up));
-        if (which) a.dst.vc[(((size_t)kvh * (a.dst.cap / T) + unit) * HD + d) * T + r] = v;
-        else a.dst.kc[((size_t)kvh * a.dst.cap + unit * T + r) * HD + d] = v;
+    if (tid < T) up[tid] = tid < n ? es[tid] - be[tid >> a.dst.lb] : 0;
+    __syncthreads();
+    auto moved = [](int c, int by) { return (int)rintf(ldexpf((float)c, by)); };
+    if (which == 0) {
+        u32x4 *dst = (u32x4 *)(a.dst.kc + ((size_t)kvh * a.dst.cap + unit * T) * HD);
+#pragma unroll
+        for (int k = 0; k < NP; k++) {
+            const int i = tid + k * WG, by = up[i / PPR];
+            if (i / PPR >= n) continue;
+            if (by)
+#pragma unroll
+                for (int c = 0; c < 4; c++)
+                    w[k][c] = pack4(moved(byte_of(w[k][c], 0), by), moved(byte_of(w[k][c], 1), by),
+                                    moved(byte_of(w[k][c], 2), by), moved(byte_of(w[k][c], 3), by));
+            dst[i] = w[k];
+        }
+        return;
+    }
+    int8_t *dst = a.dst.vc + ((size_t)kvh * a.dst.cap + unit * T) * HD + vd * T + vr;
+    const int by[4] = {up[vr], up[vr + 1], up[vr + 2], up[vr + 3]};
+    const bool any = by[0] | by[1] | by[2] | by[3];
+#pragma unroll
+    for (int k = 0; k < NV; k++) {
+        if (any)
+            v[k] = pack4(moved(byte_of(v[k], 0), by[0]), moved(byte_of(v[k], 1), by[1]), moved(byte_of(v[k], 2), by[2]),
+                         moved(byte_of(v[k], 3), by[3]));
+        if (vr + 4 <= n) {
+            *(uint32_t *)(dst + k * 16 * T) = v[k];
+        } else {
+#pragma unroll
+            for (int j = 0; j < 4; j++)
+                if (vr + j < n) dst[k * 16 * T + j] = (int8_t)byte_of(v[k], j);
+        }
     }
 }
 

@@ -26,7 +26,6 @@ namespace {
 
 typedef _Float16 f16x8 __attribute__((ext_vector_type(8)));
 typedef _Float16 f16x2 __attribute__((ext_vector_type(2)));
-typedef float f32x4 __attribute__((ext_vector_type(4)));
 
 constexpr int T = KV8_TILE;
 constexpr float NEG = -3.402823466e38f;  // the running maximum before any slot

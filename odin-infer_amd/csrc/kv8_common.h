@@ -5,6 +5,8 @@
 
 namespace oi {
 
+typedef float f32x4 __attribute__((ext_vector_type(4)));
+
 static __device__ __forceinline__ int kv8_past(const Kv8Past &p, int n, int cap) {
     return p.dev ? min(max(*p.dev, 0), cap - n) : p.past;
 }
