@@ -156,7 +156,7 @@ int64_t oi_kv8_attn_workspace_bytes(const oi_kv8_dims *d, int32_t n_heads, int32
     const int group = n_heads / d->n_kv_heads;
     const int s = std::max(kv8_attn_splits(d->n_kv_heads, group, n, d->capacity, d->head_dim, false),
                            kv8_attn_splits(d->n_kv_heads, group, n, d->capacity, d->head_dim, true));
-    return (int64_t)kv8_attn_workspace(n_heads, n, d->head_dim, s);
+    return (int64_t)kv8_attn_workspace(n_heads, group, n, d->capacity, d->head_dim, s, true);
 }
 
 int oi_kv8_attn_launch(const oi_kv8_dims *d, const void *cache, int32_t n_heads, int32_t type, const void *q,
@@ -178,9 +178,9 @@ int oi_kv8_attn_launch(const oi_kv8_dims *d, const void *cache, int32_t n_heads,
         if (!rows_ok(q, type, q_stride, row) || !rows_ok(out, type, out_stride, row)) return err(OI_E_ARG, W, BAD_ROWS);
         const int group = n_heads / d->n_kv_heads;
         if ((int64_t)n * group > 65535 * 16) return err(OI_E_RANGE, W, "too many rows in one call");
-        const int splits = kv8_attn_splits(d->n_kv_heads, group, n, n_past_dev ? d->capacity : n_past + n, d->head_dim,
-                                           type == OI_TYPE_F16);
-        const int64_t need = (int64_t)kv8_attn_workspace(n_heads, n, d->head_dim, splits);
+        const int end = n_past_dev ? d->capacity : n_past + n;
+        const int splits = kv8_attn_splits(d->n_kv_heads, group, n, end, d->head_dim, type == OI_TYPE_F16);
+        const int64_t need = (int64_t)kv8_attn_workspace(n_heads, group, n, end, d->head_dim, splits, mass);
         if (workspace_bytes < need)
             return err(OI_E_ARG, W, "workspace of " + std::to_string(workspace_bytes) + " bytes, " +
                                         std::to_string(need) + " needed");
@@ -200,10 +200,18 @@ int oi_kv8_attn_launch(const oi_kv8_dims *d, const void *cache, int32_t n_heads,
         a.past = {n_past, n_past_dev};
         a.mass = mass;
         a.splits = splits;
-        a.part = (float *)workspace;
-        const size_t rows = (size_t)n * n_heads, parts = splits > 1 ? rows * splits : 0;
-        a.ml = (float2 *)(a.part + parts * d->head_dim);
-        a.lse = mass ? (float *)(a.ml + parts) : nullptr;
+        // the saved weights first (16-byte stores), then the splits' results
+        const size_t rows = (size_t)n * n_heads, parts = rows * splits;
+        float *ws = (float *)workspace;
+        if (mass && kv8_attn_saves(group, n)) {
+            a.save_units = (end + KV8_TILE - 1) / KV8_TILE;
+            a.save = ws;
+            a.save_m = ws + rows * a.save_units * KV8_TILE;
+            ws = a.save_m + (rows * a.save_units + 3) / 4 * 4;
+        }
+        a.part = ws;
+        a.ml = (float2 *)(a.part + (splits > 1 ? parts * d->head_dim : 0));
+        a.norm = mass ? a.ml + parts : nullptr;
         return launched(launch_kv8_attn(a, (hipStream_t)stream), W);
     });
 }

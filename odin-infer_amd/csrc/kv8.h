@@ -54,13 +54,17 @@ struct Kv8AttnArgs {
     Kv8Past past;
     float *mass;          // [n_kv][cap] or null
     float *part;          // [n * n_heads][splits][hd], where splits > 1: the splits' o
-    float2 *ml;           // [n * n_heads][splits]: their m and l
-    float *lse;           // [n * n_heads], where mass is set
-    int32_t splits;
+    float2 *ml;           // [n * n_heads][splits]: their m and l (few rows, or splits > 1)
+    float2 *norm;         // [n * n_heads], where mass is set: m and 2^15 / l of a row
+    // few rows with mass: every weight as it was formed [n_kv][save_units][rows][64]
+    // and its row's maximum then [n_kv][save_units][rows]; null otherwise
+    float *save, *save_m;
+    int32_t save_units, splits;
 };
 // splits over the slots for a call that sees at most `end` of them, and the workspace that they take
 int kv8_attn_splits(int n_kv, int group, int n, int end, int hd, bool f16);
-size_t kv8_attn_workspace(int n_heads, int n, int hd, int splits);
+bool kv8_attn_saves(int group, int n);
+size_t kv8_attn_workspace(int n_heads, int group, int n, int end, int hd, int splits, bool mass);
 hipError_t launch_kv8_attn(const Kv8AttnArgs &a, hipStream_t st);
 
 struct Kv8EvictArgs {

@@ -56,6 +56,18 @@ __global__ __launch_bounds__(WG) void kv8_append_kernel(Kv8AppendArgs a) {
     if (unit * T >= end) return;
     const int s0 = unit * T + 16 * wave, col = lane % (HD / 4), r0 = lane / (HD / 4);
     const int64_t stride = a.stride[which];
+    const int blk = s0 >> a.c.lb, b0 = blk << a.c.lb;
+    int8_t *ep = (which ? a.c.ve : a.c.ke) + (size_t)kvh * (a.c.cap >> a.c.lb) + blk;
+    const bool old = b0 < past;  // the block holds earlier slots
+    // what the call may have to keep is requested with the new rows: the exponent, and V's
+    // pieces of 16 slots that are not all new
+    const int8_t e_was = old ? *ep : 0;
+    const bool whole = s0 >= past && s0 + 16 <= end, any = s0 < end && s0 + 16 > past;
+    u32x4 vp[HD / WAVE];
+    u32x4 *const vat = (u32x4 *)(a.c.vc + (((size_t)kvh * (a.c.cap / T) + unit) * HD + lane) * T + 16 * wave);
+    if (which && !whole && (any || (old && s0 < past)))
+#pragma unroll
+        for (int k = 0; k < HD / WAVE; k++) vp[k] = vat[k * WAVE * T / 16];
     float x[NR][4];
 #pragma unroll
     for (int j = 0; j < NR; j++) {
@@ -89,12 +101,9 @@ __global__ __launch_bounds__(WG) void kv8_append_kernel(Kv8AppendArgs a) {
     __syncthreads();
     const int nw = 1 << (a.c.lb - 4), w0 = wave & ~(nw - 1);  // waves of this block, its first
     for (int w = 0; w < nw; w++) amax = fmaxf(amax, wmax[w0 + w]);
-    const int blk = s0 >> a.c.lb, b0 = blk << a.c.lb;
-    int8_t *ep = (which ? a.c.ve : a.c.ke) + (size_t)kvh * (a.c.cap >> a.c.lb) + blk;
     int e = exp_for(amax), e_old = e;
-    const bool old = b0 < past;  // the block holds earlier slots
     if (old) {
-        e_old = kv8_exp(*ep);
+        e_old = kv8_exp(e_was);
         e = max(e, e_old);
     }
     const bool touched = b0 < end && b0 + (1 << a.c.lb) > past;
@@ -122,15 +131,12 @@ __global__ __launch_bounds__(WG) void kv8_append_kernel(Kv8AppendArgs a) {
         for (int j = 0; j < NR; j++) tile[16 * wave + j * RPL + r0][col] = q[j];
         __builtin_amdgcn_wave_barrier();  // this wave's 16 rows only
         // 16 slots of a dimension: one 16-byte piece of its row
-        const bool whole = s0 >= past && s0 + 16 <= end;
-        const bool any = s0 < end && s0 + 16 > past;
         if (any || (requant && s0 < past)) {
             const uint8_t *tb = (const uint8_t *)&tile[16 * wave][0];
 #pragma unroll
             for (int k = 0; k < HD / WAVE; k++) {
                 const int d = lane + k * WAVE;
-                u32x4 *p = (u32x4 *)(a.c.vc + (((size_t)kvh * (a.c.cap / T) + unit) * HD + d) * T + 16 * wave);
-                u32x4 w = whole ? u32x4{0u, 0u, 0u, 0u} : *p;
+                u32x4 w = whole ? u32x4{0u, 0u, 0u, 0u} : vp[k];
 #pragma unroll
                 for (int c = 0; c < 4; c++) {
                     uint32_t r = 0;
@@ -144,11 +150,10 @@ __global__ __launch_bounds__(WG) void kv8_append_kernel(Kv8AppendArgs a) {
                     }
                     w[c] = r;
                 }
-                *p = w;
+                vat[k * WAVE * T / 16] = w;
             }
         }
     }
-    __syncthreads();  // every wave of the block has read the old exponent
     if (touched && lane == 0 && wave == w0) *ep = (int8_t)e;
 }
 
@@ -189,7 +194,7 @@ __global__ __launch_bounds__(WG) void kv8_read_kernel(Kv8ReadArgs a) {
             *(u32x2 *)((uint16_t *)a.out[which] + at) =
                 u32x2{f2h(y[0]) | (uint32_t)f2h(y[1]) << 16, f2h(y[2]) | (uint32_t)f2h(y[3]) << 16};
         else
-            *(float4 *)((float *)a.out[which] + at) = make_float4(y[0], y[1], y[2], y[3]);
+            __builtin_nontemporal_store(f32x4{y[0], y[1], y[2], y[3]}, (f32x4 *)((float *)a.out[which] + at));
     }
 }
 

@@ -172,7 +172,7 @@ __device__ __forceinline__ size_t row_id(const Kv8AttnArgs &a, int r, int kvh) {
 }
 
 // A wave takes a unit of 64 slots at a time for 16 rows of one kv head (the
-// (token, query head) pairs that share it), four waves a workgroup, alternate
+// (token, query head) pairs that share it), the waves of a workgroup alternate
 // units.  Scores are formed transposed, K the first operand: a lane then holds
 // 16 scores of one row, and with K's rows taken in the order
 //   operand row 4 g' + i of tile t  <-  slot 16 g' + 4 t + i
@@ -181,12 +181,12 @@ __device__ __forceinline__ size_t row_id(const Kv8AttnArgs &a, int r, int kvh) {
 // the row maximum.  K and V go from memory to the operand registers without
 // LDS, 16 bytes a lane; K of the next unit is requested when this unit's scores
 // are done, V when its product is.  The waves' results meet in LDS.
-template <int HD, int MODE>
+template <int HD, int MODE, bool SAVE>
 __global__ __launch_bounds__(WG) void kv8_rows_kernel(Kv8AttnArgs a) {
-    constexpr int NK = HD / 64, ND = HD / 16, PD = HD + 4, R = tile_rows(MODE);
+    constexpr int NW = WG / WAVE, NK = HD / 64, ND = HD / 16, PD = HD + 4, R = tile_rows(MODE), TPR = WG / R;
     constexpr bool F16 = MODE == ROWS_F16;
-    __shared__ __attribute__((aligned(16))) float so[4][R][PD];
-    __shared__ float sm[4][R], sl[4][R];
+    __shared__ __attribute__((aligned(16))) float so[NW][R][PD];
+    __shared__ float sm[NW][R], sl[NW][R];
     const int tid = threadIdx.x, lane = tid & (WAVE - 1), wave = tid / WAVE;
     const int c = lane & 15, g = lane >> 4;
     const int kvh = blockIdx.x, rt = blockIdx.y, split = blockIdx.z;
@@ -235,13 +235,13 @@ __global__ __launch_bounds__(WG) void kv8_rows_kernel(Kv8AttnArgs a) {
     }
     q.make(qraw, ok, a.scale < 0.f, lower);
     const float scale = fabsf(a.scale);
-    for (; u < u1; u += 4) {
+    for (; u < u1; u += NW) {
         f32x4 s[4];
 #pragma unroll
         for (int t = 0; t < 4; t++) s[t] = scores<HD, MODE>(kr[t], q);
         const float mul = fmaxf(ldexpf(scale, kv8_exp((int8_t)kexp) + q.e), FLT_MIN);  // above 0: -inf stays -inf
         const int ev = kv8_exp((int8_t)vexp);
-        if (u + 4 < u1) load_k(u + 4);
+        if (u + NW < u1) load_k(u + NW);
         if (u * T + T > first_limit) {  // some row does not see all of the unit
             const int p0 = u * T + 16 * g;
 #pragma unroll
@@ -256,19 +256,30 @@ __global__ __launch_bounds__(WG) void kv8_rows_kernel(Kv8AttnArgs a) {
 #pragma unroll
             for (int i = 0; i < 4; i++) top = fmaxf(top, s[t][i]);
         top = col_max(fmaf(top, mul, (float)ev));
-        const float m1 = fmaxf(m, top), bias = (float)ev - m1 + PSCALE;
+        const float m1 = fmaxf(m, ceilf(top)), bias = (float)ev - m1 + (F16 ? PSCALE : 0.f);
         float sum = 0.f;
         f16x8 ph[2], pl[2];
+        f32x4 w[SAVE ? 4 : 1];
 #pragma unroll
         for (int t = 0; t < 4; t++)
 #pragma unroll
             for (int i = 0; i < 4; i++) {
-                const float p = ex2(fmaf(s[t][i], mul, bias));
+                const float p = ex2(fmaf(s[t][i], mul, bias)) * (F16 ? 1.f : 32768.f);
+                if constexpr (SAVE) w[t][i] = p;
                 sum += p;
                 const _Float16 h = (_Float16)p;
                 ph[t / 2][4 * (t & 1) + i] = h;
                 if constexpr (!F16) pl[t / 2][4 * (t & 1) + i] = (_Float16)(p - (float)h);
             }
+        if constexpr (SAVE) {  // weights without V's exponent, for the mass, and the maximum that they go by
+            const size_t at = ((size_t)kvh * a.save_units + u) * rows + c;
+            const float un = pow2i(-ev);
+            if (c < min(R, rows)) {
+#pragma unroll
+                for (int t = 0; t < 4; t++) *(f32x4 *)(a.save + at * T + 16 * g + 4 * t) = w[t] * un;
+                if (g == 0) a.save_m[at] = m1;
+            }
+        }
         if constexpr (MODE == ROWS_PACK) {
             ph[0] = lower ? pl[0] : ph[0];
             ph[1] = lower ? pl[1] : ph[1];
@@ -289,7 +300,7 @@ __global__ __launch_bounds__(WG) void kv8_rows_kernel(Kv8AttnArgs a) {
                 o[d] = mfma(w, ph[h], o[d]);
                 if constexpr (MODE == ROWS_F32) o[d] = mfma(w, pl[h], o[d]);
             }
-        if (u + 4 < u1) load_v(u + 4);
+        if (u + NW < u1) load_v(u + NW);
     }
     // the four waves' results in LDS; their weights once per row, then the sum
     l = col_sum(l);
@@ -307,29 +318,24 @@ __global__ __launch_bounds__(WG) void kv8_rows_kernel(Kv8AttnArgs a) {
         }
     }
     __syncthreads();
-    if (tid >= 16 * R) return;
-    float M = NEG, W[4], L = 0.f;
-    {
-        const int r = tid / 16;  // 16 threads a row from here on
-#pragma unroll
-        for (int w = 0; w < 4; w++) M = fmaxf(M, sm[w][r]);
-#pragma unroll
-        for (int w = 0; w < 4; w++) {
-            W[w] = ex2(sm[w][r] - M);
-            L += sl[w][r] * W[w];
-        }
-    }
-    const int r = tid / 16, gr = rt * R + r;
+    const int r = tid / TPR, gr = rt * R + r;  // TPR threads a row from here on
     if (gr >= rows) return;
+    float M = NEG, W[NW], L = 0.f;
+#pragma unroll
+    for (int w = 0; w < NW; w++) M = fmaxf(M, sm[w][r]);
+#pragma unroll
+    for (int w = 0; w < NW; w++) {
+        W[w] = ex2(sm[w][r] - M);
+        L += sl[w][r] * W[w];
+    }
     const size_t id = row_id(a, gr, kvh);
     const bool last = a.splits == 1;
     const float inv = last ? 1.f / L : 1.f;
 #pragma unroll
-    for (int k = 0; k < HD / 64; k++) {
-        const int d = 64 * k + 4 * (tid & 15);
+    for (int d = 4 * (tid % TPR); d < HD; d += 4 * TPR) {
         f32x4 y = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll
-        for (int w = 0; w < 4; w++) y += *(const f32x4 *)&so[w][r][d] * W[w];
+        for (int w = 0; w < NW; w++) y += *(const f32x4 *)&so[w][r][d] * W[w];
         y *= inv;
         if (!last) {
             *(f32x4 *)(a.part + (id * a.splits + split) * HD + d) = y;
@@ -342,9 +348,9 @@ __global__ __launch_bounds__(WG) void kv8_rows_kernel(Kv8AttnArgs a) {
                 *(f32x4 *)((float *)a.out + at) = y;
         }
     }
-    if ((tid & 15) == 0) {
-        if (!last) a.ml[id * a.splits + split] = make_float2(M, L);
-        else if (a.lse) a.lse[id] = M + log2f(L) - PSCALE;
+    if (tid % TPR == 0) {
+        a.ml[id * a.splits + split] = make_float2(M, L);
+        if (last && a.norm) a.norm[id] = make_float2(M, 32768.f / L);
     }
 }
 
@@ -353,14 +359,18 @@ __global__ __launch_bounds__(WG) void kv8_rows_kernel(Kv8AttnArgs a) {
 // up to MS * 8 splits; the weights 2^(m - M) are formed once, in LDS.
 constexpr int MW = 512, MPRE = 8;  // threads; splits per thread in the first round trip
 constexpr int KV8_MAX_SPLITS = 1024;
+template <int HD>
+struct MergeLds {
+    static constexpr int LPR = HD / 4, MS = MW / LPR;  // lanes of a row, splits at a time
+    float wt[KV8_MAX_SPLITS];
+    __attribute__((aligned(16))) float red[MS][HD];
+    float wmax[MW / WAVE], wsum[MW / WAVE];
+};
 template <int HD, bool F16>
-__global__ __launch_bounds__(MW) void kv8_merge_kernel(Kv8AttnArgs a) {
-    constexpr int LPR = HD / 4, MS = MW / LPR;  // lanes of a row, splits at a time
-    __shared__ float wt[KV8_MAX_SPLITS];
-    __shared__ __attribute__((aligned(16))) float red[MS][HD];
-    __shared__ float wmax[MW / WAVE], wsum[MW / WAVE];
+__device__ __forceinline__ void merge_row(const Kv8AttnArgs &a, int token, int head, MergeLds<HD> &lds) {
+    constexpr int LPR = MergeLds<HD>::LPR, MS = MergeLds<HD>::MS;
     const int tid = threadIdx.x, lane = tid & (WAVE - 1), wave = tid / WAVE, S = a.splits;
-    const size_t id = (size_t)blockIdx.y * a.n_heads + blockIdx.x;
+    const size_t id = (size_t)token * a.n_heads + head;
     const int col = tid % LPR, s0 = tid / LPR;
     const float *pt = a.part + id * S * HD + 4 * col;
     const float2 *ml = a.ml + id * S;
@@ -374,42 +384,47 @@ __global__ __launch_bounds__(MW) void kv8_merge_kernel(Kv8AttnArgs a) {
         pre[k] = s < S ? *(const f32x4 *)(pt + (size_t)s * HD) : f32x4{0.f, 0.f, 0.f, 0.f};
     }
     const float m = wave_max_all(fmaxf(mine[0].x, mine[1].x));
-    if (lane == 0) wmax[wave] = m;
+    if (lane == 0) lds.wmax[wave] = m;
     __syncthreads();
-    float M = wmax[0];
+    float M = lds.wmax[0];
 #pragma unroll
-    for (int w = 1; w < MW / WAVE; w++) M = fmaxf(M, wmax[w]);
+    for (int w = 1; w < MW / WAVE; w++) M = fmaxf(M, lds.wmax[w]);
     float L = 0.f;
 #pragma unroll
     for (int k = 0; k < 2; k++) {
         const float f = ex2(mine[k].x - M);
-        if (tid + k * MW < S) wt[tid + k * MW] = f;
+        if (tid + k * MW < S) lds.wt[tid + k * MW] = f;
         L += mine[k].y * f;
     }
     L = wave_sum(L);
-    if (lane == 0) wsum[wave] = L;
+    if (lane == 0) lds.wsum[wave] = L;
     __syncthreads();
     L = 0.f;
 #pragma unroll
-    for (int w = 0; w < MW / WAVE; w++) L += wsum[w];
+    for (int w = 0; w < MW / WAVE; w++) L += lds.wsum[w];
     f32x4 y = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll
     for (int k = 0; k < MPRE; k++)
-        if (s0 + k * MS < S) y += pre[k] * wt[s0 + k * MS];
+        if (s0 + k * MS < S) y += pre[k] * lds.wt[s0 + k * MS];
 #pragma unroll 4
-    for (int s = s0 + MPRE * MS; s < S; s += MS) y += *(const f32x4 *)(pt + (size_t)s * HD) * wt[s];
-    *(f32x4 *)&red[s0][4 * col] = y;
+    for (int s = s0 + MPRE * MS; s < S; s += MS) y += *(const f32x4 *)(pt + (size_t)s * HD) * lds.wt[s];
+    *(f32x4 *)&lds.red[s0][4 * col] = y;
     __syncthreads();
     if (tid < HD) {
         float v = 0.f;
 #pragma unroll
-        for (int k = 0; k < MS; k++) v += red[k][tid];
+        for (int k = 0; k < MS; k++) v += lds.red[k][tid];
         v /= L;
-        const int64_t at = (int64_t)blockIdx.y * a.out_stride + (int64_t)blockIdx.x * HD + tid;
+        const int64_t at = token * a.out_stride + (int64_t)head * HD + tid;
         if constexpr (F16) ((uint16_t *)a.out)[at] = f2h(v);
         else ((float *)a.out)[at] = v;
     }
-    if (tid == 0 && a.lse) a.lse[id] = M + log2f(L) - PSCALE;
+    if (tid == 0 && a.norm) a.norm[id] = make_float2(M, 32768.f / L);
+}
+template <int HD, bool F16>
+__global__ __launch_bounds__(MW) void kv8_merge_kernel(Kv8AttnArgs a) {
+    __shared__ MergeLds<HD> lds;
+    merge_row<HD, F16>(a, blockIdx.y, blockIdx.x, lds);
 }
 
 // ------------------------------------------------------------- prompts --
@@ -602,7 +617,7 @@ __global__ __launch_bounds__(NW *WAVE, HD == 128 ? 2 : 1) void kv8_prompt_kernel
                 }
                 top = half_reduce(top, [](float y, float z) { return fmaxf(y, z); });
                 if (__any(top > m + LAZY)) {
-                    const float m1 = fmaxf(m, top), alpha = ex2(m - m1);
+                    const float m1 = fmaxf(m, ceilf(top)), alpha = ex2(m - m1);
                     m = m1;
                     l *= alpha;
 #pragma unroll
@@ -612,11 +627,11 @@ __global__ __launch_bounds__(NW *WAVE, HD == 128 ? 2 : 1) void kv8_prompt_kernel
                 }
 #pragma unroll
                 for (int b = 0; b < 2; b++) {
-                    const float bias = ev[2 * x + b] - m + PS;
+                    const float bias = ev[2 * x + b] - m + (F16 ? PS : 0.f);
                     float sum = 0.f;
 #pragma unroll
                     for (int i = 0; i < 8; i++) {
-                        const float p = ex2(fmaf(s[8 * b + i], mul[b], bias));
+                        const float p = ex2(fmaf(s[8 * b + i], mul[b], bias)) * (F16 ? 1.f : 32768.f);
                         sum += p;
                         const _Float16 t = (_Float16)p;
                         ph[b][i] = t;
@@ -642,11 +657,12 @@ __global__ __launch_bounds__(NW *WAVE, HD == 128 ? 2 : 1) void kv8_prompt_kernel
         if (u + 1 < u1) st.store(lds[buf ^ 1][0], lds[buf ^ 1][1], es[buf ^ 1], tid);
         __syncthreads();
     }
-    l = half_reduce(l, [](float x, float y) { return x + y; });
+    constexpr float UP = F16 ? 128.f : 1.f;  // 2^(PSCALE - PS): results leave at 2^15 as from the other kernel
+    l = half_reduce(l, [](float x, float y) { return x + y; }) * UP;
     if (r >= rows) return;
     const size_t id = row_id(a, r, kvh);
     const bool last = a.splits == 1;
-    const float inv = last ? 1.f / l : 1.f;
+    const float inv = last ? UP / l : UP;
     const int64_t to = row_at(a, r, kvh, a.out_stride, HD);
 #pragma unroll
     for (int d = 0; d < DT; d++)
@@ -663,68 +679,72 @@ __global__ __launch_bounds__(NW *WAVE, HD == 128 ? 2 : 1) void kv8_prompt_kernel
                 *(f32x4 *)((float *)a.out + to + dim) = y;
         }
     if (h == 0 && d0 == 0) {
-        if (!last) a.ml[id * a.splits + split] = make_float2(m + (PSCALE - PS), l);
-        else if (a.lse) a.lse[id] = m + log2f(l) - PS;
+        if (!last) a.ml[id * a.splits + split] = make_float2(m, l);
+        else if (a.norm) a.norm[id] = make_float2(m, 32768.f / l);
     }
 }
 
 // The weight that every slot receives from the call's rows, summed in f32 over
-// all of them: scores formed again from K (half of the cache) and each row's
-// log-sum.  Every sum is in a fixed order.
+// all of them: scores formed again from K (half of the cache), 2^(t - m) times
+// 2^15 / l of the row.  Every sum is in a fixed order.
 //
-// One tile of rows (decode): q stays in registers and a wave takes unit after
-// unit, K of the next one requested before this one's products.
-template <int HD, int MODE>
-__global__ __launch_bounds__(WG) void kv8_mass_few_kernel(Kv8AttnArgs a) {
-    constexpr int NK = HD / 64, R = tile_rows(MODE);
+// One tile of rows (decode): the rows kernel has left every weight relative to
+// its row's maximum so far, and that maximum (an integer, so what is left to
+// multiply is an exact power of two and the row's 2^15 / l).  The workgroups before
+// `merges` merge a (token, query head) each; of the others a wave takes unit after
+// unit, a slot per lane.  Both read the splits' (m, l) by themselves, so one launch
+// does for both.  At 100004 slots of 4 kv heads 8 us (scores formed again from K:
+// 18; reads of 2 KB a unit instead of 8).
+constexpr int FEW_MASS_ROWS = 16;
+template <int HD, bool F16>
+__global__ __launch_bounds__(MW) void kv8_mass_few_kernel(Kv8AttnArgs a, int merges) {
+    constexpr int NW = MW / WAVE, R = FEW_MASS_ROWS, AHEAD = 4;
+    __shared__ union {
+        MergeLds<HD> merge;
+        float2 norm[R];
+    } lds;
+    if ((int)blockIdx.x < merges) {
+        const int token = blockIdx.x / a.n_heads;
+        merge_row<HD, F16>(a, token, blockIdx.x - token * a.n_heads, lds.merge);
+        return;
+    }
+    const int at = blockIdx.x - merges, kvh = at % a.c.n_kv, nth = at / a.c.n_kv;
     const int tid = threadIdx.x, lane = tid & (WAVE - 1), wave = tid / WAVE;
-    const int c = lane & 15, g = lane >> 4, kvh = blockIdx.x;
     const int rows = a.n * a.group, past = kv8_past(a.past, a.n, a.c.cap), end = past + a.n;
-    const int units = (end + T - 1) / T, step = gridDim.y * 4;
-    const int rr = min(c % R, rows - 1);
-    const int limit = c < min(R, rows) ? past + row_token(a, rr) + 1 : 0;  // each row once
-    QTile<HD, MODE> q;
-    typename QTile<HD, MODE>::Raw raw;
-    QTile<HD, MODE>::fetch(raw, a.q, row_at(a, rr, kvh, a.q_stride, HD), g);
-    const float lse = a.lse[row_id(a, rr, kvh)];
-    const int8_t *kb = a.c.kc + (size_t)kvh * a.c.cap * HD;
-    const int8_t *ke = a.c.ke + (size_t)kvh * (a.c.cap >> a.c.lb);
+    const int units = (end + T - 1) / T, step = (gridDim.x - merges) / a.c.n_kv * NW;
+    // the rows' m and 1 / l (the weights' 2^15 is in both): a wave per row over its splits
+    for (int r = wave; r < rows; r += NW) {
+        const float2 *ml = a.ml + row_id(a, r, kvh) * a.splits;
+        float M = NEG, L = 0.f;
+        for (int s = lane; s < a.splits; s += WAVE) {
+            const float2 x = ml[s];
+            const float m1 = fmaxf(M, x.x);
+            L = L * ex2(M - m1) + x.y * ex2(x.x - m1);
+            M = m1;
+        }
+        const float all = wave_max_all(M);
+        L = wave_sum(L * ex2(M - all));
+        if (lane == 0) lds.norm[r] = make_float2(all, 1.f / L);
+    }
+    __syncthreads();
+    const float2 norm = lds.norm[min(lane, rows - 1)];
     float *mass = a.mass + (size_t)kvh * a.c.cap;
-    const int krow = 16 * (c >> 2) + (c & 3);
-    u32x4 kr[4][NK];
-    int kexp = 0;
-    float was = 0.f;
-    auto load = [&](int u) {
-#pragma unroll
-        for (int t = 0; t < 4; t++)
-#pragma unroll
-            for (int k = 0; k < NK; k++)
-                kr[t][k] = *(const u32x4 *)(kb + (size_t)(u * T + krow + 4 * t) * HD + 64 * k + 16 * g);
-        kexp = ke[(u * T + 16 * g) >> a.c.lb];
-        was = u * T + lane < past ? mass[u * T + lane] : 0.f;
-    };
-    int u = blockIdx.y * 4 + wave;
-    if (u < units) load(u);
-    q.make(raw, c % R < rows, a.scale < 0.f, c >= R);
-    const float scale = fabsf(a.scale);
-    for (; u < units; u += step) {
-        f32x4 s[4];
-#pragma unroll
-        for (int t = 0; t < 4; t++) s[t] = scores<HD, MODE>(kr[t], q);
-        const float mul = ldexpf(scale, kv8_exp((int8_t)kexp) + q.e), had = was;
-        if (u + step < units) load(u + step);
-        const int p0 = u * T + 16 * g;
-        // slot 16 g + 4 t + i summed over the 16 rows, kept by lane c = 4 t + i
+    for (int u = nth * NW + wave; u < units; u += step) {
+        const size_t from = ((size_t)kvh * a.save_units + u) * rows;
+        const int s = u * T + lane;
+        const float *w = a.save + from * T + lane;
+        const float had = s < past ? mass[s] : 0.f;
+        const float f = ex2(a.save_m[from + min(lane, rows - 1)] - norm.x) * norm.y;  // lane r: of row r
         float sum = 0.f;
+        for (int r0 = 0; r0 < rows; r0 += AHEAD) {
+            float x[AHEAD];
 #pragma unroll
-        for (int t = 0; t < 4; t++)
+            for (int i = 0; i < AHEAD; i++) x[i] = w[min(r0 + i, rows - 1) * T];
 #pragma unroll
-            for (int i = 0; i < 4; i++) {
-                const float p = p0 + 4 * t + i < limit ? ex2(fmaf(s[t][i], mul, -lse)) : 0.f;
-                const float v = lane_group_sum(p, 16);
-                sum = c == 4 * t + i ? v : sum;
-            }
-        if (u * T + lane < end) mass[u * T + lane] = had + sum;
+            for (int i = 0; i < AHEAD; i++)
+                if (r0 + i < rows) sum = fmaf(x[i], lane_value(f, r0 + i), sum);
+        }
+        if (s < end) mass[s] = had + sum;
     }
 }
 
@@ -736,7 +756,8 @@ template <int HD, bool F16, int X>
 __global__ __launch_bounds__(WG, 2) void kv8_mass_kernel(Kv8AttnArgs a) {
     constexpr int NF = HD / 16, QR = 64, PC = F16 ? 1 : 2, TPR = WG / QR, EL = HD / TPR, WS = 32 * X, GS = 2 * WS;
     __shared__ __attribute__((aligned(16))) f16x8 qs[2][PC][QR * HD / 8];
-    __shared__ float qmul[2][QR], qlse[2][QR], sum[2][GS];
+    __shared__ float qmul[2][QR], sum[2][GS];
+    __shared__ float2 qnorm[2][QR];
     const int tid = threadIdx.x, lane = tid & (WAVE - 1), wave = tid / WAVE;
     const int c = lane & 31, h = lane >> 5, kvh = blockIdx.x, s0 = blockIdx.y * GS + (wave & 1) * WS;
     const int rows = a.n * a.group, past = kv8_past(a.past, a.n, a.c.cap), end = past + a.n;
@@ -746,7 +767,7 @@ __global__ __launch_bounds__(WG, 2) void kv8_mass_kernel(Kv8AttnArgs a) {
     // the tile's rows into registers, four threads a row, then as halves into LDS
     const int qr = tid / TPR, qj = tid % TPR;
     u32x4 raw[F16 ? EL / 8 : EL / 4];
-    float raw_lse = 0.f;
+    float2 raw_norm = make_float2(0.f, 0.f);
     auto fetch = [&](int t0) {
         const int r = min(t0 + qr, rows - 1);
         const int64_t at = row_at(a, r, kvh, a.q_stride, HD) + qj * EL;
@@ -754,7 +775,7 @@ __global__ __launch_bounds__(WG, 2) void kv8_mass_kernel(Kv8AttnArgs a) {
         for (int i = 0; i < (F16 ? EL / 8 : EL / 4); i++)
             raw[i] = F16 ? *(const u32x4 *)((const uint16_t *)a.q + at + 8 * i)
                          : *(const u32x4 *)((const float *)a.q + at + 4 * i);
-        raw_lse = a.lse[row_id(a, r, kvh)];
+        raw_norm = a.norm[row_id(a, r, kvh)];
     };
     auto store = [&](int b) {
         int e = 0;
@@ -797,7 +818,7 @@ __global__ __launch_bounds__(WG, 2) void kv8_mass_kernel(Kv8AttnArgs a) {
         }
         if (qj == 0) {
             qmul[b][qr] = ldexpf(scale, e);
-            qlse[b][qr] = raw_lse;
+            qnorm[b][qr] = raw_norm;
         }
     };
     // K: row c of each half unit; its 16-byte loads supply two operands, dimensions 32 m + 16 h + 0..7 and + 8..15
@@ -833,7 +854,8 @@ __global__ __launch_bounds__(WG, 2) void kv8_mass_kernel(Kv8AttnArgs a) {
         const int r_last = min(t0 + 32 * (wave >> 1) + 31, rows - 1);
         if (s0 < past + row_token(a, r_last) + 1 && t0 + 32 * (wave >> 1) < rows) {
             const int limit = r < rows ? past + row_token(a, r) + 1 : 0;
-            const float qm = qmul[b][lr], lse = qlse[b][lr];
+            const float qm = qmul[b][lr];
+            const float2 norm = qnorm[b][lr];
             const bool edge = s0 + WS > past + row_token(a, t0 + 32 * (wave >> 1)) + 1 || t0 + QR > rows;
 #pragma unroll
             for (int x = 0; x < X; x++) {
@@ -849,12 +871,13 @@ __global__ __launch_bounds__(WG, 2) void kv8_mass_kernel(Kv8AttnArgs a) {
                 if (edge) {
 #pragma unroll
                     for (int i = 0; i < 16; i++) {
-                        const float p = ex2(fmaf(s[i], step[2 * x + i / 8] * qm, -lse));
+                        const float p = ex2(fmaf(s[i], step[2 * x + i / 8] * qm, -norm.x)) * norm.y;
                         acc[x][i] += s0 + 32 * x + 8 * (i / 4) + 4 * h + i % 4 < limit ? p : 0.f;
                     }
                 } else {
 #pragma unroll
-                    for (int i = 0; i < 16; i++) acc[x][i] += ex2(fmaf(s[i], step[2 * x + i / 8] * qm, -lse));
+                    for (int i = 0; i < 16; i++)
+                        acc[x][i] = fmaf(ex2(fmaf(s[i], step[2 * x + i / 8] * qm, -norm.x)), norm.y, acc[x][i]);
                 }
             }
         }
@@ -923,8 +946,12 @@ int kv8_attn_splits(int n_kv, int group, int n, int end, int hd, bool f16) {
     return best;
 }
 
-size_t kv8_attn_workspace(int n_heads, int n, int hd, int splits) {
-    return (size_t)n * n_heads * ((splits > 1 ? (size_t)splits * (hd + 2) : 0) + 1) * 4;
+bool kv8_attn_saves(int group, int n) { return (int64_t)n * group <= FEW_MASS_ROWS; }
+
+size_t kv8_attn_workspace(int n_heads, int group, int n, int end, int hd, int splits, bool mass) {
+    const size_t rows = (size_t)n * n_heads, units = ((size_t)end + T - 1) / T;
+    const size_t saved = mass && kv8_attn_saves(group, n) ? rows * units * T + (rows * units + 3) / 4 * 4 : 0;
+    return (saved + rows * ((splits > 1 ? (size_t)splits * hd : 0) + 2 * (size_t)splits + 2)) * 4;
 }
 
 namespace {
@@ -935,10 +962,11 @@ void launch(const Kv8AttnArgs &a, hipStream_t st) {
     constexpr bool F16 = MODE == ROWS_F16;
     const int rows = a.n * a.group;
     const int end = a.past.dev ? a.c.cap : a.past.past + a.n, units = (end + T - 1) / T;
+    const dim3 merge_grid((unsigned)a.n_heads, (unsigned)a.n);
     if (rows <= FEW_ROWS) {
-        hipLaunchKernelGGL((kv8_rows_kernel<HD, MODE>),
-                           dim3((unsigned)a.c.n_kv, (unsigned)((rows + R - 1) / R), (unsigned)a.splits), dim3(WG), 0, st,
-                           a);
+        const dim3 grid((unsigned)a.c.n_kv, (unsigned)((rows + R - 1) / R), (unsigned)a.splits);
+        if (a.save) hipLaunchKernelGGL((kv8_rows_kernel<HD, MODE, true>), grid, dim3(WG), 0, st, a);
+        else hipLaunchKernelGGL((kv8_rows_kernel<HD, MODE, false>), grid, dim3(WG), 0, st, a);
     } else if constexpr (MODE != ROWS_PACK) {
         const PromptPlan p = prompt_plan(HD, F16, a.c.n_kv, rows);
         const dim3 grid((unsigned)a.c.n_kv, (unsigned)((rows + p.rows - 1) / p.rows), (unsigned)a.splits);
@@ -947,13 +975,15 @@ void launch(const Kv8AttnArgs &a, hipStream_t st) {
         else if constexpr (F16) go(kv8_prompt_kernel<HD, F16, 8, 2>);
         else go(kv8_prompt_kernel<HD, F16, 4, 1>);
     }
-    if (a.splits > 1)
-        hipLaunchKernelGGL((kv8_merge_kernel<HD, F16>), dim3((unsigned)a.n_heads, (unsigned)a.n), dim3(MW), 0, st, a);
+    if (a.save) {
+        const int merges = a.splits > 1 ? a.n * a.n_heads : 0;
+        const int wgs = std::max(1, std::min((units + 7) / 8, 2 * CUS / a.c.n_kv)) * a.c.n_kv;
+        hipLaunchKernelGGL((kv8_mass_few_kernel<HD, F16>), dim3((unsigned)(merges + wgs)), dim3(MW), 0, st, a, merges);
+        return;
+    }
+    if (a.splits > 1) hipLaunchKernelGGL((kv8_merge_kernel<HD, F16>), merge_grid, dim3(MW), 0, st, a);
     if (!a.mass) return;
-    if (rows <= R) {
-        const int wgs = std::max(1, std::min((units + 3) / 4, 512 / a.c.n_kv));
-        hipLaunchKernelGGL((kv8_mass_few_kernel<HD, MODE>), dim3((unsigned)a.c.n_kv, (unsigned)wgs), dim3(WG), 0, st, a);
-    } else if constexpr (MODE != ROWS_PACK) {
+    if constexpr (MODE != ROWS_PACK) {
         constexpr int X = HD == 128 ? 2 : 1;  // 64 slots of K a wave, 32 where a row is twice as long
         hipLaunchKernelGGL((kv8_mass_kernel<HD, F16, X>),
                            dim3((unsigned)a.c.n_kv, (unsigned)((end + 64 * X - 1) / (64 * X))), dim3(WG), 0, st, a);

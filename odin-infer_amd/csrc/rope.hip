@@ -94,13 +94,22 @@ __global__ __launch_bounds__(WG) void rope_axes_kernel(RopeArgs a, int per) {
     const int t = blockIdx.x, tid = threadIdx.x, lane = tid & (WAVE - 1), wave = tid / WAVE;
     const int half = a.rotary / 2, heads = a.n_heads + a.n_kv;
     const int h0 = blockIdx.y * per, h1 = min(h0 + per, heads);
+    auto load = [&](int h, float (&x)[E]) {
+        if (h < a.n_heads) load_row<E>(a.q, t * a.q_stride + h * a.q_head + E * lane, a.in_f16, x);
+        else load_row<E>(a.k, t * a.k_stride + (int64_t)(h - a.n_heads) * HD + E * lane, a.in_f16, x);
+    };
+    // the next head is requested before this one is worked on, the first before the angles
+    float x[E], next[E];
+    int h = h0 + wave;
+    if (h < h1) load(h, next);
     if (tid < half) turn(a.pos[(int64_t)rope_axis(a, tid) * a.n + t], a.inv_freq[tid], cs[tid], sn[tid]);
     __syncthreads();
-    for (int h = h0 + wave; h < h1; h += WG / WAVE) {
+    for (; h < h1; h += WG / WAVE) {
         const bool is_q = h < a.n_heads;
-        float x[E], y[E];
-        if (is_q) load_row<E>(a.q, t * a.q_stride + h * a.q_head + E * lane, a.in_f16, x);
-        else load_row<E>(a.k, t * a.k_stride + (int64_t)(h - a.n_heads) * HD + E * lane, a.in_f16, x);
+        float y[E];
+#pragma unroll
+        for (int e = 0; e < E; e++) x[e] = next[e];
+        if (h + WG / WAVE < h1) load(h + WG / WAVE, next);
         const float *w = is_q ? a.q_norm : a.k_norm;
         if (w) {
             float ss = 0.f;
