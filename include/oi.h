@@ -471,8 +471,8 @@ typedef struct {
  * pointers.  q: head h of token t at t * q_stride + h * q_head_stride (in
  * elements; a q projection with a gate beside each head has head stride
  * 2 * head_dim); k, q_out and k_out: heads one after the other.  Types F32 or
- * F16 each way; q_out may be q and k_out k where type and strides are the same.
- * Pointers 16-byte aligned, strides multiples of 16 bytes; OI_E_ARG otherwise.
+ * F16 each way; q_out may be q and k_out k where type and strides are the same
+ * (OI_E_ARG otherwise); outputs overlap nothing else.  Pointers 16-byte aligned, strides multiples of 16 bytes; OI_E_ARG otherwise.
  * head_dim 128 or 256.  Enqueued on `stream`. */
 int oi_rope_axes_launch(const oi_rope_axes_dims *d, int32_t n, const int32_t *pos, const float *inv_freq,
                         const float *q_norm, const float *k_norm, int32_t in_type, const void *q, int64_t q_stride,
@@ -525,8 +525,9 @@ int oi_kv8_append_launch(const oi_kv8_dims *d, void *cache, int32_t type, const 
 int oi_kv8_read_launch(const oi_kv8_dims *d, const void *cache, int32_t slot0, int32_t n, int32_t type, void *k,
                        void *v, void *stream);
 
-/* Workspace that oi_kv8_attn_launch needs for n tokens at any length up to the
- * capacity; 0 for bad arguments. */
+/* Workspace that oi_kv8_attn_launch needs for n tokens (exactly n: fewer may need
+ * more) at any length up to the capacity, with mass or without, 16-byte aligned;
+ * 0 for bad arguments. */
 int64_t oi_kv8_attn_workspace_bytes(const oi_kv8_dims *d, int32_t n_heads, int32_t n);
 
 /* Causal attention of n tokens over the cache, which already holds them (append
@@ -539,7 +540,10 @@ int64_t oi_kv8_attn_workspace_bytes(const oi_kv8_dims *d, int32_t n_heads, int32
  * head, is added to slots below n_past and stored in slots n_past ..
  * n_past+n-1 (a new slot starts at nothing); slots past those stay as they are.
  * Every sum is in a fixed order.  `out` may be `q` where the strides are the
- * same and mass is NULL. */
+ * same and mass is NULL (OI_E_ARG otherwise); it overlaps nothing else.  With
+ * n_past_dev the work is laid out for the whole capacity, so that one captured
+ * call serves every length; sums then may be in another order than with n_past.
+ * At most 1048560 rows (n * n_heads / n_kv_heads). */
 int oi_kv8_attn_launch(const oi_kv8_dims *d, const void *cache, int32_t n_heads, int32_t type, const void *q,
                        int64_t q_stride, float scale, int32_t n, int32_t n_past, const int32_t *n_past_dev,
                        float *mass, void *out, int64_t out_stride, void *workspace, int64_t workspace_bytes,
@@ -552,7 +556,7 @@ int oi_kv8_attn_launch(const oi_kv8_dims *d, const void *cache, int32_t n_heads,
  * exponents of their new blocks (exact where that does not rise, otherwise
  * rounded to half to even once), masses, positions (src_pos and dst_pos int32
  * [n_kv_heads][capacity], both NULL or neither) and, in kept [n_kv_heads][keep],
- * the slots they came from.  dst may differ from src in capacity and block.  The
+ * the slots they came from.  src_mass 16-byte aligned.  dst may differ from src in capacity and block.  The
  * buffers of the two caches must not overlap (OI_E_ARG): a program keeps one
  * spare and exchanges them. */
 int oi_kv8_evict_launch(const oi_kv8_dims *src_dims, const void *src, const float *src_mass, const int32_t *src_pos,

@@ -112,6 +112,7 @@ int oi_kv8_append_launch(const oi_kv8_dims *d, void *cache, int32_t type, const 
         if (!type_ok(type)) return err(OI_E_ARG, W, "type must be F32 or F16");
         if (!cache || !k || !v) return err(OI_E_ARG, W, "null argument");
         if (!aligned(cache, 256)) return err(OI_E_ARG, W, "the cache must be 256-byte aligned");
+        if (!aligned(n_past_dev, 4)) return err(OI_E_ARG, W, "misaligned n_past_dev");
         if (int rc = range_ok(d, n, n_past, n_past_dev, W)) return rc;
         const int64_t row = (int64_t)d->n_kv_heads * d->head_dim;
         if (!rows_ok(k, type, k_stride, row) || !rows_ok(v, type, v_stride, row)) return err(OI_E_ARG, W, BAD_ROWS);
@@ -171,11 +172,13 @@ int oi_kv8_attn_launch(const oi_kv8_dims *d, const void *cache, int32_t n_heads,
         if (!type_ok(type)) return err(OI_E_ARG, W, "type must be F32 or F16");
         if (!cache || !q || !out || !workspace) return err(OI_E_ARG, W, "null argument");
         if (!aligned(cache, 256)) return err(OI_E_ARG, W, "the cache must be 256-byte aligned");
-        if (!aligned(workspace, 16) || !aligned(mass, 4)) return err(OI_E_ARG, W, "misaligned workspace or mass");
+        if (!aligned(workspace, 16) || !aligned(mass, 4) || !aligned(n_past_dev, 4)) return err(OI_E_ARG, W, "misaligned workspace, mass or n_past_dev");
         if (int rc = range_ok(d, n, n_past, n_past_dev, W)) return rc;
         if (!std::isfinite(scale)) return err(OI_E_ARG, W, "scale is not finite");
         const int64_t row = (int64_t)n_heads * d->head_dim;
         if (!rows_ok(q, type, q_stride, row) || !rows_ok(out, type, out_stride, row)) return err(OI_E_ARG, W, BAD_ROWS);
+        if (out == q && (q_stride != out_stride || mass))
+            return err(OI_E_ARG, W, "out may be q only with the same stride and without mass");
         const int group = n_heads / d->n_kv_heads;
         if ((int64_t)n * group > 65535 * 16) return err(OI_E_RANGE, W, "too many rows in one call");
         const int end = n_past_dev ? d->capacity : n_past + n;
@@ -282,6 +285,11 @@ int oi_rope_axes_launch(const oi_rope_axes_dims *d, int32_t n, const int32_t *po
             !rows_ok(q_out, out_type, q_out_stride, d->n_heads * hd) ||
             !rows_ok(k_out, out_type, k_out_stride, d->n_kv_heads * hd))
             return err(OI_E_ARG, W, BAD_ROWS);
+        if ((q_out == q && (in_type != out_type || q_stride != q_out_stride || q_head_stride != hd)) ||
+            (k_out == k && (in_type != out_type || k_stride != k_out_stride)))
+            return err(OI_E_ARG, W, "in place needs the same type and strides");
+        if (!aligned(pos, 4) || !aligned(inv_freq, 4) || !aligned(q_norm, 4) || !aligned(k_norm, 4))
+            return err(OI_E_ARG, W, "misaligned positions, frequencies or norm weights");
         if (int rc = stream_ok(stream, W)) return rc;
         RopeArgs a{};
         a.q = q; a.k = k; a.qo = q_out; a.ko = k_out;

@@ -759,9 +759,10 @@ __global__ __launch_bounds__(WG, 2) void kv8_mass_kernel(Kv8AttnArgs a) {
     __shared__ float qmul[2][QR], sum[2][GS];
     __shared__ float2 qnorm[2][QR];
     const int tid = threadIdx.x, lane = tid & (WAVE - 1), wave = tid / WAVE;
-    const int c = lane & 31, h = lane >> 5, kvh = blockIdx.x, s0 = blockIdx.y * GS + (wave & 1) * WS;
+    const int c = lane & 31, h = lane >> 5, kvh = blockIdx.x % a.c.n_kv, blk = blockIdx.x / a.c.n_kv;
+    const int s0 = blk * GS + (wave & 1) * WS;
     const int rows = a.n * a.group, past = kv8_past(a.past, a.n, a.c.cap), end = past + a.n;
-    if ((int)blockIdx.y * GS >= end) return;
+    if (blk * GS >= end) return;
     const float scale = fabsf(a.scale);
     const bool neg = a.scale < 0.f;
     // the tile's rows into registers, four threads a row, then as halves into LDS
@@ -844,7 +845,7 @@ __global__ __launch_bounds__(WG, 2) void kv8_mass_kernel(Kv8AttnArgs a) {
 #pragma unroll
         for (int i = 0; i < 16; i++) acc[x][i] = 0.f;
     // from the tile of rows that first sees one of the slots
-    const int first = max(0, (int)blockIdx.y * GS - past) * a.group / QR * QR;
+    const int first = max(0, blk * GS - past) * a.group / QR * QR;
     fetch(first);
     store(0);
     __syncthreads();
@@ -894,7 +895,7 @@ __global__ __launch_bounds__(WG, 2) void kv8_mass_kernel(Kv8AttnArgs a) {
             if (c == 0) sum[wave >> 1][(wave & 1) * WS + 32 * x + 8 * (i / 4) + 4 * h + i % 4] = v;
         }
     __syncthreads();
-    const int s = blockIdx.y * GS + tid;
+    const int s = blk * GS + tid;
     if (tid < GS && s < end) {
         float *m = a.mass + (size_t)kvh * a.c.cap + s;
         const float v = sum[0][tid] + sum[1][tid];
@@ -922,6 +923,7 @@ static PromptPlan prompt_plan(int hd, bool f16, int n_kv, int64_t rows) {
 
 int kv8_attn_splits(int n_kv, int group, int n, int end, int hd, bool f16) {
     const int64_t units = (end + T - 1) / T, rows = (int64_t)n * group;
+    if (n > 65535) return 1;  // the merge's grid
     if (rows <= FEW_ROWS) {
         // a unit per wave, up to two workgroups a CU
         const int64_t tiles = (rows + 15) / 16 * n_kv, most = (2 * CUS + tiles - 1) / tiles;
@@ -985,8 +987,8 @@ void launch(const Kv8AttnArgs &a, hipStream_t st) {
     if (!a.mass) return;
     if constexpr (MODE != ROWS_PACK) {
         constexpr int X = HD == 128 ? 2 : 1;  // 64 slots of K a wave, 32 where a row is twice as long
-        hipLaunchKernelGGL((kv8_mass_kernel<HD, F16, X>),
-                           dim3((unsigned)a.c.n_kv, (unsigned)((end + 64 * X - 1) / (64 * X))), dim3(WG), 0, st, a);
+        hipLaunchKernelGGL((kv8_mass_kernel<HD, F16, X>), dim3((unsigned)a.c.n_kv * ((end + 64 * X - 1) / (64 * X))),
+                           dim3(WG), 0, st, a);
     }
 }
 

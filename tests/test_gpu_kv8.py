@@ -82,7 +82,8 @@ def test_append(t, n_kv, hd, block, calls):
     plan, ref, buf = both(rng, n_kv, hd, cap, block)
     past = 0
     for i, n in enumerate(calls):
-        k, v = rows(rng, n, n_kv, hd, t), rows(rng, n, n_kv, hd, t) * NP[t](0.1 * 3 ** i)
+        with np.errstate(over="ignore"):  # the last calls of an f16 case hold infinities
+            k, v = rows(rng, n, n_kv, hd, t), rows(rng, n, n_kv, hd, t) * NP[t](0.1 * 3 ** i)
         ref.append(k, v, past)
         kd, vd = dev(k), dev(v)
         plan.append(buf.data_ptr(), t, kd.data_ptr(), vd.data_ptr(), n, past)

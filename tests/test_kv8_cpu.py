@@ -87,6 +87,13 @@ def test_attn_refusals():
         a[at] = bad
         assert L.oi_kv8_attn_launch(*a) == code, (at, bad)
         assert b"kv8 attention" in L.oi_last_error()
+    for out, stride, mass in [(P, 1024, None), (P, 512, 8 * P)]:  # in place: another stride, or with mass
+        a = list(ok)
+        a[10], a[11], a[12] = mass, out, stride
+        assert L.oi_kv8_attn_launch(*a) == E_ARG
+    a = list(ok)
+    a[9] = P + 2  # the device length
+    assert L.oi_kv8_attn_launch(*a) == E_ARG
     for heads, n in [(3, 1), (0, 1), (4, 0), (4, 257), (-4, 1)]:
         assert L.oi_kv8_attn_workspace_bytes(r, heads, n) == 0
 
@@ -100,7 +107,7 @@ def test_evict_refusals():
                           (11, None, E_ARG), (12, None, E_ARG), (1, P + 64, E_ARG), (9, far + 64, E_ARG),
                           (4, 0, E_RANGE), (4, 257, E_RANGE), (5, 0, E_RANGE), (5, 201, E_RANGE), (5, 129, E_RANGE),
                           (6, -1, E_RANGE), (7, -1, E_RANGE), (6, 93, E_RANGE), (7, 2 ** 31 - 1, E_RANGE),
-                          (9, P, E_ARG), (9, P + 256, E_ARG), (10, 4 * P, E_ARG), (11, 6 * P + 512, E_ARG)]:
+                          (2, 4 * P + 4, E_ARG), (12, far + 8 * P + 2, E_ARG), (9, P, E_ARG), (9, P + 256, E_ARG), (10, 4 * P, E_ARG), (11, 6 * P + 512, E_ARG)]:
         a = list(ok)
         a[at] = bad
         assert L.oi_kv8_evict_launch(*a) == code, (at, bad)
@@ -117,7 +124,7 @@ def test_rope_refusals():
         return _native.RopeAxesDims(h, kv, hd, rot, (ctypes.c_int32 * 3)(*s), il, eps)
 
     good = D()
-    ok = [ctypes.byref(good), 3, P, P, P, P, 0, P, 512, 128, P, 256, 1, P, 512, P, 256, None]
+    ok = [ctypes.byref(good), 3, P, P, P, P, 0, P, 512, 128, P, 256, 1, 4 * P, 512, 8 * P, 256, None]
     for at, bad, code in [(1, 0, E_RANGE), (1, -1, E_RANGE), (2, None, E_ARG), (3, None, E_ARG), (6, 2, E_ARG),
                           (12, 8, E_ARG), (7, None, E_ARG), (10, None, E_ARG), (13, None, E_ARG), (15, None, E_ARG),
                           (7, P + 4, E_ARG), (8, 508, E_ARG), (8, 514, E_ARG), (9, 64, E_ARG), (9, 130, E_ARG),
@@ -134,6 +141,17 @@ def test_rope_refusals():
     a = list(ok)
     a[0] = None
     assert L.oi_rope_axes_launch(*a) == E_ARG
+    # in place with another type, another row stride, a gate beside each head, another k stride
+    for at, bad in [((13,), (P,)), ((12, 13, 14), (0, P, 1024)), ((8, 9, 12, 13, 14), (1024, 256, 0, P, 1024)),
+                    ((12, 10, 15, 16), (0, 2 * P, 2 * P, 512))]:
+        a = list(ok)
+        for i, b in zip(at, bad):
+            a[i] = b
+        assert L.oi_rope_axes_launch(*a) == E_ARG, (at, bad)
+    for at in (2, 3, 4, 5):
+        a = list(ok)
+        a[at] = P + 2
+        assert L.oi_rope_axes_launch(*a) == E_ARG, at
 
 
 def test_format_one_rounding():
