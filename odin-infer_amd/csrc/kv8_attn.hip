@@ -77,63 +77,109 @@ constexpr int tile_rows(int mode) { return mode == ROWS_PACK ? 8 : 16; }
 
 // A tile of q as that operand: lane (column c, group g) holds dimensions
 // 64 k + 16 g + 8 h + 0..7 of its row, the order in which its 16-byte loads of K
-// fall.  f32 rows: two halves of q 2^-e, e the row's exponent.  A negative scale
-// turns q's sign, so that the largest score is that of the largest product.
+// fall.  f32 rows are made into two halves of q 2^-e (e the row's exponent) by the
+// workgroup together, a row by 256 / R threads, and pass through LDS: each wave
+// for itself took 1.8 us more at head_dim 256, in one long run of instructions.  A negative scale turns q's sign, so that the largest score is that
+// of the largest product.
 template <int HD, int MODE>
 struct QTile {
-    static constexpr int NF = HD / 32;
+    static constexpr int NF = HD / 32, R = tile_rows(MODE);
     static constexpr bool F16 = MODE == ROWS_F16, TWO = MODE == ROWS_F32;
+    static constexpr int TPR = WG / R, EL = HD / TPR;  // f32: threads of a row, elements of a thread
+    struct Lds {
+        f16x8 half[2][R][HD / 8];  // upper, lower; piece j of row r at j ^ (r & 7)
+        int e[R];
+    };
     f16x8 hi[NF], lo[TWO ? NF : 1];
     int e = 0;
+    u32x4 raw[F16 ? NF : EL / 4];
 
-    // the row's loads (row `at` exists), then the operands (zero with ok = false)
-    struct Raw {
-        u32x4 w[F16 ? NF : 2 * NF];
-    };
-    static __device__ __forceinline__ void fetch(Raw &r, const void *q, int64_t at, int g) {
+    // f16: the loads of row `at`, this lane's; f32: `at` is the row of thread tid / TPR
+    __device__ __forceinline__ void fetch(const void *q, int64_t at, int tid) {
+        if constexpr (F16) {
+            const int g = (tid & (WAVE - 1)) >> 4;
 #pragma unroll
-        for (int f = 0; f < NF; f++) {
-            const int64_t d = at + 64 * (f / 2) + 16 * g + 8 * (f & 1);
-            if constexpr (F16) {
-                r.w[f] = *(const u32x4 *)((const uint16_t *)q + d);
-            } else {
-                r.w[2 * f] = *(const u32x4 *)((const float *)q + d);
-                r.w[2 * f + 1] = *(const u32x4 *)((const float *)q + d + 4);
-            }
+            for (int f = 0; f < NF; f++)
+                raw[f] = *(const u32x4 *)((const uint16_t *)q + at + 64 * (f / 2) + 16 * g + 8 * (f & 1));
+        } else {
+#pragma unroll
+            for (int i = 0; i < EL / 4; i++)
+                raw[i] = *(const u32x4 *)((const float *)q + at + tid % TPR * EL + 4 * i);
         }
     }
-    __device__ __forceinline__ void make(const Raw &r, bool ok, bool neg, bool lower) {
+    // f32: the halves into LDS (a barrier follows)
+    __device__ __forceinline__ void split(Lds &lds, int tid, bool neg) {
+        if constexpr (!F16) {
+            const int r = tid / TPR, j = tid % TPR;
+            float amax = 0.f;
+#pragma unroll
+            for (int i = 0; i < EL / 4; i++)
+#pragma unroll
+                for (int k = 0; k < 4; k++) {
+                    const uint32_t bits = raw[i][k];
+                    amax = fmaxf(amax, fabsf(__uint_as_float(bits)));
+                }
+            amax = fmaxf(amax, OI_DPP(amax, 0xB1));
+            amax = fmaxf(amax, OI_DPP(amax, 0x4E));
+            amax = fmaxf(amax, OI_DPP(amax, 0x141));
+            amax = fmaxf(amax, OI_DPP(amax, 0x140));
+            if constexpr (TPR == 32) {
+                const auto w = __builtin_amdgcn_permlane16_swap(__float_as_uint(amax), __float_as_uint(amax), false, false);
+                amax = fmaxf(__uint_as_float(w[0]), __uint_as_float(w[1]));
+            }
+            const int ex = amax > 0.f ? (int)(__float_as_uint(amax) >> 23) - 127 - 14 : 0;
+            uint32_t h[EL / 2], l[EL / 2];
+#pragma unroll
+            for (int i = 0; i < EL / 2; i++) {
+                f16x2 th, tl;
+#pragma unroll
+                for (int k = 0; k < 2; k++) {
+                    const uint32_t bits = raw[i / 2][2 * (i & 1) + k];
+                    const float x = __uint_as_float(bits), y = ldexpf(neg ? -x : x, -ex);
+                    const _Float16 t = (_Float16)y;
+                    th[k] = t;
+                    tl[k] = (_Float16)(y - (float)t);
+                }
+                h[i] = __builtin_bit_cast(uint32_t, th);
+                l[i] = __builtin_bit_cast(uint32_t, tl);
+            }
+            // pieces of 8 elements; a thread of 4 elements writes half of one
+            constexpr int W = EL < 8 ? EL / 2 : 4;  // words of a piece per thread
+#pragma unroll
+            for (int i = 0; i < (EL + 7) / 8; i++) {
+                const int el = j * EL + 8 * i;
+                uint32_t *ph = (uint32_t *)&lds.half[0][r][(el / 8) ^ (r & 7)] + el % 8 / 2,
+                         *pl = (uint32_t *)&lds.half[1][r][(el / 8) ^ (r & 7)] + el % 8 / 2;
+#pragma unroll
+                for (int k = 0; k < W; k++) {
+                    ph[k] = h[4 * i + k];
+                    pl[k] = l[4 * i + k];
+                }
+            }
+            if (j == 0) lds.e[r] = ex;
+        }
+    }
+    // the operands, zero with ok = false
+    __device__ __forceinline__ void make(const Lds &lds, int tid, bool ok, bool neg) {
+        const int c = tid & 15, g = (tid & (WAVE - 1)) >> 4;
         if constexpr (F16) {
             const uint32_t sign = neg ? 0x80008000u : 0u;
 #pragma unroll
             for (int f = 0; f < NF; f++) {
                 u32x4 w;
 #pragma unroll
-                for (int i = 0; i < 4; i++) w[i] = ok ? r.w[f][i] ^ sign : 0u;
+                for (int i = 0; i < 4; i++) w[i] = ok ? raw[f][i] ^ sign : 0u;
                 hi[f] = __builtin_bit_cast(f16x8, w);
             }
         } else {
-            float amax = 0.f;
+            const int r = c % R;
+            e = lds.e[r];
 #pragma unroll
-            for (int f = 0; f < 2 * NF; f++)
-#pragma unroll
-                for (int i = 0; i < 4; i++) amax = fmaxf(amax, fabsf(__uint_as_float(r.w[f][i])));
-            amax = ok ? col_max(amax) : 0.f;
-            e = amax > 0.f ? (int)(__float_as_uint(amax) >> 23) - 127 - 14 : 0;
-#pragma unroll
-            for (int f = 0; f < NF; f++)
-#pragma unroll
-                for (int i = 0; i < 8; i++) {
-                    const float x = __uint_as_float(r.w[2 * f + i / 4][i & 3]);
-                    const float y = ok ? ldexpf(neg ? -x : x, -e) : 0.f;
-                    const _Float16 h = (_Float16)y, l = (_Float16)(y - (float)h);
-                    if constexpr (TWO) {
-                        hi[f][i] = h;
-                        lo[f][i] = l;
-                    } else {
-                        hi[f][i] = lower ? l : h;
-                    }
-                }
+            for (int f = 0; f < NF; f++) {
+                const int at = (8 * (f / 2) + 2 * g + (f & 1)) ^ (r & 7);
+                hi[f] = lds.half[TWO ? 0 : c / R][r][at];
+                if constexpr (TWO) lo[f] = lds.half[1][r][at];
+            }
         }
     }
 };
@@ -185,8 +231,12 @@ template <int HD, int MODE, bool SAVE>
 __global__ __launch_bounds__(WG) void kv8_rows_kernel(Kv8AttnArgs a) {
     constexpr int NW = WG / WAVE, NK = HD / 64, ND = HD / 16, PD = HD + 4, R = tile_rows(MODE), TPR = WG / R;
     constexpr bool F16 = MODE == ROWS_F16;
-    __shared__ __attribute__((aligned(16))) float so[NW][R][PD];
+    __shared__ __attribute__((aligned(16))) union {
+        float o[NW][R][PD];
+        typename QTile<HD, MODE>::Lds q;
+    } lds;
     __shared__ float sm[NW][R], sl[NW][R];
+    auto &so = lds.o;
     const int tid = threadIdx.x, lane = tid & (WAVE - 1), wave = tid / WAVE;
     const int c = lane & 15, g = lane >> 4;
     const int kvh = blockIdx.x, rt = blockIdx.y, split = blockIdx.z;
@@ -199,9 +249,9 @@ __global__ __launch_bounds__(WG) void kv8_rows_kernel(Kv8AttnArgs a) {
     const int last_limit = past + row_token(a, min(rt * R + R - 1, rows - 1)) + 1;
     const int units = (last_limit + T - 1) / T;
     const int u0 = (int)((int64_t)split * units / a.splits), u1 = (int)((int64_t)(split + 1) * units / a.splits);
+    const bool neg = a.scale < 0.f;
     QTile<HD, MODE> q;
-    typename QTile<HD, MODE>::Raw qraw;
-    QTile<HD, MODE>::fetch(qraw, a.q, row_at(a, rr, kvh, a.q_stride, HD), g);
+    q.fetch(a.q, row_at(a, F16 ? rr : min(rt * R + tid / TPR, rows - 1), kvh, a.q_stride, HD), tid);
 
     const int krow = 16 * (c >> 2) + (c & 3);
     const int8_t *kb = a.c.kc + (size_t)kvh * a.c.cap * HD + krow * HD + 16 * g;
@@ -233,7 +283,11 @@ __global__ __launch_bounds__(WG) void kv8_rows_kernel(Kv8AttnArgs a) {
         load_k(u);
         load_v(u);
     }
-    q.make(qraw, ok, a.scale < 0.f, lower);
+    if constexpr (!F16) {
+        q.split(lds.q, tid, neg);
+        __syncthreads();
+    }
+    q.make(lds.q, tid, ok, neg);
     const float scale = fabsf(a.scale);
     for (; u < u1; u += NW) {
         f32x4 s[4];
@@ -309,6 +363,7 @@ __global__ __launch_bounds__(WG) void kv8_rows_kernel(Kv8AttnArgs a) {
         for (int d = 0; d < ND; d++)
 #pragma unroll
             for (int i = 0; i < 4; i++) o[d][i] = half_sum(o[d][i]);
+    if constexpr (!F16) __syncthreads();  // every wave has read q
     if (!lower) {
 #pragma unroll
         for (int d = 0; d < ND; d++) *(f32x4 *)&so[wave][c][16 * d + 4 * g] = o[d];
@@ -486,9 +541,11 @@ struct QRows {
     }
 };
 
-// A unit of 64 slots, K and V as halves in LDS, 16-byte pieces (8 values)
-// placed so that 8 neighbouring rows' equal pieces fall on different banks:
-// piece j of row r at j ^ (r & 7).  K row r holds the slot with bits 2 and 3 of r
+// A unit of 64 slots, K and V as halves in LDS, in 16-byte pieces (8 values).
+// Lanes read equal pieces of neighbouring rows, sixteen at a time over the 64
+// banks (256 bytes): a K row of 256 or 512 bytes has its piece j at j ^ (r & 15),
+// V rows of 128 bytes, two to a round of the banks, at j ^ (r / 2 & 7).  (With r & 7
+// for both, 46% of the LDS cycles were conflicts.)  K row r holds the slot with bits 2 and 3 of r
 // exchanged: the products then leave a lane the scores of slots 8 h + 0..7 of
 // each 16, those whose weights it supplies to the product with V.
 template <int HD, int NT>
@@ -513,11 +570,11 @@ struct Stage {
             const int at = tid + i * NT;
             const int s = at / (HD / 16), j = at % (HD / 16) * 2;
             const int r = (s & ~12) | (s & 4) << 1 | (s & 8) >> 1;
-            ks[r * (HD / 8) + (j ^ (r & 7))] = bytes_h(k[i][0], k[i][1]);
-            ks[r * (HD / 8) + ((j + 1) ^ (r & 7))] = bytes_h(k[i][2], k[i][3]);
+            ks[r * (HD / 8) + (j ^ (r & 15))] = bytes_h(k[i][0], k[i][1]);
+            ks[r * (HD / 8) + ((j + 1) ^ (r & 15))] = bytes_h(k[i][2], k[i][3]);
             const int d = at / 4, m = at % 4 * 2;
-            vs[d * 8 + (m ^ (d & 7))] = bytes_h(v[i][0], v[i][1]);
-            vs[d * 8 + ((m + 1) ^ (d & 7))] = bytes_h(v[i][2], v[i][3]);
+            vs[d * 8 + (m ^ (d >> 1 & 7))] = bytes_h(v[i][0], v[i][1]);
+            vs[d * 8 + ((m + 1) ^ (d >> 1 & 7))] = bytes_h(v[i][2], v[i][3]);
         }
     }
 };
@@ -572,9 +629,9 @@ __global__ __launch_bounds__(NW *WAVE, HD == 128 ? 2 : 1) void kv8_prompt_kernel
         if (u + 1 < u1) st.load(kb, vb, ke, ve, a.c.lb, u + 1, tid);
         if (u * T < mine) {
             const f32x4 kmul = *(const f32x4 *)&es[buf][0] * scale, ev = *(const f32x4 *)&es[buf][4];
-            auto k_at = [&](int x, int f) { return kt[(32 * x + c) * (HD / 8) + ((2 * f + h) ^ (c & 7))]; };
+            auto k_at = [&](int x, int f) { return kt[(32 * x + c) * (HD / 8) + ((2 * f + h) ^ (c & 15))]; };
             auto v_at = [&](int x, int b, int d) {
-                return vt[(32 * (d0 + d) + c) * 8 + ((4 * x + 2 * b + h) ^ (c & 7))];
+                return vt[(32 * (d0 + d) + c) * 8 + ((4 * x + 2 * b + h) ^ (c >> 1 & 7))];
             };
             f16x8 kf[AHEAD ? NF : 1], vf[AHEAD ? DT : 1][2];
             if constexpr (AHEAD)
@@ -787,7 +844,7 @@ __global__ __launch_bounds__(WG, 2) void kv8_mass_kernel(Kv8AttnArgs a) {
                 u32x4 w = raw[i];
 #pragma unroll
                 for (int k = 0; k < 4; k++) w[k] ^= sign;
-                qs[b][0][qr * (HD / 8) + ((qj * (EL / 8) + i) ^ (qr & 7))] = __builtin_bit_cast(f16x8, w);
+                qs[b][0][qr * (HD / 8) + ((qj * (EL / 8) + i) ^ (qr & 15))] = __builtin_bit_cast(f16x8, w);
             }
         } else {
             float amax = 0.f;
@@ -812,7 +869,7 @@ __global__ __launch_bounds__(WG, 2) void kv8_mass_kernel(Kv8AttnArgs a) {
                     hi[k] = t;
                     lo[k] = (_Float16)(y - (float)t);
                 }
-                const int at = qr * (HD / 8) + ((qj * (EL / 8) + i) ^ (qr & 7));
+                const int at = qr * (HD / 8) + ((qj * (EL / 8) + i) ^ (qr & 15));
                 qs[b][0][at] = hi;
                 qs[b][PC - 1][at] = lo;
             }
@@ -865,7 +922,7 @@ __global__ __launch_bounds__(WG, 2) void kv8_mass_kernel(Kv8AttnArgs a) {
                 for (int i = 0; i < 16; i++) s[i] = 0.f;
 #pragma unroll
                 for (int f = 0; f < NF; f++) {
-                    const int at = lr * (HD / 8) + ((4 * (f / 2) + 2 * h + (f & 1)) ^ (lr & 7));
+                    const int at = lr * (HD / 8) + ((4 * (f / 2) + 2 * h + (f & 1)) ^ (lr & 15));
                     s = mfma32(kf[x][f], qs[b][0][at], s);
                     if constexpr (!F16) s = mfma32(kf[x][f], qs[b][PC - 1][at], s);
                 }
