@@ -215,6 +215,11 @@ int oi_kv8_attn_launch(const oi_kv8_dims *d, const void *cache, int32_t n_heads,
         a.part = ws;
         a.ml = (float2 *)(a.part + (splits > 1 ? parts * d->head_dim : 0));
         a.norm = mass ? a.ml + parts : nullptr;
+        if (mass && !a.save) {
+            a.msplits = kv8_mass_splits(d->n_kv_heads, group, n, end, d->head_dim);
+            a.msum_slots = end;
+            a.msum = (float *)(a.norm + rows);
+        }
         return launched(launch_kv8_attn(a, (hipStream_t)stream), W);
     });
 }

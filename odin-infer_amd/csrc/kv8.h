@@ -60,10 +60,14 @@ struct Kv8AttnArgs {
     // and its row's maximum then [n_kv][save_units][rows]; null otherwise
     float *save, *save_m;
     int32_t save_units, splits;
+    // many rows with mass: splits of the rows, and where msplits > 1 their sums [msplits][n_kv][msum_slots]
+    float *msum;
+    int32_t msum_slots, msplits;
 };
 // splits over the slots for a call that sees at most `end` of them, and the workspace that they take
 int kv8_attn_splits(int n_kv, int group, int n, int end, int hd, bool f16);
 bool kv8_attn_saves(int group, int n);
+int kv8_mass_splits(int n_kv, int group, int n, int end, int hd);
 size_t kv8_attn_workspace(int n_heads, int group, int n, int end, int hd, int splits, bool mass);
 hipError_t launch_kv8_attn(const Kv8AttnArgs &a, hipStream_t st);
 

@@ -482,6 +482,35 @@ __global__ __launch_bounds__(MW) void kv8_merge_kernel(Kv8AttnArgs a) {
     merge_row<HD, F16>(a, blockIdx.y, blockIdx.x, lds);
 }
 
+// Merge of a few splits of many rows: four dimensions a thread, WG * 4 / HD rows a
+// workgroup (a workgroup per row took 30 us for two splits of 16000 rows).
+constexpr int MERGE_FEW = 16;
+template <int HD, bool F16>
+__global__ __launch_bounds__(WG) void kv8_merge_many_kernel(Kv8AttnArgs a) {
+    constexpr int LPR = HD / 4, RPW = WG / LPR;
+    const int h = blockIdx.x * RPW + threadIdx.x / LPR, d = threadIdx.x % LPR * 4, S = a.splits;
+    if (h >= a.n_heads) return;
+    const size_t id = (size_t)blockIdx.y * a.n_heads + h;
+    const float2 *ml = a.ml + id * S;
+    const float *pt = a.part + id * S * HD + d;
+    float M = NEG, L = 0.f;
+    f32x4 y = {0.f, 0.f, 0.f, 0.f};
+    for (int s = 0; s < S; s++) M = fmaxf(M, ml[s].x);
+    for (int s = 0; s < S; s++) {
+        const float f = ex2(ml[s].x - M);
+        L += ml[s].y * f;
+        y += *(const f32x4 *)(pt + (size_t)s * HD) * f;
+    }
+    y *= 1.f / L;
+    const int64_t at = blockIdx.y * a.out_stride + (int64_t)h * HD + d;
+    if constexpr (F16)
+        *(u32x2 *)((uint16_t *)a.out + at) =
+            u32x2{f2h(y[0]) | (uint32_t)f2h(y[1]) << 16, f2h(y[2]) | (uint32_t)f2h(y[3]) << 16};
+    else
+        *(f32x4 *)((float *)a.out + at) = y;
+    if (d == 0 && a.norm) a.norm[id] = make_float2(M, 32768.f / L);
+}
+
 // ------------------------------------------------------------- prompts --
 
 typedef float f32x16 __attribute__((ext_vector_type(16)));
@@ -808,7 +837,10 @@ __global__ __launch_bounds__(MW) void kv8_mass_few_kernel(Kv8AttnArgs a, int mer
 // Many rows: a workgroup owns 64 X slots, a wave 32 X of them (K in its operand
 // registers, converted once) and every other 32 rows of the tiles of 64 rows of q
 // that pass through LDS (two buffers).  The sums over rows stay in registers; at
-// the end they cross the lanes and meet, two waves a slot, in LDS.
+// the end they cross the lanes and meet, two waves a slot, in LDS.  Where slots are
+// too few to fill the card, the rows are split over workgroups too, whose sums a
+// second launch adds (1000 rows of 16 heads of 2 kv heads at 5000 slots, head_dim
+// 256: 168 us in one split, 96 in three).
 template <int HD, bool F16, int X>
 __global__ __launch_bounds__(WG, 2) void kv8_mass_kernel(Kv8AttnArgs a) {
     constexpr int NF = HD / 16, QR = 64, PC = F16 ? 1 : 2, TPR = WG / QR, EL = HD / TPR, WS = 32 * X, GS = 2 * WS;
@@ -820,8 +852,6 @@ __global__ __launch_bounds__(WG, 2) void kv8_mass_kernel(Kv8AttnArgs a) {
     const int s0 = blk * GS + (wave & 1) * WS;
     const int rows = a.n * a.group, past = kv8_past(a.past, a.n, a.c.cap), end = past + a.n;
     if (blk * GS >= end) return;
-    const float scale = fabsf(a.scale);
-    const bool neg = a.scale < 0.f;
     // the tile's rows into registers, four threads a row, then as halves into LDS
     const int qr = tid / TPR, qj = tid % TPR;
     u32x4 raw[F16 ? EL / 8 : EL / 4];
@@ -838,14 +868,9 @@ __global__ __launch_bounds__(WG, 2) void kv8_mass_kernel(Kv8AttnArgs a) {
     auto store = [&](int b) {
         int e = 0;
         if constexpr (F16) {
-            const uint32_t sign = neg ? 0x80008000u : 0u;
 #pragma unroll
-            for (int i = 0; i < EL / 8; i++) {
-                u32x4 w = raw[i];
-#pragma unroll
-                for (int k = 0; k < 4; k++) w[k] ^= sign;
-                qs[b][0][qr * (HD / 8) + ((qj * (EL / 8) + i) ^ (qr & 15))] = __builtin_bit_cast(f16x8, w);
-            }
+            for (int i = 0; i < EL / 8; i++)
+                qs[b][0][qr * (HD / 8) + ((qj * (EL / 8) + i) ^ (qr & 15))] = __builtin_bit_cast(f16x8, raw[i]);
         } else {
             float amax = 0.f;
 #pragma unroll
@@ -864,7 +889,7 @@ __global__ __launch_bounds__(WG, 2) void kv8_mass_kernel(Kv8AttnArgs a) {
 #pragma unroll
                 for (int k = 0; k < 8; k++) {
                     const uint32_t bits = raw[2 * i + k / 4][k & 3];
-                    const float x = __uint_as_float(bits), y = ldexpf(neg ? -x : x, -e);
+                    const float y = ldexpf(__uint_as_float(bits), -e);
                     const _Float16 t = (_Float16)y;
                     hi[k] = t;
                     lo[k] = (_Float16)(y - (float)t);
@@ -875,7 +900,7 @@ __global__ __launch_bounds__(WG, 2) void kv8_mass_kernel(Kv8AttnArgs a) {
             }
         }
         if (qj == 0) {
-            qmul[b][qr] = ldexpf(scale, e);
+            qmul[b][qr] = ldexpf(a.scale, e);
             qnorm[b][qr] = raw_norm;
         }
     };
@@ -901,13 +926,17 @@ __global__ __launch_bounds__(WG, 2) void kv8_mass_kernel(Kv8AttnArgs a) {
     for (int x = 0; x < X; x++)
 #pragma unroll
         for (int i = 0; i < 16; i++) acc[x][i] = 0.f;
-    // from the tile of rows that first sees one of the slots
-    const int first = max(0, blk * GS - past) * a.group / QR * QR;
-    fetch(first);
-    store(0);
+    // from the tile of rows that first sees one of the slots, this split's part of the tiles
+    const int first = max(0, blk * GS - past) * a.group / QR, tiles = (rows + QR - 1) / QR - first;
+    const int from = (first + (int)((int64_t)blockIdx.y * tiles / gridDim.y)) * QR,
+              to = (first + (int)((int64_t)(blockIdx.y + 1) * tiles / gridDim.y)) * QR;
+    if (from < to) {
+        fetch(from);
+        store(0);
+    }
     __syncthreads();
-    for (int t0 = first, b = 0; t0 < rows; t0 += QR, b ^= 1) {
-        if (t0 + QR < rows) fetch(t0 + QR);
+    for (int t0 = from, b = 0; t0 < to; t0 += QR, b ^= 1) {
+        if (t0 + QR < to) fetch(t0 + QR);
         const int lr = 32 * (wave >> 1) + c, r = t0 + lr;  // my column's row
         const int r_last = min(t0 + 32 * (wave >> 1) + 31, rows - 1);
         if (s0 < past + row_token(a, r_last) + 1 && t0 + 32 * (wave >> 1) < rows) {
@@ -915,31 +944,37 @@ __global__ __launch_bounds__(WG, 2) void kv8_mass_kernel(Kv8AttnArgs a) {
             const float qm = qmul[b][lr];
             const float2 norm = qnorm[b][lr];
             const bool edge = s0 + WS > past + row_token(a, t0 + 32 * (wave >> 1)) + 1 || t0 + QR > rows;
+            f32x16 s[X];
+#pragma unroll
+            for (int x = 0; x < X; x++)
+#pragma unroll
+                for (int i = 0; i < 16; i++) s[x][i] = 0.f;
+#pragma unroll
+            for (int f = 0; f < NF; f++) {
+                const int at = lr * (HD / 8) + ((4 * (f / 2) + 2 * h + (f & 1)) ^ (lr & 15));
+                const f16x8 hi = qs[b][0][at], lo = qs[b][PC - 1][at];
+#pragma unroll
+                for (int x = 0; x < X; x++) {
+                    s[x] = mfma32(kf[x][f], hi, s[x]);
+                    if constexpr (!F16) s[x] = mfma32(kf[x][f], lo, s[x]);
+                }
+            }
 #pragma unroll
             for (int x = 0; x < X; x++) {
-                f32x16 s;
-#pragma unroll
-                for (int i = 0; i < 16; i++) s[i] = 0.f;
-#pragma unroll
-                for (int f = 0; f < NF; f++) {
-                    const int at = lr * (HD / 8) + ((4 * (f / 2) + 2 * h + (f & 1)) ^ (lr & 15));
-                    s = mfma32(kf[x][f], qs[b][0][at], s);
-                    if constexpr (!F16) s = mfma32(kf[x][f], qs[b][PC - 1][at], s);
-                }
                 if (edge) {
 #pragma unroll
                     for (int i = 0; i < 16; i++) {
-                        const float p = ex2(fmaf(s[i], step[2 * x + i / 8] * qm, -norm.x)) * norm.y;
+                        const float p = ex2(fmaf(s[x][i], step[2 * x + i / 8] * qm, -norm.x)) * norm.y;
                         acc[x][i] += s0 + 32 * x + 8 * (i / 4) + 4 * h + i % 4 < limit ? p : 0.f;
                     }
                 } else {
 #pragma unroll
                     for (int i = 0; i < 16; i++)
-                        acc[x][i] = fmaf(ex2(fmaf(s[i], step[2 * x + i / 8] * qm, -norm.x)), norm.y, acc[x][i]);
+                        acc[x][i] = fmaf(ex2(fmaf(s[x][i], step[2 * x + i / 8] * qm, -norm.x)), norm.y, acc[x][i]);
                 }
             }
         }
-        if (t0 + QR < rows) store(b ^ 1);
+        if (t0 + QR < to) store(b ^ 1);
         __syncthreads();
     }
 #pragma unroll
@@ -954,10 +989,23 @@ __global__ __launch_bounds__(WG, 2) void kv8_mass_kernel(Kv8AttnArgs a) {
     __syncthreads();
     const int s = blk * GS + tid;
     if (tid < GS && s < end) {
-        float *m = a.mass + (size_t)kvh * a.c.cap + s;
         const float v = sum[0][tid] + sum[1][tid];
+        if (gridDim.y > 1) {
+            a.msum[((size_t)blockIdx.y * a.c.n_kv + kvh) * a.msum_slots + s] = v;
+            return;
+        }
+        float *m = a.mass + (size_t)kvh * a.c.cap + s;
         *m = s < past ? *m + v : v;
     }
+}
+// the row splits' sums, in order
+__global__ __launch_bounds__(WG) void kv8_mass_sum_kernel(Kv8AttnArgs a, int splits) {
+    const int past = kv8_past(a.past, a.n, a.c.cap), s = blockIdx.x * WG + threadIdx.x, kvh = blockIdx.y;
+    if (s >= past + a.n) return;
+    float v = 0.f;
+    for (int y = 0; y < splits; y++) v += a.msum[((size_t)y * a.c.n_kv + kvh) * a.msum_slots + s];
+    float *m = a.mass + (size_t)kvh * a.c.cap + s;
+    *m = s < past ? *m + v : v;
 }
 
 }  // namespace
@@ -1007,10 +1055,22 @@ int kv8_attn_splits(int n_kv, int group, int n, int end, int hd, bool f16) {
 
 bool kv8_attn_saves(int group, int n) { return (int64_t)n * group <= FEW_MASS_ROWS; }
 
+// slots of a workgroup of the mass of many rows: 64 of K a wave, 32 where a row is twice as long
+static int mass_slots(int hd) { return hd == 128 ? 128 : 64; }
+
+// Splits of the rows for the mass of many rows: workgroups for two a CU, but a
+// dozen tiles of 64 rows each
+int kv8_mass_splits(int n_kv, int group, int n, int end, int hd) {
+    const int64_t wgs = ((int64_t)end + mass_slots(hd) - 1) / mass_slots(hd) * n_kv, tiles = ((int64_t)n * group + 63) / 64;
+    return (int)std::max<int64_t>(1, std::min((2 * CUS + wgs / 2) / wgs, tiles / 12));
+}
+
 size_t kv8_attn_workspace(int n_heads, int group, int n, int end, int hd, int splits, bool mass) {
     const size_t rows = (size_t)n * n_heads, units = ((size_t)end + T - 1) / T;
     const size_t saved = mass && kv8_attn_saves(group, n) ? rows * units * T + (rows * units + 3) / 4 * 4 : 0;
-    return (saved + rows * ((splits > 1 ? (size_t)splits * hd : 0) + 2 * (size_t)splits + 2)) * 4;
+    const int n_kv = n_heads / group, ms = mass && !kv8_attn_saves(group, n) ? kv8_mass_splits(n_kv, group, n, end, hd) : 1;
+    const size_t sums = ms > 1 ? (size_t)ms * n_kv * end : 0;
+    return (saved + rows * ((splits > 1 ? (size_t)splits * hd : 0) + 2 * (size_t)splits + 2) + sums) * 4;
 }
 
 namespace {
@@ -1040,12 +1100,22 @@ void launch(const Kv8AttnArgs &a, hipStream_t st) {
         hipLaunchKernelGGL((kv8_mass_few_kernel<HD, F16>), dim3((unsigned)(merges + wgs)), dim3(MW), 0, st, a, merges);
         return;
     }
-    if (a.splits > 1) hipLaunchKernelGGL((kv8_merge_kernel<HD, F16>), merge_grid, dim3(MW), 0, st, a);
+    if (a.splits > 1 && a.splits <= MERGE_FEW && rows > FEW_ROWS) {
+        constexpr int RPW = WG * 4 / HD;
+        hipLaunchKernelGGL((kv8_merge_many_kernel<HD, F16>),
+                           dim3((unsigned)((a.n_heads + RPW - 1) / RPW), (unsigned)a.n), dim3(WG), 0, st, a);
+    } else if (a.splits > 1) {
+        hipLaunchKernelGGL((kv8_merge_kernel<HD, F16>), merge_grid, dim3(MW), 0, st, a);
+    }
     if (!a.mass) return;
     if constexpr (MODE != ROWS_PACK) {
-        constexpr int X = HD == 128 ? 2 : 1;  // 64 slots of K a wave, 32 where a row is twice as long
-        hipLaunchKernelGGL((kv8_mass_kernel<HD, F16, X>), dim3((unsigned)a.c.n_kv * ((end + 64 * X - 1) / (64 * X))),
-                           dim3(WG), 0, st, a);
+        constexpr int X = HD == 128 ? 2 : 1;
+        hipLaunchKernelGGL((kv8_mass_kernel<HD, F16, X>),
+                           dim3((unsigned)a.c.n_kv * ((end + 64 * X - 1) / (64 * X)), (unsigned)a.msplits), dim3(WG), 0, st,
+                           a);
+        if (a.msplits > 1)
+            hipLaunchKernelGGL(kv8_mass_sum_kernel, dim3((unsigned)((end + WG - 1) / WG), (unsigned)a.c.n_kv), dim3(WG), 0,
+                               st, a, a.msplits);
     }
 }
 
