@@ -213,8 +213,8 @@ int oi_kv8_attn_launch(const oi_kv8_dims *d, const void *cache, int32_t n_heads,
             ws = a.save_m + (rows * a.save_units + 3) / 4 * 4;
         }
         a.part = ws;
-        a.ml = (float2 *)(a.part + (splits > 1 ? parts * d->head_dim : 0));
-        a.norm = mass ? a.ml + parts : nullptr;
+        a.ml = (float4 *)(a.part + (splits > 1 ? parts * d->head_dim : 0));
+        a.norm = mass ? (float2 *)(a.ml + parts) : nullptr;
         if (mass && !a.save) {
             a.msplits = kv8_mass_splits(d->n_kv_heads, group, n, end, d->head_dim);
             a.msum_slots = end;

@@ -54,7 +54,7 @@ struct Kv8AttnArgs {
     Kv8Past past;
     float *mass;          // [n_kv][cap] or null
     float *part;          // [n * n_heads][splits][hd], where splits > 1: the splits' o
-    float2 *ml;           // [n * n_heads][splits]: their m and l (few rows, or splits > 1)
+    float4 *ml;           // [n * n_heads][splits]: their m, l of the products' weights, l of the exact ones
     float2 *norm;         // [n * n_heads], where mass is set: m and 2^15 / l of a row
     // few rows with mass: every weight as it was formed [n_kv][save_units][rows][64]
     // and its row's maximum then [n_kv][save_units][rows]; null otherwise

@@ -11,7 +11,8 @@
 // take f16 operands: a and b are exact there; q and p of an f32 call are each
 // the sum of two halves (22 bits, q scaled by a power of two per row), of an
 // f16 call q is exact and p is rounded once to 11 bits (the size of the output's
-// own rounding).  2^15 is where the largest weight sits in f16: a weight keeps
+// own rounding; its l is the sum of the rounded p, so a weight that dominates
+// loses nothing, and the mass takes the sum of p before the rounding).  2^15 is where the largest weight sits in f16: a weight keeps
 // all its bits down to 2^-29 of it and is lost below 2^-40.
 
 #include <algorithm>
@@ -64,6 +65,17 @@ __device__ __forceinline__ float col_sum(float v) {
 // v and that of the column 8 away.  By value: __builtin_bit_cast of a vector's
 // element (inside OI_DPP) takes the vector's first one.
 __device__ __forceinline__ float half_sum(float v) { return v + OI_DPP(v, 0x128); }
+// the sum of 8 halves in f32, one mixed multiply-add each (v_dot2_f32_f16 took 3% more of a prompt)
+__device__ __forceinline__ float sum8(f16x8 p) {
+    float lo = 0.f, hi = 0.f;
+#pragma unroll
+    for (int i = 0; i < 4; i++) {
+        const uint32_t w = __builtin_bit_cast(uint32_t, f16x2{p[2 * i], p[2 * i + 1]});
+        asm("v_fma_mix_f32 %0, %1, 1.0, %0 op_sel_hi:[1,0,0]" : "+v"(lo) : "v"(w));
+        asm("v_fma_mix_f32 %0, %1, 1.0, %0 op_sel:[1,0,0] op_sel_hi:[1,0,0]" : "+v"(hi) : "v"(w));
+    }
+    return lo + hi;
+}
 // 2^x; results below the normal numbers are 0
 __device__ __forceinline__ float ex2(float x) { return __builtin_amdgcn_exp2f(x); }
 
@@ -235,7 +247,7 @@ __global__ __launch_bounds__(WG) void kv8_rows_kernel(Kv8AttnArgs a) {
         float o[NW][R][PD];
         typename QTile<HD, MODE>::Lds q;
     } lds;
-    __shared__ float sm[NW][R], sl[NW][R];
+    __shared__ float sm[NW][R], sl[NW][R], sx[NW][R];
     auto &so = lds.o;
     const int tid = threadIdx.x, lane = tid & (WAVE - 1), wave = tid / WAVE;
     const int c = lane & 15, g = lane >> 4;
@@ -274,7 +286,7 @@ __global__ __launch_bounds__(WG) void kv8_rows_kernel(Kv8AttnArgs a) {
 #pragma unroll
         for (int d = 0; d < ND; d++) vr[d] = *(const u32x4 *)(p + 16 * d * T);
     };
-    float m = NEG, l = 0.f;
+    float m = NEG, l = 0.f, lx = 0.f;  // lx: of the weights before their rounding to f16
     f32x4 o[ND];
 #pragma unroll
     for (int d = 0; d < ND; d++) o[d] = f32x4{0.f, 0.f, 0.f, 0.f};
@@ -341,11 +353,13 @@ __global__ __launch_bounds__(WG) void kv8_rows_kernel(Kv8AttnArgs a) {
         if (__any(m1 != m)) {  // a row's maximum rose
             const float alpha = ex2(m - m1);
             l *= alpha;
+            lx *= alpha;
 #pragma unroll
             for (int d = 0; d < ND; d++) o[d] *= alpha;
             m = m1;
         }
-        l += sum * pow2i(-ev);
+        lx += sum * pow2i(-ev);
+        if constexpr (F16) l += (sum8(ph[0]) + sum8(ph[1])) * pow2i(-ev);
 #pragma unroll
         for (int d = 0; d < ND; d++)
 #pragma unroll
@@ -357,7 +371,8 @@ __global__ __launch_bounds__(WG) void kv8_rows_kernel(Kv8AttnArgs a) {
         if (u + NW < u1) load_v(u + NW);
     }
     // the four waves' results in LDS; their weights once per row, then the sum
-    l = col_sum(l);
+    lx = col_sum(lx);
+    l = F16 ? col_sum(l) : lx;
     if constexpr (MODE == ROWS_PACK)
 #pragma unroll
         for (int d = 0; d < ND; d++)
@@ -370,18 +385,20 @@ __global__ __launch_bounds__(WG) void kv8_rows_kernel(Kv8AttnArgs a) {
         if (g == 0) {
             sm[wave][c] = m;
             sl[wave][c] = l;
+            sx[wave][c] = lx;
         }
     }
     __syncthreads();
     const int r = tid / TPR, gr = rt * R + r;  // TPR threads a row from here on
     if (gr >= rows) return;
-    float M = NEG, W[NW], L = 0.f;
+    float M = NEG, W[NW], L = 0.f, X = 0.f;
 #pragma unroll
     for (int w = 0; w < NW; w++) M = fmaxf(M, sm[w][r]);
 #pragma unroll
     for (int w = 0; w < NW; w++) {
         W[w] = ex2(sm[w][r] - M);
         L += sl[w][r] * W[w];
+        X += sx[w][r] * W[w];
     }
     const size_t id = row_id(a, gr, kvh);
     const bool last = a.splits == 1;
@@ -404,8 +421,8 @@ __global__ __launch_bounds__(WG) void kv8_rows_kernel(Kv8AttnArgs a) {
         }
     }
     if (tid % TPR == 0) {
-        a.ml[id * a.splits + split] = make_float2(M, L);
-        if (last && a.norm) a.norm[id] = make_float2(M, 32768.f / L);
+        a.ml[id * a.splits + split] = make_float4(M, L, X, 0.f);
+        if (last && a.norm) a.norm[id] = make_float2(M, 32768.f / X);
     }
 }
 
@@ -419,7 +436,7 @@ struct MergeLds {
     static constexpr int LPR = HD / 4, MS = MW / LPR;  // lanes of a row, splits at a time
     float wt[KV8_MAX_SPLITS];
     __attribute__((aligned(16))) float red[MS][HD];
-    float wmax[MW / WAVE], wsum[MW / WAVE];
+    float wmax[MW / WAVE], wsum[MW / WAVE], wsumx[MW / WAVE];
 };
 template <int HD, bool F16>
 __device__ __forceinline__ void merge_row(const Kv8AttnArgs &a, int token, int head, MergeLds<HD> &lds) {
@@ -428,11 +445,11 @@ __device__ __forceinline__ void merge_row(const Kv8AttnArgs &a, int token, int h
     const size_t id = (size_t)token * a.n_heads + head;
     const int col = tid % LPR, s0 = tid / LPR;
     const float *pt = a.part + id * S * HD + 4 * col;
-    const float2 *ml = a.ml + id * S;
+    const float4 *ml = a.ml + id * S;
     f32x4 pre[MPRE];
-    float2 mine[2];
+    float4 mine[2];
 #pragma unroll
-    for (int k = 0; k < 2; k++) mine[k] = tid + k * MW < S ? ml[tid + k * MW] : make_float2(NEG, 0.f);
+    for (int k = 0; k < 2; k++) mine[k] = tid + k * MW < S ? ml[tid + k * MW] : make_float4(NEG, 0.f, 0.f, 0.f);
 #pragma unroll
     for (int k = 0; k < MPRE; k++) {
         const int s = s0 + k * MS;
@@ -444,19 +461,27 @@ __device__ __forceinline__ void merge_row(const Kv8AttnArgs &a, int token, int h
     float M = lds.wmax[0];
 #pragma unroll
     for (int w = 1; w < MW / WAVE; w++) M = fmaxf(M, lds.wmax[w]);
-    float L = 0.f;
+    float L = 0.f, X = 0.f;
 #pragma unroll
     for (int k = 0; k < 2; k++) {
         const float f = ex2(mine[k].x - M);
         if (tid + k * MW < S) lds.wt[tid + k * MW] = f;
         L += mine[k].y * f;
+        X += mine[k].z * f;
     }
     L = wave_sum(L);
-    if (lane == 0) lds.wsum[wave] = L;
+    X = wave_sum(X);
+    if (lane == 0) {
+        lds.wsum[wave] = L;
+        lds.wsumx[wave] = X;
+    }
     __syncthreads();
-    L = 0.f;
+    L = X = 0.f;
 #pragma unroll
-    for (int w = 0; w < MW / WAVE; w++) L += lds.wsum[w];
+    for (int w = 0; w < MW / WAVE; w++) {
+        L += lds.wsum[w];
+        X += lds.wsumx[w];
+    }
     f32x4 y = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll
     for (int k = 0; k < MPRE; k++)
@@ -474,7 +499,7 @@ __device__ __forceinline__ void merge_row(const Kv8AttnArgs &a, int token, int h
         if constexpr (F16) ((uint16_t *)a.out)[at] = f2h(v);
         else ((float *)a.out)[at] = v;
     }
-    if (tid == 0 && a.norm) a.norm[id] = make_float2(M, 32768.f / L);
+    if (tid == 0 && a.norm) a.norm[id] = make_float2(M, 32768.f / X);
 }
 template <int HD, bool F16>
 __global__ __launch_bounds__(MW) void kv8_merge_kernel(Kv8AttnArgs a) {
@@ -491,14 +516,15 @@ __global__ __launch_bounds__(WG) void kv8_merge_many_kernel(Kv8AttnArgs a) {
     const int h = blockIdx.x * RPW + threadIdx.x / LPR, d = threadIdx.x % LPR * 4, S = a.splits;
     if (h >= a.n_heads) return;
     const size_t id = (size_t)blockIdx.y * a.n_heads + h;
-    const float2 *ml = a.ml + id * S;
+    const float4 *ml = a.ml + id * S;
     const float *pt = a.part + id * S * HD + d;
-    float M = NEG, L = 0.f;
+    float M = NEG, L = 0.f, X = 0.f;
     f32x4 y = {0.f, 0.f, 0.f, 0.f};
     for (int s = 0; s < S; s++) M = fmaxf(M, ml[s].x);
     for (int s = 0; s < S; s++) {
         const float f = ex2(ml[s].x - M);
         L += ml[s].y * f;
+        X += ml[s].z * f;
         y += *(const f32x4 *)(pt + (size_t)s * HD) * f;
     }
     y *= 1.f / L;
@@ -508,7 +534,7 @@ __global__ __launch_bounds__(WG) void kv8_merge_many_kernel(Kv8AttnArgs a) {
             u32x2{f2h(y[0]) | (uint32_t)f2h(y[1]) << 16, f2h(y[2]) | (uint32_t)f2h(y[3]) << 16};
     else
         *(f32x4 *)((float *)a.out + at) = y;
-    if (d == 0 && a.norm) a.norm[id] = make_float2(M, 32768.f / L);
+    if (d == 0 && a.norm) a.norm[id] = make_float2(M, 32768.f / X);
 }
 
 // ------------------------------------------------------------- prompts --
@@ -617,7 +643,7 @@ struct Stage {
 // maximum rises by more than 2^7: their weights then reach 2^15 at most, from 2^8
 // (a weight keeps its bits down to 2^-22 of the largest and is lost below 2^-33,
 // 2^17 of which are below the output's rounding).
-template <int HD, bool F16, int NW, int DS>
+template <int HD, bool F16, int NW, int DS, bool NORM>
 __global__ __launch_bounds__(NW *WAVE, HD == 128 ? 2 : 1) void kv8_prompt_kernel(Kv8AttnArgs a) {
     constexpr int NF = HD / 16, DT = HD / 32 / DS, R = 32 * NW / DS;
     constexpr bool AHEAD = HD == 128;  // registers left to request operands from LDS ahead of their use
@@ -640,7 +666,7 @@ __global__ __launch_bounds__(NW *WAVE, HD == 128 ? 2 : 1) void kv8_prompt_kernel
     const int8_t *ke = a.c.ke + (size_t)kvh * (a.c.cap >> a.c.lb);
     const int8_t *ve = a.c.ve + (size_t)kvh * (a.c.cap >> a.c.lb);
     const float scale = fabsf(a.scale);
-    float m = NEG, l = 0.f;
+    float m = NEG, l = 0.f, lx = 0.f;  // lx: of the weights before their rounding to f16 (f32 rows, and NORM)
     f32x16 o[DT];
 #pragma unroll
     for (int d = 0; d < DT; d++)
@@ -706,6 +732,7 @@ __global__ __launch_bounds__(NW *WAVE, HD == 128 ? 2 : 1) void kv8_prompt_kernel
                     const float m1 = fmaxf(m, ceilf(top)), alpha = ex2(m - m1);
                     m = m1;
                     l *= alpha;
+                    lx *= alpha;
 #pragma unroll
                     for (int d = 0; d < DT; d++)
 #pragma unroll
@@ -723,7 +750,9 @@ __global__ __launch_bounds__(NW *WAVE, HD == 128 ? 2 : 1) void kv8_prompt_kernel
                         ph[b][i] = t;
                         if constexpr (!F16) pl[b][i] = (_Float16)(p - (float)t);
                     }
-                    l = fmaf(sum, pow2i(-(int)ev[2 * x + b]), l);
+                    const float un = pow2i(-(int)ev[2 * x + b]);
+                    if constexpr (F16) l = fmaf(sum8(ph[b]), un, l);
+                    if constexpr (!F16 || NORM) lx = fmaf(sum, un, lx);
                 }
                 if constexpr (AHEAD)
                     if (x == 0) {
@@ -744,7 +773,8 @@ __global__ __launch_bounds__(NW *WAVE, HD == 128 ? 2 : 1) void kv8_prompt_kernel
         __syncthreads();
     }
     constexpr float UP = F16 ? 128.f : 1.f;  // 2^(PSCALE - PS): results leave at 2^15 as from the other kernel
-    l = half_reduce(l, [](float x, float y) { return x + y; }) * UP;
+    lx = half_reduce(lx, [](float x, float y) { return x + y; }) * UP;
+    l = F16 ? half_reduce(l, [](float x, float y) { return x + y; }) * UP : lx;
     if (r >= rows) return;
     const size_t id = row_id(a, r, kvh);
     const bool last = a.splits == 1;
@@ -765,8 +795,8 @@ __global__ __launch_bounds__(NW *WAVE, HD == 128 ? 2 : 1) void kv8_prompt_kernel
                 *(f32x4 *)((float *)a.out + to + dim) = y;
         }
     if (h == 0 && d0 == 0) {
-        if (!last) a.ml[id * a.splits + split] = make_float2(m, l);
-        else if (a.norm) a.norm[id] = make_float2(m, 32768.f / l);
+        if (!last) a.ml[id * a.splits + split] = make_float4(m, l, lx, 0.f);
+        else if (NORM) a.norm[id] = make_float2(m, 32768.f / lx);
     }
 }
 
@@ -800,12 +830,12 @@ __global__ __launch_bounds__(MW) void kv8_mass_few_kernel(Kv8AttnArgs a, int mer
     const int units = (end + T - 1) / T, step = (gridDim.x - merges) / a.c.n_kv * NW;
     // the rows' m and 1 / l (the weights' 2^15 is in both): a wave per row over its splits
     for (int r = wave; r < rows; r += NW) {
-        const float2 *ml = a.ml + row_id(a, r, kvh) * a.splits;
+        const float4 *ml = a.ml + row_id(a, r, kvh) * a.splits;
         float M = NEG, L = 0.f;
         for (int s = lane; s < a.splits; s += WAVE) {
-            const float2 x = ml[s];
+            const float4 x = ml[s];
             const float m1 = fmaxf(M, x.x);
-            L = L * ex2(M - m1) + x.y * ex2(x.x - m1);
+            L = L * ex2(M - m1) + x.z * ex2(x.x - m1);
             M = m1;
         }
         const float all = wave_max_all(M);
@@ -1070,7 +1100,7 @@ size_t kv8_attn_workspace(int n_heads, int group, int n, int end, int hd, int sp
     const size_t saved = mass && kv8_attn_saves(group, n) ? rows * units * T + (rows * units + 3) / 4 * 4 : 0;
     const int n_kv = n_heads / group, ms = mass && !kv8_attn_saves(group, n) ? kv8_mass_splits(n_kv, group, n, end, hd) : 1;
     const size_t sums = ms > 1 ? (size_t)ms * n_kv * end : 0;
-    return (saved + rows * ((splits > 1 ? (size_t)splits * hd : 0) + 2 * (size_t)splits + 2) + sums) * 4;
+    return (saved + rows * ((splits > 1 ? (size_t)splits * hd : 0) + 4 * (size_t)splits + 2) + sums) * 4;
 }
 
 namespace {
@@ -1090,9 +1120,15 @@ void launch(const Kv8AttnArgs &a, hipStream_t st) {
         const PromptPlan p = prompt_plan(HD, F16, a.c.n_kv, rows);
         const dim3 grid((unsigned)a.c.n_kv, (unsigned)((rows + p.rows - 1) / p.rows), (unsigned)a.splits);
         auto go = [&](auto kernel) { hipLaunchKernelGGL(kernel, grid, dim3((unsigned)(p.waves * WAVE)), 0, st, a); };
-        if constexpr (HD == 128) p.waves == 8 ? go(kv8_prompt_kernel<HD, F16, 8, 1>) : go(kv8_prompt_kernel<HD, F16, 4, 1>);
-        else if constexpr (F16) go(kv8_prompt_kernel<HD, F16, 8, 2>);
-        else go(kv8_prompt_kernel<HD, F16, 4, 1>);
+        auto by_norm = [&](auto norm) {
+            constexpr bool N = decltype(norm)::value;
+            if constexpr (HD == 128)
+                p.waves == 8 ? go(kv8_prompt_kernel<HD, F16, 8, 1, N>) : go(kv8_prompt_kernel<HD, F16, 4, 1, N>);
+            else if constexpr (F16) go(kv8_prompt_kernel<HD, F16, 8, 2, N>);
+            else go(kv8_prompt_kernel<HD, F16, 4, 1, N>);
+        };
+        if (a.norm) by_norm(std::integral_constant<bool, true>{});
+        else by_norm(std::integral_constant<bool, false>{});
     }
     if (a.save) {
         const int merges = a.splits > 1 ? a.n * a.n_heads : 0;
