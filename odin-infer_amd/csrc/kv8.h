@@ -56,7 +56,7 @@ struct Kv8AttnArgs {
     float *part;          // [n * n_heads][splits][hd], where splits > 1: the splits' o
     float4 *ml;           // [n * n_heads][splits]: their m, l of the products' weights, l of the exact ones
     float2 *norm;         // [n * n_heads], where mass is set: m and 2^15 / l of a row
-    // few rows with mass: every weight as it was formed [n_kv][save_units][rows][64]
+    // few rows with mass: every weight as it was formed [n_kv][save_units][4][rows][16]
     // and its row's maximum then [n_kv][save_units][rows]; null otherwise
     float *save, *save_m;
     int32_t save_units, splits;

@@ -411,13 +411,13 @@ __global__ __launch_bounds__(EV) void kv8_select_kernel(Kv8EvictArgs a) {
 // `kept`, brought to the exponent that their new block needs (a left shift is
 // exact, a right shift rounds half to even; most need none), from registers to
 // registers.  K rows are read where they lie, 16 bytes a thread.  Of V a slot is a
-// byte column: a thread reads four slots' bytes of a dimension, a workgroup 64
-// slots of it, which lie in a few neighbouring 64-byte rows (tiles brought through
-// LDS whole took 49 us against 20 for 8192 of 40960 slots: 45 KB a workgroup).
-// Bound by memory: K reads what is kept, V every row that holds a kept slot.
+// byte column: the lanes of a wave are the 64 slots of one dimension, which lie in
+// a few neighbouring 64-byte rows.  Bound by memory: K reads what is kept, V every
+// row that holds a kept slot.  21 us for 8192 of 40960 slots of 8 heads of 128
+// (with V's tiles brought through LDS 49, four dimensions a wave 27).
 template <int HD>
 __global__ __launch_bounds__(WG) void kv8_gather_kernel(Kv8EvictArgs a) {
-    constexpr int PPR = HD / 16, NP = T * PPR / WG, NV = HD / 16;  // K: 16-byte pieces of a row, of a thread; V: words
+    constexpr int PPR = HD / 16, NP = T * PPR / WG, NV = HD * T / WG;  // K: 16-byte pieces of a row, of a thread; V: bytes of a thread
     __shared__ int slot[T], es[T], mx[T], be[4], up[T];
     const int tid = threadIdx.x;
     const int unit = blockIdx.x, kvh = blockIdx.y, which = blockIdx.z, n = min(T, a.keep - unit * T);
@@ -435,8 +435,8 @@ __global__ __launch_bounds__(WG) void kv8_gather_kernel(Kv8EvictArgs a) {
     }
     __syncthreads();
     u32x4 w[NP];
-    uint32_t v[NV];
-    const int vr = 4 * (tid % 16), vd = tid / 16;  // V: my four slots, my first dimension
+    int8_t v[NV];
+    const int vr = tid % T, vd = tid / T;  // V: my slot, my first dimension
     if (which == 0) {
 #pragma unroll
         for (int k = 0; k < NP; k++) {
@@ -453,27 +453,14 @@ __global__ __launch_bounds__(WG) void kv8_gather_kernel(Kv8EvictArgs a) {
             atomicMax(&mx[(tid + k * WG) / PPR], x);
         }
     } else {
-        const int8_t *from[4];
+        const int s = slot[vr];
+        const int8_t *from = a.src.vc + ((size_t)kvh * a.src.cap + (s & ~(T - 1))) * HD + vd * T + (s & (T - 1));
 #pragma unroll
-        for (int j = 0; j < 4; j++) {
-            const int s = slot[vr + j];
-            from[j] = a.src.vc + ((size_t)kvh * a.src.cap + (s & ~(T - 1))) * HD + vd * T + (s & (T - 1));
-        }
-        int8_t b[NV][4];
+        for (int k = 0; k < NV; k++) v[k] = from[k * (WG / T) * T];
+        int big = 0;
 #pragma unroll
-        for (int k = 0; k < NV; k++)
-#pragma unroll
-            for (int j = 0; j < 4; j++) b[k][j] = from[j][k * 16 * T];
-        int big[4] = {0, 0, 0, 0};
-#pragma unroll
-        for (int k = 0; k < NV; k++) {
-            v[k] = pack4(b[k][0], b[k][1], b[k][2], b[k][3]);
-#pragma unroll
-            for (int j = 0; j < 4; j++) big[j] = max(big[j], abs((int)b[k][j]));
-        }
-#pragma unroll
-        for (int j = 0; j < 4; j++)
-            if (vr + j < n) atomicMax(&mx[vr + j], big[j]);
+        for (int k = 0; k < NV; k++) big = max(big, abs((int)v[k]));
+        atomicMax(&mx[vr], big);
     }
     __syncthreads();
     const int B = 1 << a.dst.lb;
@@ -503,22 +490,11 @@ __global__ __launch_bounds__(WG) void kv8_gather_kernel(Kv8EvictArgs a) {
         }
         return;
     }
+    if (vr >= n) return;
     int8_t *dst = a.dst.vc + ((size_t)kvh * a.dst.cap + unit * T) * HD + vd * T + vr;
-    const int by[4] = {up[vr], up[vr + 1], up[vr + 2], up[vr + 3]};
-    const bool any = by[0] | by[1] | by[2] | by[3];
+    const int by = up[vr];
 #pragma unroll
-    for (int k = 0; k < NV; k++) {
-        if (any)
-            v[k] = pack4(moved(byte_of(v[k], 0), by[0]), moved(byte_of(v[k], 1), by[1]), moved(byte_of(v[k], 2), by[2]),
-                         moved(byte_of(v[k], 3), by[3]));
-        if (vr + 4 <= n) {
-            *(uint32_t *)(dst + k * 16 * T) = v[k];
-        } else {
-#pragma unroll
-            for (int j = 0; j < 4; j++)
-                if (vr + j < n) dst[k * 16 * T + j] = (int8_t)byte_of(v[k], j);
-        }
-    }
+    for (int k = 0; k < NV; k++) dst[k * (WG / T) * T] = (int8_t)(by ? moved(v[k], by) : v[k]);
 }
 
 }  // namespace

@@ -337,13 +337,15 @@ __global__ __launch_bounds__(WG) void kv8_rows_kernel(Kv8AttnArgs a) {
                 ph[t / 2][4 * (t & 1) + i] = h;
                 if constexpr (!F16) pl[t / 2][4 * (t & 1) + i] = (_Float16)(p - (float)h);
             }
-        if constexpr (SAVE) {  // weights without V's exponent, for the mass, and the maximum that they go by
-            const size_t at = ((size_t)kvh * a.save_units + u) * rows + c;
+        if constexpr (SAVE) {
+            // weights without V's exponent, for the mass, and the maximum that they go by; slot
+            // 16 g + 4 t + i of a row at 16 (t rows + row) + 4 g + i: each store is contiguous
+            const size_t at = ((size_t)kvh * a.save_units + u) * rows;
             const float un = pow2i(-ev);
             if (c < min(R, rows)) {
 #pragma unroll
-                for (int t = 0; t < 4; t++) *(f32x4 *)(a.save + at * T + 16 * g + 4 * t) = w[t] * un;
-                if (g == 0) a.save_m[at] = m1;
+                for (int t = 0; t < 4; t++) *(f32x4 *)(a.save + at * T + 16 * (t * rows + c) + 4 * g) = w[t] * un;
+                if (g == 0) a.save_m[at + c] = m1;
             }
         }
         if constexpr (MODE == ROWS_PACK) {
@@ -848,14 +850,14 @@ __global__ __launch_bounds__(MW) void kv8_mass_few_kernel(Kv8AttnArgs a, int mer
     for (int u = nth * NW + wave; u < units; u += step) {
         const size_t from = ((size_t)kvh * a.save_units + u) * rows;
         const int s = u * T + lane;
-        const float *w = a.save + from * T + lane;
+        const float *w = a.save + from * T + 16 * ((lane >> 2 & 3) * rows) + 4 * (lane >> 4) + (lane & 3);
         const float had = s < past ? mass[s] : 0.f;
         const float f = ex2(a.save_m[from + min(lane, rows - 1)] - norm.x) * norm.y;  // lane r: of row r
         float sum = 0.f;
         for (int r0 = 0; r0 < rows; r0 += AHEAD) {
             float x[AHEAD];
 #pragma unroll
-            for (int i = 0; i < AHEAD; i++) x[i] = w[min(r0 + i, rows - 1) * T];
+            for (int i = 0; i < AHEAD; i++) x[i] = w[min(r0 + i, rows - 1) * 16];
 #pragma unroll
             for (int i = 0; i < AHEAD; i++)
                 if (r0 + i < rows) sum = fmaf(x[i], lane_value(f, r0 + i), sum);
