@@ -1062,8 +1062,8 @@ int kv8_attn_splits(int n_kv, int group, int n, int end, int hd, bool f16) {
     const int64_t units = (end + T - 1) / T, rows = (int64_t)n * group;
     if (n > 65535) return 1;  // the merge's grid
     if (rows <= FEW_ROWS) {
-        // a unit per wave, up to two workgroups a CU
-        const int64_t tiles = (rows + 15) / 16 * n_kv, most = (2 * CUS + tiles - 1) / tiles;
+        // a unit per wave, up to two workgroups a CU (one for head_dim 256, whose registers leave room for one)
+        const int64_t tiles = (rows + 15) / 16 * n_kv, room = hd == 128 ? 2 * CUS : CUS, most = (room + tiles - 1) / tiles;
         return (int)std::max<int64_t>(1, std::min((units + 3) / 4, most));
     }
     // The least of rounds * (units of a split + 3 for its beginning and end) + the
