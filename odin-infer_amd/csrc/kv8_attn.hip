@@ -510,7 +510,8 @@ __global__ __launch_bounds__(MW) void kv8_merge_kernel(Kv8AttnArgs a) {
 }
 
 // Merge of a few splits of many rows: four dimensions a thread, WG * 4 / HD rows a
-// workgroup (a workgroup per row took 30 us for two splits of 16000 rows).
+// workgroup (a workgroup per row took 30 us for two splits of 16000 rows, this 9;
+// for 11 splits of 768 rows it is the other way, 5 us against 8).
 constexpr int MERGE_FEW = 16;
 template <int HD, bool F16>
 __global__ __launch_bounds__(WG) void kv8_merge_many_kernel(Kv8AttnArgs a) {
@@ -1042,13 +1043,24 @@ __global__ __launch_bounds__(WG) void kv8_mass_sum_kernel(Kv8AttnArgs a, int spl
 
 }  // namespace
 
-// Up to FEW_ROWS rows of a kv head go by 16 (kv8_rows_kernel), more to the prompt
-// kernel: workgroups of 8 waves where they fill the card's 256 CUs (a unit is
-// converted for 256 rows at a time), of 4 waves, two to a CU, otherwise; for
-// head_dim 256 the registers of f16 rows allow 8 waves in pairs that share 32 rows
-// and hold half of the dimensions each, those of f32 rows 4 waves.
-constexpr int FEW_ROWS = 64, CUS = 256;
+constexpr int CUS = 256;
 
+// Whether rows go by 16 over many splits (kv8_rows_kernel) or by 128 and 256 with
+// units converted once for all of them (kv8_prompt_kernel).  Always the former
+// where a tile of rows is all; else up to 512 rows while tiles of 16 rows x units
+// stay below a bound, both measured at 24 to 480 rows and 500 to 30000 slots:
+//   head_dim 128  f32 20000: 45 us against 49, 37700: 90 / 70
+//                 f16  7500: 23 / 26 (24 rows), 3960: 22 / 25 (240), 3020: 20 / 17 (96), 20000: 40 / 33
+//   head_dim 256  f32  3840: 43 / 55   f16 1020: 21 / 26, 1510: 27 / 25, 2810: 38 / 24
+static bool by_sixteen(int hd, bool f16, int n_kv, int64_t rows, int64_t units) {
+    const int64_t most = hd == 128 ? (f16 ? 8000 : 24000) : (f16 ? 2000 : 5000);
+    return rows <= 16 || (rows <= 512 && (rows + 15) / 16 * n_kv * units <= most);
+}
+
+// The prompt kernel's workgroups: 8 waves where they fill the card's CUs (a unit is
+// converted for 256 rows at a time), 4 waves, two to a CU, otherwise; for head_dim
+// 256 the registers of f16 rows allow 8 waves in pairs that share 32 rows and hold
+// half of the dimensions each, those of f32 rows 4 waves.
 struct PromptPlan {
     int waves, rows, resident;  // of a workgroup; workgroups at a time
 };
@@ -1061,7 +1073,7 @@ static PromptPlan prompt_plan(int hd, bool f16, int n_kv, int64_t rows) {
 int kv8_attn_splits(int n_kv, int group, int n, int end, int hd, bool f16) {
     const int64_t units = (end + T - 1) / T, rows = (int64_t)n * group;
     if (n > 65535) return 1;  // the merge's grid
-    if (rows <= FEW_ROWS) {
+    if (by_sixteen(hd, f16, n_kv, rows, units)) {
         // a unit per wave, up to two workgroups a CU (one for head_dim 256, whose registers leave room for one)
         const int64_t tiles = (rows + 15) / 16 * n_kv, room = hd == 128 ? 2 * CUS : CUS, most = (room + tiles - 1) / tiles;
         return (int)std::max<int64_t>(1, std::min((units + 3) / 4, most));
@@ -1074,7 +1086,7 @@ int kv8_attn_splits(int n_kv, int group, int n, int end, int hd, bool f16) {
     const double merge = (double)rows * n_kv * hd * 8 / 5e6 / 2.7;
     int best = 1;
     double least = 1e30;
-    for (int64_t s = 1; s <= 64 && s <= (units + 1) / 2; s++) {
+    for (int64_t s = 1; s <= 256 && s <= (units + 1) / 2; s++) {
         const double c = (double)((tiles * s + p.resident - 1) / p.resident) * ((double)units / s + 3) +
                          (s > 1 ? 2 + merge * s : 0);
         if (c < least) {
@@ -1114,11 +1126,11 @@ void launch(const Kv8AttnArgs &a, hipStream_t st) {
     const int rows = a.n * a.group;
     const int end = a.past.dev ? a.c.cap : a.past.past + a.n, units = (end + T - 1) / T;
     const dim3 merge_grid((unsigned)a.n_heads, (unsigned)a.n);
-    if (rows <= FEW_ROWS) {
+    if (by_sixteen(HD, F16, a.c.n_kv, rows, units)) {
         const dim3 grid((unsigned)a.c.n_kv, (unsigned)((rows + R - 1) / R), (unsigned)a.splits);
         if (a.save) hipLaunchKernelGGL((kv8_rows_kernel<HD, MODE, true>), grid, dim3(WG), 0, st, a);
         else hipLaunchKernelGGL((kv8_rows_kernel<HD, MODE, false>), grid, dim3(WG), 0, st, a);
-    } else if constexpr (MODE != ROWS_PACK) {
+    } else if constexpr (MODE != ROWS_PACK) {  // (at most 8 rows always go by 16)
         const PromptPlan p = prompt_plan(HD, F16, a.c.n_kv, rows);
         const dim3 grid((unsigned)a.c.n_kv, (unsigned)((rows + p.rows - 1) / p.rows), (unsigned)a.splits);
         auto go = [&](auto kernel) { hipLaunchKernelGGL(kernel, grid, dim3((unsigned)(p.waves * WAVE)), 0, st, a); };
@@ -1138,7 +1150,7 @@ void launch(const Kv8AttnArgs &a, hipStream_t st) {
         hipLaunchKernelGGL((kv8_mass_few_kernel<HD, F16>), dim3((unsigned)(merges + wgs)), dim3(MW), 0, st, a, merges);
         return;
     }
-    if (a.splits > 1 && a.splits <= MERGE_FEW && rows > FEW_ROWS) {
+    if (a.splits > 1 && a.splits <= MERGE_FEW && a.n * a.n_heads >= (a.splits <= 4 ? 512 : 4096)) {
         constexpr int RPW = WG * 4 / HD;
         hipLaunchKernelGGL((kv8_merge_many_kernel<HD, F16>),
                            dim3((unsigned)((a.n_heads + RPW - 1) / RPW), (unsigned)a.n), dim3(WG), 0, st, a);
