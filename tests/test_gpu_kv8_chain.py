@@ -250,3 +250,65 @@ def test_captured_eviction():
             torch.cuda.synchronize()
             results.append([x.clone() for x in (buf, mass, out, dbuf, dmass, kept)])
         assert all(torch.equal(a, b) for a, b in zip(*results)), i
+
+
+@pytest.mark.parametrize("t", [F32, F16])
+@pytest.mark.parametrize("n_heads,n_kv,hd,block,n,past", [
+    (8, 1, 128, 16, 90, 37),      # 720 rows, five and a half workgroups' tiles
+    (7, 1, 128, 64, 75, 0),       # 525 rows of groups of 7, nothing before them
+    (16, 2, 128, 32, 65, 1000),   # splits that the first rows see whole and the last in part
+    (8, 1, 256, 16, 66, 200),
+    (12, 2, 256, 64, 100, 0),
+    (16, 1, 256, 32, 40, 1500),
+    (513, 1, 128, 64, 1, 100),    # one token of more heads than go by sixteen
+    (6, 6, 128, 32, 530, 3),      # no sharing
+])
+def test_many_rows(t, n_heads, n_kv, hd, block, n, past):
+    """More than 512 rows of a kv head: the prompt kernel in each of its forms,
+    with the mass, host and device length (other splits)."""
+    rng = np.random.default_rng(n_heads + n + past)
+    end, cap = past + n, (past + n + 63) // 64 * 64 + 640
+    plan, ref, buf = filled(rng, n_kv, hd, cap, block, end)
+    q = (1.5 * rng.standard_normal((n, n_heads, hd))).astype(NP[t])
+    mass0 = rng.random((n_kv, cap)).astype(np.float32)
+    mass0[:, past:] = np.nan
+    want, wmass, A = kv8ref.attend(ref, q, hd ** -0.5, n, past, mass0)
+    vmax = np.abs(ref.values("v", end)).max()
+    plain = attn(plan, buf, q, n, past, t)
+    check(plain, want, A, vmax, t, end)
+    pd = torch.tensor([past], dtype=torch.int32, device="cuda")
+    for dev_past in (None, pd):
+        mass = dev(mass0)
+        got = attn(plan, buf, q, n, past if dev_past is None else -9, t, mass=mass, past_dev=dev_past, pad=8)
+        check(got, want, A, vmax, t, end)
+        m = mass.cpu().numpy().astype(np.float64)
+        assert np.all(np.isnan(m[:, end:]))
+        added = wmass[:, :end] - np.where(np.arange(end) < past, mass0[:, :end].astype(np.float64), 0)
+        tol = 2 * weight_error(A) + 2.0 ** -22 + 2.0 ** -24 * (n * n_heads / n_kv + 4)
+        assert np.all(np.abs(m[:, :end] - wmass[:, :end]) <= tol * added + 2.0 ** -23 * wmass[:, :end] + 1e-30)
+    same_bytes(ref, buf)
+
+
+@pytest.mark.parametrize("t", [F32, F16])
+def test_many_rows_extremes(t):
+    """Rows of zero, of infinity and of NaN, blocks of very different size, a
+    negative scale: in the prompt kernel."""
+    rng = np.random.default_rng(81)
+    n, heads, past = 70, 8, 150
+    plan, ref, _ = filled(rng, 1, 128, 256, 16, 220)
+    ref.ve[0] = rng.integers(-14, 7, ref.ve.shape[1])
+    ref.ke[0] = rng.integers(-12, -4, ref.ke.shape[1])
+    buf = dev(ref.buf)
+    q = rng.standard_normal((n, heads, 128)).astype(NP[t])
+    q[0] = 0
+    q[1] *= NP[t](1e-6)
+    q[2] *= NP[t](100)
+    clean = q.copy()
+    q[3, 0, 7] = np.inf
+    q[4, 1, 9] = np.nan
+    want, _, A = kv8ref.attend(ref, clean, -0.1, n, past)
+    got = attn(plan, buf, q, n, past, t, scale=-0.1)
+    assert np.all(np.isnan(got[4, 1])) and not np.any(np.isfinite(got[3, 0]))
+    ok = np.ones((n, heads), bool)
+    ok[3, 0] = ok[4, 1] = False
+    check(got[ok], want[ok], A, np.abs(ref.values("v", 220)).max(), t, 220)
