@@ -238,7 +238,13 @@ __device__ __forceinline__ size_t row_id(const Kv8AttnArgs &a, int r, int kvh) {
 // weights the lane supplies to the second product: nothing crosses lanes but
 // the row maximum.  K and V go from memory to the operand registers without
 // LDS, 16 bytes a lane; K of the next unit is requested when this unit's scores
-// are done, V when its product is.  The waves' results meet in LDS.
+// are done, V when its product is.  The waves' results meet in LDS.  The running
+// maximum is raised to whole numbers: the rescaling is exact then, and so is the
+// sum of V's exponent, the maximum and the offset in front of the exponential.
+// Long caches are bound by memory: 100004 slots of 4 kv heads of 128 (102 MB)
+// 22 us, where a read of that size by itself takes about 6.5 us + bytes / 7 TB/s;
+// short ones by one wave's chain of loads, products and the merge: 1031 slots
+// 7 us.  SAVE (26 us) leaves the weights for the mass.
 template <int HD, int MODE, bool SAVE>
 __global__ __launch_bounds__(WG) void kv8_rows_kernel(Kv8AttnArgs a) {
     constexpr int NW = WG / WAVE, NK = HD / 64, ND = HD / 16, PD = HD + 4, R = tile_rows(MODE), TPR = WG / R;
@@ -645,7 +651,13 @@ struct Stage {
 // 32x32x16 products, for half a unit at a time.  f16 rows rescale o only when a
 // maximum rises by more than 2^7: their weights then reach 2^15 at most, from 2^8
 // (a weight keeps its bits down to 2^-22 of the largest and is lost below 2^-33,
-// 2^17 of which are below the output's rounding).
+// 2^17 of which are below the output's rounding).  2047 tokens of 32 heads of 128
+// over 8 at 8048 slots: 282 us in f16 (836 TFLOP/s), 450 in f32 (twice the
+// products).  Vector instructions fill 61% of its cycles (softmax, and the bytes'
+// conversion for 256 rows), the matrix units 44%, at the 1.7 GHz that the card
+// holds under them.  Measured and not kept: 64 rows a wave (one wave a SIMD, 428);
+// the waves of a SIMD half a unit apart with three buffers (311); a raised wave
+// priority around the products (f16 the same, f32 600).
 template <int HD, bool F16, int NW, int DS, bool NORM>
 __global__ __launch_bounds__(NW *WAVE, HD == 128 ? 2 : 1) void kv8_prompt_kernel(Kv8AttnArgs a) {
     constexpr int NF = HD / 16, DT = HD / 32 / DS, R = 32 * NW / DS;
@@ -873,7 +885,9 @@ __global__ __launch_bounds__(MW) void kv8_mass_few_kernel(Kv8AttnArgs a, int mer
 // the end they cross the lanes and meet, two waves a slot, in LDS.  Where slots are
 // too few to fill the card, the rows are split over workgroups too, whose sums a
 // second launch adds (1000 rows of 16 heads of 2 kv heads at 5000 slots, head_dim
-// 256: 168 us in one split, 96 in three).
+// 256: 168 us in one split, 96 in three).  2047 tokens of 32 heads at 8048 slots:
+// 193 us, 610 TFLOP/s; 56% of its cycles are vector instructions (an exponential
+// and two multiply-adds a score), 31% the matrix units.
 template <int HD, bool F16, int X>
 __global__ __launch_bounds__(WG, 2) void kv8_mass_kernel(Kv8AttnArgs a) {
     constexpr int NF = HD / 16, QR = 64, PC = F16 ? 1 : 2, TPR = WG / QR, EL = HD / TPR, WS = 32 * X, GS = 2 * WS;
