@@ -154,10 +154,7 @@ int oi_kv8_read_launch(const oi_kv8_dims *d, const void *cache, int32_t slot0, i
 
 int64_t oi_kv8_attn_workspace_bytes(const oi_kv8_dims *d, int32_t n_heads, int32_t n) {
     if (!dims_ok(d) || n_heads <= 0 || n_heads > 4096 || n_heads % d->n_kv_heads || n <= 0 || n > d->capacity) return 0;
-    const int group = n_heads / d->n_kv_heads;
-    const int s = std::max(kv8_attn_splits(d->n_kv_heads, group, n, d->capacity, d->head_dim, false),
-                           kv8_attn_splits(d->n_kv_heads, group, n, d->capacity, d->head_dim, true));
-    return (int64_t)kv8_attn_workspace(n_heads, group, n, d->capacity, d->head_dim, s, true);
+    return (int64_t)kv8_attn_workspace_most(n_heads, n_heads / d->n_kv_heads, n, d->capacity, d->head_dim);
 }
 
 int oi_kv8_attn_launch(const oi_kv8_dims *d, const void *cache, int32_t n_heads, int32_t type, const void *q,

@@ -69,6 +69,7 @@ int kv8_attn_splits(int n_kv, int group, int n, int end, int hd, bool f16);
 bool kv8_attn_saves(int group, int n);
 int kv8_mass_splits(int n_kv, int group, int n, int end, int hd);
 size_t kv8_attn_workspace(int n_heads, int group, int n, int end, int hd, int splits, bool mass);
+size_t kv8_attn_workspace_most(int n_heads, int group, int n, int cap, int hd);  // at any length, with mass
 hipError_t launch_kv8_attn(const Kv8AttnArgs &a, hipStream_t st);
 
 struct Kv8EvictArgs {

@@ -1066,9 +1066,9 @@ constexpr int CUS = 256;
 //   head_dim 128  f32 20000: 45 us against 49, 37700: 90 / 70
 //                 f16  7500: 23 / 26 (24 rows), 3960: 22 / 25 (240), 3020: 20 / 17 (96), 20000: 40 / 33
 //   head_dim 256  f32  3840: 43 / 55   f16 1020: 21 / 26, 1510: 27 / 25, 2810: 38 / 24
+static int64_t most_by_sixteen(int hd, bool f16) { return hd == 128 ? (f16 ? 8000 : 24000) : (f16 ? 2000 : 5000); }
 static bool by_sixteen(int hd, bool f16, int n_kv, int64_t rows, int64_t units) {
-    const int64_t most = hd == 128 ? (f16 ? 8000 : 24000) : (f16 ? 2000 : 5000);
-    return rows <= 16 || (rows <= 512 && (rows + 15) / 16 * n_kv * units <= most);
+    return rows <= 16 || (rows <= 512 && (rows + 15) / 16 * n_kv * units <= most_by_sixteen(hd, f16));
 }
 
 // The prompt kernel's workgroups: 8 waves where they fill the card's CUs (a unit is
@@ -1129,6 +1129,31 @@ size_t kv8_attn_workspace(int n_heads, int group, int n, int end, int hd, int sp
     const int n_kv = n_heads / group, ms = mass && !kv8_attn_saves(group, n) ? kv8_mass_splits(n_kv, group, n, end, hd) : 1;
     const size_t sums = ms > 1 ? (size_t)ms * n_kv * end : 0;
     return (saved + rows * ((splits > 1 ? (size_t)splits * hd : 0) + 4 * (size_t)splits + 2) + sums) * 4;
+}
+
+// What a call of n tokens may need at any length up to the capacity.  The splits over
+// the slots grow with the length in either form (more units to share out), but may
+// fall where the form changes; the mass's row splits fall as its slots fill the card,
+// in steps, just before which their sums take the most.
+size_t kv8_attn_workspace_most(int n_heads, int group, int n, int cap, int hd) {
+    const int n_kv = n_heads / group;
+    const int64_t rows = (int64_t)n * group, units = cap / T;
+    int splits = 1;
+    for (const bool f16 : {false, true}) {
+        splits = std::max(splits, kv8_attn_splits(n_kv, group, n, cap, hd, f16));
+        const int64_t last = std::min(units, most_by_sixteen(hd, f16) / ((rows + 15) / 16 * n_kv));
+        if (last > 0) splits = std::max(splits, kv8_attn_splits(n_kv, group, n, (int)(last * T), hd, f16));
+    }
+    size_t sums = 0;
+    if (!kv8_attn_saves(group, n))
+        for (int64_t end = mass_slots(hd), e = 0; e < cap; end += mass_slots(hd)) {
+            e = std::min<int64_t>(end, cap);
+            const int ms = kv8_mass_splits(n_kv, group, n, (int)e, hd);
+            if (ms == 1) break;  // and at every greater length
+            sums = std::max(sums, (size_t)ms * n_kv * e * 4);
+        }
+    const size_t all = kv8_attn_workspace(n_heads, group, n, cap, hd, splits, true);
+    return std::max(all, kv8_attn_workspace(n_heads, group, n, cap, hd, splits, false) + sums);
 }
 
 namespace {

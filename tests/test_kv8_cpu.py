@@ -3,6 +3,7 @@ the entries refuse (before anything reaches a device), and the properties of the
 format that the header states, on the plain form that the GPU tests compare
 with."""
 import ctypes
+import re
 
 import numpy as np
 import pytest
@@ -96,6 +97,29 @@ def test_attn_refusals():
     assert L.oi_kv8_attn_launch(*a) == E_ARG
     for heads, n in [(3, 1), (0, 1), (4, 0), (4, 257), (-4, 1)]:
         assert L.oi_kv8_attn_workspace_bytes(r, heads, n) == 0
+
+
+@pytest.mark.parametrize("hd", [128, 256])
+def test_workspace_covers_every_length(hd):
+    """The stated workspace is enough at every length, type, and with or without mass
+    (a call with none says what it needs)."""
+    L = lib()
+
+    def needed(r, heads, t, n, past, mass):
+        assert L.oi_kv8_attn_launch(r, P, heads, t, 2 * P, heads * hd, 1.0, n, past, None, 4 * P if mass else None,
+                                    8 * P, heads * hd, 16 * P, 0, None) == E_ARG
+        return int(re.search(rb"bytes, (\d+) needed", L.oi_last_error()).group(1))
+
+    for n_kv, group, cap, n in [(1, 3, 116032, 2078), (16, 16, 960, 298), (8, 2, 7488, 901), (1, 8, 27840, 195),
+                                (1, 4, 10048, 1230), (8, 8, 40960, 3), (8, 4, 9600, 30), (2, 2, 64, 9),
+                                (4, 1, 100032, 1), (16, 16, 960, 298), (8, 4, 33024, 2047)]:
+        D = dims(n_kv, hd, cap, 64)
+        r = ctypes.byref(D)
+        most = L.oi_kv8_attn_workspace_bytes(r, n_kv * group, n)
+        for past in sorted({*range(0, cap - n + 1, max(1, cap // 1500)), cap - n}):
+            for t in (0, 1):
+                for mass in (False, True):
+                    assert needed(r, n_kv * group, t, n, past, mass) <= most, (n_kv, group, cap, n, past, t, mass)
 
 
 def test_evict_refusals():
