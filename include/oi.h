@@ -472,8 +472,10 @@ typedef struct {
  * elements; a q projection with a gate beside each head has head stride
  * 2 * head_dim); k, q_out and k_out: heads one after the other.  Types F32 or
  * F16 each way; q_out may be q and k_out k where type and strides are the same
- * (OI_E_ARG otherwise); outputs overlap nothing else.  Pointers 16-byte aligned, strides multiples of 16 bytes; OI_E_ARG otherwise.
- * head_dim 128 or 256.  Enqueued on `stream`. */
+ * (OI_E_ARG otherwise); outputs overlap nothing else (OI_E_ARG; rows of one
+ * stride may lie between each other, of two strides not).  Pointers 16-byte
+ * aligned, strides multiples of 16 bytes; OI_E_ARG otherwise.  head_dim 128 or
+ * 256, n below 2^24.  Enqueued on `stream`. */
 int oi_rope_axes_launch(const oi_rope_axes_dims *d, int32_t n, const int32_t *pos, const float *inv_freq,
                         const float *q_norm, const float *k_norm, int32_t in_type, const void *q, int64_t q_stride,
                         int64_t q_head_stride, const void *k, int64_t k_stride, int32_t out_type, void *q_out,
@@ -484,7 +486,8 @@ int oi_rope_axes_launch(const oi_rope_axes_dims *d, int32_t n, const int32_t *po
 /* A layer's cache in half the bytes of the f16 one (no counterpart in the
  * reference).  A value is code * 2^exponent: a signed byte in [-127, 127] and an
  * exponent in [-24, 10] (the range of f16; a byte outside counts as the nearest
- * in it) per kv head and block of slots, apart for K and V.  One buffer of oi_kv8_bytes, 256-byte aligned:
+ * in it) per kv head and block of slots, apart for K and V.  One buffer of
+ * oi_kv8_bytes, 256-byte aligned:
  *   K codes     int8 [n_kv_heads][capacity][head_dim]
  *   V codes     int8 [n_kv_heads][capacity / 64][head_dim][64]
  *   K exponents int8 [n_kv_heads][capacity / block]
@@ -497,8 +500,10 @@ int oi_rope_axes_launch(const oi_rope_axes_dims *d, int32_t n, const int32_t *po
  * Slots are places in the cache, not positions: after an eviction they differ,
  * and the caller rotates q and k by positions before they get here.
  * The launches allocate nothing and may be captured.  `stream` must belong to
- * the current device (OI_E_ARG otherwise).  Calls on one cache, mass or
- * workspace that overlap in time race. */
+ * the current device (OI_E_ARG otherwise).  An output (cache, mass, workspace,
+ * rows) that shares memory with another argument of its call is OI_E_ARG, except
+ * where said; rows of one stride may lie between each other.  Calls on one cache,
+ * mass or workspace that overlap in time race. */
 typedef struct {
     int32_t n_kv_heads, head_dim, capacity, block;
 } oi_kv8_dims;

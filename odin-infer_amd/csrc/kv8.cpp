@@ -89,8 +89,20 @@ int range_ok(const oi_kv8_dims *d, int32_t n, int32_t past, const int32_t *past_
     return OI_OK;
 }
 
-bool overlap(const void *a, int64_t na, const void *b, int64_t nb) {
-    return (const char *)a < (const char *)b + nb && (const char *)b < (const char *)a + na;
+// n pieces of `len` bytes, `stride` apart
+struct Span {
+    const void *p;
+    int64_t len, n = 1, stride = 0;
+};
+// Whether any two pieces may meet: equal strides are looked at within one stride (q, k and v
+// in one row of a projection lie between each other), others as a whole.
+bool overlap(const Span &a, const Span &b) {
+    if (!a.p || !b.p) return false;
+    const __int128 x = (uintptr_t)a.p, y = (uintptr_t)b.p;  // n * stride may pass 64 bits
+    if (x >= y + (__int128)(b.n - 1) * b.stride + b.len || y >= x + (__int128)(a.n - 1) * a.stride + a.len) return false;
+    if (a.n == 1 || b.n == 1 || a.stride != b.stride) return true;
+    const int64_t s = a.stride, by = (int64_t)((y - x) % s), r = by < 0 ? by + s : by;  // b's place behind a piece of a
+    return r < a.len || s - r < b.len;
 }
 
 }  // namespace
@@ -116,6 +128,10 @@ int oi_kv8_append_launch(const oi_kv8_dims *d, void *cache, int32_t type, const 
         if (int rc = range_ok(d, n, n_past, n_past_dev, W)) return rc;
         const int64_t row = (int64_t)d->n_kv_heads * d->head_dim;
         if (!rows_ok(k, type, k_stride, row) || !rows_ok(v, type, v_stride, row)) return err(OI_E_ARG, W, BAD_ROWS);
+        const int64_t es = size_of(type);
+        const Span all{cache, oi_kv8_bytes(d)};
+        if (overlap(all, {k, row * es, n, k_stride * es}) || overlap(all, {v, row * es, n, v_stride * es}))
+            return err(OI_E_ARG, W, "k or v lies in the cache");
         if (int rc = stream_ok(stream, W)) return rc;
         Kv8AppendArgs a{};
         a.c = parts(d, cache);
@@ -140,6 +156,9 @@ int oi_kv8_read_launch(const oi_kv8_dims *d, const void *cache, int32_t slot0, i
         if (!aligned(cache, 256)) return err(OI_E_ARG, W, "the cache must be 256-byte aligned");
         if (!aligned(k, 16) || !aligned(v, 16)) return err(OI_E_ARG, W, "outputs must be 16-byte aligned");
         if (int rc = range_ok(d, n, slot0, nullptr, W)) return rc;
+        const int64_t bytes = (int64_t)d->n_kv_heads * n * d->head_dim * size_of(type);
+        const Span all{cache, oi_kv8_bytes(d)}, ko{k, bytes}, vo{v, bytes};
+        if (overlap(all, ko) || overlap(all, vo) || overlap(ko, vo)) return err(OI_E_ARG, W, "outputs overlap");
         if (int rc = stream_ok(stream, W)) return rc;
         Kv8ReadArgs a{};
         a.c = parts(d, cache);
@@ -184,6 +203,13 @@ int oi_kv8_attn_launch(const oi_kv8_dims *d, const void *cache, int32_t n_heads,
         if (workspace_bytes < need)
             return err(OI_E_ARG, W, "workspace of " + std::to_string(workspace_bytes) + " bytes, " +
                                         std::to_string(need) + " needed");
+        const int64_t es = size_of(type);
+        const Span all{cache, oi_kv8_bytes(d)}, qs{q, row * es, n, q_stride * es}, os{out, row * es, n, out_stride * es},
+            ws_span{workspace, need}, ms{mass, (int64_t)d->n_kv_heads * d->capacity * 4};
+        if ((out != q && overlap(os, qs)) || overlap(os, all) || overlap(os, ws_span) || overlap(os, ms) ||
+            overlap(ws_span, all) || overlap(ws_span, qs) || overlap(ws_span, ms) || overlap(ms, all) ||
+            overlap(ms, qs))
+            return err(OI_E_ARG, W, "out, workspace or mass overlaps another argument");
         if (int rc = stream_ok(stream, W)) return rc;
         Kv8AttnArgs a{};
         a.c = parts(d, cache);
@@ -240,9 +266,14 @@ int oi_kv8_evict_launch(const oi_kv8_dims *src_dims, const void *src, const floa
         if (n_first < 0 || n_last < 0 || (int64_t)n_first + n_last > keep)
             return err(OI_E_RANGE, W, "n_first + n_last outside 0..keep");
         const int64_t h = src_dims->n_kv_heads, sm = h * src_dims->capacity * 4, dm = h * dst_dims->capacity * 4;
-        if (overlap(src, oi_kv8_bytes(src_dims), dst, oi_kv8_bytes(dst_dims)) || overlap(src_mass, sm, dst_mass, dm) ||
-            (src_pos && overlap(src_pos, sm, dst_pos, dm)))
-            return err(OI_E_ARG, W, "the two caches overlap");
+        const Span in[] = {{src, oi_kv8_bytes(src_dims)}, {src_mass, sm}, {src_pos, sm}},
+                   to[] = {{dst, oi_kv8_bytes(dst_dims)}, {dst_mass, dm}, {dst_pos, dm}, {kept, h * keep * 4}};
+        for (int i = 0; i < 4; i++) {
+            for (const Span &s : in)
+                if (overlap(to[i], s)) return err(OI_E_ARG, W, "the two caches overlap");
+            for (int j = 0; j < i; j++)
+                if (overlap(to[i], to[j])) return err(OI_E_ARG, W, "outputs overlap");
+        }
         if (int rc = stream_ok(stream, W)) return rc;
         Kv8EvictArgs a{};
         a.src = parts(src_dims, src);
@@ -277,7 +308,7 @@ int oi_rope_axes_launch(const oi_rope_axes_dims *d, int32_t n, const int32_t *po
         }
         if (pairs != d->rotary_dim / 2) return err(OI_E_ARG, W, "the sections' sum is not rotary_dim / 2");
         if (!(d->eps >= 0.f) || !std::isfinite(d->eps)) return err(OI_E_ARG, W, "bad eps");
-        if (n <= 0) return err(OI_E_RANGE, W, "n must be positive");
+        if (n <= 0 || n >= 1 << 24) return err(OI_E_RANGE, W, "n outside 1 .. 2^24 - 1");  // 256 threads each in one grid
         if (!type_ok(in_type) || !type_ok(out_type)) return err(OI_E_ARG, W, "type must be F32 or F16");
         if (!q || !k || !q_out || !k_out || (d->rotary_dim && (!pos || !inv_freq)))
             return err(OI_E_ARG, W, "null argument");
@@ -290,6 +321,12 @@ int oi_rope_axes_launch(const oi_rope_axes_dims *d, int32_t n, const int32_t *po
         if ((q_out == q && (in_type != out_type || q_stride != q_out_stride || q_head_stride != hd)) ||
             (k_out == k && (in_type != out_type || k_stride != k_out_stride)))
             return err(OI_E_ARG, W, "in place needs the same type and strides");
+        const int64_t ei = size_of(in_type), eo = size_of(out_type);
+        const Span qs{q, qr * ei, n, q_stride * ei}, ks{k, d->n_kv_heads * hd * ei, n, k_stride * ei},
+            qo{q_out, d->n_heads * hd * eo, n, q_out_stride * eo}, ko{k_out, d->n_kv_heads * hd * eo, n, k_out_stride * eo};
+        if ((q_out != q && overlap(qo, qs)) || (k_out != k && overlap(ko, ks)) || overlap(qo, ks) || overlap(ko, qs) ||
+            overlap(qo, ko))
+            return err(OI_E_ARG, W, "an output overlaps another argument");
         if (!aligned(pos, 4) || !aligned(inv_freq, 4) || !aligned(q_norm, 4) || !aligned(k_norm, 4))
             return err(OI_E_ARG, W, "misaligned positions, frequencies or norm weights");
         if (int rc = stream_ok(stream, W)) return rc;

@@ -312,3 +312,58 @@ def test_many_rows_extremes(t):
     ok = np.ones((n, heads), bool)
     ok[3, 0] = ok[4, 1] = False
     check(got[ok], want[ok], A, np.abs(ref.values("v", 220)).max(), t, 220)
+
+
+@pytest.mark.parametrize("t", [F32, F16])
+@pytest.mark.parametrize("n", [1, 300])
+def test_one_projection_in_place(t, n):
+    """q, k and v in the rows of one projection: rotated where they lie, appended and
+    attended from there, the result back over q.  Bit for bit as from buffers of
+    their own."""
+    rng = np.random.default_rng(71 + n)
+    heads, n_kv, hd, past = 4, 2, 128, 40
+    plan, turn = kv8.KV8(n_kv, hd, 384, 32), rope.RopeAxes(heads, n_kv, hd, 64, (12, 10, 10), False, 1e-6)
+    a, b = heads * hd, (heads + n_kv) * hd
+    row = b + n_kv * hd
+    x = rng.standard_normal((n, row)).astype(NP[t])
+    fill = rng.integers(0, 256, plan.nbytes).astype(np.uint8)
+    kv0 = dev(rng.standard_normal((2, past, n_kv, hd)).astype(NP[t]))
+    pos = dev(np.stack([np.arange(n), np.arange(n) // 7, np.arange(n) % 7]).astype(np.int32) + past)
+    f, w = dev((1e4 ** (-np.arange(32) / 32)).astype(np.float32)), dev((1 + 0.1 * rng.standard_normal((2, hd))).astype(np.float32))
+    ws = torch.empty(plan.attn_workspace_bytes(heads, n), dtype=torch.uint8, device="cuda")
+
+    def run(q, k, v, qs, ks, vs, out):
+        buf = dev(fill)
+        plan.append(buf.data_ptr(), t, kv0[0].data_ptr(), kv0[1].data_ptr(), past, 0)
+        turn.launch(n, pos.data_ptr(), f.data_ptr(), w[0].data_ptr(), w[1].data_ptr(), t, q, k, t, q, k, q_stride=qs,
+                    k_stride=ks, q_out_stride=qs, k_out_stride=ks)
+        plan.append(buf.data_ptr(), t, k, v, n, past, k_stride=ks, v_stride=vs)
+        plan.attn(buf.data_ptr(), heads, t, q, n, past, out, ws.data_ptr(), ws.numel(), q_stride=qs, out_stride=qs)
+        torch.cuda.synchronize()
+        return buf.cpu().numpy()
+
+    one = dev(x)
+    p, es = one.data_ptr(), one.element_size()
+    got = run(p, p + a * es, p + b * es, row, row, row, p)
+    q, k, v = (dev(np.ascontiguousarray(x[:, i:j])) for i, j in ((0, a), (a, b), (b, row)))
+    out = torch.empty_like(q)
+    want = run(q.data_ptr(), k.data_ptr(), v.data_ptr(), a, b - a, b - a, out.data_ptr())
+    assert np.array_equal(got, want)
+    assert torch.equal(one[:, :a], out) and torch.equal(one[:, a:b], k) and torch.equal(one[:, b:], v)
+
+
+@pytest.mark.parametrize("t", [F32, F16])
+def test_stated_workspace_is_enough_where_rows_are_split(t):
+    """A prompt whose mass splits its rows at this length and at the capacity does not."""
+    rng = np.random.default_rng(81 + t)
+    heads, n_kv, hd, cap, n, past = 8, 8, 128, 5632, 1664, 1024
+    plan, ref, buf = filled(rng, n_kv, hd, cap, 64, past + n)
+    q = rng.standard_normal((n, heads, hd)).astype(NP[t])
+    mass0 = np.zeros((n_kv, cap), np.float32)
+    mass = dev(mass0)
+    want, wmass, A = kv8ref.attend(ref, q, hd ** -0.5, n, past, mass0)
+    got = attn(plan, buf, q, n, past, t, mass=mass)
+    check(got, want, A, np.abs(ref.values("v", past + n)).max(), t, past + n)
+    tol = 2 * weight_error(A) + 2.0 ** -22 + 2.0 ** -24 * (n + 4)
+    m = mass.cpu().numpy()
+    assert np.all(np.abs(m - wmass) <= tol * wmass + 1e-30)

@@ -178,6 +178,57 @@ def test_rope_refusals():
         assert L.oi_rope_axes_launch(*a) == E_ARG, at
 
 
+def test_overlap_refusals():
+    """An output that shares memory with another argument, whole or in part."""
+    L, D = lib(), dims()
+    r, size, M = ctypes.byref(D), kv8.KV8(2, 128, 256, 32).nbytes, 1 << 24
+    c, row = M, 256 * 4  # the cache; a K or V row's bytes
+
+    for k, v in [(c, 2 * M), (2 * M, c + size - 256), (c - row, 2 * M), (c - 9 * 2 * row + 16, 2 * M)]:
+        assert L.oi_kv8_append_launch(r, c, 0, k, 512, v, 256, 10, 0, None, None) == E_ARG, (k, v)
+        assert b"in the cache" in L.oi_last_error()
+    for k, v in [(c, 2 * M), (2 * M, c + size - 256), (2 * M, 2 * M), (2 * M, 2 * M + 10 * row - 16)]:
+        assert L.oi_kv8_read_launch(r, c, 0, 10, 0, k, v, None) == E_ARG, (k, v)
+        assert b"overlap" in L.oi_last_error()
+
+    need, row = L.oi_kv8_attn_workspace_bytes(r, 4, 3), 512 * 4
+    q, out, ws, mass = 2 * M, 3 * M, 4 * M, 5 * M
+    for a in [dict(out=q + 16), dict(out=q + 2 * row - 16), dict(out=c + size - 256), dict(out=ws + 16),
+              dict(out=mass - 3 * row + 16), dict(ws=c), dict(ws=q + 2 * row), dict(ws=mass), dict(mass=c + 16),
+              dict(mass=q + 4), dict(out=q + row, stride=1024), dict(out=q + 512, stride=1024, q_stride=1024),
+              dict(out=q - 512 + 4096, stride=1024, q_stride=1024), dict(q=M >> 1, q_stride=1 << 40)]:
+        b = dict(dict(q=q, out=out, ws=ws, mass=mass, stride=512, q_stride=512), **a)
+        assert L.oi_kv8_attn_launch(r, c, 4, 0, b["q"], b["q_stride"], 0.1, 3, 5, None, b["mass"], b["out"],
+                                    b["stride"], b["ws"], need, None) == E_ARG, a
+        assert b"overlaps" in L.oi_last_error()
+
+    other = ctypes.byref(dims(cap=128, block=64))
+    for at, bad in [(9, 3 * M), (10, 2 * M + 512), (10, c), (11, 3 * M + 512), (11, 2 * M), (12, 3 * M), (12, 2 * M),
+                    (12, 5 * M), (12, 6 * M + 1020), (12, 7 * M + 4), (10, 7 * M), (10, 5 * M), (11, 5 * M + 64)]:
+        a = [r, c, 2 * M, 3 * M, 200, 100, 4, 8, other, 5 * M, 6 * M, 7 * M, 8 * M, None]
+        a[at] = bad
+        assert L.oi_kv8_evict_launch(*a) == E_ARG, (at, bad)
+        assert b"overlap" in L.oi_last_error()
+
+    D = _native.RopeAxesDims(4, 2, 128, 128, (ctypes.c_int32 * 3)(24, 20, 20), 1, 1e-6)
+    # q and k of one projection's rows (q, k, v: 1024 elements), f32; then the outputs
+    q, k, row = 2 * M, 2 * M + 512 * 4, 1024 * 4
+    for qo, ko, qs, ks in [(q + 16, 3 * M, 1024, 256), (k, 3 * M, 1024, 256), (3 * M, q + 512, 256 * 4, 1024),
+                           (3 * M, k + 512, 256 * 4, 1024), (3 * M, 3 * M, 512, 256), (3 * M, 3 * M + 2047, 512, 256),
+                           (q, k - 16, 1024, 1024), (q, k + row - 16, 1024, 256), (q + 9 * row + 2048 - 16, 3 * M, 512, 256)]:
+        a = [ctypes.byref(D), 10, M, M, None, None, 0, q, 1024, 128, k, 1024, 0, qo, qs, ko & ~15, ks, None]
+        assert L.oi_rope_axes_launch(*a) == E_ARG, (qo, ko)
+        assert b"overlaps" in L.oi_last_error(), (qo, ko)
+    # in place in the projection's rows, or beside it: what is refused here is the positions' alignment
+    for qo, ko, qs, ks in [(q, k, 1024, 1024), (q, 3 * M, 1024, 256), (3 * M, k, 512, 1024), (q, k + 1024, 1024, 1024)]:
+        a = [ctypes.byref(D), 10, M + 2, M, None, None, 0, q, 1024, 128, k, 1024, 0, qo, qs, ko, ks, None]
+        assert L.oi_rope_axes_launch(*a) == E_ARG, (qo, ko)
+        assert b"misaligned" in L.oi_last_error(), (qo, ko)
+    for n, code in [(1 << 24, E_RANGE), (2 ** 31 - 1, E_RANGE)]:
+        a = [ctypes.byref(D), n, M, M, None, None, 0, q, 1024, 128, k, 1024, 0, q, 1024, k, 1024, None]
+        assert L.oi_rope_axes_launch(*a) == code
+
+
 def test_format_one_rounding():
     """A value stored once is off by at most half a step, and the step is the
     least power of two that holds the block."""
