@@ -249,7 +249,8 @@ __device__ __forceinline__ uint32_t block_before(uint32_t v, uint32_t *ws, uint3
 // per wave, the counts summed up, and each finds its place; of equal keys at the
 // border the lowest slots stay.  Bound by its instructions on one CU, three passes
 // over the slots: 27 us for 40960, 9 us for 4096 (three digits with a pass each and
-// slots one at a time took 45).
+// slots one at a time took 45; the masses held in registers from one pass to the next
+// in unrolled loops, 37 and 18: they spill, and the code is fetched for a single use).
 constexpr int EV_TILE = 4 * EV, EV_CH = 64, EV_LIST = 8192;  // slots of a chunk; chunks counted at a time; the list
 __global__ __launch_bounds__(EV) void kv8_select_kernel(Kv8EvictArgs a) {
     constexpr int NW = EV / WAVE;

@@ -496,3 +496,27 @@ def test_evict_many_slots():
         torch.cuda.synchronize()
         assert np.array_equal(kd.cpu().numpy(), want)
         assert np.array_equal(md.cpu().numpy()[0, :keep], mass[0, want])
+
+
+@pytest.mark.parametrize("n", [4095, 4097, 24577, 65536, 65537])
+@pytest.mark.parametrize("kind", ["spread", "levels", "equal"])
+def test_evict_around_the_sizes_of_the_selection(n, kind):
+    rng = np.random.default_rng(n)
+    cap, keep = (n + 63) // 64 * 64, n // 3
+    plan, dplan = kv8.KV8(2, 128, cap, 32), kv8.KV8(2, 128, (keep + 63) // 64 * 64, 32)
+    buf = torch.zeros(plan.nbytes, dtype=torch.uint8, device="cuda")
+    dbuf = torch.zeros(dplan.nbytes, dtype=torch.uint8, device="cuda")
+    mass = {"spread": np.exp(3 * rng.standard_normal((2, cap))), "levels": rng.integers(0, 3, (2, cap)),
+            "equal": np.full((2, cap), 0.25)}[kind].astype(np.float32)
+    mass[:, n:] = np.inf  # behind the slots in use
+    first, last = 4, 64
+    sm, md = dev(mass), torch.zeros(2, dplan.capacity, device="cuda")
+    kd = torch.zeros(2, keep, dtype=torch.int32, device="cuda")
+    plan.evict(buf.data_ptr(), sm.data_ptr(), None, n, keep, first, last, dplan, dbuf.data_ptr(), md.data_ptr(), None,
+               kd.data_ptr())
+    torch.cuda.synchronize()
+    for h in range(2):
+        order = np.argsort(-mass[h, first:n - last], kind="stable")[:keep - first - last] + first
+        want = np.sort(np.concatenate([np.arange(first), order, np.arange(n - last, n)]))
+        assert np.array_equal(kd[h].cpu().numpy(), want), h
+        assert np.array_equal(md[h].cpu().numpy()[:keep], mass[h, want])
