@@ -10,10 +10,14 @@
 // again exactly (a power of two).  m, l and o are 32-bit.  The matrix products
 // take f16 operands: a and b are exact there; q and p of an f32 call are each
 // the sum of two halves (22 bits, q scaled by a power of two per row), of an
-// f16 call q is exact and p is rounded once to 11 bits (the size of the output's
-// own rounding; its l is the sum of the rounded p, so a weight that dominates
-// loses nothing, and the mass takes the sum of p before the rounding).  2^15 is where the largest weight sits in f16: a weight keeps
-// all its bits down to 2^-29 of it and is lost below 2^-40.
+// f16 call q is exact.  Its p is the sum of two halves where at most 8 rows share a
+// kv head (half of a product's columns are free for the second; the error of one
+// token over 37000 slots is then that of the output's rounding, 1.7e-4, and was
+// 2.9e-4, in the same time), with more rows rounded once to 11 bits (2.2e-4 against
+// 2.0e-4; a second product each would cost a third of the rate): l is then the sum
+// of the rounded p, so a weight that dominates loses nothing, and the mass takes the
+// sum of p before the rounding.  2^15 is where the largest weight sits in f16: a
+// weight keeps all its bits down to 2^-29 of it and is lost below 2^-40.
 
 #include <algorithm>
 #include <cfloat>
@@ -84,8 +88,11 @@ enum {
     ROWS_F16 = 0,   // 16 rows of an f16 q
     ROWS_F32 = 1,   // 16 rows of an f32 q, two operands each (upper and lower half)
     ROWS_PACK = 2,  // 8 rows of an f32 q: upper halves in columns 0..7, lower halves in 8..15, one product for both
+    ROWS_F16_PACK = 3,  // 8 rows of an f16 q, twice; only the weights p are packed so
 };
-constexpr int tile_rows(int mode) { return mode == ROWS_PACK ? 8 : 16; }
+constexpr bool rows_packed(int mode) { return mode == ROWS_PACK || mode == ROWS_F16_PACK; }
+constexpr bool rows_f16(int mode) { return mode == ROWS_F16 || mode == ROWS_F16_PACK; }
+constexpr int tile_rows(int mode) { return rows_packed(mode) ? 8 : 16; }
 
 // A tile of q as that operand: lane (column c, group g) holds dimensions
 // 64 k + 16 g + 8 h + 0..7 of its row, the order in which its 16-byte loads of K
@@ -96,7 +103,7 @@ constexpr int tile_rows(int mode) { return mode == ROWS_PACK ? 8 : 16; }
 template <int HD, int MODE>
 struct QTile {
     static constexpr int NF = HD / 32, R = tile_rows(MODE);
-    static constexpr bool F16 = MODE == ROWS_F16, TWO = MODE == ROWS_F32;
+    static constexpr bool F16 = rows_f16(MODE), TWO = MODE == ROWS_F32;
     static constexpr int TPR = WG / R, EL = HD / TPR;  // f32: threads of a row, elements of a thread
     struct Lds {
         f16x8 half[2][R][HD / 8];  // upper, lower; piece j of row r at j ^ (r & 7)
@@ -248,7 +255,7 @@ __device__ __forceinline__ size_t row_id(const Kv8AttnArgs &a, int r, int kvh) {
 template <int HD, int MODE, bool SAVE>
 __global__ __launch_bounds__(WG) void kv8_rows_kernel(Kv8AttnArgs a) {
     constexpr int NW = WG / WAVE, NK = HD / 64, ND = HD / 16, PD = HD + 4, R = tile_rows(MODE), TPR = WG / R;
-    constexpr bool F16 = MODE == ROWS_F16;
+    constexpr bool F16 = rows_f16(MODE), PACK = rows_packed(MODE), ROUND = F16 && !PACK;  // ROUND: p in 11 bits
     __shared__ __attribute__((aligned(16))) union {
         float o[NW][R][PD];
         typename QTile<HD, MODE>::Lds q;
@@ -328,7 +335,7 @@ __global__ __launch_bounds__(WG) void kv8_rows_kernel(Kv8AttnArgs a) {
 #pragma unroll
             for (int i = 0; i < 4; i++) top = fmaxf(top, s[t][i]);
         top = col_max(fmaf(top, mul, (float)ev));
-        const float m1 = fmaxf(m, ceilf(top)), bias = (float)ev - m1 + (F16 ? PSCALE : 0.f);
+        const float m1 = fmaxf(m, ceilf(top)), bias = (float)ev - m1 + (ROUND ? PSCALE : 0.f);
         float sum = 0.f;
         f16x8 ph[2], pl[2];
         f32x4 w[SAVE ? 4 : 1];
@@ -336,12 +343,12 @@ __global__ __launch_bounds__(WG) void kv8_rows_kernel(Kv8AttnArgs a) {
         for (int t = 0; t < 4; t++)
 #pragma unroll
             for (int i = 0; i < 4; i++) {
-                const float p = ex2(fmaf(s[t][i], mul, bias)) * (F16 ? 1.f : 32768.f);
+                const float p = ex2(fmaf(s[t][i], mul, bias)) * (ROUND ? 1.f : 32768.f);
                 if constexpr (SAVE) w[t][i] = p;
                 sum += p;
                 const _Float16 h = (_Float16)p;
                 ph[t / 2][4 * (t & 1) + i] = h;
-                if constexpr (!F16) pl[t / 2][4 * (t & 1) + i] = (_Float16)(p - (float)h);
+                if constexpr (!ROUND) pl[t / 2][4 * (t & 1) + i] = (_Float16)(p - (float)h);
             }
         if constexpr (SAVE) {
             // weights without V's exponent, for the mass, and the maximum that they go by; slot
@@ -354,7 +361,7 @@ __global__ __launch_bounds__(WG) void kv8_rows_kernel(Kv8AttnArgs a) {
                 if (g == 0) a.save_m[at + c] = m1;
             }
         }
-        if constexpr (MODE == ROWS_PACK) {
+        if constexpr (PACK) {
             ph[0] = lower ? pl[0] : ph[0];
             ph[1] = lower ? pl[1] : ph[1];
         }
@@ -367,7 +374,7 @@ __global__ __launch_bounds__(WG) void kv8_rows_kernel(Kv8AttnArgs a) {
             m = m1;
         }
         lx += sum * pow2i(-ev);
-        if constexpr (F16) l += (sum8(ph[0]) + sum8(ph[1])) * pow2i(-ev);
+        if constexpr (ROUND) l += (sum8(ph[0]) + sum8(ph[1])) * pow2i(-ev);
 #pragma unroll
         for (int d = 0; d < ND; d++)
 #pragma unroll
@@ -380,8 +387,8 @@ __global__ __launch_bounds__(WG) void kv8_rows_kernel(Kv8AttnArgs a) {
     }
     // the four waves' results in LDS; their weights once per row, then the sum
     lx = col_sum(lx);
-    l = F16 ? col_sum(l) : lx;
-    if constexpr (MODE == ROWS_PACK)
+    l = ROUND ? col_sum(l) : lx;
+    if constexpr (PACK)
 #pragma unroll
         for (int d = 0; d < ND; d++)
 #pragma unroll
@@ -1161,7 +1168,7 @@ namespace {
 template <int HD, int MODE>
 void launch(const Kv8AttnArgs &a, hipStream_t st) {
     constexpr int R = tile_rows(MODE);
-    constexpr bool F16 = MODE == ROWS_F16;
+    constexpr bool F16 = rows_f16(MODE);
     const int rows = a.n * a.group;
     const int end = a.past.dev ? a.c.cap : a.past.past + a.n, units = (end + T - 1) / T;
     const dim3 merge_grid((unsigned)a.n_heads, (unsigned)a.n);
@@ -1169,7 +1176,7 @@ void launch(const Kv8AttnArgs &a, hipStream_t st) {
         const dim3 grid((unsigned)a.c.n_kv, (unsigned)((rows + R - 1) / R), (unsigned)a.splits);
         if (a.save) hipLaunchKernelGGL((kv8_rows_kernel<HD, MODE, true>), grid, dim3(WG), 0, st, a);
         else hipLaunchKernelGGL((kv8_rows_kernel<HD, MODE, false>), grid, dim3(WG), 0, st, a);
-    } else if constexpr (MODE != ROWS_PACK) {  // (at most 8 rows always go by 16)
+    } else if constexpr (!rows_packed(MODE)) {  // (at most 8 rows always go by 16)
         const PromptPlan p = prompt_plan(HD, F16, a.c.n_kv, rows);
         const dim3 grid((unsigned)a.c.n_kv, (unsigned)((rows + p.rows - 1) / p.rows), (unsigned)a.splits);
         auto go = [&](auto kernel) { hipLaunchKernelGGL(kernel, grid, dim3((unsigned)(p.waves * WAVE)), 0, st, a); };
@@ -1197,7 +1204,7 @@ void launch(const Kv8AttnArgs &a, hipStream_t st) {
         hipLaunchKernelGGL((kv8_merge_kernel<HD, F16>), merge_grid, dim3(MW), 0, st, a);
     }
     if (!a.mass) return;
-    if constexpr (MODE != ROWS_PACK) {
+    if constexpr (!rows_packed(MODE)) {
         constexpr int X = HD == 128 ? 2 : 1;
         hipLaunchKernelGGL((kv8_mass_kernel<HD, F16, X>),
                            dim3((unsigned)a.c.n_kv * ((end + 64 * X - 1) / (64 * X)), (unsigned)a.msplits), dim3(WG), 0, st,
@@ -1211,10 +1218,12 @@ void launch(const Kv8AttnArgs &a, hipStream_t st) {
 }  // namespace
 
 hipError_t launch_kv8_attn(const Kv8AttnArgs &a, hipStream_t st) {
-    const int mode = a.f16 ? ROWS_F16 : a.n * a.group <= 8 ? ROWS_PACK : ROWS_F32;
+    const bool pack = a.n * a.group <= 8;
+    const int mode = a.f16 ? (pack ? ROWS_F16_PACK : ROWS_F16) : pack ? ROWS_PACK : ROWS_F32;
     auto by_mode = [&](auto hd) {
         constexpr int HD = decltype(hd)::value;
         if (mode == ROWS_F16) launch<HD, ROWS_F16>(a, st);
+        else if (mode == ROWS_F16_PACK) launch<HD, ROWS_F16_PACK>(a, st);
         else if (mode == ROWS_PACK) launch<HD, ROWS_PACK>(a, st);
         else launch<HD, ROWS_F32>(a, st);
     };

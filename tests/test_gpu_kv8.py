@@ -274,6 +274,23 @@ def test_attn_long_split_context():
             check(attn(plan, buf, q, n, past, F32), want, A, np.abs(ref.values("v", past + n)).max(), F32, past + n)
 
 
+@pytest.mark.parametrize("hd,heads", [(128, 8), (256, 3)])
+def test_f16_token_keeps_its_weights(hd, heads):
+    """Two slots of opposite values and nearly equal weights: what is left of them is
+    the weights' difference, to an f32 call's error and the output's one rounding."""
+    rng = np.random.default_rng(91 + hd)
+    plan = kv8.KV8(1, hd, 64, 16)
+    ref = kv8ref.Cache(1, hd, 64, 16, noise(rng, plan))
+    u, x = 0.05 * rng.standard_normal((2, hd))
+    ref.append(np.stack([u, -u])[:, None].astype(np.float32), np.stack([x, -x])[:, None].astype(np.float32), 0)
+    q = rng.standard_normal((1, heads, hd)).astype(np.float16)
+    want, _, A = kv8ref.attend(ref, q, hd ** -0.5, 1, 1, None)
+    got = attn(plan, dev(ref.buf), q, 1, 1, F16)
+    tol = 2 * weight_error(A) + 2.0 ** -22 + 2.0 ** -23 * 41
+    err = np.abs(got - want) - 2.0 ** -11 * np.abs(want) - 2.0 ** -25
+    assert err.max() <= tol * np.abs(ref.values("v", 2)).max()
+
+
 @pytest.mark.parametrize("t", [F32, F16])
 @pytest.mark.parametrize("n", [1, 40])
 def test_attn_blocks_of_very_different_size(t, n):
