@@ -14,10 +14,15 @@
 // kv head (half of a product's columns are free for the second; the error of one
 // token over 37000 slots is then that of the output's rounding, 1.7e-4, and was
 // 2.9e-4, in the same time), with more rows rounded once to 11 bits (2.2e-4 against
-// 2.0e-4; a second product each would cost a third of the rate): l is then the sum
-// of the rounded p, so a weight that dominates loses nothing, and the mass takes the
-// sum of p before the rounding.  2^15 is where the largest weight sits in f16: a
-// weight keeps all its bits down to 2^-29 of it and is lost below 2^-40.
+// 2.0e-4; a second product each would cost a third of the rate).
+// 2^15 is where the row's largest p sits in f16: another keeps all its bits down to
+// 2^-29 of it and is lost below 2^-40, from o, where both count with their blocks'
+// steps.  In l they count without: a slot in a block of small V (of zeros, step
+// 2^-24) may hold most of the row's weight while its p is far below f16's numbers.  So l
+// is the sum of p before the rounding, but for 11-bit weights where V's steps are
+// near each other: there it is the sum of the rounded p (a weight that dominates
+// loses nothing, 2.1e-4 against 2.8e-4), near as stated at NEAR_SUM and NEAR_EXP.
+// The mass takes the sum of p before the rounding.
 
 #include <algorithm>
 #include <cfloat>
@@ -35,6 +40,14 @@ typedef _Float16 f16x2 __attribute__((ext_vector_type(2)));
 constexpr int T = KV8_TILE;
 constexpr float NEG = -3.402823466e38f;  // the running maximum before any slot
 constexpr float PSCALE = 15.f;
+// Where l takes rounded weights.  Half a subnormal of f16 is 2^-25.
+// Rows kernel: a lane's 16 slots, of one block, where their sum is at least this: what
+// subnormals lose is below 2^-18 of it.
+constexpr float NEAR_SUM = 0.125f;
+// Prompt kernel: a unit whose exponents of V are all up to this far below the largest so
+// far: the slot with the largest score then has put 2^(7 - that largest) or more into l,
+// and a subnormal loses 2^-28 of that at most.
+constexpr float NEAR_EXP = 4.f;
 
 // 8 signed bytes as halves: byte ^ 128 behind 0x64 is 1024 + 128 + byte
 __device__ __forceinline__ f16x8 bytes_h(uint32_t lo, uint32_t hi) {
@@ -374,7 +387,10 @@ __global__ __launch_bounds__(WG) void kv8_rows_kernel(Kv8AttnArgs a) {
             m = m1;
         }
         lx += sum * pow2i(-ev);
-        if constexpr (ROUND) l += (sum8(ph[0]) + sum8(ph[1])) * pow2i(-ev);
+        if constexpr (ROUND) {
+            const float rounded = sum8(ph[0]) + sum8(ph[1]);
+            l += (rounded >= NEAR_SUM ? rounded : sum) * pow2i(-ev);
+        }
 #pragma unroll
         for (int d = 0; d < ND; d++)
 #pragma unroll
@@ -619,11 +635,12 @@ struct QRows {
 // for both, 46% of the LDS cycles were conflicts.)  K row r holds the slot with bits 2 and 3 of r
 // exchanged: the products then leave a lane the scores of slots 8 h + 0..7 of
 // each 16, those whose weights it supplies to the product with V.
-template <int HD, int NT>
+template <int HD, int NT, bool F16>
 struct Stage {
     static constexpr int N = T * HD / 16 / NT;  // 16-byte pieces of codes per thread
     u32x4 k[N], v[N];
     int8_t e;  // thread 4 w + b: of K (w = 0) or V (w = 1), slots 16 b ..
+    float vmax = KV8_EMIN;  // V's threads: the largest exponent so far
     __device__ __forceinline__ void load(const int8_t *kb, const int8_t *vb, const int8_t *ke, const int8_t *ve, int lb,
                                          int u, int tid) {
         if (tid < 8) e = (tid < 4 ? ke : ve)[(u * T + 16 * (tid & 3)) >> lb];
@@ -634,8 +651,21 @@ struct Stage {
             v[i] = vp[tid + i * NT];
         }
     }
-    __device__ __forceinline__ void store(f16x8 *ks, f16x8 *vs, float *es, int tid) const {
+    // unit u.  es: K's steps, V's exponents and, for f16 rows, 2^-v of V's exponents or, where one of
+    // them is more than NEAR_EXP below the largest so far, 0.  Bytes behind the `end` slots in use count for nothing.
+    __device__ __forceinline__ void store(f16x8 *ks, f16x8 *vs, float *es, int u, int end, int tid) {
         if (tid < 8) es[tid] = tid < 4 ? pow2i(kv8_exp(e)) : (float)kv8_exp(e);
+        if constexpr (F16)
+            if (tid < 8) {
+                const int x = kv8_exp(e);
+                const bool used = u * T + 16 * (tid & 3) < end;
+                float lo = used ? (float)x : (float)KV8_EMAX, hi = used ? (float)x : (float)KV8_EMIN;
+                lo = fminf(lo, OI_DPP(lo, 0xB1));
+                hi = fmaxf(hi, OI_DPP(hi, 0xB1));
+                lo = fminf(lo, OI_DPP(lo, 0x4E));
+                vmax = fmaxf(vmax, fmaxf(hi, OI_DPP(hi, 0x4E)));
+                if (tid >= 4) es[tid + 4] = lo < vmax - NEAR_EXP ? 0.f : pow2i(-x);
+            }
 #pragma unroll
         for (int i = 0; i < N; i++) {
             const int at = tid + i * NT;
@@ -657,8 +687,9 @@ struct Stage {
 // before and stored after this one's products).  Scores transposed as above, on
 // 32x32x16 products, for half a unit at a time.  f16 rows rescale o only when a
 // maximum rises by more than 2^7: their weights then reach 2^15 at most, from 2^8
-// (a weight keeps its bits down to 2^-22 of the largest and is lost below 2^-33,
-// 2^17 of which are below the output's rounding).  2047 tokens of 32 heads of 128
+// (a p keeps its bits down to 2^-22 of the largest and is lost from o below 2^-33,
+// 2^17 of which are below the output's rounding; l as stated above.  A unit whose V
+// lies far apart forms its exponentials twice: 375 us where every unit does, 304 else).  2047 tokens of 32 heads of 128
 // over 8 at 8048 slots: 282 us in f16 (836 TFLOP/s), 450 in f32 (twice the
 // products).  Vector instructions fill 61% of its cycles (softmax, and the bytes'
 // conversion for 256 rows), the matrix units 44%, at the 1.7 GHz that the card
@@ -671,7 +702,7 @@ __global__ __launch_bounds__(NW *WAVE, HD == 128 ? 2 : 1) void kv8_prompt_kernel
     constexpr bool AHEAD = HD == 128;  // registers left to request operands from LDS ahead of their use
     constexpr float PS = F16 ? 8.f : PSCALE, LAZY = F16 ? 7.f : 0.f;
     __shared__ __attribute__((aligned(16))) f16x8 lds[2][2][T * HD / 8];  // [buffer][K, V]
-    __shared__ __attribute__((aligned(16))) float es[2][8];  // K's steps and V's exponents, per 16 slots
+    __shared__ __attribute__((aligned(16))) float es[2][F16 ? 12 : 8];  // per 16 slots, as Stage::store leaves them
     const int tid = threadIdx.x, lane = tid & (WAVE - 1), wave = tid / WAVE;
     const int c = lane & 31, h = lane >> 5;
     const int kvh = blockIdx.x, rt = gridDim.y - 1 - blockIdx.y, split = blockIdx.z;  // the longest first
@@ -694,10 +725,10 @@ __global__ __launch_bounds__(NW *WAVE, HD == 128 ? 2 : 1) void kv8_prompt_kernel
     for (int d = 0; d < DT; d++)
 #pragma unroll
         for (int i = 0; i < 16; i++) o[d][i] = 0.f;
-    Stage<HD, NW * WAVE> st;
+    Stage<HD, NW * WAVE, F16> st;
     if (u0 < u1) {
         st.load(kb, vb, ke, ve, a.c.lb, u0, tid);
-        st.store(lds[0][0], lds[0][1], es[0], tid);
+        st.store(lds[0][0], lds[0][1], es[0], u0, past + a.n, tid);
     }
     __syncthreads();
     for (int u = u0; u < u1; u++) {
@@ -706,6 +737,13 @@ __global__ __launch_bounds__(NW *WAVE, HD == 128 ? 2 : 1) void kv8_prompt_kernel
         if (u + 1 < u1) st.load(kb, vb, ke, ve, a.c.lb, u + 1, tid);
         if (u * T < mine) {
             const f32x4 kmul = *(const f32x4 *)&es[buf][0] * scale, ev = *(const f32x4 *)&es[buf][4];
+            // 2^-v, or 0 in a far unit, whose weights are summed before their rounding
+            f32x4 un;
+            bool far = false;
+            if constexpr (F16) {
+                un = *(const f32x4 *)&es[buf][8];
+                far = __builtin_amdgcn_readfirstlane(__float_as_int(un[0])) == 0;
+            }
             auto k_at = [&](int x, int f) { return kt[(32 * x + c) * (HD / 8) + ((2 * f + h) ^ (c & 15))]; };
             auto v_at = [&](int x, int b, int d) {
                 return vt[(32 * (d0 + d) + c) * 8 + ((4 * x + 2 * b + h) ^ (c >> 1 & 7))];
@@ -750,7 +788,7 @@ __global__ __launch_bounds__(NW *WAVE, HD == 128 ? 2 : 1) void kv8_prompt_kernel
                     top = fmaxf(top, fmaf(t8, mul[b], ev[2 * x + b]));
                 }
                 top = half_reduce(top, [](float y, float z) { return fmaxf(y, z); });
-                if (__any(top > m + LAZY)) {
+                if (__any(top > m + LAZY) || far) {
                     const float m1 = fmaxf(m, ceilf(top)), alpha = ex2(m - m1);
                     m = m1;
                     l *= alpha;
@@ -759,6 +797,17 @@ __global__ __launch_bounds__(NW *WAVE, HD == 128 ? 2 : 1) void kv8_prompt_kernel
                     for (int d = 0; d < DT; d++)
 #pragma unroll
                         for (int i = 0; i < 16; i++) o[d][i] *= alpha;
+                    if (far)
+#pragma unroll
+                        for (int b = 0; b < 2; b++) {
+                            const float bias = ev[2 * x + b] - m + PS;
+                            float sum = 0.f;
+#pragma unroll
+                            for (int i = 0; i < 8; i++) sum += ex2(fmaf(s[8 * b + i], mul[b], bias));
+                            sum *= pow2i(-(int)ev[2 * x + b]);
+                            l += sum;
+                            lx += sum;
+                        }
                 }
 #pragma unroll
                 for (int b = 0; b < 2; b++) {
@@ -772,9 +821,8 @@ __global__ __launch_bounds__(NW *WAVE, HD == 128 ? 2 : 1) void kv8_prompt_kernel
                         ph[b][i] = t;
                         if constexpr (!F16) pl[b][i] = (_Float16)(p - (float)t);
                     }
-                    const float un = pow2i(-(int)ev[2 * x + b]);
-                    if constexpr (F16) l = fmaf(sum8(ph[b]), un, l);
-                    if constexpr (!F16 || NORM) lx = fmaf(sum, un, lx);
+                    if constexpr (F16) l = fmaf(sum8(ph[b]), un[2 * x + b], l);
+                    if constexpr (!F16 || NORM) lx = fmaf(sum, F16 ? un[2 * x + b] : pow2i(-(int)ev[2 * x + b]), lx);
                 }
                 if constexpr (AHEAD)
                     if (x == 0) {
@@ -791,7 +839,7 @@ __global__ __launch_bounds__(NW *WAVE, HD == 128 ? 2 : 1) void kv8_prompt_kernel
                     }
             }
         }
-        if (u + 1 < u1) st.store(lds[buf ^ 1][0], lds[buf ^ 1][1], es[buf ^ 1], tid);
+        if (u + 1 < u1) st.store(lds[buf ^ 1][0], lds[buf ^ 1][1], es[buf ^ 1], u + 1, past + a.n, tid);
         __syncthreads();
     }
     constexpr float UP = F16 ? 128.f : 1.f;  // 2^(PSCALE - PS): results leave at 2^15 as from the other kernel
