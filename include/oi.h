@@ -486,7 +486,9 @@ int oi_rope_axes_launch(const oi_rope_axes_dims *d, int32_t n, const int32_t *po
 /* A layer's cache in half the bytes of the f16 one (no counterpart in the
  * reference).  A value is code * 2^exponent: a signed byte in [-127, 127] and an
  * exponent in [-24, 10] (the range of f16; a byte outside counts as the nearest
- * in it) per kv head and block of slots, apart for K and V.  One buffer of
+ * in it) per kv head and block of slots, apart for K and V.  The largest
+ * exponent's values go past f16's largest number (an f16 65504 may round to
+ * 65536): where outputs are OI_TYPE_F16 they come out as +-65504.  One buffer of
  * oi_kv8_bytes, 256-byte aligned:
  *   K codes     int8 [n_kv_heads][capacity][head_dim]
  *   V codes     int8 [n_kv_heads][capacity / 64][head_dim][64]

@@ -196,7 +196,7 @@ __global__ __launch_bounds__(WG) void kv8_read_kernel(Kv8ReadArgs a) {
         const float y[4] = {(float)c[0] * step, (float)c[1] * step, (float)c[2] * step, (float)c[3] * step};
         if constexpr (F16)
             *(u32x2 *)((uint16_t *)a.out[which] + at) =
-                u32x2{f2h(y[0]) | (uint32_t)f2h(y[1]) << 16, f2h(y[2]) | (uint32_t)f2h(y[3]) << 16};
+                u32x2{f2h_top(y[0]) | (uint32_t)f2h_top(y[1]) << 16, f2h_top(y[2]) | (uint32_t)f2h_top(y[3]) << 16};
         else
             __builtin_nontemporal_store(f32x4{y[0], y[1], y[2], y[3]}, (f32x4 *)((float *)a.out[which] + at));
     }

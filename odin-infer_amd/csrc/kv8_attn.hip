@@ -446,7 +446,7 @@ __global__ __launch_bounds__(WG) void kv8_rows_kernel(Kv8AttnArgs a) {
             const int64_t at = row_at(a, gr, kvh, a.out_stride, HD) + d;
             if constexpr (F16)
                 *(u32x2 *)((uint16_t *)a.out + at) =
-                    u32x2{f2h(y[0]) | (uint32_t)f2h(y[1]) << 16, f2h(y[2]) | (uint32_t)f2h(y[3]) << 16};
+                    u32x2{f2h_top(y[0]) | (uint32_t)f2h_top(y[1]) << 16, f2h_top(y[2]) | (uint32_t)f2h_top(y[3]) << 16};
             else
                 *(f32x4 *)((float *)a.out + at) = y;
         }
@@ -527,7 +527,7 @@ __device__ __forceinline__ void merge_row(const Kv8AttnArgs &a, int token, int h
         for (int k = 0; k < MS; k++) v += lds.red[k][tid];
         v /= L;
         const int64_t at = token * a.out_stride + (int64_t)head * HD + tid;
-        if constexpr (F16) ((uint16_t *)a.out)[at] = f2h(v);
+        if constexpr (F16) ((uint16_t *)a.out)[at] = f2h_top(v);
         else ((float *)a.out)[at] = v;
     }
     if (tid == 0 && a.norm) a.norm[id] = make_float2(M, 32768.f / X);
@@ -563,7 +563,7 @@ __global__ __launch_bounds__(WG) void kv8_merge_many_kernel(Kv8AttnArgs a) {
     const int64_t at = blockIdx.y * a.out_stride + (int64_t)h * HD + d;
     if constexpr (F16)
         *(u32x2 *)((uint16_t *)a.out + at) =
-            u32x2{f2h(y[0]) | (uint32_t)f2h(y[1]) << 16, f2h(y[2]) | (uint32_t)f2h(y[3]) << 16};
+            u32x2{f2h_top(y[0]) | (uint32_t)f2h_top(y[1]) << 16, f2h_top(y[2]) | (uint32_t)f2h_top(y[3]) << 16};
     else
         *(f32x4 *)((float *)a.out + at) = y;
     if (d == 0 && a.norm) a.norm[id] = make_float2(M, 32768.f / X);
@@ -860,7 +860,7 @@ __global__ __launch_bounds__(NW *WAVE, HD == 128 ? 2 : 1) void kv8_prompt_kernel
                 *(f32x4 *)(a.part + (id * a.splits + split) * HD + dim) = y;
             else if constexpr (F16)
                 *(u32x2 *)((uint16_t *)a.out + to + dim) =
-                    u32x2{f2h(y[0]) | (uint32_t)f2h(y[1]) << 16, f2h(y[2]) | (uint32_t)f2h(y[3]) << 16};
+                    u32x2{f2h_top(y[0]) | (uint32_t)f2h_top(y[1]) << 16, f2h_top(y[2]) | (uint32_t)f2h_top(y[3]) << 16};
             else
                 *(f32x4 *)((float *)a.out + to + dim) = y;
         }
