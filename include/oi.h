@@ -472,8 +472,9 @@ typedef struct {
  * elements; a q projection with a gate beside each head has head stride
  * 2 * head_dim); k, q_out and k_out: heads one after the other.  Types F32 or
  * F16 each way; q_out may be q and k_out k where type and strides are the same
- * (OI_E_ARG otherwise); outputs overlap nothing else (OI_E_ARG; rows of one
- * stride may lie between each other, of two strides not).  Pointers 16-byte
+ * (OI_E_ARG otherwise); outputs overlap nothing else, positions, frequencies and
+ * norm weights among it (OI_E_ARG; rows of one stride may lie between each other,
+ * anything else between an output's rows counts as overlapping).  Pointers 16-byte
  * aligned, strides multiples of 16 bytes; OI_E_ARG otherwise.  head_dim 128 or
  * 256, n below 2^24.  Enqueued on `stream`. */
 int oi_rope_axes_launch(const oi_rope_axes_dims *d, int32_t n, const int32_t *pos, const float *inv_freq,
@@ -503,8 +504,9 @@ int oi_rope_axes_launch(const oi_rope_axes_dims *d, int32_t n, const int32_t *po
  * and the caller rotates q and k by positions before they get here.
  * The launches allocate nothing and may be captured.  `stream` must belong to
  * the current device (OI_E_ARG otherwise).  An output (cache, mass, workspace,
- * rows) that shares memory with another argument of its call is OI_E_ARG, except
- * where said; rows of one stride may lie between each other.  Calls on one cache,
+ * rows) that shares memory with another argument of its call, *n_past_dev among
+ * them, is OI_E_ARG, except where said; rows of one stride may lie between each
+ * other, anything else between an output's rows counts as shared.  Calls on one cache,
  * mass or workspace that overlap in time race. */
 typedef struct {
     int32_t n_kv_heads, head_dim, capacity, block;

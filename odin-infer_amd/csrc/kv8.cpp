@@ -132,6 +132,7 @@ int oi_kv8_append_launch(const oi_kv8_dims *d, void *cache, int32_t type, const 
         const Span all{cache, oi_kv8_bytes(d)};
         if (overlap(all, {k, row * es, n, k_stride * es}) || overlap(all, {v, row * es, n, v_stride * es}))
             return err(OI_E_ARG, W, "k or v lies in the cache");
+        if (overlap(all, {n_past_dev, 4})) return err(OI_E_ARG, W, "n_past_dev lies in the cache");
         if (int rc = stream_ok(stream, W)) return rc;
         Kv8AppendArgs a{};
         a.c = parts(d, cache);
@@ -205,10 +206,10 @@ int oi_kv8_attn_launch(const oi_kv8_dims *d, const void *cache, int32_t n_heads,
                                         std::to_string(need) + " needed");
         const int64_t es = size_of(type);
         const Span all{cache, oi_kv8_bytes(d)}, qs{q, row * es, n, q_stride * es}, os{out, row * es, n, out_stride * es},
-            ws_span{workspace, need}, ms{mass, (int64_t)d->n_kv_heads * d->capacity * 4};
+            ws_span{workspace, need}, ms{mass, (int64_t)d->n_kv_heads * d->capacity * 4}, past{n_past_dev, 4};
         if ((out != q && overlap(os, qs)) || overlap(os, all) || overlap(os, ws_span) || overlap(os, ms) ||
             overlap(ws_span, all) || overlap(ws_span, qs) || overlap(ws_span, ms) || overlap(ms, all) ||
-            overlap(ms, qs))
+            overlap(ms, qs) || overlap(past, os) || overlap(past, ws_span) || overlap(past, ms))
             return err(OI_E_ARG, W, "out, workspace or mass overlaps another argument");
         if (int rc = stream_ok(stream, W)) return rc;
         Kv8AttnArgs a{};
@@ -327,6 +328,12 @@ int oi_rope_axes_launch(const oi_rope_axes_dims *d, int32_t n, const int32_t *po
         if ((q_out != q && overlap(qo, qs)) || (k_out != k && overlap(ko, ks)) || overlap(qo, ks) || overlap(ko, qs) ||
             overlap(qo, ko))
             return err(OI_E_ARG, W, "an output overlaps another argument");
+        if (d->rotary_dim)  // not read otherwise
+            for (const Span &s : {Span{pos, (int64_t)n * 12}, Span{inv_freq, (int64_t)d->rotary_dim * 2}})
+                if (overlap(qo, s) || overlap(ko, s)) return err(OI_E_ARG, W, "an output overlaps the positions or frequencies");
+        for (const float *p : {q_norm, k_norm})
+            if (overlap(qo, {p, hd * 4}) || overlap(ko, {p, hd * 4}))
+                return err(OI_E_ARG, W, "an output overlaps a norm's weights");
         if (!aligned(pos, 4) || !aligned(inv_freq, 4) || !aligned(q_norm, 4) || !aligned(k_norm, 4))
             return err(OI_E_ARG, W, "misaligned positions, frequencies or norm weights");
         if (int rc = stream_ok(stream, W)) return rc;
