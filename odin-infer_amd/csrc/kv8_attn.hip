@@ -879,7 +879,8 @@ __global__ __launch_bounds__(NW *WAVE, HD == 128 ? 2 : 1) void kv8_prompt_kernel
 // multiply is an exact power of two and the row's 2^15 / l).  The workgroups before
 // `merges` merge a (token, query head) each; of the others a wave takes unit after
 // unit, a slot per lane.  Both read the splits' (m, l) by themselves, so one launch
-// does for both.  At 100004 slots of 4 kv heads 8 us (scores formed again from K:
+// does for both.  A slot takes nothing from rows that do not see it, not 0 times their
+// 1 / l either (NaN of a row that holds NaN).  At 100004 slots of 4 kv heads 8 us (scores formed again from K:
 // 18; reads of 2 KB a unit instead of 8).
 constexpr int FEW_MASS_ROWS = 16;
 template <int HD, bool F16>
@@ -928,7 +929,7 @@ __global__ __launch_bounds__(MW) void kv8_mass_few_kernel(Kv8AttnArgs a, int mer
             for (int i = 0; i < AHEAD; i++) x[i] = w[min(r0 + i, rows - 1) * 16];
 #pragma unroll
             for (int i = 0; i < AHEAD; i++)
-                if (r0 + i < rows) sum = fmaf(x[i], lane_value(f, r0 + i), sum);
+                if (r0 + i < rows && row_token(a, r0 + i) >= s - past) sum = fmaf(x[i], lane_value(f, r0 + i), sum);
         }
         if (s < end) mass[s] = had + sum;
     }
