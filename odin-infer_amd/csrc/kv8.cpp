@@ -191,7 +191,8 @@ int oi_kv8_attn_launch(const oi_kv8_dims *d, const void *cache, int32_t n_heads,
         if (!aligned(cache, 256)) return err(OI_E_ARG, W, "the cache must be 256-byte aligned");
         if (!aligned(workspace, 16) || !aligned(mass, 4) || !aligned(n_past_dev, 4)) return err(OI_E_ARG, W, "misaligned workspace, mass or n_past_dev");
         if (int rc = range_ok(d, n, n_past, n_past_dev, W)) return rc;
-        if (!std::isfinite(scale)) return err(OI_E_ARG, W, "scale is not finite");
+        const float scale2 = (float)((double)scale * 1.4426950408889634);  // exponents are formed in base 2
+        if (!std::isfinite(scale2)) return err(OI_E_ARG, W, "scale (times log2 e) is not finite");
         const int64_t row = (int64_t)n_heads * d->head_dim;
         if (!rows_ok(q, type, q_stride, row) || !rows_ok(out, type, out_stride, row)) return err(OI_E_ARG, W, BAD_ROWS);
         if (out == q && (q_stride != out_stride || mass))
@@ -218,7 +219,7 @@ int oi_kv8_attn_launch(const oi_kv8_dims *d, const void *cache, int32_t n_heads,
         a.q_stride = q_stride;
         a.out = out;
         a.out_stride = out_stride;
-        a.scale = (float)((double)scale * 1.4426950408889634);
+        a.scale = scale2;
         a.f16 = type == OI_TYPE_F16;
         a.n = n;
         a.n_heads = n_heads;

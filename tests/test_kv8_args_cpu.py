@@ -1,5 +1,5 @@
 """What the entries of the 8-bit cache and of the rotation refuse before anything
-reaches a device: small inputs inside an output."""
+reaches a device: small inputs inside an output, a scale that f32 does not hold."""
 import ctypes
 
 import pytest
@@ -59,3 +59,12 @@ def test_rotation_without_norm_or_turn_has_no_such_inputs():
     keep.rotary_dim, keep.sections = 0, (ctypes.c_int32 * 3)(0, 0, 0)
     a[2] = a[3] = 7 * M
     assert L.oi_rope_axes_launch(*a) == E_ARG and b"misaligned" in L.oi_last_error()
+
+
+@pytest.mark.parametrize("scale", [3.4e38, -3.0e38, 2.5e38])
+def test_scale_that_f32_does_not_hold_in_base_2(scale):
+    """scale * log2(e) is what the kernels multiply by: infinite, every output would be NaN."""
+    L, r = lib(), dims()
+    need = L.oi_kv8_attn_workspace_bytes(r, 4, 3)
+    rc = L.oi_kv8_attn_launch(r, M, 4, 0, 2 * M, 512, scale, 3, 5, None, None, 3 * M, 512, 4 * M, need, None)
+    assert rc == E_ARG and b"scale" in L.oi_last_error()
