@@ -544,12 +544,15 @@ int64_t oi_kv8_attn_workspace_bytes(const oi_kv8_dims *d, int32_t n_heads, int32
  * with q_stride and out_stride elements from a token to the next, both of
  * `type`, 16-byte aligned, strides multiples of 16 bytes; query head h reads kv
  * head h / (n_heads / n_kv_heads).  out = softmax(scale * q K) V with 32-bit
- * sums; scale * log2(e) must be finite in f32 (OI_E_ARG).  mass (NULL: none),
- * f32 [n_kv_heads][capacity]: what each slot receives, the softmax weight summed
- * over the call's tokens and the query heads of its kv head, is added to slots
- * below n_past and stored in slots n_past .. n_past+n-1 (a new slot starts at
- * nothing); slots past those stay as they are.  Every sum is in a fixed order.
- * `out` may be `q` where the strides are the
+ * sums; scale * log2(e) must be finite in f32 (OI_E_ARG).  Weights multiply V in 22
+ * bits, in f16 calls of more than 8 rows a kv head (n * n_heads / n_kv_heads) in
+ * 11; a slot whose weight times its block's step of V is below 2^-40 of the row's
+ * largest such product (f16 prompts: 2^-33) counts in the sum alone.  mass
+ * (NULL: none), f32 [n_kv_heads][capacity]: what each slot receives, the softmax
+ * weight summed over the call's tokens and the query heads of its kv head, is
+ * added to slots below n_past and stored in slots n_past .. n_past+n-1 (a new
+ * slot starts at nothing); slots past those stay as they are.  Every sum is in a
+ * fixed order.  `out` may be `q` where the strides are the
  * same and mass is NULL (OI_E_ARG otherwise); it overlaps nothing else.  With
  * n_past_dev the work is laid out for the whole capacity, so that one captured
  * call serves every length; sums then may be in another order than with n_past.

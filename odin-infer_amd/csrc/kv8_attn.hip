@@ -17,11 +17,13 @@
 // 2.0e-4; a second product each would cost a third of the rate).
 // 2^15 is where the row's largest p sits in f16: another keeps all its bits down to
 // 2^-29 of it and is lost below 2^-40, from o, where both count with their blocks'
-// steps.  In l they count without: a slot in a block of small V (of zeros, step
-// 2^-24) may hold most of the row's weight while its p is far below f16's numbers.  So l
-// is the sum of p before the rounding, but for 11-bit weights where V's steps are
-// near each other: there it is the sum of the rounded p (a weight that dominates
-// loses nothing, 2.1e-4 against 2.8e-4), near as stated at NEAR_SUM and NEAR_EXP.
+// steps.  A slot loses less than 2^-30 of half the step of the largest one's block, which
+// storing that one's V may have cost (2^-24 in the prompt's f16 form).
+// In l they count without the steps: a slot in a block of small V (of zeros, step 2^-24)
+// may hold most of the row's weight while its p is far below f16's numbers.  So l is
+// the sum of p before the rounding, but for 11-bit weights where V's steps are near
+// each other: there it is the sum of the rounded p (a weight that dominates loses
+// nothing, 2.1e-4 against 2.8e-4), near as stated at NEAR_SUM and NEAR_EXP.
 // The mass takes the sum of p before the rounding.
 
 #include <algorithm>
@@ -111,8 +113,8 @@ constexpr int tile_rows(int mode) { return rows_packed(mode) ? 8 : 16; }
 // 64 k + 16 g + 8 h + 0..7 of its row, the order in which its 16-byte loads of K
 // fall.  f32 rows are made into two halves of q 2^-e (e the row's exponent) by the
 // workgroup together, a row by 256 / R threads, and pass through LDS: each wave
-// for itself took 1.8 us more at head_dim 256, in one long run of instructions.  A negative scale turns q's sign, so that the largest score is that
-// of the largest product.
+// for itself took 1.8 us more at head_dim 256, in one long run of instructions.  A
+// negative scale turns q's sign, so that the largest score is that of the largest product.
 template <int HD, int MODE>
 struct QTile {
     static constexpr int NF = HD / 32, R = tile_rows(MODE);
@@ -689,10 +691,12 @@ struct Stage {
 // maximum rises by more than 2^7: their weights then reach 2^15 at most, from 2^8
 // (a p keeps its bits down to 2^-22 of the largest and is lost from o below 2^-33,
 // 2^17 of which are below the output's rounding; l as stated above.  A unit whose V
-// lies far apart forms its exponentials twice: 375 us where every unit does, 304 else).  2047 tokens of 32 heads of 128
-// over 8 at 8048 slots: 282 us in f16 (836 TFLOP/s), 450 in f32 (twice the
-// products).  Vector instructions fill 61% of its cycles (softmax, and the bytes'
-// conversion for 256 rows), the matrix units 44%, at the 1.7 GHz that the card
+// lies far apart forms its exponentials twice: 375 us where every unit does).
+// 2047 tokens of 32 heads of 128 over 8 at 8048 slots: 304 us in f16 (776 TFLOP/s;
+// 314 with the sums that the mass needs), 477 in f32 (twice the products); 1000 tokens
+// of 16 heads of 256 over 2 at 5000 slots: 147 us in f16 (500 TFLOP/s), 317 in f32
+// (233).  Vector instructions fill 64% of its cycles (softmax, and the bytes'
+// conversion for 256 rows), the matrix units 41%, at the 1.8 GHz that the card
 // holds under them.  Measured and not kept: 64 rows a wave (one wave a SIMD, 428);
 // the waves of a SIMD half a unit apart with three buffers (311); a raised wave
 // priority around the products (f16 the same, f32 600).
@@ -880,8 +884,8 @@ __global__ __launch_bounds__(NW *WAVE, HD == 128 ? 2 : 1) void kv8_prompt_kernel
 // `merges` merge a (token, query head) each; of the others a wave takes unit after
 // unit, a slot per lane.  Both read the splits' (m, l) by themselves, so one launch
 // does for both.  A slot takes nothing from rows that do not see it, not 0 times their
-// 1 / l either (NaN of a row that holds NaN).  At 100004 slots of 4 kv heads 8 us (scores formed again from K:
-// 18; reads of 2 KB a unit instead of 8).
+// 1 / l either (NaN of a row that holds NaN).  At 100004 slots of 4 kv heads 8 us
+// (scores formed again from K: 18; reads of 2 KB a unit instead of 8).
 constexpr int FEW_MASS_ROWS = 16;
 template <int HD, bool F16>
 __global__ __launch_bounds__(MW) void kv8_mass_few_kernel(Kv8AttnArgs a, int merges) {
@@ -942,8 +946,8 @@ __global__ __launch_bounds__(MW) void kv8_mass_few_kernel(Kv8AttnArgs a, int mer
 // too few to fill the card, the rows are split over workgroups too, whose sums a
 // second launch adds (1000 rows of 16 heads of 2 kv heads at 5000 slots, head_dim
 // 256: 168 us in one split, 96 in three).  2047 tokens of 32 heads at 8048 slots:
-// 193 us, 610 TFLOP/s; 56% of its cycles are vector instructions (an exponential
-// and two multiply-adds a score), 31% the matrix units.
+// 192 us, 613 TFLOP/s; 54% of its cycles are vector instructions (an exponential
+// and two multiply-adds a score), 32% the matrix units.
 template <int HD, bool F16, int X>
 __global__ __launch_bounds__(WG, 2) void kv8_mass_kernel(Kv8AttnArgs a) {
     constexpr int NF = HD / 16, QR = 64, PC = F16 ? 1 : 2, TPR = WG / QR, EL = HD / TPR, WS = 32 * X, GS = 2 * WS;

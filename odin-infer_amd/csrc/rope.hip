@@ -7,7 +7,7 @@
 // sine and cosine of the remainder are 32-bit.  One workgroup takes a token (a
 // few heads of it where tokens are few): the angles are formed once for all its
 // heads, then a wave takes a head at a time.  2311 tokens of 16 + 2 heads of 256 to
-// f16 (64 MB) 17 us, bound by memory (about 6.5 us + bytes / 7 TB/s); a single token
+// f16 (64 MB) 18 us, bound by memory (about 6.5 us + bytes / 7 TB/s); a single token
 // of 32 + 8 heads 3.6 us, the chain of load, norm and store.
 
 #include "device_common.h"
