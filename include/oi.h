@@ -536,7 +536,7 @@ int oi_kv8_read_launch(const oi_kv8_dims *d, const void *cache, int32_t slot0, i
 
 /* Workspace that oi_kv8_attn_launch needs for n tokens (exactly n: fewer may need
  * more) at any length up to the capacity, with mass or without, 16-byte aligned;
- * 0 for bad arguments. */
+ * 0 for bad arguments, more rows than one call takes among them. */
 int64_t oi_kv8_attn_workspace_bytes(const oi_kv8_dims *d, int32_t n_heads, int32_t n);
 
 /* Causal attention of n tokens over the cache, which already holds them (append

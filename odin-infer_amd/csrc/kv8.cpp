@@ -80,6 +80,8 @@ int stream_ok(void *stream, const char *what) {
     return OI_OK;
 }
 
+constexpr int64_t MAX_ROWS = 65535 * 16;  // of a kv head in one attention call: the grid of tiles of 16
+
 // `past` slots in use, then `n` more
 int range_ok(const oi_kv8_dims *d, int32_t n, int32_t past, const int32_t *past_dev, const char *what) {
     if (n <= 0 || n > d->capacity) return err(OI_E_RANGE, what, "n=" + std::to_string(n) + " outside 1..capacity");
@@ -174,6 +176,7 @@ int oi_kv8_read_launch(const oi_kv8_dims *d, const void *cache, int32_t slot0, i
 
 int64_t oi_kv8_attn_workspace_bytes(const oi_kv8_dims *d, int32_t n_heads, int32_t n) {
     if (!dims_ok(d) || n_heads <= 0 || n_heads > 4096 || n_heads % d->n_kv_heads || n <= 0 || n > d->capacity) return 0;
+    if ((int64_t)n * (n_heads / d->n_kv_heads) > MAX_ROWS) return 0;
     return (int64_t)kv8_attn_workspace_most(n_heads, n_heads / d->n_kv_heads, n, d->capacity, d->head_dim);
 }
 
@@ -198,7 +201,7 @@ int oi_kv8_attn_launch(const oi_kv8_dims *d, const void *cache, int32_t n_heads,
         if (out == q && (q_stride != out_stride || mass))
             return err(OI_E_ARG, W, "out may be q only with the same stride and without mass");
         const int group = n_heads / d->n_kv_heads;
-        if ((int64_t)n * group > 65535 * 16) return err(OI_E_RANGE, W, "too many rows in one call");
+        if ((int64_t)n * group > MAX_ROWS) return err(OI_E_RANGE, W, "too many rows in one call");
         const int end = n_past_dev ? d->capacity : n_past + n;
         const int splits = kv8_attn_splits(d->n_kv_heads, group, n, end, d->head_dim, type == OI_TYPE_F16);
         const int64_t need = (int64_t)kv8_attn_workspace(n_heads, group, n, end, d->head_dim, splits, mass);

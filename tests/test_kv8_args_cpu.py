@@ -68,3 +68,15 @@ def test_scale_that_f32_does_not_hold_in_base_2(scale):
     need = L.oi_kv8_attn_workspace_bytes(r, 4, 3)
     rc = L.oi_kv8_attn_launch(r, M, 4, 0, 2 * M, 512, scale, 3, 5, None, None, 3 * M, 512, 4 * M, need, None)
     assert rc == E_ARG and b"scale" in L.oi_last_error()
+
+
+def test_workspace_of_a_call_that_is_refused():
+    """More rows than one call takes: no size, as for other arguments that the call refuses."""
+    L, r = lib(), dims(cap=1 << 21)
+    for heads, n in [(8, 262140), (4, 524280), (2, 1048560)]:
+        assert L.oi_kv8_attn_workspace_bytes(r, heads, n) > 0
+        assert L.oi_kv8_attn_workspace_bytes(r, heads, n + 1) == 0
+        need = 1 << 60
+        rc = L.oi_kv8_attn_launch(r, M, heads, 0, 1 << 50, 128 * heads, 0.1, n + 1, 0, None, None, 1 << 52, 128 * heads,
+                                  1 << 54, need, None)
+        assert rc == -6 and b"too many rows" in L.oi_last_error()
