@@ -576,6 +576,96 @@ int oi_kv8_evict_launch(const oi_kv8_dims *src_dims, const void *src, const floa
                         int32_t n, int32_t keep, int32_t n_first, int32_t n_last, const oi_kv8_dims *dst_dims,
                         void *dst, float *dst_mass, int32_t *dst_pos, int32_t *kept, void *stream);
 
+/* ----------------------------------------------------- paged K/V cache --- */
+
+/* One layer's f16 cache for many sequences (no counterpart in the reference): a pool
+ * of pages of `page` slots.  Slot j of a sequence lies in page table[sequence][j / page]
+ * at j % page; its number in the pool is page_id * page + j % page.  One buffer of
+ * oi_paged_bytes, 256-byte aligned, binary16:
+ *   K [n_pages][n_kv_heads][page][head_dim]
+ *   V [n_pages][n_kv_heads][page / 8][head_dim][8]   (eights of slots)
+ * head_dim 128 or 256, page 16, 32 or 64, n_pages * page at most 2^28.  The memory
+ * needs no initialization: a call reads values only of slots below the lengths that it
+ * is given.  Lengths, tables and the list of free pages are int32 in device memory and
+ * serve all layers: plan once a step, then append and attend in each layer's buffer.
+ * Numbers there are not checked on the host: a length past the table's row counts as
+ * the row's slots, a page id that the pool does not have as its last page (none in
+ * slots), a negative number as 0.
+ * The launches allocate nothing, wait for nothing and may be captured: a replay goes
+ * by the numbers that it finds.  `stream` must belong to the current device (OI_E_ARG
+ * otherwise).  An output (cache, table, list, maps, rows, workspace) that shares memory
+ * with another argument of its call is OI_E_ARG, except where said; rows of one stride
+ * may lie between each other, anything else between an output's rows counts as shared.
+ * Calls on one cache, table, list or workspace that overlap in time race. */
+typedef struct {
+    int32_t n_kv_heads, head_dim, n_pages, page;
+} oi_paged_dims;
+
+/* Bytes of a cache buffer; 0 for bad dims. */
+int64_t oi_paged_bytes(const oi_paged_dims *d);
+
+/* Room for a step's tokens: sequence i holds n_past[i] slots and gets n_new[i] more
+ * (negative: 0), in pages from the end of the list free_pages[0 .. *n_free)
+ * (int32 [n_pages]; at first all page ids, *n_free = n_pages), in the sequences' order.
+ * A sequence is served unless its tokens do not fit its table row (table_stride
+ * entries) or the n_rows rows of the step, or it needs a page and the list does not
+ * hold what it and the sequences before it need.  Written: new entries of table
+ * [n_seqs][table_stride]; *n_free; lens [n_seqs], the slots held now, 0 where not
+ * served; starts [n_seqs + 1], the packed rows' begins (sums of n_new, at most n_rows);
+ * slots [n_rows], each row's slot number, -1 for rows not served or behind the last;
+ * pos (NULL: none) [3][n_rows], its place in the sequence on three axes as
+ * oi_rope_axes_launch takes them, 0 for such rows.  n_seqs at most 65536, n_rows at
+ * most 2^24 (0: no rows).  One step needs one call for all layers. */
+int oi_paged_plan_launch(const oi_paged_dims *d, int32_t n_seqs, const int32_t *n_past, const int32_t *n_new,
+                         int32_t *table, int32_t table_stride, const int32_t *free_pages, int32_t *n_free,
+                         int32_t n_rows, int32_t *lens, int32_t *starts, int32_t *slots, int32_t *pos, void *stream);
+
+/* Pages back to the list: sequence i holds n_held[i] slots and keeps the first
+ * n_keep[i] of them (NULL: none, the sequences have ended).  A release of what the last
+ * plan took leaves list and count as they were before it.  Where the list would hold
+ * more than n_pages, nothing is released. */
+int oi_paged_release_launch(const oi_paged_dims *d, int32_t n_seqs, const int32_t *n_held, const int32_t *n_keep,
+                            const int32_t *table, int32_t table_stride, int32_t *free_pages, int32_t *n_free,
+                            void *stream);
+
+/* Store K and V of n packed rows, [n][n_kv_heads][head_dim] with k_stride and v_stride
+ * elements from a row to the next, OI_TYPE_F32 or OI_TYPE_F16, 16-byte aligned, strides
+ * multiples of 16 bytes, in slots[row] (oi_paged_plan_launch; a number that the pool does
+ * not have: the row is passed over).  Values are rounded to nearest even; those past
+ * f16's range, infinities among them, are stored as +-65504, NaN as 0.  Of two rows
+ * with one slot either may be stored, element by element. */
+int oi_paged_append_launch(const oi_paged_dims *d, void *cache, int32_t type, const void *k, int64_t k_stride,
+                           const void *v, int64_t v_stride, int32_t n, const int32_t *slots, void *stream);
+
+/* Workspace of the calls below, 16-byte aligned, at any lengths; 0 for arguments that
+ * the call refuses. */
+int64_t oi_paged_tokens_workspace_bytes(const oi_paged_dims *d, int32_t n_heads, int32_t n_seqs, int32_t n_q);
+int64_t oi_paged_prompts_workspace_bytes(const oi_paged_dims *d, int32_t n_heads, int32_t n_seqs, int32_t n_rows);
+
+/* Causal attention of the newest n_q (1 .. 16) tokens of each sequence, which the cache
+ * already holds: token j of a sequence of lens[i] slots sees slots 0 .. lens[i] - n_q + j
+ * (none: its rows come out 0, as for a sequence that was not served).  q and out
+ * [n_seqs * n_q][n_heads][head_dim], q_stride and out_stride elements from a token to the
+ * next, both of `type` (F32 or F16), 16-byte aligned, strides multiples of 16 bytes.
+ * Query head h reads kv head h / (n_heads / n_kv_heads).  out = softmax(scale * q K) V
+ * with 32-bit sums in a fixed order and weights of 22 bits; scale * log2(e) must be finite
+ * in f32 (OI_E_ARG).  Cached values below the lengths must be finite (as the append
+ * leaves them).  `out` may be `q` where the strides are the same. */
+int oi_paged_tokens_launch(const oi_paged_dims *d, const void *cache, int32_t n_heads, int32_t type, const void *q,
+                           int64_t q_stride, float scale, int32_t n_seqs, int32_t n_q, const int32_t *lens,
+                           const int32_t *table, int32_t table_stride, void *out, int64_t out_stride, void *workspace,
+                           int64_t workspace_bytes, void *stream);
+
+/* The same for packed rows: sequence i's tokens are the rows starts[i] .. starts[i+1]-1
+ * of n_rows (starts [n_seqs + 1], rising; numbers outside 0 .. n_rows count as the nearer
+ * end), its newest; rows of no sequence stay as they are.  For whole prompts, chunks
+ * behind cached slots, and drafts of differing lengths.  Weights have 22 bits, in F16
+ * calls 11.  n_rows at most 2^24 and n_rows * (n_heads / n_kv_heads)^2 below 2^32. */
+int oi_paged_prompts_launch(const oi_paged_dims *d, const void *cache, int32_t n_heads, int32_t type, const void *q,
+                            int64_t q_stride, float scale, int32_t n_seqs, int32_t n_rows, const int32_t *starts,
+                            const int32_t *lens, const int32_t *table, int32_t table_stride, void *out,
+                            int64_t out_stride, void *workspace, int64_t workspace_bytes, void *stream);
+
 #ifdef __cplusplus
 }
 #endif

@@ -39,12 +39,12 @@ def build(verbose=False):
     jobs = []
     objs = []
     for src in ["kernels.hip", "gemv.hip", "attn.hip", "gemm.hip", "prefill.hip", "deltanet.hip", "qwen35_attn.hip", "noalloc.hip", "sample.hip", "prefill_hybrid.hip",
-                "kv8.hip", "kv8_attn.hip", "rope.hip"]:
+                "kv8.hip", "kv8_attn.hip", "rope.hip", "paged.hip", "paged_attn.hip"]:
         obj = os.path.join(BUILD, src + ".o")
         objs.append(obj)
         jobs.append([HIPCC, "--offload-arch=" + ARCH, *COMMON, *DEVICE_FLAGS, "-x", "hip", "-c",
                      os.path.join(CSRC, src), "-o", obj])
-    for src in ["engine.cpp", "gguf.cpp", "oikv.cpp", "state.cpp", "kv8.cpp"]:
+    for src in ["engine.cpp", "gguf.cpp", "oikv.cpp", "state.cpp", "kv8.cpp", "paged.cpp"]:
         obj = os.path.join(BUILD, src + ".o")
         objs.append(obj)
         jobs.append([HIPCC, *COMMON, "-D__HIP_PLATFORM_AMD__", "-c", os.path.join(CSRC, src), "-o", obj])

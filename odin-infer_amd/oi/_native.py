@@ -41,6 +41,10 @@ class KV8Dims(ctypes.Structure):
     _fields_ = [("n_kv_heads", c_i32), ("head_dim", c_i32), ("capacity", c_i32), ("block", c_i32)]
 
 
+class PagedDims(ctypes.Structure):
+    _fields_ = [("n_kv_heads", c_i32), ("head_dim", c_i32), ("n_pages", c_i32), ("page", c_i32)]
+
+
 class Opts(ctypes.Structure):
     _fields_ = [("max_ctx", c_i32), ("use_hip", c_i32), ("num_threads", c_i32), ("device", c_i32)]
 
@@ -122,6 +126,16 @@ HIP_SYMBOLS = {
     "oi_kv8_attn_launch": (c_i32, [c_vp, c_vp, c_i32, c_i32, c_vp, c_i64, c_f, c_i32, c_i32, c_vp, c_vp, c_vp, c_i64,
                                    c_vp, c_i64, c_vp]),
     "oi_kv8_evict_launch": (c_i32, [c_vp, c_vp, c_vp, c_vp] + [c_i32] * 4 + [c_vp] * 6),
+    "oi_paged_bytes": (c_i64, [c_vp]),
+    "oi_paged_plan_launch": (c_i32, [c_vp, c_i32, c_vp, c_vp, c_vp, c_i32, c_vp, c_vp, c_i32] + [c_vp] * 5),
+    "oi_paged_release_launch": (c_i32, [c_vp, c_i32, c_vp, c_vp, c_vp, c_i32, c_vp, c_vp, c_vp]),
+    "oi_paged_append_launch": (c_i32, [c_vp, c_vp, c_i32, c_vp, c_i64, c_vp, c_i64, c_i32, c_vp, c_vp]),
+    "oi_paged_tokens_workspace_bytes": (c_i64, [c_vp, c_i32, c_i32, c_i32]),
+    "oi_paged_tokens_launch": (c_i32, [c_vp, c_vp, c_i32, c_i32, c_vp, c_i64, c_f, c_i32, c_i32, c_vp, c_vp, c_i32, c_vp,
+                                       c_i64, c_vp, c_i64, c_vp]),
+    "oi_paged_prompts_workspace_bytes": (c_i64, [c_vp, c_i32, c_i32, c_i32]),
+    "oi_paged_prompts_launch": (c_i32, [c_vp, c_vp, c_i32, c_i32, c_vp, c_i64, c_f, c_i32, c_i32, c_vp, c_vp, c_vp, c_i32,
+                                        c_vp, c_i64, c_vp, c_i64, c_vp]),
 }
 
 
