@@ -81,8 +81,9 @@ Workspace workspace(int workers, int part_rows, int hd) {
 bool tokens_fit(int32_t n_seqs, int32_t n_q) {
     return n_seqs > 0 && n_seqs <= MAX_SEQS && n_q > 0 && n_q <= MAX_DRAFT;
 }
-Workspace tokens_workspace(const oi_paged_dims *d, int32_t n_heads, int32_t n_q) {
-    return workspace(paged_tokens_workers(d->head_dim), std::min(16, n_q * (n_heads / d->n_kv_heads)), d->head_dim);
+Workspace tokens_workspace(const oi_paged_dims *d, int32_t n_heads, int32_t n_q, bool f16) {
+    const int rows = n_q * (n_heads / d->n_kv_heads);
+    return workspace(paged_tokens_workers(d->head_dim), std::min(paged_tokens_rows(d->head_dim, rows, f16), rows), d->head_dim);
 }
 bool prompts_fit(const oi_paged_dims *d, int32_t n_heads, int32_t n_seqs, int32_t n_rows) {
     const int64_t g = n_heads / d->n_kv_heads;
@@ -139,6 +140,7 @@ int attention(PagedAttnArgs &a, const char *what, const oi_paged_dims *d, const 
     a.lens = lens;
     a.table = table;
     a.stride = stride;
+    a.cap = (int)std::min<int64_t>(cap, INT32_MAX - 64);  // rounding up to units stays in range
     a.workers = w.workers;
     a.part_rows = w.part_rows;
     a.at = (PagedAt *)ws;
@@ -250,7 +252,7 @@ int oi_paged_append_launch(const oi_paged_dims *d, void *cache, int32_t type, co
 
 int64_t oi_paged_tokens_workspace_bytes(const oi_paged_dims *d, int32_t n_heads, int32_t n_seqs, int32_t n_q) {
     if (!dims_ok(d) || !heads_ok(d, n_heads) || !tokens_fit(n_seqs, n_q)) return 0;
-    return (int64_t)tokens_workspace(d, n_heads, n_q).bytes;
+    return (int64_t)std::max(tokens_workspace(d, n_heads, n_q, true).bytes, tokens_workspace(d, n_heads, n_q, false).bytes);
 }
 
 int oi_paged_tokens_launch(const oi_paged_dims *d, const void *cache, int32_t n_heads, int32_t type, const void *q,
@@ -265,10 +267,16 @@ int oi_paged_tokens_launch(const oi_paged_dims *d, const void *cache, int32_t n_
         if (!tokens_fit(n_seqs, n_q)) return err(OI_E_RANGE, W, "n_seqs outside 1 .. 65536 or n_q outside 1 .. 16");
         PagedAttnArgs a{};
         a.n_q = n_q;
-        const Workspace w = tokens_workspace(d, n_heads, n_q);
+        const Workspace w = tokens_workspace(d, n_heads, n_q, type == OI_TYPE_F16);
         if (int rc = attention(a, W, d, cache, n_heads, type, q, q_stride, scale, n_seqs, (int64_t)n_seqs * n_q, nullptr, lens,
                                table, table_stride, out, out_stride, workspace, workspace_bytes, w, stream))
             return rc;
+        a.tile_rows = paged_tokens_rows(d->head_dim, n_q * a.group, a.f16);
+        a.groups = paged_tokens_groups(d->head_dim, n_q * a.group, a.f16);
+        a.tiles = (n_q * a.group + a.tile_rows - 1) / a.tile_rows;
+        // the whole cost in 31 bits
+        const int64_t tiles = (int64_t)n_seqs * d->n_kv_heads * a.tiles;
+        while (tiles * ((a.cap / 32 >> a.shift) + 3) >= INT32_MAX) a.shift++;
         return launched(launch_paged_tokens(a, (hipStream_t)stream), W);
     });
 }

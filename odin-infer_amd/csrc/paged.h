@@ -56,7 +56,10 @@ struct PagedAttnArgs {
     uint32_t magic;                // ceil(2^32 / group), 0 for a group of 1
     int32_t n_seqs, n_q, n_rows;   // n_q: tokens of each sequence (tokens call)
     const int32_t *starts, *lens, *table;  // starts: prompts call
-    int32_t stride;                // entries of a table row
+    int32_t stride, cap;           // entries of a table row, and its slots
+    // tokens call: rows of an item, a sequence and kv head's items; log2 of the groups of waves
+    // and of the units that costs count
+    int32_t tile_rows, tiles, groups, shift;
     // workspace
     int32_t workers, part_rows;    // part_rows: rows of a partial result
     PagedAt *at;                   // [workers + 1], the last: {used workers, 0, 0, 0}
@@ -65,6 +68,9 @@ struct PagedAttnArgs {
 };
 // the workers of a call and the bytes that they take
 int paged_tokens_workers(int hd);
+// rows of an item, given those of a sequence and kv head, and log2 of its groups of waves
+int paged_tokens_rows(int hd, int rows, bool f16);
+int paged_tokens_groups(int hd, int rows, bool f16);
 int paged_prompts_workers(int hd, bool f16);
 int paged_prompts_tile(int hd, bool f16);  // rows of a tile
 hipError_t launch_paged_tokens(const PagedAttnArgs &a, hipStream_t st);

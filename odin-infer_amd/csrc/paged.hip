@@ -196,7 +196,7 @@ constexpr int APPEND_T = 8, APPEND_E = 512;  // packed rows and elements of a wo
 // 16-byte piece per dimension; it belongs to the workgroup of its first row.  64 rows
 // of 8 heads of 128 (f32) 4.4 us, one chain; 8231 f16 rows 19 us: 4 TB/s, the rate of a copy.
 template <bool F16>
-__global__ __launch_bounds__(WG) void paged_append_kernel(PagedAppendArgs a) {
+__global__ __launch_bounds__(WG, 4) void paged_append_kernel(PagedAppendArgs a) {
     constexpr int NR = 2 * APPEND_T - 1;
     const int t0 = blockIdx.x * APPEND_T, e0 = blockIdx.y * APPEND_E, tid = threadIdx.x, lane = tid & (WAVE - 1);
     const int wave = __builtin_amdgcn_readfirstlane(tid / WAVE);

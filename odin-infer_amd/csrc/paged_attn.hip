@@ -22,6 +22,7 @@
 // short ones keeps the whole card busy, and the grid and the workspace do not depend on
 // lengths: a captured call serves all of them.
 
+#include <algorithm>
 #include <cfloat>
 
 #include "device_common.h"
@@ -43,9 +44,8 @@ constexpr int PU = 64;                   // of the prompts kernel
 
 __device__ __forceinline__ float ex2(float x) { return __builtin_amdgcn_exp2f(x); }
 
-__device__ __forceinline__ int seq_len(const PagedAttnArgs &a, int s) {
-    return (int)min((int64_t)max(a.lens[s], 0), (int64_t)a.stride << a.c.lp);
-}
+// a number of the call's arrays, through the scalar cache where s is uniform
+__device__ __forceinline__ int seq_len(const PagedAttnArgs &a, int s) { return min(max(a.lens[s], 0), a.cap); }
 // The token of row r of a sequence and kv head (token-major): r / group by a
 // multiplication (exact while r * group < 2^32)
 __device__ __forceinline__ int row_token(const PagedAttnArgs &a, int r) {
@@ -63,83 +63,133 @@ __device__ __forceinline__ int page_ok(const PagedAttnArgs &a, int id) {
 
 // ------------------------------------------------------------- sharing out --
 
-// x / y of numbers below 2^53 (y > 0)
+__device__ __forceinline__ uint32_t quot(uint32_t x, uint32_t y) { return x / y; }
+// numbers below 2^53 (x >= 0, y > 0)
 __device__ __forceinline__ int64_t quot(int64_t x, int64_t y) {
+    if (((x | y) >> 32) == 0) return (uint32_t)x / (uint32_t)y;
     int64_t q = (int64_t)((double)x / (double)y);
     if (q * y > x) q--;
     else if ((q + 1) * y <= x) q++;
     return q;
 }
 
-// The tiles of a sequence and their costs.  Tokens: `tiles` alike.  Prompts: a tile
-// of R rows more sees R / group slots more, and costs are slots times the group.
-struct SeqWork {
-    int len, tokens, tiles;
-    int64_t first, step;  // a tile's cost: first + t * step
-    __device__ __forceinline__ int64_t upto(int64_t t) const { return t * first + step * (t * (t - 1) / 2); }
-};
+// The tiles of a sequence and their costs.
+// Tokens: tiles alike, costs in units (where 32 bits do not hold their sum, 2^shift of them).
 struct TokensWork {
-    static constexpr int OWN = 1, LEAST = 4, PARTS = 256;  // a tile's own cost, a worker's least, a tile's most parts
-    __device__ static __forceinline__ SeqWork of(const PagedAttnArgs &a, int s) {
-        SeqWork w;
-        w.len = seq_len(a, s);
-        w.tokens = a.n_q;
-        w.tiles = (a.n_q * a.group + 15) / 16;
-        w.first = (w.len + TU - 1) / TU + OWN;
-        w.step = 0;
-        return w;
+    using Cost = uint32_t;
+    static constexpr int UNIT = TU, OWN = 1, LEAST = 4, PARTS = 256;  // a tile's own cost, a worker's least, a tile's most parts
+    int len, tokens, tiles;
+    Cost first;
+    __device__ __forceinline__ TokensWork(const PagedAttnArgs &a, int s) {
+        len = seq_len(a, s);
+        tokens = a.n_q;
+        tiles = a.tiles;
+        first = ((uint32_t)((len + TU - 1) / TU + (1 << a.shift) - 1) >> a.shift) + OWN;
     }
-    __device__ static __forceinline__ int64_t unit(const PagedAttnArgs &) { return 1; }
-    __device__ static __forceinline__ int units(const PagedAttnArgs &, const SeqWork &w, int) {
-        return (w.len + TU - 1) / TU;
+    __device__ static __forceinline__ Cost unit(const PagedAttnArgs &) { return 1; }
+    __device__ __forceinline__ Cost all() const { return tiles * first; }
+    __device__ __forceinline__ Cost most() const { return first; }
+    __device__ __forceinline__ int units(const PagedAttnArgs &, int) const { return (len + TU - 1) / TU; }
+    // the tile that x falls into, and the unit there
+    __device__ __forceinline__ int find(const PagedAttnArgs &a, Cost x, int &u) const {
+        const Cost t = quot(x, first), in = x - t * first;
+        u = in <= (Cost)OWN ? 0 : (int)min((in - OWN) << a.shift, (Cost)units(a, 0));
+        return (int)t;
     }
+    __device__ static __forceinline__ int near(const PagedAttnArgs &a, Cost share) { return (int)(share / 8 << a.shift); }
 };
+// Prompts: a tile of R rows more sees R / group slots more; costs are slots times the group.
 template <int R>
 struct PromptsWork {
-    static constexpr int OWN = 1, LEAST = 4, PARTS = 128;
-    __device__ static __forceinline__ SeqWork of(const PagedAttnArgs &a, int s) {
-        SeqWork w;
+    using Cost = int64_t;
+    static constexpr int UNIT = PU, OWN = 1, LEAST = 4, PARTS = 128;
+    int len, tokens, tiles;
+    Cost first;  // of tile 0, each further one R more
+    __device__ __forceinline__ PromptsWork(const PagedAttnArgs &a, int s) {
         const int r0 = min(max(a.starts[s], 0), a.n_rows), r1 = min(max(a.starts[s + 1], r0), a.n_rows);
-        w.len = seq_len(a, s);
-        w.tokens = r1 - r0;
-        w.tiles = (int)(((int64_t)w.tokens * a.group + R - 1) / R);
-        w.first = (int64_t)a.group * (max(w.len - w.tokens, 0) + OWN * PU) + R;
-        w.step = R;
-        return w;
+        len = seq_len(a, s);
+        tokens = r1 - r0;
+        tiles = (int)(((int64_t)tokens * a.group + R - 1) / R);
+        first = (int64_t)a.group * (max(len - tokens, 0) + OWN * PU) + R;
     }
-    __device__ static __forceinline__ int64_t unit(const PagedAttnArgs &a) { return (int64_t)a.group * PU; }
-    __device__ static __forceinline__ int units(const PagedAttnArgs &a, const SeqWork &w, int tile) {
-        const int last = row_token(a, min(tile * R + R, w.tokens * a.group) - 1);
-        return (max(w.len - w.tokens + last + 1, 0) + PU - 1) / PU;
+    __device__ static __forceinline__ Cost unit(const PagedAttnArgs &a) { return (int64_t)a.group * PU; }
+    __device__ __forceinline__ Cost upto(int64_t t) const { return t * first + R * (t * (t - 1) / 2); }
+    __device__ __forceinline__ Cost all() const { return upto(tiles); }
+    __device__ __forceinline__ Cost most() const { return tiles ? first + (int64_t)(tiles - 1) * R : 0; }
+    __device__ __forceinline__ int units(const PagedAttnArgs &a, int tile) const {
+        const int last = row_token(a, min(tile * R + R, tokens * a.group) - 1);
+        return (max(len - tokens + last + 1, 0) + PU - 1) / PU;
     }
+    __device__ __forceinline__ int find(const PagedAttnArgs &a, Cost x, int &u) const {
+        // the last t with upto(t) <= x
+        const float b = (float)first - 0.5f * R;
+        int64_t t = (int64_t)((sqrtf(b * b + 2.f * R * (float)x) - b) * (1.f / R));
+        t = min(max(t, (int64_t)0), (int64_t)tiles - 1);
+        while (t > 0 && upto(t) > x) t--;
+        while (t + 1 < tiles && upto(t + 1) <= x) t++;
+        const int64_t in = x - upto(t), own = OWN * unit(a);
+        u = in <= own ? 0 : (int)quot((in - own) * units(a, (int)t), first + t * R - own);
+        return (int)t;
+    }
+    __device__ static __forceinline__ int near(const PagedAttnArgs &a, Cost share) { return (int)quot(share, 8 * unit(a)); }
 };
 
-// The border at x of the whole cost: sequence s holds it, x less the sequences before.
-template <class W>
-__device__ PagedAt border(const PagedAttnArgs &a, int s, int64_t x, int64_t share) {
-    const SeqWork w = W::of(a, s);
-    const int64_t one = w.upto(w.tiles), u1 = W::unit(a);
-    int head = (int)quot(x, one);
-    x -= head * one;
-    // the last tile with upto(t) <= x
-    int64_t t;
-    if (w.step == 0) {
-        t = quot(x, w.first);
-    } else {
-        const double b = (double)w.first - 0.5 * w.step;
-        t = (int64_t)((sqrt(b * b + 2.0 * w.step * x) - b) / w.step);
-        t = min(max(t, (int64_t)0), (int64_t)w.tiles - 1);
-        while (t > 0 && w.upto(t) > x) t--;
-        while (t + 1 < w.tiles && w.upto(t + 1) <= x) t++;
+// Sums over the lanes up to each, and a lane's value for all.
+__device__ __forceinline__ uint32_t scan_lanes(uint32_t v) {
+#define OI_SCAN(ctrl, rows) v += (uint32_t)__builtin_amdgcn_update_dpp(0, (int)v, ctrl, rows, 0xF, false)
+    OI_SCAN(0x111, 0xF);  // rows of 16: 1, 2, 4, 8 lanes back
+    OI_SCAN(0x112, 0xF);
+    OI_SCAN(0x114, 0xF);
+    OI_SCAN(0x118, 0xF);
+    OI_SCAN(0x142, 0xA);  // the last lane of rows 0 and 2 to the row behind
+    OI_SCAN(0x143, 0xC);  // lane 31 to rows 2 and 3
+#undef OI_SCAN
+    return v;
+}
+__device__ __forceinline__ int64_t scan_lanes(int64_t v) {
+#pragma unroll
+    for (int d = 1; d < WAVE; d *= 2) {
+        const int64_t o = __shfl_up(v, d);
+        if ((int)__lane_id() >= d) v += o;
     }
-    const int64_t in = x - w.upto(t), cost = w.first + t * w.step, own = W::OWN * u1;
-    const int units = W::units(a, w, (int)t);
-    int u = in <= own ? 0 : (int)quot((in - own) * units, cost - own);
-    const int near = (int)quot(share, 8 * u1);
-    int tile = (int)t;
+    return v;
+}
+__device__ __forceinline__ uint32_t of_lane(uint32_t v, int i) { return (uint32_t)__builtin_amdgcn_readlane((int)v, i); }
+__device__ __forceinline__ int64_t of_lane(int64_t v, int i) {
+    return (int64_t)((uint64_t)of_lane((uint32_t)((uint64_t)v >> 32), i) << 32 | of_lane((uint32_t)(uint64_t)v, i));
+}
+
+// The border at x of the whole cost (below its end), given each lane's sum of `per`
+// neighbouring sequences (own) and that of the lanes up to it (run).
+template <class W>
+__device__ PagedAt border(const PagedAttnArgs &a, typename W::Cost x, typename W::Cost share, typename W::Cost own,
+                          typename W::Cost run, int per) {
+    using Cost = typename W::Cost;
+    const int lane = __lane_id();
+    int at = __ffsll((unsigned long long)__ballot(x < run)) - 1;
+    x -= of_lane(run, at) - of_lane(own, at);
+    int s = at * per;
+    if (per > 1) {  // these sequences, a lane each
+        for (int s1 = min(s + per, a.n_seqs);; s += WAVE) {
+            const Cost c = s + lane < s1 ? W(a, min(s + lane, s1 - 1)).all() * a.c.n_kv : (Cost)0, r = scan_lanes(c);
+            const unsigned long long hit = __ballot(x < r);
+            if (hit) {
+                at = __ffsll(hit) - 1;
+                x -= of_lane(r, at) - of_lane(c, at);
+                s += at;
+                break;
+            }
+            x -= of_lane(r, WAVE - 1);
+        }
+    }
+    const W w(a, s);
+    const Cost one = w.all();
+    int head = (int)quot(x, one), u;
+    int tile = w.find(a, x - head * one, u);
+    const int near = W::near(a, share);
     if (u <= near) {
         u = 0;
-    } else if (units - u <= near) {
+    } else if (w.units(a, tile) - u <= near) {
         u = 0;
         if (++tile == w.tiles) {
             tile = 0;
@@ -149,80 +199,41 @@ __device__ PagedAt border(const PagedAttnArgs &a, int s, int64_t x, int64_t shar
             }
         }
     }
-    return {s, head, tile, u};
+    return {__builtin_amdgcn_readfirstlane(s), __builtin_amdgcn_readfirstlane(head), __builtin_amdgcn_readfirstlane(tile),
+            __builtin_amdgcn_readfirstlane(u)};
 }
 
-struct ShareLds {
-    int64_t sum[WG / WAVE];
-    int64_t most[WG / WAVE];
-    PagedAt at[2];
-};
-// Worker's stretch, [at[0], at[1]); the number of workers used is returned.  All WG
-// threads take part; each sums a run of neighbouring sequences.  `spread`: neighbouring
-// workers go to one XCD (blocks are dealt to the 8 in turn), whose cache then holds
-// what they share.
+// A worker's stretch, [begin, end); the number of workers used is returned (this one is
+// idle if it is not below).  Every wave does it for itself, without LDS: a lane sums a run
+// of neighbouring sequences.  SPREAD: neighbouring workers go to one XCD (blocks are
+// dealt to the 8 in turn), whose cache then holds what they share.
 template <class W, bool SPREAD>
-__device__ int share_out(const PagedAttnArgs &a, ShareLds &lds, int &worker) {
-    const int tid = threadIdx.x, lane = tid & (WAVE - 1), wave = tid / WAVE;
-    const int per = (a.n_seqs + WG - 1) / WG, s0 = min(tid * per, a.n_seqs), s1 = min(s0 + per, a.n_seqs);
-    int64_t sum = 0, most = 0;
+__device__ int share_out(const PagedAttnArgs &a, int &worker, PagedAt &begin, PagedAt &end) {
+    using Cost = typename W::Cost;
+    const int lane = __lane_id(), per = (a.n_seqs + WAVE - 1) / WAVE;
+    const int s0 = min(lane * per, a.n_seqs), s1 = min(s0 + per, a.n_seqs);
+    Cost own = 0, most = 0;
     for (int s = s0; s < s1; s++) {
-        const SeqWork w = W::of(a, s);
-        sum += w.upto(w.tiles) * a.c.n_kv;
-        if (w.tiles) most = max(most, w.first + (w.tiles - 1) * w.step);
+        const W w(a, s);
+        own += w.all() * a.c.n_kv;
+        most = max(most, w.most());
     }
-    int64_t run = sum;
-#pragma unroll
-    for (int d = 1; d < WAVE; d *= 2) {
-        const int64_t o = __shfl_up(run, d);
-        if (lane >= d) run += o;
-        most = max(most, (int64_t)__shfl_xor(most, d));
+    const Cost run = scan_lanes(own), total = of_lane(run, WAVE - 1);
+    Cost share = max(quot((Cost)(total + a.workers - 1), (Cost)a.workers), (Cost)(W::LEAST * W::unit(a)));
+    // a tile that would have more than PARTS parts
+    for (unsigned long long m = __ballot(most > share * W::PARTS); m; m = __ballot(most > share * W::PARTS)) {
+        const Cost x = of_lane(most, __ffsll(m) - 1);
+        share = quot((Cost)(x + W::PARTS - 1), (Cost)W::PARTS);
     }
-    if (lane == WAVE - 1) {
-        lds.sum[wave] = run;
-        lds.most[wave] = most;
-    }
-    if (tid < 2) lds.at[tid] = {a.n_seqs, 0, 0, 0};
-    __syncthreads();
-    int64_t before = 0, total = 0;
-    most = 0;
-#pragma unroll
-    for (int w = 0; w < WG / WAVE; w++) {
-        const int64_t x = lds.sum[w];
-        before += w < wave ? x : 0;
-        total += x;
-        most = max(most, lds.most[w]);
-    }
-    run += before - sum;  // the sequences before this thread's
-    int64_t share = quot(total + a.workers - 1, a.workers);
-    share = max(share, max(W::LEAST * W::unit(a), quot(most + W::PARTS - 1, (int64_t)W::PARTS)));
-    const int used = (int)quot(total + share - 1, share);
+    const int used = (int)quot((Cost)(total + share - 1), share);
     const int each = (used + 7) / 8, b = blockIdx.x;
     worker = SPREAD ? (b / 8 < each ? (b & 7) * each + b / 8 : used) : b;
     if (worker < used) {
-#pragma unroll
-        for (int k = 0; k < 2; k++) {
-            int64_t x = (worker + k) * share;
-            if (x < run || x >= run + sum) continue;  // past the end of all: as set
-            x -= run;
-            for (int s = s0; s < s1; s++) {
-                const SeqWork w = W::of(a, s);
-                const int64_t c = w.upto(w.tiles) * a.c.n_kv;
-                if (x < c) {
-                    lds.at[k] = border<W>(a, s, x, share);
-                    break;
-                }
-                x -= c;
-            }
-        }
+        begin = border<W>(a, (Cost)worker * share, share, own, run, per);
+        end = {a.n_seqs, 0, 0, 0};
+        if (worker + 1 < used) end = border<W>(a, (Cost)(worker + 1) * share, share, own, run, per);
     }
-    __syncthreads();
-    return used;
-}
-// the same in every lane, in scalar registers
-__device__ __forceinline__ PagedAt uniform(const PagedAt &x) {
-    return {__builtin_amdgcn_readfirstlane(x.seq), __builtin_amdgcn_readfirstlane(x.head),
-            __builtin_amdgcn_readfirstlane(x.tile), __builtin_amdgcn_readfirstlane(x.u)};
+    return __builtin_amdgcn_readfirstlane(used);
 }
 __device__ __forceinline__ bool same_tile(const PagedAt &x, const PagedAt &y) {
     return x.seq == y.seq && x.head == y.head && x.tile == y.tile;
@@ -241,9 +252,9 @@ template <class W, class F>
 __device__ __forceinline__ void each_piece(const PagedAttnArgs &a, PagedAt at, const PagedAt end, F f) {
     while (at.seq < end.seq || (at.seq == end.seq && (at.head < end.head || (at.head == end.head &&
                                (at.tile < end.tile || (at.tile == end.tile && at.u < end.u)))))) {
-        const SeqWork w = W::of(a, at.seq);
+        const W w(a, at.seq);
         if (w.tiles) {
-            const int units = W::units(a, w, at.tile);
+            const int units = w.units(a, at.tile);
             f(w, at, units, at.u, same_tile(at, end) ? end.u : units);
         }
         at.u = 0;
@@ -314,13 +325,15 @@ struct QPieces {
             }
             amax = reduce(amax);
             e = ok && amax > 0.f ? (int)(__float_as_uint(amax) >> 23) - 127 - 14 : 0;
+            // 2^-e as two factors that f32 holds, the sign in one; 0 for no row
+            const float s0 = ok ? ldexpf(neg ? -1.f : 1.f, -e / 2) : 0.f, s1 = ldexpf(1.f, -e - -e / 2);
 #pragma unroll
             for (int f = 0; f < NF; f++) {  // read again: the row is in cache, its registers are not free
                 const f32x4 u = *(const f32x4 *)(p + PART * f), w = *(const f32x4 *)(p + PART * f + 4);
 #pragma unroll
                 for (int i = 0; i < 8; i++) {
                     const float x = i < 4 ? u[i & 3] : w[i & 3];
-                    const float y = ok ? ldexpf(neg ? -x : x, -e) : 0.f;
+                    const float y = x * s0 * s1;
                     const _Float16 t = (_Float16)y;
                     hi[f][i] = t;
                     lo[f][i] = (_Float16)(y - (float)t);
@@ -352,30 +365,37 @@ __device__ __forceinline__ float inverse(float l) { return l == 0.f ? 0.f : 1.f 
 // 16 bytes a lane without LDS; K of the next unit is requested when this one's scores
 // are done, V when its product is, pages one unit ahead of both.  The maximum is raised
 // to whole numbers, so rescaling is exact.
-template <int HD, bool F16>
-__global__ __launch_bounds__(WG) void paged_tokens_kernel(PagedAttnArgs a) {
-    constexpr int NW = WG / WAVE, NK = HD / 32, ND = HD / 16, PD = HD + 4, R = 16, TPR = WG / R;
-    __shared__ __attribute__((aligned(16))) float so[NW][R][PD];
-    __shared__ float sm[NW][R], sl[NW][R];
-    __shared__ ShareLds share;
+// Workgroups of a CU, as registers allow.
+template <int HD, bool F16, int NT>
+struct TokensShape {
+    static constexpr int PER_CU = HD == 128 ? 2 : 1;
+};
+template <int HD, bool F16, int NT, bool GROUPS>
+__global__ __launch_bounds__(WG, (TokensShape<HD, F16, NT>::PER_CU)) void paged_tokens_kernel(PagedAttnArgs a) {
+    constexpr int NW = WG / WAVE, NK = HD / 32, ND = HD / 16, PD = HD + 4;
+    using W = TokensWork;
+    __shared__ __attribute__((aligned(16))) float so[NW][16][PD];
+    __shared__ float sm[NW][16], sl[NW][16];
     int worker;
-    const int used = share_out<TokensWork, false>(a, share, worker);
+    PagedAt begin, end;
+    const int used = share_out<W, true>(a, worker, begin, end);
     const int tid = threadIdx.x, lane = tid & (WAVE - 1), wave = tid / WAVE;
     if (blockIdx.x == 0 && tid == 0) a.at[a.workers] = {used, 0, 0, 0};
     if (worker >= used) return;
-    const PagedAt begin = uniform(share.at[0]), end = uniform(share.at[1]);
     leave_border(a, worker, begin, end);
     const int c = lane & 15, g = lane >> 4, lp = a.c.lp, P = 1 << lp;
     const bool neg = a.scale < 0.f;
     const float scale = fabsf(a.scale);
-    const int kslot = 8 * (c >> 2) + (c & 3);  // of tile 0; 4 more in tile 1
+    const int kslot = 8 * (c >> 2) + (c & 3);  // of a product's first 16 slots; 4 more in its second
     const size_t page_elems = ((size_t)a.c.n_kv << lp) * HD;
+    const int rows = a.n_q * a.group;
+    const int lg = GROUPS ? a.groups : 0, ng = 1 << lg;  // groups of waves
+    const int group = wave & (ng - 1), turn = wave >> lg, step = NW >> lg;
 
-    each_piece<TokensWork>(a, begin, end, [&](const SeqWork &w, const PagedAt &at, int units, int u0, int u1) {
-        const int rows = a.n_q * a.group, rt = at.tile, len = w.len;
-        const int row = rt * R + c, rr = min(row, rows - 1);
-        const int limit = len - a.n_q + row_token(a, rr) + 1;  // slots that this row sees
-        const int first_limit = len - a.n_q + row_token(a, rt * R) + 1;
+    each_piece<W>(a, begin, end, [&](const W &w, const PagedAt &at, int units, int u0, int u1) {
+        const int row0 = at.tile * a.tile_rows + 16 * NT * group;
+        const int len = w.len, seen0 = len - a.n_q + 1;  // slots that the first token sees
+        const int first_limit = seen0 + row_token(a, min(row0, rows - 1));
         const int32_t *table = a.table + (int64_t)at.seq * a.stride;
         const uint16_t *kb = a.c.k + ((size_t)at.head << lp) * HD + 8 * g;
         const uint16_t *vb = a.c.v + ((size_t)at.head << lp) * HD + 8 * c;
@@ -398,72 +418,88 @@ __global__ __launch_bounds__(WG) void paged_tokens_kernel(PagedAttnArgs a) {
 #pragma unroll
             for (int d = 0; d < ND; d++) vr[d] = *(const u32x4 *)(p + 16 * d * 8);
         };
-        float m = NEG, l = 0.f;
-        f32x4 o[ND];
-#pragma unroll
-        for (int d = 0; d < ND; d++) o[d] = f32x4{0.f, 0.f, 0.f, 0.f};
-        int u = u0 + wave;
+        float m[NT], l[NT], mul[NT];
+        int limit[NT];  // slots that this lane's rows see
+        f32x4 o[NT][ND];
+        int u = row0 < rows ? u0 + turn : u1;
         if (u < u1) {
             pages(u, kp, vp);
-            if (u + NW < u1) pages(u + NW, kn, vn);
+            if (u + step < u1) pages(u + step, kn, vn);
         }
-        QPieces<NK, 32, F16> q;
-        q.load(a.q, row_at(a, at.seq * a.n_q, rr, at.head, a.q_stride) + 8 * g, row < rows, neg,
-               [](float x) { return col_reduce(x, Max()); });
+        QPieces<NK, 32, F16> q[NT];
+#pragma unroll
+        for (int n = 0; n < NT; n++) {
+            const int row = row0 + 16 * n + c, rr = min(row, rows - 1);
+            limit[n] = seen0 + row_token(a, rr);
+            q[n].load(a.q, row_at(a, at.seq * a.n_q, rr, at.head, a.q_stride) + 8 * g, row < rows, neg,
+                      [](float x) { return col_reduce(x, Max()); });
+            mul[n] = fmaxf(ldexpf(scale, q[n].e), FLT_MIN);  // above 0: -inf stays -inf
+            m[n] = NEG;
+            l[n] = 0.f;
+#pragma unroll
+            for (int d = 0; d < ND; d++) o[n][d] = f32x4{0.f, 0.f, 0.f, 0.f};
+        }
         if (u < u1) {
             load_k(u);
             load_v(u, vp);
         }
-        const float mul = fmaxf(ldexpf(scale, q.e), FLT_MIN);  // above 0: -inf stays -inf
-        for (; u < u1; u += NW) {
-            f32x4 s[2];
+        for (; u < u1; u += step) {
+            f32x4 s[NT][2];
 #pragma unroll
-            for (int t = 0; t < 2; t++) {
-                s[t] = f32x4{0.f, 0.f, 0.f, 0.f};
+            for (int n = 0; n < NT; n++)
+#pragma unroll
+                for (int t = 0; t < 2; t++) s[n][t] = f32x4{0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+            for (int t = 0; t < 2; t++)
 #pragma unroll
                 for (int f = 0; f < NK; f++) {
                     const f16x8 k = __builtin_bit_cast(f16x8, kr[t][f]);
-                    s[t] = mfma(k, q.hi[f], s[t]);
-                    if constexpr (!F16) s[t] = mfma(k, q.lo[f], s[t]);
+#pragma unroll
+                    for (int n = 0; n < NT; n++) {
+                        s[n][t] = mfma(k, q[n].hi[f], s[n][t]);
+                        if constexpr (!F16) s[n][t] = mfma(k, q[n].lo[f], s[n][t]);
+                    }
                 }
-            }
             kp = kn;
-            if (u + NW < u1) load_k(u + NW);
-            const int p0 = u * TU + 8 * g;  // the slot of s[0][0]
-            if (u * TU + TU > first_limit) {  // some row does not see all of the unit
+            if (u + step < u1) load_k(u + step);
+            const int p0 = u * TU + 8 * g;  // the slot of s[n][0][0]
+            f16x8 ph[NT], pl[NT];
+#pragma unroll
+            for (int n = 0; n < NT; n++) {
+                if (u * TU + TU > first_limit) {  // some row does not see all of the unit
+#pragma unroll
+                    for (int t = 0; t < 2; t++)
+#pragma unroll
+                        for (int i = 0; i < 4; i++)
+                            if (p0 + 4 * t + i >= limit[n]) s[n][t][i] = -INFINITY;
+                }
+                float top = s[n][0][0];
 #pragma unroll
                 for (int t = 0; t < 2; t++)
 #pragma unroll
-                    for (int i = 0; i < 4; i++)
-                        if (p0 + 4 * t + i >= limit) s[t][i] = -INFINITY;
-            }
-            float top = s[0][0];
+                    for (int i = 0; i < 4; i++) top = fmaxf(top, s[n][t][i]);
+                top = col_reduce(top * mul[n], Max());
+                const float m1 = fmaxf(m[n], ceilf(top));
+                float sum = 0.f;
 #pragma unroll
-            for (int t = 0; t < 2; t++)
+                for (int t = 0; t < 2; t++)
 #pragma unroll
-                for (int i = 0; i < 4; i++) top = fmaxf(top, s[t][i]);
-            top = col_reduce(top * mul, Max());
-            const float m1 = fmaxf(m, ceilf(top));
-            f16x8 ph, pl;
-            float sum = 0.f;
+                    for (int i = 0; i < 4; i++) {
+                        const float p = ex2(fmaf(s[n][t][i], mul[n], -m1)) * 32768.f;
+                        sum += p;
+                        const _Float16 h = (_Float16)p;
+                        ph[n][4 * t + i] = h;
+                        pl[n][4 * t + i] = (_Float16)(p - (float)h);
+                    }
+                if (__any(m1 != m[n])) {  // a row's maximum rose
+                    const float alpha = ex2(m[n] - m1);
+                    l[n] *= alpha;
 #pragma unroll
-            for (int t = 0; t < 2; t++)
-#pragma unroll
-                for (int i = 0; i < 4; i++) {
-                    const float p = ex2(fmaf(s[t][i], mul, -m1)) * 32768.f;
-                    sum += p;
-                    const _Float16 h = (_Float16)p;
-                    ph[4 * t + i] = h;
-                    pl[4 * t + i] = (_Float16)(p - (float)h);
+                    for (int d = 0; d < ND; d++) o[n][d] *= alpha;
+                    m[n] = m1;
                 }
-            if (__any(m1 != m)) {  // a row's maximum rose
-                const float alpha = ex2(m - m1);
-                l *= alpha;
-#pragma unroll
-                for (int d = 0; d < ND; d++) o[d] *= alpha;
-                m = m1;
+                l[n] += sum;
             }
-            l += sum;
             if (u * TU + TU > len) {  // bytes behind the sequence's end count for nothing
                 u32x4 keep;
 #pragma unroll
@@ -475,119 +511,220 @@ __global__ __launch_bounds__(WG) void paged_tokens_kernel(PagedAttnArgs a) {
 #pragma unroll
             for (int d = 0; d < ND; d++) {
                 const f16x8 v = __builtin_bit_cast(f16x8, vr[d]);
-                o[d] = mfma(v, ph, o[d]);
-                o[d] = mfma(v, pl, o[d]);
+#pragma unroll
+                for (int n = 0; n < NT; n++) o[n][d] = mfma(v, ph[n], o[n][d]);
+#pragma unroll
+                for (int n = 0; n < NT; n++) o[n][d] = mfma(v, pl[n], o[n][d]);
             }
-            if (u + NW < u1) {
-                load_v(u + NW, vn);
-                if (u + 2 * NW < u1) pages(u + 2 * NW, kn, vn);
+            if (u + step < u1) {
+                load_v(u + step, vn);
+                if (u + 2 * step < u1) pages(u + 2 * step, kn, vn);
             }
         }
-        // the four waves' results meet in LDS
-        l = col_reduce(l, Add());
+        // the waves' results meet in LDS, 16 rows of each group at a time
+        const bool whole = u0 == 0 && u1 == units;
 #pragma unroll
-        for (int d = 0; d < ND; d++) *(f32x4 *)&so[wave][c][16 * d + 4 * g] = o[d];
-        if (g == 0) {
-            sm[wave][c] = m;
-            sl[wave][c] = l;
-        }
-        __syncthreads();
-        const int r = tid / TPR, gr = rt * R + r;  // TPR threads a row from here on
-        if (gr < rows) {
-            float M = NEG, wt[NW], L = 0.f;
+        for (int n = 0; n < NT; n++) {
+            if (n > 0 && at.tile * a.tile_rows + 16 * n >= rows) break;
+            const float ls = col_reduce(l[n], Add());
 #pragma unroll
-            for (int k = 0; k < NW; k++) M = fmaxf(M, sm[k][r]);
-#pragma unroll
-            for (int k = 0; k < NW; k++) {
-                wt[k] = ex2(sm[k][r] - M);
-                L += sl[k][r] * wt[k];
+            for (int d = 0; d < ND; d++) *(f32x4 *)&so[wave][c][16 * d + 4 * g] = o[n][d];
+            if (g == 0) {
+                sm[wave][c] = m[n];
+                sl[wave][c] = ls;
             }
-            const bool whole = u0 == 0 && u1 == units;
-            const size_t slot = ((size_t)worker * 2 + (u0 == 0)) * a.part_rows + r;
-            const float inv = whole ? inverse(L) : 1.f;
-            const int64_t to = row_at(a, at.seq * a.n_q, gr, at.head, a.out_stride);
+            __syncthreads();
+            // a group's rows over its `step` waves, 4 step threads a row
+            const int tpr = 16 >> lg, tr = tid & ((WG >> lg) - 1), r = tr >> (4 - lg), sg = tid >> (8 - lg);
+            const int row = 16 * (NT * sg + n) + r, gr = at.tile * a.tile_rows + row;
+            if (gr < rows) {
+                float M = NEG, wt[NW], L = 0.f;
 #pragma unroll
-            for (int d = 4 * (tid % TPR); d < HD; d += 4 * TPR) {
-                f32x4 y = {0.f, 0.f, 0.f, 0.f};
+                for (int k = 0; k < NW; k++)
+                    if (k < step) M = fmaxf(M, sm[sg + k * ng][r]);
 #pragma unroll
-                for (int k = 0; k < NW; k++) y += *(const f32x4 *)&so[k][r][d] * wt[k];
-                y *= inv;
-                if (whole) store_out(a.out, F16, to + d, y);
-                else *(f32x4 *)(a.part + slot * HD + d) = y;
+                for (int k = 0; k < NW; k++)
+                    if (k < step) {
+                        wt[k] = ex2(sm[sg + k * ng][r] - M);
+                        L += sl[sg + k * ng][r] * wt[k];
+                    }
+                const size_t slot = ((size_t)worker * 2 + (u0 == 0)) * a.part_rows + row;
+                const float inv = whole ? inverse(L) : 1.f;
+                const int64_t to = row_at(a, at.seq * a.n_q, gr, at.head, a.out_stride);
+                for (int d = 4 * (tr & (tpr - 1)); d < HD; d += 4 * tpr) {
+                    f32x4 y = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+                    for (int k = 0; k < NW; k++)
+                        if (k < step) y += *(const f32x4 *)&so[sg + k * ng][r][d] * wt[k];
+                    y *= inv;
+                    if (whole) store_out(a.out, F16, to + d, y);
+                    else *(f32x4 *)(a.part + slot * HD + d) = y;
+                }
+                if (!whole && (tr & (tpr - 1)) == 0) a.ml[slot] = make_float2(M, L);
             }
-            if (!whole && tid % TPR == 0) a.ml[slot] = make_float2(M, L);
+            __syncthreads();  // LDS is read before it is written again
         }
-        __syncthreads();  // LDS is read before the next piece is written there
     });
 }
 
 // ------------------------------------------------------------------- join --
 
 // The parts of a tile that the border behind worker w cuts first: part 1 of w, then
-// part 0 of the workers after it while they begin inside the tile.  A workgroup takes
-// `JR` of its rows.
-constexpr int JR = 8;
-template <class W, int HD, int R>
-__global__ __launch_bounds__(WG) void paged_join_kernel(PagedAttnArgs a) {
-    constexpr int LPR = HD / 4, MS = WG / LPR;  // lanes of a row, parts at a time
-    __shared__ int parts;
+// part 0 of the workers after it while they begin inside the tile.
+__device__ __forceinline__ bool first_cut(const PagedAt &at, const PagedAt &prev) {
+    return at.u > 0 && !(same_tile(at, prev) && prev.u > 0);
+}
+
+// A row of a tile, whose parts may be many: a workgroup takes it.  BY_TILE: a workgroup
+// per tile (few of them) looks for the border in it; otherwise per border.  (m, l) and the
+// first results of every thread are requested together.
+constexpr int JPRE = 8;  // parts of a thread in the first round trip
+template <int HD, bool BY_TILE>
+__global__ __launch_bounds__(WG, 4) void paged_join_kernel(PagedAttnArgs a) {
+    constexpr int LPR = HD / 4, MS = WG / LPR, MOST = 512, KP = MOST / WG;  // lanes of a row, parts at a time
+    constexpr int NB = BY_TILE ? 2 : KP;                                    // borders of a thread
+    static_assert(TokensWork::PARTS + 2 <= MOST, "a tile's parts fit");
+    __shared__ float wt[MOST];
     __shared__ __attribute__((aligned(16))) float red[MS][HD];
-    __shared__ float redl[MS], redm[MS];
-    const int w = blockIdx.x, tid = threadIdx.x, used = a.at[a.workers].seq;
-    if (w + 1 >= used) return;
-    const PagedAt at = a.at[w + 1], prev = a.at[w];
-    if (at.u == 0 || (same_tile(at, prev) && prev.u > 0)) return;
-    const SeqWork sw = W::of(a, at.seq);
-    const int rows = min(sw.tokens * a.group - at.tile * R, R), r0 = blockIdx.y * JR;
-    if (r0 >= rows) return;
-    if (tid == 0) parts = 1;
-    __syncthreads();
-    int n = 0;
-    for (int k = w + 1 + tid; k < used; k += WG) {
-        const PagedAt x = a.at[k];
-        if (!same_tile(x, at) || x.u == 0) break;
-        n++;
+    __shared__ float wmax[WG / WAVE], wsum[WG / WAVE];
+    __shared__ int count[WG / WAVE], least[WG / WAVE];
+    const int r = blockIdx.y, tid = threadIdx.x, lane = tid & (WAVE - 1), wave = tid / WAVE;
+    const int used = a.at[a.workers].seq;
+    PagedAt at;
+    int w0 = blockIdx.x;  // the border looked at first is w0 + 1
+    if constexpr (BY_TILE) {
+        const int head = (int)((uint32_t)blockIdx.x / (uint32_t)a.tiles), seq = (int)((uint32_t)head / (uint32_t)a.c.n_kv);
+        at = {seq, head - seq * a.c.n_kv, (int)blockIdx.x - head * a.tiles, 0};
+        w0 = 0;
+    } else {
+        at = a.at[w0 + 1];
+        const PagedAt prev = a.at[w0];
+        if (w0 + 1 >= used || !first_cut(at, prev)) return;
     }
-    if (n) atomicAdd(&parts, n);
+    if (r >= a.n_q * a.group - at.tile * a.tile_rows) return;
+    // borders inside the tile are neighbours
+    int n = 0, first = INT32_MAX;
+#pragma unroll
+    for (int i = 0; i < NB; i++) {
+        const int k = w0 + 1 + tid + i * WG;
+        const PagedAt x = k < a.workers ? a.at[k] : PagedAt{-1, 0, 0, 0};
+        const unsigned long long in = __ballot(k < used && same_tile(x, at) && x.u > 0);
+        n += __popcll(in);
+        if (in) first = min(first, k - lane + __ffsll(in) - 1);
+    }
+    if (lane == 0) {
+        count[wave] = n;
+        least[wave] = first;
+    }
     __syncthreads();
-    n = parts;
-    const int base = a.starts ? min(max(a.starts[at.seq], 0), a.n_rows) : at.seq * a.n_q;
+    n = 0;
+#pragma unroll
+    for (int i = 0; i < WG / WAVE; i++) {
+        n += count[i];
+        first = min(first, least[i]);
+    }
+    if (n == 0) return;
+    n++;
+    const int w = first - 1;  // its part 1, then part 0 of those behind it
+    auto slot = [&](int k) { return ((size_t)(w + k) * 2 + (k == 0)) * a.part_rows + r; };
+    float2 ml[KP];
+    f32x4 pre[JPRE];
     const int col = tid % LPR, k0 = tid / LPR;
-    for (int r = r0; r < min(r0 + JR, rows); r++) {
-        float M = NEG, L = 0.f;
-        f32x4 y = {0.f, 0.f, 0.f, 0.f};
-        for (int k = k0; k < n; k += MS) {
+#pragma unroll
+    for (int i = 0; i < KP; i++) ml[i] = tid + i * WG < n ? a.ml[slot(tid + i * WG)] : make_float2(NEG, 0.f);
+#pragma unroll
+    for (int i = 0; i < JPRE; i++) {
+        const int k = k0 + i * MS;
+        pre[i] = k < n ? *(const f32x4 *)(a.part + slot(k) * HD + 4 * col) : f32x4{0.f, 0.f, 0.f, 0.f};
+    }
+    float m = NEG;
+#pragma unroll
+    for (int i = 0; i < KP; i++) m = fmaxf(m, ml[i].x);
+    m = wave_max_all(m);
+    if (lane == 0) wmax[wave] = m;
+    __syncthreads();
+#pragma unroll
+    for (int i = 0; i < WG / WAVE; i++) m = fmaxf(m, wmax[i]);
+    float l = 0.f;
+#pragma unroll
+    for (int i = 0; i < KP; i++) {
+        const float f = ex2(ml[i].x - m);
+        // 0 for a part that saw nothing (an empty one has no results to read)
+        if (tid + i * WG < n) wt[tid + i * WG] = ml[i].y == 0.f ? 0.f : f;
+        l += ml[i].y * f;
+    }
+    l = wave_sum(l);
+    if (lane == 0) wsum[wave] = l;
+    __syncthreads();
+    l = 0.f;
+#pragma unroll
+    for (int i = 0; i < WG / WAVE; i++) l += wsum[i];
+    f32x4 y = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+    for (int i = 0; i < JPRE; i++) {
+        const float f = k0 + i * MS < n ? wt[k0 + i * MS] : 0.f;
+        if (f != 0.f) y += pre[i] * f;
+    }
+#pragma unroll 8
+    for (int k = k0 + JPRE * MS; k < n; k += MS) {
+        const f32x4 p = *(const f32x4 *)(a.part + slot(k) * HD + 4 * col);
+        const float f = wt[k];
+        if (f != 0.f) y += p * f;
+    }
+    *(f32x4 *)&red[k0][4 * col] = y;
+    __syncthreads();
+    if (tid < LPR) {
+#pragma unroll
+        for (int k = 1; k < MS; k++) y += *(const f32x4 *)&red[k][4 * col];
+        store_out(a.out, a.f16, row_at(a, at.seq * a.n_q, at.tile * a.tile_rows + r, at.head, a.out_stride) + 4 * col,
+                  y * inverse(l));
+    }
+}
+
+// Many rows of few parts: four dimensions a thread.
+template <int HD, int R>
+__global__ __launch_bounds__(WG) void paged_join_rows_kernel(PagedAttnArgs a) {
+    constexpr int LPR = HD / 4, RPW = WG / LPR;
+    const int w = blockIdx.x, tid = threadIdx.x, lane = tid & (WAVE - 1);
+    const int used = a.at[a.workers].seq;
+    const PagedAt at = a.at[w + 1], prev = a.at[w];
+    const PagedAt next = w + 1 + lane < a.workers ? a.at[w + 1 + lane] : PagedAt{-1, 0, 0, 0};
+    if (w + 1 >= used || !first_cut(at, prev)) return;
+    const PromptsWork<R> sw(a, at.seq);
+    const int rows = min(sw.tokens * a.group - at.tile * R, R);
+    const int r = blockIdx.y * RPW + tid / LPR, col = tid % LPR;
+    if ((int)blockIdx.y * RPW >= rows) return;
+    // neighbours all: 1 and those of the next 64 that begin inside the tile, and so on
+    int n = 1 + __popcll(__ballot(w + 1 + lane < used && same_tile(next, at) && next.u > 0));
+    for (int k = w + 1 + WAVE; n == k - w && k < used; k += WAVE) {
+        const PagedAt x = k + lane < used ? a.at[k + lane] : PagedAt{-1, 0, 0, 0};
+        n += __popcll(__ballot(same_tile(x, at) && x.u > 0));
+    }
+    if (r >= rows) return;
+    float M = NEG, L = 0.f;
+    f32x4 y = {0.f, 0.f, 0.f, 0.f};
+    constexpr int B = 4;
+    for (int k0 = 0; k0 < n; k0 += B) {
+        float2 ml[B];
+        f32x4 p[B];
+#pragma unroll
+        for (int i = 0; i < B; i++) {
+            const int k = min(k0 + i, n - 1);
             const size_t slot = ((size_t)(w + k) * 2 + (k == 0)) * a.part_rows + r;
-            const float2 ml = a.ml[slot];
-            f32x4 p = *(const f32x4 *)(a.part + slot * HD + 4 * col);
-            if (ml.y == 0.f) p = f32x4{0.f, 0.f, 0.f, 0.f};  // saw nothing, or an empty part that nobody wrote
-            const float m1 = fmaxf(M, ml.x), f0 = ex2(M - m1), f1 = ex2(ml.x - m1);
-            L = L * f0 + ml.y * f1;
-            y = y * f0 + p * f1;
+            ml[i] = a.ml[slot];
+            p[i] = *(const f32x4 *)(a.part + slot * HD + 4 * col);
+        }
+#pragma unroll
+        for (int i = 0; i < B; i++) {
+            if (k0 + i >= n || ml[i].y == 0.f) continue;  // saw nothing: an empty part has no results
+            const float m1 = fmaxf(M, ml[i].x), f0 = ex2(M - m1), f1 = ex2(ml[i].x - m1);
+            L = L * f0 + ml[i].y * f1;
+            y = y * f0 + p[i] * f1;
             M = m1;
         }
-        *(f32x4 *)&red[k0][4 * col] = y;
-        if (col == 0) {
-            redl[k0] = L;
-            redm[k0] = M;
-        }
-        __syncthreads();
-        if (tid < LPR) {
-            M = NEG;
-#pragma unroll
-            for (int k = 0; k < MS; k++) M = fmaxf(M, redm[k]);
-            L = 0.f;
-            y = f32x4{0.f, 0.f, 0.f, 0.f};
-#pragma unroll
-            for (int k = 0; k < MS; k++) {
-                const float f = ex2(redm[k] - M);
-                L += redl[k] * f;
-                y += *(const f32x4 *)&red[k][4 * col] * f;
-            }
-            store_out(a.out, a.f16, row_at(a, base, at.tile * R + r, at.head, a.out_stride) + 4 * col, y * inverse(L));
-        }
-        __syncthreads();
     }
+    const int base = min(max(a.starts[at.seq], 0), a.n_rows);
+    store_out(a.out, a.f16, row_at(a, base, at.tile * R + r, at.head, a.out_stride) + 4 * col, y * inverse(L));
 }
 
 // ---------------------------------------------------------------- prompts --
@@ -626,13 +763,12 @@ __global__ __launch_bounds__(WG, (PromptShape<HD, F16>::PER_CU)) void paged_prom
     using W = PromptsWork<R>;
     static_assert(S::NW * WAVE == WG, "the sharing out takes WG threads");
     __shared__ __attribute__((aligned(16))) f16x8 lds[2][2][PIECES];  // [buffer][K, V]
-    __shared__ ShareLds share;
     int worker;
-    const int used = share_out<W, true>(a, share, worker);
+    PagedAt begin, end;
+    const int used = share_out<W, true>(a, worker, begin, end);
     const int tid = threadIdx.x, lane = tid & (WAVE - 1), wave = __builtin_amdgcn_readfirstlane(tid / WAVE);
     if (blockIdx.x == 0 && tid == 0) a.at[a.workers] = {used, 0, 0, 0};
     if (worker >= used) return;
-    const PagedAt begin = uniform(share.at[0]), end = uniform(share.at[1]);
     leave_border(a, worker, begin, end);
     const int c = lane & 31, h = lane >> 5, lp = a.c.lp, P = 1 << lp;
     const float scale = fabsf(a.scale);
@@ -646,7 +782,7 @@ __global__ __launch_bounds__(WG, (PromptShape<HD, F16>::PER_CU)) void paged_prom
         ksrc[i] = (uint32_t)(s16 * HD + 8 * (j ^ r)) * 2;
     }
 
-    each_piece<W>(a, begin, end, [&](const SeqWork &w, const PagedAt &at, int units, int u0, int u1) {
+    each_piece<W>(a, begin, end, [&](const W &w, const PagedAt &at, int units, int u0, int u1) {
         const int rows = w.tokens * a.group, past = w.len - w.tokens;
         const int base = min(max(a.starts[at.seq], 0), a.n_rows);
         const int row0 = at.tile * R + wave * 32;  // my rows
@@ -797,22 +933,38 @@ template <int HD, bool F16>
 void prompts(const PagedAttnArgs &a, hipStream_t st) {
     constexpr int R = PromptShape<HD, F16>::R;
     hipLaunchKernelGGL((paged_prompts_kernel<HD, F16>), dim3((unsigned)a.workers), dim3(WG), 0, st, a);
-    hipLaunchKernelGGL((paged_join_kernel<PromptsWork<R>, HD, R>), dim3((unsigned)a.workers - 1, (unsigned)((a.part_rows + JR - 1) / JR)),
+    constexpr int RPW = WG * 4 / HD;
+    hipLaunchKernelGGL((paged_join_rows_kernel<HD, R>), dim3((unsigned)a.workers - 1, (unsigned)((a.part_rows + RPW - 1) / RPW)),
                        dim3(WG), 0, st, a);
 }
-template <int HD>
+template <int HD, bool F16, int NT>
 void tokens(const PagedAttnArgs &a, hipStream_t st) {
-    if (a.f16) hipLaunchKernelGGL((paged_tokens_kernel<HD, true>), dim3((unsigned)a.workers), dim3(WG), 0, st, a);
-    else hipLaunchKernelGGL((paged_tokens_kernel<HD, false>), dim3((unsigned)a.workers), dim3(WG), 0, st, a);
-    hipLaunchKernelGGL((paged_join_kernel<TokensWork, HD, 16>), dim3((unsigned)a.workers - 1, (unsigned)((a.part_rows + JR - 1) / JR)),
-                       dim3(WG), 0, st, a);
+    if (a.groups) hipLaunchKernelGGL((paged_tokens_kernel<HD, F16, NT, true>), dim3((unsigned)a.workers), dim3(WG), 0, st, a);
+    else hipLaunchKernelGGL((paged_tokens_kernel<HD, F16, NT, false>), dim3((unsigned)a.workers), dim3(WG), 0, st, a);
+    const int64_t items = (int64_t)a.n_seqs * a.c.n_kv * a.tiles;
+    if (items < a.workers)
+        hipLaunchKernelGGL((paged_join_kernel<HD, true>), dim3((unsigned)items, (unsigned)a.part_rows), dim3(WG), 0, st, a);
+    else
+        hipLaunchKernelGGL((paged_join_kernel<HD, false>), dim3((unsigned)a.workers - 1, (unsigned)a.part_rows), dim3(WG), 0, st, a);
 }
 
 constexpr int CUS = 256;
 
 }  // namespace
 
-int paged_tokens_workers(int hd) { return hd == 128 ? 3 * CUS : 2 * CUS; }
+// 16-row tiles of a wave (two where registers allow) and, as a power of two, its workgroup's
+// groups of waves, which read the same slots for other rows
+static int tokens_tiles(int hd, int rows, bool f16) { return hd == 128 && f16 && rows > 16 ? 2 : 1; }
+int paged_tokens_groups(int hd, int rows, bool f16) {
+    const int r = 16 * tokens_tiles(hd, rows, f16);
+    return rows <= r ? 0 : rows <= 2 * r ? 1 : 2;
+}
+int paged_tokens_rows(int hd, int rows, bool f16) {
+    return 16 * tokens_tiles(hd, rows, f16) << paged_tokens_groups(hd, rows, f16);
+}
+int paged_tokens_workers(int hd) {
+    return CUS * (hd == 128 ? TokensShape<128, true, 1>::PER_CU : TokensShape<256, true, 1>::PER_CU);
+}
 int paged_prompts_workers(int hd, bool f16) { return hd == 256 && !f16 ? CUS : 2 * CUS; }
 int paged_prompts_tile(int hd, bool f16) {
     return hd == 128 ? (f16 ? PromptShape<128, true>::R : PromptShape<128, false>::R)
@@ -820,8 +972,12 @@ int paged_prompts_tile(int hd, bool f16) {
 }
 
 hipError_t launch_paged_tokens(const PagedAttnArgs &a, hipStream_t st) {
-    if (a.c.hd == 128) tokens<128>(a, st);
-    else if (a.c.hd == 256) tokens<256>(a, st);
+    const int nt = tokens_tiles(a.c.hd, a.n_q * a.group, a.f16);
+    if (a.c.hd == 128 && a.f16 && nt == 2) tokens<128, true, 2>(a, st);
+    else if (a.c.hd == 128 && a.f16) tokens<128, true, 1>(a, st);
+    else if (a.c.hd == 128) tokens<128, false, 1>(a, st);
+    else if (a.c.hd == 256 && a.f16) tokens<256, true, 1>(a, st);
+    else if (a.c.hd == 256) tokens<256, false, 1>(a, st);
     else return hipErrorInvalidValue;
     return hipGetLastError();
 }
