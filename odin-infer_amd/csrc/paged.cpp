@@ -90,9 +90,8 @@ bool prompts_fit(const oi_paged_dims *d, int32_t n_heads, int32_t n_seqs, int32_
     return n_seqs > 0 && n_seqs <= MAX_SEQS && n_rows > 0 && n_rows <= MAX_TOKENS && n_rows * g * g < ((int64_t)1 << 32);
 }
 Workspace prompts_workspace(const oi_paged_dims *d, int32_t n_heads, int32_t n_rows, bool f16) {
-    const int64_t rows = (int64_t)n_rows * (n_heads / d->n_kv_heads);
     return workspace(paged_prompts_workers(d->head_dim, f16),
-                     (int)std::min<int64_t>(paged_prompts_tile(d->head_dim, f16), rows), d->head_dim);
+                     (int)std::min<int64_t>(paged_prompts_rows(), (int64_t)n_rows * (n_heads / d->n_kv_heads)), d->head_dim);
 }
 
 // What both attention calls have alike.  n_rows: tokens of q and out.

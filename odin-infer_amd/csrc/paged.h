@@ -57,8 +57,8 @@ struct PagedAttnArgs {
     int32_t n_seqs, n_q, n_rows;   // n_q: tokens of each sequence (tokens call)
     const int32_t *starts, *lens, *table;  // starts: prompts call
     int32_t stride, cap;           // entries of a table row, and its slots
-    // tokens call: rows of an item, a sequence and kv head's items; log2 of the groups of waves
-    // and of the units that costs count
+    // tokens call: rows of a tile, a sequence and kv head's tiles; log2 of the groups of waves and
+    // of the units that costs count
     int32_t tile_rows, tiles, groups, shift;
     // workspace
     int32_t workers, part_rows;    // part_rows: rows of a partial result
@@ -72,7 +72,7 @@ int paged_tokens_workers(int hd);
 int paged_tokens_rows(int hd, int rows, bool f16);
 int paged_tokens_groups(int hd, int rows, bool f16);
 int paged_prompts_workers(int hd, bool f16);
-int paged_prompts_tile(int hd, bool f16);  // rows of a tile
+int paged_prompts_rows();  // of a tile
 hipError_t launch_paged_tokens(const PagedAttnArgs &a, hipStream_t st);
 hipError_t launch_paged_prompts(const PagedAttnArgs &a, hipStream_t st);
 

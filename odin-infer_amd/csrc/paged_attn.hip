@@ -9,8 +9,10 @@
 // row), an f16 q exact.  Weights are the sum of two halves (22 bits) but for f16
 // prompts, whose outputs hold no more than 11 bits: there p is rounded once and l is
 // the sum of the rounded weights.  2^15 is where the row's largest p sits in f16:
-// another keeps all its bits down to 2^-29 of it and is lost below 2^-40 (f16 prompts:
-// 2^-22 and 2^-33).  Cached values are finite (the append sees to it): a slot that a
+// another keeps all its bits down to 2^-29 of it and is lost below 2^-40.  Prompts leave
+// room above the maximum instead, so that few rises of it rescale o: from 2^3 in f16,
+// where a weight below 2^-28 is lost (2^17 of the largest such make one rounding of the
+// output), from 2^9 in f32 (2^-34).  Cached values are finite (the append sees to it): a slot that a
 // row does not see has weight 0, and slots past a sequence's end count as zeros.
 //
 // Work is shared out on the device, since the lengths are there: every tile of rows
@@ -77,7 +79,7 @@ __device__ __forceinline__ int64_t quot(int64_t x, int64_t y) {
 // Tokens: tiles alike, costs in units (where 32 bits do not hold their sum, 2^shift of them).
 struct TokensWork {
     using Cost = uint32_t;
-    static constexpr int UNIT = TU, OWN = 1, LEAST = 4, PARTS = 256;  // a tile's own cost, a worker's least, a tile's most parts
+    static constexpr int OWN = 1, LEAST = 4, PARTS = 256;  // a tile's own cost, a worker's least, a tile's most parts
     int len, tokens, tiles;
     Cost first;
     __device__ __forceinline__ TokensWork(const PagedAttnArgs &a, int s) {
@@ -96,13 +98,12 @@ struct TokensWork {
         u = in <= (Cost)OWN ? 0 : (int)min((in - OWN) << a.shift, (Cost)units(a, 0));
         return (int)t;
     }
-    __device__ static __forceinline__ int near(const PagedAttnArgs &a, Cost share) { return (int)(share / 8 << a.shift); }
+    __device__ static __forceinline__ int near(const PagedAttnArgs &a, Cost share) { return (int)(min(share / 8, (Cost)2) << a.shift); }
 };
 // Prompts: a tile of R rows more sees R / group slots more; costs are slots times the group.
-template <int R>
 struct PromptsWork {
     using Cost = int64_t;
-    static constexpr int UNIT = PU, OWN = 1, LEAST = 4, PARTS = 128;
+    static constexpr int R = 128, OWN = 1, LEAST = 4, PARTS = 128;
     int len, tokens, tiles;
     Cost first;  // of tile 0, each further one R more
     __device__ __forceinline__ PromptsWork(const PagedAttnArgs &a, int s) {
@@ -131,7 +132,7 @@ struct PromptsWork {
         u = in <= own ? 0 : (int)quot((in - own) * units(a, (int)t), first + t * R - own);
         return (int)t;
     }
-    __device__ static __forceinline__ int near(const PagedAttnArgs &a, Cost share) { return (int)quot(share, 8 * unit(a)); }
+    __device__ static __forceinline__ int near(const PagedAttnArgs &a, Cost share) { return (int)min(quot(share, 8 * unit(a)), (Cost)4); }
 };
 
 // Sums over the lanes up to each, and a lane's value for all.
@@ -205,9 +206,9 @@ __device__ PagedAt border(const PagedAttnArgs &a, typename W::Cost x, typename W
 
 // A worker's stretch, [begin, end); the number of workers used is returned (this one is
 // idle if it is not below).  Every wave does it for itself, without LDS: a lane sums a run
-// of neighbouring sequences.  SPREAD: neighbouring workers go to one XCD (blocks are
-// dealt to the 8 in turn), whose cache then holds what they share.
-template <class W, bool SPREAD>
+// of neighbouring sequences.  Neighbouring workers go to one XCD (blocks are dealt to the
+// 8 in turn), whose cache then holds what they share.
+template <class W>
 __device__ int share_out(const PagedAttnArgs &a, int &worker, PagedAt &begin, PagedAt &end) {
     using Cost = typename W::Cost;
     const int lane = __lane_id(), per = (a.n_seqs + WAVE - 1) / WAVE;
@@ -227,7 +228,7 @@ __device__ int share_out(const PagedAttnArgs &a, int &worker, PagedAt &begin, Pa
     }
     const int used = (int)quot((Cost)(total + share - 1), share);
     const int each = (used + 7) / 8, b = blockIdx.x;
-    worker = SPREAD ? (b / 8 < each ? (b & 7) * each + b / 8 : used) : b;
+    worker = b / 8 < each ? (b & 7) * each + b / 8 : used;
     if (worker < used) {
         begin = border<W>(a, (Cost)worker * share, share, own, run, per);
         end = {a.n_seqs, 0, 0, 0};
@@ -378,7 +379,7 @@ __global__ __launch_bounds__(WG, (TokensShape<HD, F16, NT>::PER_CU)) void paged_
     __shared__ float sm[NW][16], sl[NW][16];
     int worker;
     PagedAt begin, end;
-    const int used = share_out<W, true>(a, worker, begin, end);
+    const int used = share_out<W>(a, worker, begin, end);
     const int tid = threadIdx.x, lane = tid & (WAVE - 1), wave = tid / WAVE;
     if (blockIdx.x == 0 && tid == 0) a.at[a.workers] = {used, 0, 0, 0};
     if (worker >= used) return;
@@ -682,7 +683,7 @@ __global__ __launch_bounds__(WG, 4) void paged_join_kernel(PagedAttnArgs a) {
 }
 
 // Many rows of few parts: four dimensions a thread.
-template <int HD, int R>
+template <int HD>
 __global__ __launch_bounds__(WG) void paged_join_rows_kernel(PagedAttnArgs a) {
     constexpr int LPR = HD / 4, RPW = WG / LPR;
     const int w = blockIdx.x, tid = threadIdx.x, lane = tid & (WAVE - 1);
@@ -690,7 +691,8 @@ __global__ __launch_bounds__(WG) void paged_join_rows_kernel(PagedAttnArgs a) {
     const PagedAt at = a.at[w + 1], prev = a.at[w];
     const PagedAt next = w + 1 + lane < a.workers ? a.at[w + 1 + lane] : PagedAt{-1, 0, 0, 0};
     if (w + 1 >= used || !first_cut(at, prev)) return;
-    const PromptsWork<R> sw(a, at.seq);
+    constexpr int R = PromptsWork::R;
+    const PromptsWork sw(a, at.seq);
     const int rows = min(sw.tokens * a.group - at.tile * R, R);
     const int r = blockIdx.y * RPW + tid / LPR, col = tid % LPR;
     if ((int)blockIdx.y * RPW >= rows) return;
@@ -729,194 +731,288 @@ __global__ __launch_bounds__(WG) void paged_join_rows_kernel(PagedAttnArgs a) {
 
 // ---------------------------------------------------------------- prompts --
 
-__device__ __forceinline__ float sum8(f16x8 p, float to) {
-    const f16x2 one = {(_Float16)1.f, (_Float16)1.f};
-#pragma unroll
-    for (int i = 0; i < 4; i++) to = __builtin_amdgcn_fdot2(f16x2{p[2 * i], p[2 * i + 1]}, one, to, false);
-    return to;
-}
-
+// Workgroups of a CU, as registers and LDS allow.
 template <int HD, bool F16>
-struct PromptShape {
-    static constexpr int NW = 4, R = 32 * NW;  // waves, rows
-    static constexpr int SLOTS = HD == 128 ? 64 : 32;  // of a staged step
-    static constexpr int PER_CU = HD == 256 && !F16 ? 1 : 2;
+struct PromptsShape {
+    static constexpr int PER_CU = HD == 128 && F16 ? 2 : 1;
 };
+constexpr int PR = PromptsWork::R;  // rows of a tile
 
-// A worker of NW waves takes tiles of 32 NW rows of one kv head, a wave 32 of them,
-// and the tile's slots step after step through two buffers in LDS, filled straight from
-// memory while the other is worked on.  Scores transposed, on 32x32x16 products.  K's
-// piece j (8 dimensions) of LDS row r lies at j ^ (r & 15), and row r holds the slot with
-// bits 2 and 3 of r exchanged: the products then leave a lane the scores of slots 8 h +
-// 0..7 of each 16, those whose weights it supplies to the product with V; V's pieces (8
-// slots of a dimension) lie as in the cache.  Either way sixteen lanes read all banks
-// once.  f16 rows rescale o only when a maximum rises by more than 2^7: their weights
-// then reach 2^15 at most, from 2^8.
+// A worker of four waves takes tiles of 128 rows of one kv head, a wave 32 of them, and the
+// tile's slots 64 at a time through two buffers of K and two of V in LDS, filled straight from
+// memory (K a step ahead of V) while the others are worked on.  Scores transposed, on 32x32x16
+// products.  K's piece j (8 dimensions) of LDS row r lies at j ^ (r & 15), and row r holds the
+// slot with bits 2 and 3 of r exchanged: the products then leave a lane the scores of slots 8 h +
+// 0..7 of each 16, those whose weights it supplies to the product with V; V's pieces (8 slots of
+// a dimension) lie as in the cache.  Either way sixteen lanes read all banks once.
+// A wave's work is a pipeline over halves of 32 slots: while the vector units turn half i's
+// scores to weights, the matrix units form half i + 1's scores and the products of half i -
+// 1's weights with V.  A row's maximum is raised only when another is more than 2^LAZY above it
+// (weights then reach 2^15 at most, from 2^PS), and o follows after the products that go by the
+// old one.
 template <int HD, bool F16>
-__global__ __launch_bounds__(WG, (PromptShape<HD, F16>::PER_CU)) void paged_prompts_kernel(PagedAttnArgs a) {
-    using S = PromptShape<HD, F16>;
-    constexpr int NF = HD / 16, DT = HD / 32, R = S::R, ST = S::SLOTS, X = ST / 32;
-    constexpr int PIECES = ST * HD / 8;           // of K, and of V, in a step
-    constexpr int CH = PIECES / WAVE / S::NW;     // a wave's stretches of 64 pieces, of each
-    constexpr int RPC = WAVE / (HD / 8);          // K rows of a stretch
-    constexpr float PS = F16 ? 8.f : 15.f, LAZY = F16 ? 7.f : 0.f;
-    using W = PromptsWork<R>;
-    static_assert(S::NW * WAVE == WG, "the sharing out takes WG threads");
-    __shared__ __attribute__((aligned(16))) f16x8 lds[2][2][PIECES];  // [buffer][K, V]
+__global__ __launch_bounds__(WG, (PromptsShape<HD, F16>::PER_CU)) void paged_prompts_kernel(PagedAttnArgs a) {
+    constexpr int NW = WG / WAVE, NF = HD / 16, DT = HD / 32;
+    constexpr int PIECES = PU * HD / 8;     // of K, and of V, in a step
+    constexpr int CH = PIECES / WAVE / NW;  // a wave's stretches of 64 pieces, of each
+    constexpr int RPC = WAVE / (HD / 8);    // K rows of a stretch
+    constexpr float PS = F16 ? 3.f : 9.f, LAZY = 15.f - PS;
+    using W = PromptsWork;
+    __shared__ __attribute__((aligned(16))) f16x8 kl[2][PIECES], vl[2][PIECES];
     int worker;
     PagedAt begin, end;
-    const int used = share_out<W, true>(a, worker, begin, end);
+    const int used = share_out<W>(a, worker, begin, end);
     const int tid = threadIdx.x, lane = tid & (WAVE - 1), wave = __builtin_amdgcn_readfirstlane(tid / WAVE);
     if (blockIdx.x == 0 && tid == 0) a.at[a.workers] = {used, 0, 0, 0};
     if (worker >= used) return;
     leave_border(a, worker, begin, end);
     const int c = lane & 31, h = lane >> 5, lp = a.c.lp, P = 1 << lp;
     const float scale = fabsf(a.scale);
-    const size_t page_elems = ((size_t)a.c.n_kv << lp) * HD;
-    // a lane's place in the sources of its stretches: stretch i of a wave is number i NW + wave
-    uint32_t ksrc[CH];
+    const uint32_t page_bytes = ((uint32_t)a.c.n_kv << lp) * HD * 2;
+    // a lane's place in the sixteens that its stretches come from: stretch i of a wave is number
+    // i NW + wave
+    uint32_t ksrc[CH], vsrc[CH];
 #pragma unroll
     for (int i = 0; i < CH; i++) {
-        const int r = ((i * S::NW + wave) * RPC + lane / (HD / 8)) & 15, j = lane % (HD / 8);
+        const int st = i * NW + wave, r = (st * RPC + lane / (HD / 8)) & 15, j = lane % (HD / 8);
         const int s16 = (r & 3) | (r & 4) << 1 | (r & 8) >> 1;
         ksrc[i] = (uint32_t)(s16 * HD + 8 * (j ^ r)) * 2;
+        vsrc[i] = (uint32_t)((st * WAVE + lane) % (2 * HD)) * 16;
     }
 
     each_piece<W>(a, begin, end, [&](const W &w, const PagedAt &at, int units, int u0, int u1) {
         const int rows = w.tokens * a.group, past = w.len - w.tokens;
         const int base = min(max(a.starts[at.seq], 0), a.n_rows);
-        const int row0 = at.tile * R + wave * 32;  // my rows
-        const int r = row0 + c, rr = min(r, rows - 1), limit = past + row_token(a, rr) + 1;
-        const int mine = row0 < rows ? past + row_token(a, min(row0 + 31, rows - 1)) + 1 : 0;  // slots my rows see
-        const int first_limit = past + row_token(a, min(row0, rows - 1)) + 1;
-        const int s_end = min(u1 * PU, units * PU), s_begin = u0 * PU;
+        const int row0 = at.tile * PR + wave * 32, r = row0 + c, rr = min(r, rows - 1);  // my rows
+        const int s_end = u1 * PU;
+        const int mine = row0 < rows ? past + row_token(a, min(row0 + 32, rows) - 1) + 1 : 0;  // slots my rows see
+        const int first_limit = min(past + row_token(a, min(row0, rows - 1)) + 1, s_end);
+        const int limit = min(past + row_token(a, rr) + 1, s_end);
         const int last_page = max(w.len - 1, 0) >> lp;
         const ScalarInts table = (ScalarInts)(uintptr_t)(a.table + (int64_t)at.seq * a.stride);
-        const uint16_t *kb = a.c.k + ((size_t)at.head << lp) * HD, *vb = a.c.v + ((size_t)at.head << lp) * HD;
-        auto fetch = [&](int s0, int buf) {  // slots s0 .. s0 + ST - 1
+        const char *kb = (const char *)(a.c.k + ((size_t)at.head << lp) * HD),
+                   *vb = (const char *)(a.c.v + ((size_t)at.head << lp) * HD);
+        // A step's slots lie in sixteens, each within a page: their pages, and where they begin (K and
+        // V at the same place of their halves of the cache), in bytes.
+        struct Pages {
+            int id[4];
+        };
+        struct Places {
+            uint64_t at[4];
+        };
+        auto look_up = [&](int u) {
+            Pages p;
+#pragma unroll
+            for (int j = 0; j < 4; j++) p.id[j] = table[min((u * PU + 16 * j) >> lp, last_page)];
+            return p;
+        };
+        auto place = [&](int u, const Pages &p) {
+            Places x;
+#pragma unroll
+            for (int j = 0; j < 4; j++)
+                x.at[j] = (uint64_t)(uint32_t)page_ok(a, p.id[j]) * page_bytes + (uint32_t)(((u * PU + 16 * j) & (P - 1)) * HD * 2);
+            return x;
+        };
+        auto fetch = [&](const char *from, const Places &p, const uint32_t (&src)[CH], f16x8 *to) {
 #pragma unroll
             for (int i = 0; i < CH; i++) {
-                const int st = i * S::NW + wave;
-                {
-                    const int s = s0 + (st * RPC & ~15);
-                    const int page = page_ok(a, table[min(s >> lp, last_page)]);
-                    const char *src = (const char *)(kb + page * page_elems + (size_t)(s & (P - 1)) * HD) + ksrc[i];
-                    __builtin_amdgcn_global_load_lds((const __attribute__((address_space(1))) void *)(uintptr_t)src,
-                                                     (__attribute__((address_space(3))) void *)&lds[buf][0][st * WAVE], 16,
-                                                     0, 0);
-                }
-                {
-                    const int e = st / (HD / WAVE), s = s0 + 8 * e;
-                    const int page = page_ok(a, table[min(s >> lp, last_page)]);
-                    const uint16_t *src = vb + page * page_elems + (size_t)(s & (P - 1)) * HD +
-                                          (st % (HD / WAVE) * WAVE + lane) * 8;
-                    __builtin_amdgcn_global_load_lds((const __attribute__((address_space(1))) void *)(uintptr_t)src,
-                                                     (__attribute__((address_space(3))) void *)&lds[buf][1][st * WAVE], 16,
-                                                     0, 0);
-                }
+                const char *x = from + p.at[i * NW * WAVE / (2 * HD)];
+                asm volatile("" : "+s"(x));  // a scalar address, the lane's 32-bit place behind it
+                __builtin_amdgcn_global_load_lds((const __attribute__((address_space(1))) void *)(uintptr_t)(x + src[i]),
+                                                 (__attribute__((address_space(3))) void *)(to + (i * NW + wave) * WAVE), 16, 0,
+                                                 0);
             }
         };
+        // what this wave asked for has arrived and what it read is in registers; then all waves
+        auto meet = [&]() {
+            asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)" ::: "memory");
+            __builtin_amdgcn_s_barrier();
+            asm volatile("" ::: "memory");
+        };
+        // ahead of their use: where the next steps of V and of K lie, and the pages of the one after
+        Places vp = place(u0, look_up(u0)), kp = place(u0 + 1, look_up(u0 + 1));
+        Pages ahead = look_up(u0 + 2);
+        auto go_on = [&](int u) {
+            vp = kp;
+            kp = place(u, ahead);
+            ahead = look_up(u + 1);
+        };
+        if (u0 < u1) fetch(kb, vp, ksrc, kl[u0 & 1]);
+        QPieces<NF, 16, F16> q;
+        q.load(a.q, row_at(a, base, rr, at.head, a.q_stride) + 8 * h, r < rows, a.scale < 0.f,
+               [](float x) { return half_reduce(x, Max()); });
+        const float mul = fmaxf(ldexpf(scale, q.e), FLT_MIN);
         float m = NEG, l = 0.f;
         f32x16 o[DT];
 #pragma unroll
         for (int d = 0; d < DT; d++)
 #pragma unroll
             for (int i = 0; i < 16; i++) o[d][i] = 0.f;
-        if (s_begin < s_end) fetch(s_begin, 0);
-        QPieces<NF, 16, F16> q;
-        q.load(a.q, row_at(a, base, rr, at.head, a.q_stride) + 8 * h, r < rows, a.scale < 0.f,
-               [](float x) { return half_reduce(x, Max()); });
-        const float mul = fmaxf(ldexpf(scale, q.e), FLT_MIN);
-        int buf = 0;
-        for (int s0 = s_begin; s0 < s_end; s0 += ST, buf ^= 1) {
-            // this step has arrived, and every wave is done with the other buffer
-            asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)" ::: "memory");
-            __builtin_amdgcn_s_barrier();
-            asm volatile("" ::: "memory");
-            if (s0 + ST < s_end) fetch(s0 + ST, buf ^ 1);
-            if (s0 >= mine) continue;
-            const f16x8 *kt = lds[buf][0], *vt = lds[buf][1];
+        // The softmax of a half in steps: the maximum of score pairs, the rows' new maxima, weights of a
+        // pair.  Rows rise together, so that one that climbs takes the others along and few halves
+        // rise at all; alpha: what o is to be multiplied by then.
+        float top = 0.f, alpha = 1.f, bias = 0.f;
+        bool rise = false;
+        auto higher = [&](const f32x16 &s, int i) {
+            top = i == 0 ? fmaxf(s[0], s[1]) : fmaxf(fmaxf(top, s[2 * i]), s[2 * i + 1]);
+        };
+        auto turn = [&]() {
+            top = half_reduce(top * mul, Max());
+            rise = __any(top > m + LAZY);
+            const float m1 = rise ? fmaxf(m, ceilf(top)) : m;
+            alpha = ex2(m - m1);
+            m = m1;
+            bias = PS - m1;
+            l *= alpha;
+        };
+        auto weigh = [&](const f32x16 &s, f16x8 (&ph)[2], f16x8 (&pl)[2], int i) {
+            f16x2 hi, lo;
 #pragma unroll
-            for (int x = 0; x < X; x++) {
-                f32x16 s;
-#pragma unroll
-                for (int i = 0; i < 16; i++) s[i] = 0.f;
-#pragma unroll
-                for (int f = 0; f < NF; f++) {
-                    const f16x8 k = kt[(32 * x + c) * (HD / 8) + ((2 * f + h) ^ (c & 15))];
-                    s = mfma32(k, q.hi[f], s);
-                    if constexpr (!F16) s = mfma32(k, q.lo[f], s);
-                }
-                const int p0 = s0 + 32 * x;
-                if (p0 + 32 > first_limit) {
-#pragma unroll
-                    for (int i = 0; i < 16; i++)
-                        if (p0 + 16 * (i / 8) + 8 * h + i % 8 >= limit) s[i] = -INFINITY;
-                }
-                float top = s[0];
-#pragma unroll
-                for (int i = 1; i < 16; i++) top = fmaxf(top, s[i]);
-                top = half_reduce(top * mul, Max());
-                if (__any(top > m + LAZY)) {
-                    const float m1 = fmaxf(m, ceilf(top)), alpha = ex2(m - m1);
-                    m = m1;
-                    l *= alpha;
-#pragma unroll
-                    for (int d = 0; d < DT; d++)
-#pragma unroll
-                        for (int i = 0; i < 16; i++) o[d][i] *= alpha;
-                }
-                f16x8 ph[2], pl[2];
-#pragma unroll
-                for (int b = 0; b < 2; b++) {
-                    float sum = 0.f;
-#pragma unroll
-                    for (int i = 0; i < 8; i++) {
-                        const float p = F16 ? ex2(fmaf(s[8 * b + i], mul, PS - m))
-                                            : ex2(fmaf(s[8 * b + i], mul, -m)) * 32768.f;
-                        const _Float16 t = (_Float16)p;
-                        ph[b][i] = t;
-                        if constexpr (!F16) {
-                            sum += p;
-                            pl[b][i] = (_Float16)(p - (float)t);
-                        }
-                    }
-                    if constexpr (F16) l = sum8(ph[b], l);
-                    else l += sum;
-                }
-                const bool tail = p0 + 32 > w.len;  // bytes behind the sequence's end count for nothing
-#pragma unroll
-                for (int b = 0; b < 2; b++) {
-                    u32x4 keep;
-                    if (tail) {
-                        const int s8 = p0 + 16 * b + 8 * h;
-#pragma unroll
-                        for (int i = 0; i < 4; i++)
-                            keep[i] = (s8 + 2 * i < w.len ? 0xFFFFu : 0u) | (s8 + 2 * i + 1 < w.len ? 0xFFFF0000u : 0u);
-                    }
-#pragma unroll
-                    for (int d = 0; d < DT; d++) {
-                        f16x8 v = vt[(4 * x + 2 * b + h) * HD + 32 * d + c];
-                        if (tail) v = __builtin_bit_cast(f16x8, __builtin_bit_cast(u32x4, v) & keep);
-                        o[d] = mfma32(v, ph[b], o[d]);
-                        if constexpr (!F16) o[d] = mfma32(v, pl[b], o[d]);
-                    }
+            for (int k = 0; k < 2; k++) {
+                const float p = ex2(fmaf(s[2 * i + k], mul, bias));
+                hi[k] = (_Float16)p;
+                if constexpr (!F16) {
+                    l += p;
+                    lo[k] = (_Float16)(p - (float)hi[k]);
                 }
             }
+            if constexpr (F16) l = __builtin_amdgcn_fdot2(hi, f16x2{(_Float16)1.f, (_Float16)1.f}, l, false);
+            asm volatile("" : "+v"(hi), "+v"(l));  // here, not where it is used
+            if constexpr (!F16) asm volatile("" : "+v"(lo));
+#pragma unroll
+            for (int k = 0; k < 2; k++) {
+                ph[i / 4][2 * (i % 4) + k] = hi[k];
+                if constexpr (!F16) pl[i / 4][2 * (i % 4) + k] = lo[k];
+            }
+        };
+        auto k_piece = [&](const f16x8 *kt, int x, int f) { return kt[(32 * x + c) * (HD / 8) + ((2 * f + h) ^ (c & 15))]; };
+        auto score = [&](const f16x8 &k, int f, f32x16 &s) {
+            if (f == 0) {
+#pragma unroll
+                for (int i = 0; i < 16; i++) s[i] = 0.f;
+            }
+            s = mfma32(k, q.hi[f], s);
+            if constexpr (!F16) s = mfma32(k, q.lo[f], s);
+        };
+        // o in the registers that only the matrix units use, where the others do not hold it
+        auto pin = [&]() {
+            if constexpr (PromptsShape<HD, F16>::PER_CU == 1)
+#pragma unroll
+                for (int d = 0; d < DT; d++) asm volatile("" : "+a"(o[d]));
+        };
+        // Half a step of the pipeline: weights p1 of the scores s0, the next scores s1 from half x of the K
+        // buffer, the products of the former weights p0 with half x of the V buffer.  Pieces of K, then of
+        // V come from LDS AHEAD of their use, and the vector units' work lies between their products in
+        // the order written here.
+        auto half = [&](const f16x8 *kt, const f16x8 *vt, int x, const f32x16 &s0, f32x16 &s1, const f16x8 (&ph0)[2],
+                        const f16x8 (&pl0)[2], f16x8 (&ph1)[2], f16x8 (&pl1)[2]) {
+            constexpr int N = NF + 2 * DT, AHEAD = 4, CLIMB = N / 4, STEP = N / 16;
+            f16x8 w[N];
+            auto read = [&](int j) {
+                if (j < NF) w[j] = k_piece(kt, x, j);
+                else w[j] = vt[(4 * x + 2 * ((j - NF) / DT) + h) * HD + 32 * ((j - NF) % DT) + c];
+            };
+#pragma unroll
+            for (int j = 0; j < AHEAD; j++) read(j);
+#pragma unroll
+            for (int j = 0; j < N; j++) {
+                if (j + AHEAD < N) read(j + AHEAD);
+                if (j < NF) {
+                    score(w[j], j, s1);
+                } else {
+                    const int i = (j - NF) / DT, d = (j - NF) % DT;
+                    o[d] = mfma32(w[j], ph0[i], o[d]);
+                    if constexpr (!F16) o[d] = mfma32(w[j], pl0[i], o[d]);
+                }
+                if (j < CLIMB) {
+#pragma unroll
+                    for (int i = 8 * j / CLIMB; i < 8 * (j + 1) / CLIMB; i++) higher(s0, i);
+                } else if (j == CLIMB) {
+                    turn();
+                } else if ((j - CLIMB - 1) % STEP == 0 && (j - CLIMB - 1) / STEP < 8) {
+                    weigh(s0, ph1, pl1, (j - CLIMB - 1) / STEP);
+                }
+                __builtin_amdgcn_sched_barrier(0);
+            }
+            if (__builtin_expect(rise, 0)) {
+#pragma unroll
+                for (int d = 0; d < DT; d++)
+#pragma unroll
+                    for (int i = 0; i < 16; i++) o[d][i] *= alpha;
+            }
+            pin();
+        };
+        // some row does not see all of the half
+        auto hide = [&](f32x16 &s, int p0) {
+            if (__builtin_expect(p0 + 32 > first_limit, 0)) {
+#pragma unroll
+                for (int i = 0; i < 16; i++)
+                    if (p0 + 16 * (i / 8) + 8 * h + i % 8 >= limit) s[i] = -INFINITY;
+            }
+        };
+        // step u: V of it and K of the next are here, the other two buffers free
+        auto stage = [&](int u) {
+            meet();
+            if (u + 1 < u1) fetch(vb, vp, vsrc, vl[(u + 1) & 1]);
+            if (u + 2 < u1) fetch(kb, kp, ksrc, kl[u & 1]);
+            go_on(u + 3);
+            if (__builtin_expect(u * PU + PU > w.len, 0)) {  // bytes behind the sequence's end count for nothing
+                for (int i = tid; i < PIECES; i += WG) {
+                    const int s8 = u * PU + 8 * (i / HD);
+                    u32x4 keep;
+#pragma unroll
+                    for (int k = 0; k < 4; k++)
+                        keep[k] = (s8 + 2 * k < w.len ? 0xFFFFu : 0u) | (s8 + 2 * k + 1 < w.len ? 0xFFFF0000u : 0u);
+                    f16x8 &v = vl[u & 1][i];
+                    v = __builtin_bit_cast(f16x8, __builtin_bit_cast(u32x4, v) & keep);
+                }
+                meet();
+            }
+        };
+        if (u0 < u1) {
+            meet();
+            fetch(vb, vp, vsrc, vl[u0 & 1]);
+            if (u0 + 1 < u1) fetch(kb, kp, ksrc, kl[(u0 + 1) & 1]);
+            go_on(u0 + 2);
         }
-        constexpr float UP = F16 ? 128.f : 1.f;
-        l = half_reduce(l, Add()) * UP;
+        if (mine <= u0 * PU) {  // my rows see nothing here; this wave fetches for the others
+            for (int u = u0; u < u1; u++) stage(u);
+        } else {
+            f32x16 s0, s1;
+            f16x8 ph0[2], pl0[2], ph1[2], pl1[2];
+#pragma unroll
+            for (int f = 0; f < NF; f++) score(k_piece(kl[u0 & 1], 0, f), f, s0);
+            hide(s0, u0 * PU);
+#pragma unroll
+            for (int i = 0; i < 8; i++) higher(s0, i);
+            turn();  // o is 0
+#pragma unroll
+            for (int i = 0; i < 8; i++) weigh(s0, ph0, pl0, i);
+#pragma unroll
+            for (int f = 0; f < NF; f++) score(k_piece(kl[u0 & 1], 1, f), f, s1);
+            pin();
+            // the last half's scores are of no step (K's buffer holds an older one): hidden, they weigh nothing
+            for (int u = u0; u < u1; u++) {
+                stage(u);
+                const f16x8 *kt = kl[(u + 1) & 1], *vt = vl[u & 1];
+                hide(s1, u * PU + 32);
+                half(kt, vt, 0, s1, s0, ph0, pl0, ph1, pl1);
+                hide(s0, u * PU + PU);
+                half(kt, vt, 1, s0, s1, ph1, pl1, ph0, pl0);
+            }
+        }
+        const bool whole = u0 == 0 && u1 == units;
+        l = half_reduce(l, Add());
         if (r < rows) {
-            const bool whole = u0 == 0 && u1 == units;
             const size_t slot = ((size_t)worker * 2 + (u0 == 0)) * a.part_rows + wave * 32 + c;
-            const float inv = whole ? UP * inverse(l) : UP;
+            const float inv = whole ? inverse(l) : 1.f;
             const int64_t to = row_at(a, base, r, at.head, a.out_stride);
 #pragma unroll
             for (int d = 0; d < DT; d++)
 #pragma unroll
                 for (int i = 0; i < 4; i++) {
                     const int dim = 32 * d + 8 * i + 4 * h;
-                    const f32x4 y = {o[d][4 * i] * inv, o[d][4 * i + 1] * inv, o[d][4 * i + 2] * inv, o[d][4 * i + 3] * inv};
+                    const f32x4 y = f32x4{o[d][4 * i], o[d][4 * i + 1], o[d][4 * i + 2], o[d][4 * i + 3]} * inv;
                     if (whole) store_out(a.out, F16, to + dim, y);
                     else *(f32x4 *)(a.part + slot * HD + dim) = y;
                 }
@@ -931,10 +1027,9 @@ __global__ __launch_bounds__(WG, (PromptShape<HD, F16>::PER_CU)) void paged_prom
 
 template <int HD, bool F16>
 void prompts(const PagedAttnArgs &a, hipStream_t st) {
-    constexpr int R = PromptShape<HD, F16>::R;
-    hipLaunchKernelGGL((paged_prompts_kernel<HD, F16>), dim3((unsigned)a.workers), dim3(WG), 0, st, a);
     constexpr int RPW = WG * 4 / HD;
-    hipLaunchKernelGGL((paged_join_rows_kernel<HD, R>), dim3((unsigned)a.workers - 1, (unsigned)((a.part_rows + RPW - 1) / RPW)),
+    hipLaunchKernelGGL((paged_prompts_kernel<HD, F16>), dim3((unsigned)a.workers), dim3(WG), 0, st, a);
+    hipLaunchKernelGGL((paged_join_rows_kernel<HD>), dim3((unsigned)a.workers - 1, (unsigned)((a.part_rows + RPW - 1) / RPW)),
                        dim3(WG), 0, st, a);
 }
 template <int HD, bool F16, int NT>
@@ -965,11 +1060,11 @@ int paged_tokens_rows(int hd, int rows, bool f16) {
 int paged_tokens_workers(int hd) {
     return CUS * (hd == 128 ? TokensShape<128, true, 1>::PER_CU : TokensShape<256, true, 1>::PER_CU);
 }
-int paged_prompts_workers(int hd, bool f16) { return hd == 256 && !f16 ? CUS : 2 * CUS; }
-int paged_prompts_tile(int hd, bool f16) {
-    return hd == 128 ? (f16 ? PromptShape<128, true>::R : PromptShape<128, false>::R)
-                     : (f16 ? PromptShape<256, true>::R : PromptShape<256, false>::R);
+int paged_prompts_workers(int hd, bool f16) {
+    return CUS * (hd == 128 ? (f16 ? PromptsShape<128, true>::PER_CU : PromptsShape<128, false>::PER_CU)
+                            : (f16 ? PromptsShape<256, true>::PER_CU : PromptsShape<256, false>::PER_CU));
 }
+int paged_prompts_rows() { return PR; }
 
 hipError_t launch_paged_tokens(const PagedAttnArgs &a, hipStream_t st) {
     const int nt = tokens_tiles(a.c.hd, a.n_q * a.group, a.f16);
