@@ -112,10 +112,7 @@ int attention(PagedAttnArgs &a, const char *what, const oi_paged_dims *d, const 
     if (ws_bytes < (int64_t)w.bytes)
         return err(OI_E_ARG, what, "workspace of " + std::to_string(ws_bytes) + " bytes, " + std::to_string(w.bytes) +
                                        " needed");
-    // costs are summed in whole numbers below 2^52
     const int64_t group = n_heads / d->n_kv_heads, cap = (int64_t)stride * d->page;
-    if ((double)(n_rows * group / 16 + n_seqs) * (double)group * (double)(cap + 128) * d->n_kv_heads > 4e15)
-        return err(OI_E_RANGE, what, "rows times a table's slots pass what one call takes");
     const int64_t es = size_of(type);
     const Span qs{q, row * es, n_rows, q_stride * es}, os{out, row * es, n_rows, out_stride * es}, wsp{ws, (int64_t)w.bytes},
         all{cache, oi_paged_bytes(d)}, ls{lens, (int64_t)n_seqs * 4}, ts{table, (int64_t)n_seqs * stride * 4},
@@ -273,9 +270,6 @@ int oi_paged_tokens_launch(const oi_paged_dims *d, const void *cache, int32_t n_
         a.tile_rows = paged_tokens_rows(d->head_dim, n_q * a.group, a.f16);
         a.groups = paged_tokens_groups(d->head_dim, n_q * a.group, a.f16);
         a.tiles = (n_q * a.group + a.tile_rows - 1) / a.tile_rows;
-        // the whole cost in 31 bits
-        const int64_t tiles = (int64_t)n_seqs * d->n_kv_heads * a.tiles;
-        while (tiles * ((a.cap / 32 >> a.shift) + 3) >= INT32_MAX) a.shift++;
         return launched(launch_paged_tokens(a, (hipStream_t)stream), W);
     });
 }
@@ -302,6 +296,7 @@ int oi_paged_prompts_launch(const oi_paged_dims *d, const void *cache, int32_t n
         if (int rc = attention(a, W, d, cache, n_heads, type, q, q_stride, scale, n_seqs, n_rows, starts, lens, table,
                                table_stride, out, out_stride, workspace, workspace_bytes, w, stream))
             return rc;
+        a.tile_units = (float)paged_prompts_rows() / (64.f * (float)a.group);
         return launched(launch_paged_prompts(a, (hipStream_t)stream), W);
     });
 }

@@ -57,9 +57,9 @@ struct PagedAttnArgs {
     int32_t n_seqs, n_q, n_rows;   // n_q: tokens of each sequence (tokens call)
     const int32_t *starts, *lens, *table;  // starts: prompts call
     int32_t stride, cap;           // entries of a table row, and its slots
-    // tokens call: rows of a tile, a sequence and kv head's tiles; log2 of the groups of waves and
-    // of the units that costs count
-    int32_t tile_rows, tiles, groups, shift;
+    // tokens call: rows of a tile, a sequence and kv head's tiles, log2 of the groups of waves
+    int32_t tile_rows, tiles, groups;
+    float tile_units;              // prompts call: units of slots that a tile sees more than the one before
     // workspace
     int32_t workers, part_rows;    // part_rows: rows of a partial result
     PagedAt *at;                   // [workers + 1], the last: {used workers, 0, 0, 0}

@@ -10,14 +10,22 @@ namespace {
 
 constexpr int PW = 1024;  // threads of the planning workgroup, sequences that it takes at a time
 
-// Inclusive sum over the workgroup's threads (PW of them), and the total.
-__device__ __forceinline__ int64_t scan_add(int64_t v, int64_t *lds, int64_t &total) {
+// Sum over the lanes up to each (below 2^32).
+__device__ __forceinline__ uint32_t scan_lanes(uint32_t v) {
+#define OI_SCAN(ctrl, rows) v += (uint32_t)__builtin_amdgcn_update_dpp(0, (int)v, ctrl, rows, 0xF, false)
+    OI_SCAN(0x111, 0xF);  // rows of 16: 1, 2, 4, 8 lanes back
+    OI_SCAN(0x112, 0xF);
+    OI_SCAN(0x114, 0xF);
+    OI_SCAN(0x118, 0xF);
+    OI_SCAN(0x142, 0xA);  // the last lane of rows 0 and 2 to the row behind
+    OI_SCAN(0x143, 0xC);  // lane 31 to rows 2 and 3
+#undef OI_SCAN
+    return v;
+}
+// Sum over the workgroup's threads (PW of them, below 2^25 each) up to each, and the total.
+__device__ __forceinline__ int64_t scan_add(uint32_t x, uint32_t *lds, int64_t &total) {
     const int tid = threadIdx.x, lane = tid & (WAVE - 1), wave = tid / WAVE;
-#pragma unroll
-    for (int d = 1; d < WAVE; d *= 2) {
-        const int64_t o = __shfl_up(v, d);
-        if (lane >= d) v += o;
-    }
+    const uint32_t v = scan_lanes(x);
     __syncthreads();  // the previous use of lds is complete
     if (lane == WAVE - 1) lds[wave] = v;
     __syncthreads();
@@ -25,9 +33,9 @@ __device__ __forceinline__ int64_t scan_add(int64_t v, int64_t *lds, int64_t &to
     total = 0;
 #pragma unroll
     for (int w = 0; w < PW / WAVE; w++) {
-        const int64_t x = lds[w];
-        before += w < wave ? x : 0;
-        total += x;
+        const int64_t y = lds[w];
+        before += w < wave ? y : 0;
+        total += y;
     }
     return v + before;
 }
@@ -57,8 +65,8 @@ __device__ __forceinline__ int slot_of(int page, int off, int lp, int n_pages) {
 // us: a chain of one load, two scans and two searches.
 template <bool MAPS>
 __global__ __launch_bounds__(PW) void paged_plan_kernel(PagedPlanArgs a) {
-    __shared__ int64_t red[PW / WAVE];
-    __shared__ int need0[PW], row0[PW], before[PW], past0[PW], lives[PW];
+    __shared__ uint32_t red[PW / WAVE];
+    __shared__ int need0[PW], row0[PW], before[PW], past0[PW], lives[PW], taken_by[PW / WAVE];
     const int tid = threadIdx.x, P = 1 << a.lp;
     const int n_free = min(max(*a.n_free, 0), a.n_pages);
     int64_t rows = 0, pages = 0;  // of the sequences so far
@@ -67,28 +75,35 @@ __global__ __launch_bounds__(PW) void paged_plan_kernel(PagedPlanArgs a) {
     for (int s0 = 0; s0 < a.n_seqs; s0 += PW) {
         const int s = s0 + tid, m = min(PW, a.n_seqs - s0);
         const bool real = s < a.n_seqs;
-        const int past = real ? a.past[s] : 0, fresh = real ? max(a.fresh[s], 0) : 0;
+        // more than all rows is as good as one more
+        const int past = real ? a.past[s] : 0, fresh = real ? min(max(a.fresh[s], 0), a.n_rows + 1) : 0;
         int64_t all, all_pages;
-        const int64_t end = rows + scan_add(fresh, red, all);
+        const int64_t end = rows + scan_add((uint32_t)fresh, red, all);
         const bool fits = real && past >= 0 && end <= a.n_rows && (int64_t)past + fresh <= (int64_t)a.stride << a.lp;
         const int have = fits ? pages_of(past, a.lp) : 0, need = fits ? pages_of(past + fresh, a.lp) - have : 0;
-        const int64_t run = pages + scan_add(need, red, all_pages);
+        const int64_t run = pages + scan_add((uint32_t)need, red, all_pages);
         const bool given = fits && (need == 0 || run <= n_free);
-        // given needs are the first of the sum, so a place in the list is the sum before
-        int64_t got;
-        const int64_t mine = scan_add(given ? need : 0, red, got);
-        need0[tid] = (int)(mine - (given ? need : 0));
+        // given needs are the first of the sum: a place in the list is the sum before, less what went
+        // before these sequences
+        need0[tid] = (int)min(run - need - pages, (int64_t)INT32_MAX);
         row0[tid] = (int)min(end - fresh, (int64_t)a.n_rows);
         before[tid] = have;
         past0[tid] = past;
         lives[tid] = given;
+        const int mine = given && need ? (int)(run - pages) : 0;
+        const unsigned long long takers = __ballot(mine > 0);
+        const int last = takers ? __builtin_amdgcn_readlane(mine, 63 - __clzll(takers)) : 0;
+        if ((tid & (WAVE - 1)) == 0) taken_by[tid / WAVE] = last;
         if (real) {
             a.lens[s] = given ? past + fresh : 0;
             a.starts[s + 1] = (int)min(end, (int64_t)a.n_rows);
         }
         __syncthreads();
+        int got = 0;
+#pragma unroll
+        for (int w = 0; w < PW / WAVE; w++) got = max(got, taken_by[w]);
         const int top = n_free - 1 - taken;
-        for (int k = tid; k < (int)got; k += PW) {
+        for (int k = tid; k < got; k += PW) {
             const int i = last_le(need0, m, k);
             a.table[(int64_t)(s0 + i) * a.stride + before[i] + k - need0[i]] = a.free_pages[top - k];
         }
@@ -110,7 +125,7 @@ __global__ __launch_bounds__(PW) void paged_plan_kernel(PagedPlanArgs a) {
         }
         rows += all;
         pages += all_pages;
-        taken += (int)got;
+        taken += got;
         __syncthreads();  // the sums are read before the next sequences' are written
     }
     if constexpr (MAPS)
@@ -142,7 +157,7 @@ __global__ __launch_bounds__(WG) void paged_maps_kernel(PagedPlanArgs a) {
 // Pages behind the first keep slots of each sequence go back on the list, in such
 // an order that a release of what the last plan took leaves the list as it was.
 __global__ __launch_bounds__(PW) void paged_release_kernel(PagedReleaseArgs a) {
-    __shared__ int64_t red[PW / WAVE];
+    __shared__ uint32_t red[PW / WAVE];
     __shared__ int sum0[PW], first[PW];
     const int tid = threadIdx.x;
     const int n_free = min(max(*a.n_free, 0), a.n_pages);
@@ -154,11 +169,12 @@ __global__ __launch_bounds__(PW) void paged_release_kernel(PagedReleaseArgs a) {
     };
     int64_t total = 0;
     if (a.n_seqs > PW) {
-        for (int s = tid; s < a.n_seqs; s += PW) {
+        for (int s0 = 0; s0 < a.n_seqs; s0 += PW) {
             int from;
-            total += span(s, from);
+            int64_t some;
+            scan_add(s0 + tid < a.n_seqs ? (uint32_t)span(s0 + tid, from) : 0u, red, some);
+            total += some;
         }
-        scan_add(total, red, total);
     }
     int64_t done = 0;
     for (int s0 = 0; s0 < a.n_seqs; s0 += PW) {
@@ -166,10 +182,10 @@ __global__ __launch_bounds__(PW) void paged_release_kernel(PagedReleaseArgs a) {
         int from = 0, all = 0;
         if (s < a.n_seqs) all = span(s, from);
         int64_t got;
-        const int64_t mine = scan_add(all, red, got);
+        const int64_t mine = scan_add((uint32_t)all, red, got);
         if (a.n_seqs <= PW) total = got;
         if (n_free + total > a.n_pages) return;  // more than the pool has: nothing is released
-        sum0[tid] = (int)(mine - all);
+        sum0[tid] = (int)min(mine - all, (int64_t)INT32_MAX);
         first[tid] = from;
         __syncthreads();
         for (int k = tid; k < (int)got; k += PW) {
@@ -253,10 +269,9 @@ __global__ __launch_bounds__(WG, 4) void paged_append_kernel(PagedAppendArgs a) 
     uint32_t raw[NR][F16 ? 1 : 2] = {};
 #pragma unroll
     for (int i = 0; i < NR; i++) {
-        const int t = t0 + i;
-        // rows past this workgroup's only where they go on a run
-        const bool in = slot[i + 1] >= 0 && (i < APPEND_T || ((slot[i + 1] & 7) != 0 && (slot[i + 1] & 7) >= i - APPEND_T + 1));
-        if (!in) continue;
+        const int t = min(t0 + i, a.n - 1);
+        // this workgroup's rows at once, those past them only where they go on a run
+        if (i >= APPEND_T && (slot[i + 1] < 0 || (slot[i + 1] & 7) == 0 || (slot[i + 1] & 7) < i - APPEND_T + 1)) continue;
         if constexpr (F16) {
             raw[i][0] = *(const uint32_t *)((const uint16_t *)a.x[1] + t * a.stride[1] + ev);
         } else {

@@ -46,8 +46,23 @@ constexpr int PU = 64;                   // of the prompts kernel
 
 __device__ __forceinline__ float ex2(float x) { return __builtin_amdgcn_exp2f(x); }
 
-// a number of the call's arrays, through the scalar cache where s is uniform
-__device__ __forceinline__ int seq_len(const PagedAttnArgs &a, int s) { return min(max(a.lens[s], 0), a.cap); }
+// a sequence's number in one of the call's arrays, through the scalar cache where all lanes ask for the same
+template <bool SCALAR>
+__device__ __forceinline__ int number(const int32_t *p, int s) {
+    if constexpr (SCALAR) return ((ScalarInts)(uintptr_t)p)[__builtin_amdgcn_readfirstlane(s)];
+    else return p[s];
+}
+template <bool SCALAR>
+__device__ __forceinline__ int seq_len(const PagedAttnArgs &a, int s) {
+    return min(max(number<SCALAR>(a.lens, s), 0), a.cap);
+}
+// All of the call's arguments asked for at once: a line of them at a time, where each is first
+// used, they take a chain of misses.
+__device__ __forceinline__ void ask(const PagedAttnArgs &a) {
+    asm volatile("" ::"s"(a.c.k), "s"(a.c.v), "s"(a.q), "s"(a.out), "s"(a.q_stride), "s"(a.out_stride), "s"(a.scale));
+    asm volatile("" ::"s"(a.magic), "s"(a.n_rows), "s"(a.starts), "s"(a.lens), "s"(a.table), "s"(a.stride), "s"(a.workers),
+                 "s"(a.tile_units), "s"(a.at), "s"(a.ml), "s"(a.part));
+}
 // The token of row r of a sequence and kv head (token-major): r / group by a
 // multiplication (exact while r * group < 2^32)
 __device__ __forceinline__ int row_token(const PagedAttnArgs &a, int r) {
@@ -65,79 +80,75 @@ __device__ __forceinline__ int page_ok(const PagedAttnArgs &a, int id) {
 
 // ------------------------------------------------------------- sharing out --
 
-__device__ __forceinline__ uint32_t quot(uint32_t x, uint32_t y) { return x / y; }
-// numbers below 2^53 (x >= 0, y > 0)
-__device__ __forceinline__ int64_t quot(int64_t x, int64_t y) {
-    if (((x | y) >> 32) == 0) return (uint32_t)x / (uint32_t)y;
-    int64_t q = (int64_t)((double)x / (double)y);
-    if (q * y > x) q--;
-    else if ((q + 1) * y <= x) q++;
-    return q;
-}
-
-// The tiles of a sequence and their costs.
-// Tokens: tiles alike, costs in units (where 32 bits do not hold their sum, 2^shift of them).
+// The tiles of a sequence and their costs, in units of slots (f32: a sum that f32 does not
+// hold to the unit moves borders by as much, alike for both workers at one).
+// Tokens: tiles alike.
 struct TokensWork {
-    using Cost = uint32_t;
-    static constexpr int OWN = 1, LEAST = 4, PARTS = 256;  // a tile's own cost, a worker's least, a tile's most parts
+    static constexpr int LEAST = 4, PARTS = 256, NEAR = 2;  // a worker's least, a tile's most parts, see border()
+    // A tile's own cost (its rows of q, the waves' results joined; 48 sequences 62 us with 1, 54
+    // with 4, 57 with 8)
+    static constexpr float OWN = 4.f;
     int len, tokens, tiles;
-    Cost first;
-    __device__ __forceinline__ TokensWork(const PagedAttnArgs &a, int s) {
-        len = seq_len(a, s);
-        tokens = a.n_q;
-        tiles = a.tiles;
-        first = ((uint32_t)((len + TU - 1) / TU + (1 << a.shift) - 1) >> a.shift) + OWN;
+    float first;
+    template <bool SCALAR>
+    __device__ static __forceinline__ TokensWork of(const PagedAttnArgs &a, int s) {
+        TokensWork w;
+        w.len = seq_len<SCALAR>(a, s);
+        w.tokens = a.n_q;
+        w.tiles = a.tiles;
+        w.first = (float)((w.len + TU - 1) / TU) + OWN;
+        return w;
     }
-    __device__ static __forceinline__ Cost unit(const PagedAttnArgs &) { return 1; }
-    __device__ __forceinline__ Cost all() const { return tiles * first; }
-    __device__ __forceinline__ Cost most() const { return first; }
+    __device__ __forceinline__ float all() const { return (float)tiles * first; }
+    __device__ __forceinline__ float most() const { return first; }
     __device__ __forceinline__ int units(const PagedAttnArgs &, int) const { return (len + TU - 1) / TU; }
     // the tile that x falls into, and the unit there
-    __device__ __forceinline__ int find(const PagedAttnArgs &a, Cost x, int &u) const {
-        const Cost t = quot(x, first), in = x - t * first;
-        u = in <= (Cost)OWN ? 0 : (int)min((in - OWN) << a.shift, (Cost)units(a, 0));
-        return (int)t;
+    __device__ __forceinline__ int find(const PagedAttnArgs &a, float x, int &u) const {
+        const int t = min((int)(x / first), tiles - 1);
+        u = min((int)max(x - (float)t * first - OWN, 0.f), units(a, 0));
+        return t;
     }
-    __device__ static __forceinline__ int near(const PagedAttnArgs &a, Cost share) { return (int)(min(share / 8, (Cost)2) << a.shift); }
 };
-// Prompts: a tile of R rows more sees R / group slots more; costs are slots times the group.
+// Prompts: a tile of R rows more sees R / group slots more.
 struct PromptsWork {
-    using Cost = int64_t;
-    static constexpr int R = 128, OWN = 1, LEAST = 4, PARTS = 128;
+    static constexpr int R = 128, LEAST = 4, PARTS = 128, NEAR = 8;
+    static constexpr float OWN = 4.f;  // nine short prompts 28 us with 1, 18 with 2 to 6
     int len, tokens, tiles;
-    Cost first;  // of tile 0, each further one R more
-    __device__ __forceinline__ PromptsWork(const PagedAttnArgs &a, int s) {
-        const int r0 = min(max(a.starts[s], 0), a.n_rows), r1 = min(max(a.starts[s + 1], r0), a.n_rows);
-        len = seq_len(a, s);
-        tokens = r1 - r0;
-        tiles = (int)(((int64_t)tokens * a.group + R - 1) / R);
-        first = (int64_t)a.group * (max(len - tokens, 0) + OWN * PU) + R;
+    float first, step;  // of tile 0, and what each further one costs more
+    template <bool SCALAR>
+    __device__ static __forceinline__ PromptsWork of(const PagedAttnArgs &a, int s) {
+        PromptsWork w;
+        const int r0 = min(max(number<SCALAR>(a.starts, s), 0), a.n_rows);
+        const int r1 = min(max(number<SCALAR>(a.starts, s + 1), r0), a.n_rows);
+        w.len = seq_len<SCALAR>(a, s);
+        w.tokens = r1 - r0;
+        w.tiles = (int)(((uint32_t)w.tokens * (uint32_t)a.group + R - 1) / R);  // rows stay below 2^32
+        w.step = a.tile_units;
+        w.first = (float)max(w.len - w.tokens, 0) * (1.f / PU) + OWN + w.step;
+        return w;
     }
-    __device__ static __forceinline__ Cost unit(const PagedAttnArgs &a) { return (int64_t)a.group * PU; }
-    __device__ __forceinline__ Cost upto(int64_t t) const { return t * first + R * (t * (t - 1) / 2); }
-    __device__ __forceinline__ Cost all() const { return upto(tiles); }
-    __device__ __forceinline__ Cost most() const { return tiles ? first + (int64_t)(tiles - 1) * R : 0; }
+    __device__ __forceinline__ float upto(float t) const { return t * (first + 0.5f * step * (t - 1.f)); }
+    __device__ __forceinline__ float all() const { return upto((float)tiles); }
+    __device__ __forceinline__ float most() const { return tiles ? first + (float)(tiles - 1) * step : 0.f; }
     __device__ __forceinline__ int units(const PagedAttnArgs &a, int tile) const {
         const int last = row_token(a, min(tile * R + R, tokens * a.group) - 1);
         return (max(len - tokens + last + 1, 0) + PU - 1) / PU;
     }
-    __device__ __forceinline__ int find(const PagedAttnArgs &a, Cost x, int &u) const {
-        // the last t with upto(t) <= x
-        const float b = (float)first - 0.5f * R;
-        int64_t t = (int64_t)((sqrtf(b * b + 2.f * R * (float)x) - b) * (1.f / R));
-        t = min(max(t, (int64_t)0), (int64_t)tiles - 1);
-        while (t > 0 && upto(t) > x) t--;
-        while (t + 1 < tiles && upto(t + 1) <= x) t++;
-        const int64_t in = x - upto(t), own = OWN * unit(a);
-        u = in <= own ? 0 : (int)quot((in - own) * units(a, (int)t), first + t * R - own);
-        return (int)t;
+    __device__ __forceinline__ int find(const PagedAttnArgs &a, float x, int &u) const {
+        // upto(t) = x solved, of its two forms the one that does not cancel
+        const float b = first - 0.5f * step;
+        const int t = min((int)(2.f * x / (b + sqrtf(b * b + 2.f * step * x))), tiles - 1);
+        const int n = units(a, t);
+        const float in = x - upto((float)t) - OWN, cost = first + (float)t * step - OWN;
+        u = min((int)(max(in, 0.f) / cost * (float)n), n);
+        return t;
     }
-    __device__ static __forceinline__ int near(const PagedAttnArgs &a, Cost share) { return (int)min(quot(share, 8 * unit(a)), (Cost)4); }
 };
 
 // Sums over the lanes up to each, and a lane's value for all.
-__device__ __forceinline__ uint32_t scan_lanes(uint32_t v) {
-#define OI_SCAN(ctrl, rows) v += (uint32_t)__builtin_amdgcn_update_dpp(0, (int)v, ctrl, rows, 0xF, false)
+__device__ __forceinline__ float scan_lanes(float v) {
+#define OI_SCAN(ctrl, rows) \
+    v += __int_as_float(__builtin_amdgcn_update_dpp(0, __float_as_int(v), ctrl, rows, 0xF, false))
     OI_SCAN(0x111, 0xF);  // rows of 16: 1, 2, 4, 8 lanes back
     OI_SCAN(0x112, 0xF);
     OI_SCAN(0x114, 0xF);
@@ -147,47 +158,46 @@ __device__ __forceinline__ uint32_t scan_lanes(uint32_t v) {
 #undef OI_SCAN
     return v;
 }
-__device__ __forceinline__ int64_t scan_lanes(int64_t v) {
-#pragma unroll
-    for (int d = 1; d < WAVE; d *= 2) {
-        const int64_t o = __shfl_up(v, d);
-        if ((int)__lane_id() >= d) v += o;
-    }
-    return v;
-}
-__device__ __forceinline__ uint32_t of_lane(uint32_t v, int i) { return (uint32_t)__builtin_amdgcn_readlane((int)v, i); }
-__device__ __forceinline__ int64_t of_lane(int64_t v, int i) {
-    return (int64_t)((uint64_t)of_lane((uint32_t)((uint64_t)v >> 32), i) << 32 | of_lane((uint32_t)(uint64_t)v, i));
-}
 
-// The border at x of the whole cost (below its end), given each lane's sum of `per`
-// neighbouring sequences (own) and that of the lanes up to it (run).
+// The border at x of the whole cost, given each lane's sum of `per` neighbouring sequences
+// (own) and that of the lanes up to it (run); x at or behind the end of all is that end.  It
+// rises with x, as every step of it does, so workers' stretches cover each unit once, wherever
+// rounding puts the borders.  Within NEAR units of a tile's end (an eighth of a share, if that is
+// less) it moves there.
 template <class W>
-__device__ PagedAt border(const PagedAttnArgs &a, typename W::Cost x, typename W::Cost share, typename W::Cost own,
-                          typename W::Cost run, int per) {
-    using Cost = typename W::Cost;
+__device__ PagedAt border(const PagedAttnArgs &a, float x, float share, float own, float run, int per) {
     const int lane = __lane_id();
-    int at = __ffsll((unsigned long long)__ballot(x < run)) - 1;
-    x -= of_lane(run, at) - of_lane(own, at);
+    unsigned long long hit = __ballot(x < run && own > 0.f);
+    if (!hit) return {a.n_seqs, 0, 0, 0};
+    int at = __ffsll(hit) - 1;
+    x = max(x - (lane_value(run, at) - lane_value(own, at)), 0.f);
     int s = at * per;
     if (per > 1) {  // these sequences, a lane each
-        for (int s1 = min(s + per, a.n_seqs);; s += WAVE) {
-            const Cost c = s + lane < s1 ? W(a, min(s + lane, s1 - 1)).all() * a.c.n_kv : (Cost)0, r = scan_lanes(c);
-            const unsigned long long hit = __ballot(x < r);
+        const int s1 = min(s + per, a.n_seqs);
+        int last = s;  // with tiles, so far: rounding may leave x behind them all
+        for (; s < s1; s += WAVE) {
+            const float c = s + lane < s1 ? W::template of<false>(a, min(s + lane, s1 - 1)).all() * (float)a.c.n_kv : 0.f;
+            const float r = scan_lanes(c);
+            hit = __ballot(x < r && c > 0.f);
             if (hit) {
                 at = __ffsll(hit) - 1;
-                x -= of_lane(r, at) - of_lane(c, at);
-                s += at;
+                x = max(x - (lane_value(r, at) - lane_value(c, at)), 0.f);
+                last = s + at;
                 break;
             }
-            x -= of_lane(r, WAVE - 1);
+            hit = __ballot(c > 0.f);
+            if (hit) last = s + 63 - __clzll(hit);
+            x -= lane_value(r, WAVE - 1);
         }
+        if (s >= s1) x = FLT_MAX;
+        s = last;
     }
-    const W w(a, s);
-    const Cost one = w.all();
-    int head = (int)quot(x, one), u;
-    int tile = w.find(a, x - head * one, u);
-    const int near = W::near(a, share);
+    s = __builtin_amdgcn_readfirstlane(s);
+    const W w = W::template of<true>(a, s);
+    const float one = w.all();
+    int head = min((int)min(x / one, 2e9f), a.c.n_kv - 1), u;
+    int tile = w.find(a, min(max(x - (float)head * one, 0.f), one), u);
+    const int near = (int)min(share * 0.125f, (float)W::NEAR);
     if (u <= near) {
         u = 0;
     } else if (w.units(a, tile) - u <= near) {
@@ -210,31 +220,25 @@ __device__ PagedAt border(const PagedAttnArgs &a, typename W::Cost x, typename W
 // 8 in turn), whose cache then holds what they share.
 template <class W>
 __device__ int share_out(const PagedAttnArgs &a, int &worker, PagedAt &begin, PagedAt &end) {
-    using Cost = typename W::Cost;
     const int lane = __lane_id(), per = (a.n_seqs + WAVE - 1) / WAVE;
     const int s0 = min(lane * per, a.n_seqs), s1 = min(s0 + per, a.n_seqs);
-    Cost own = 0, most = 0;
+    float own = 0.f, most = 0.f;
     for (int s = s0; s < s1; s++) {
-        const W w(a, s);
-        own += w.all() * a.c.n_kv;
+        const W w = W::template of<false>(a, s);
+        own += w.all() * (float)a.c.n_kv;
         most = max(most, w.most());
     }
-    const Cost run = scan_lanes(own), total = of_lane(run, WAVE - 1);
-    Cost share = max(quot((Cost)(total + a.workers - 1), (Cost)a.workers), (Cost)(W::LEAST * W::unit(a)));
-    // a tile that would have more than PARTS parts
-    for (unsigned long long m = __ballot(most > share * W::PARTS); m; m = __ballot(most > share * W::PARTS)) {
-        const Cost x = of_lane(most, __ffsll(m) - 1);
-        share = quot((Cost)(x + W::PARTS - 1), (Cost)W::PARTS);
-    }
-    const int used = (int)quot((Cost)(total + share - 1), share);
+    const float run = scan_lanes(own), total = lane_value(run, WAVE - 1);
+    const float share = max(max(total / (float)a.workers, (float)W::LEAST), wave_max_all(most) / (float)W::PARTS);
+    const int used = __builtin_amdgcn_readfirstlane(min((int)ceilf(total / share), a.workers));
     const int each = (used + 7) / 8, b = blockIdx.x;
     worker = b / 8 < each ? (b & 7) * each + b / 8 : used;
     if (worker < used) {
-        begin = border<W>(a, (Cost)worker * share, share, own, run, per);
+        begin = border<W>(a, (float)worker * share, share, own, run, per);
         end = {a.n_seqs, 0, 0, 0};
-        if (worker + 1 < used) end = border<W>(a, (Cost)(worker + 1) * share, share, own, run, per);
+        if (worker + 1 < used) end = border<W>(a, (float)(worker + 1) * share, share, own, run, per);
     }
-    return __builtin_amdgcn_readfirstlane(used);
+    return used;
 }
 __device__ __forceinline__ bool same_tile(const PagedAt &x, const PagedAt &y) {
     return x.seq == y.seq && x.head == y.head && x.tile == y.tile;
@@ -253,7 +257,7 @@ template <class W, class F>
 __device__ __forceinline__ void each_piece(const PagedAttnArgs &a, PagedAt at, const PagedAt end, F f) {
     while (at.seq < end.seq || (at.seq == end.seq && (at.head < end.head || (at.head == end.head &&
                                (at.tile < end.tile || (at.tile == end.tile && at.u < end.u)))))) {
-        const W w(a, at.seq);
+        const W w = W::template of<true>(a, at.seq);
         if (w.tiles) {
             const int units = w.units(a, at.tile);
             f(w, at, units, at.u, same_tile(at, end) ? end.u : units);
@@ -377,6 +381,7 @@ __global__ __launch_bounds__(WG, (TokensShape<HD, F16, NT>::PER_CU)) void paged_
     using W = TokensWork;
     __shared__ __attribute__((aligned(16))) float so[NW][16][PD];
     __shared__ float sm[NW][16], sl[NW][16];
+    ask(a);
     int worker;
     PagedAt begin, end;
     const int used = share_out<W>(a, worker, begin, end);
@@ -576,20 +581,127 @@ __device__ __forceinline__ bool first_cut(const PagedAt &at, const PagedAt &prev
     return at.u > 0 && !(same_tile(at, prev) && prev.u > 0);
 }
 
-// A row of a tile, whose parts may be many: a workgroup takes it.  BY_TILE: a workgroup
-// per tile (few of them) looks for the border in it; otherwise per border.  (m, l) and the
-// first results of every thread are requested together.
-constexpr int JPRE = 8;  // parts of a thread in the first round trip
-template <int HD, bool BY_TILE>
+// One row of n parts, a workgroup's work: (m, l) and the first results of every thread are
+// requested together.
+constexpr int JOIN_MOST = 512, JPRE = 8;  // parts of a tile; of a thread in the first round trip
+template <int HD>
+struct JoinLds {
+    static constexpr int LPR = HD / 4, MS = WG / LPR;  // lanes of a row, parts at a time
+    float wt[JOIN_MOST];
+    __attribute__((aligned(16))) float red[MS][HD];
+    float wmax[WG / WAVE], wsum[WG / WAVE];
+};
+// part 1 of worker w, then part 0 of those behind it
+__device__ __forceinline__ size_t part_at(const PagedAttnArgs &a, int w, int k, int r) {
+    return ((size_t)(w + k) * 2 + (k == 0)) * a.part_rows + r;
+}
+template <int HD>
+__device__ __forceinline__ void join_row(const PagedAttnArgs &a, int w, int n, int r, int64_t to, JoinLds<HD> &lds) {
+    constexpr int LPR = JoinLds<HD>::LPR, MS = JoinLds<HD>::MS, KP = JOIN_MOST / WG;
+    const int tid = threadIdx.x, lane = tid & (WAVE - 1), wave = tid / WAVE, col = tid % LPR, k0 = tid / LPR;
+    float2 ml[KP];
+    f32x4 pre[JPRE];
+#pragma unroll
+    for (int i = 0; i < KP; i++) ml[i] = tid + i * WG < n ? a.ml[part_at(a, w, tid + i * WG, r)] : make_float2(NEG, 0.f);
+#pragma unroll
+    for (int i = 0; i < JPRE; i++) {
+        const int k = k0 + i * MS;
+        pre[i] = k < n ? *(const f32x4 *)(a.part + part_at(a, w, k, r) * HD + 4 * col) : f32x4{0.f, 0.f, 0.f, 0.f};
+    }
+    float m = NEG;
+#pragma unroll
+    for (int i = 0; i < KP; i++) m = fmaxf(m, ml[i].x);
+    m = wave_max_all(m);
+    if (lane == 0) lds.wmax[wave] = m;
+    __syncthreads();
+#pragma unroll
+    for (int i = 0; i < WG / WAVE; i++) m = fmaxf(m, lds.wmax[i]);
+    float l = 0.f;
+#pragma unroll
+    for (int i = 0; i < KP; i++) {
+        const float f = ex2(ml[i].x - m);
+        // 0 for a part that saw nothing (an empty one has no results to read)
+        if (tid + i * WG < n) lds.wt[tid + i * WG] = ml[i].y == 0.f ? 0.f : f;
+        l += ml[i].y * f;
+    }
+    l = wave_sum(l);
+    if (lane == 0) lds.wsum[wave] = l;
+    __syncthreads();
+    l = 0.f;
+#pragma unroll
+    for (int i = 0; i < WG / WAVE; i++) l += lds.wsum[i];
+    f32x4 y = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+    for (int i = 0; i < JPRE; i++) {
+        const float f = k0 + i * MS < n ? lds.wt[k0 + i * MS] : 0.f;
+        if (f != 0.f) y += pre[i] * f;
+    }
+#pragma unroll 8
+    for (int k = k0 + JPRE * MS; k < n; k += MS) {
+        const f32x4 p = *(const f32x4 *)(a.part + part_at(a, w, k, r) * HD + 4 * col);
+        const float f = lds.wt[k];
+        if (f != 0.f) y += p * f;
+    }
+    *(f32x4 *)&lds.red[k0][4 * col] = y;
+    __syncthreads();
+    if (tid < LPR) {
+#pragma unroll
+        for (int k = 1; k < MS; k++) y += *(const f32x4 *)&lds.red[k][4 * col];
+        store_out(a.out, a.f16, to + 4 * col, y * inverse(l));
+    }
+}
+// RT rows of few parts, RT WG * 4 / HD of them apart from each other, four dimensions a thread;
+// at(r): where row r goes
+template <int HD, int RT, class F>
+__device__ __forceinline__ void join_rows(const PagedAttnArgs &a, int w, int n, int r0, int rows, F at) {
+    constexpr int LPR = HD / 4, RPW = WG / LPR, B = RT == 1 ? 4 : 2;
+    const int col = threadIdx.x % LPR, r1 = r0 + threadIdx.x / LPR;
+    float M[RT], L[RT];
+    f32x4 y[RT];
+#pragma unroll
+    for (int t = 0; t < RT; t++) {
+        M[t] = NEG;
+        L[t] = 0.f;
+        y[t] = f32x4{0.f, 0.f, 0.f, 0.f};
+    }
+    for (int k0 = 0; k0 < n; k0 += B) {
+        float2 ml[RT][B];
+        f32x4 p[RT][B];
+#pragma unroll
+        for (int t = 0; t < RT; t++)
+#pragma unroll
+            for (int i = 0; i < B; i++) {
+                const size_t slot = part_at(a, w, min(k0 + i, n - 1), min(r1 + t * RPW, rows - 1));
+                ml[t][i] = a.ml[slot];
+                p[t][i] = *(const f32x4 *)(a.part + slot * HD + 4 * col);
+            }
+#pragma unroll
+        for (int t = 0; t < RT; t++)
+#pragma unroll
+            for (int i = 0; i < B; i++) {
+                if (k0 + i >= n || ml[t][i].y == 0.f) continue;  // saw nothing: an empty part has no results
+                const float m1 = fmaxf(M[t], ml[t][i].x), f0 = ex2(M[t] - m1), f1 = ex2(ml[t][i].x - m1);
+                L[t] = L[t] * f0 + ml[t][i].y * f1;
+                y[t] = y[t] * f0 + p[t][i] * f1;
+                M[t] = m1;
+            }
+    }
+#pragma unroll
+    for (int t = 0; t < RT; t++)
+        if (r1 + t * RPW < rows) store_out(a.out, a.f16, at(r1 + t * RPW) + 4 * col, y[t] * inverse(L[t]));
+}
+
+// Tokens.  BY_TILE: a workgroup per tile (there are few) looks for the borders in it;
+// otherwise one per border.  ROWS: 1, or those that a workgroup takes at once where their parts
+// are few (3840 workgroups of a row each took 9 us for drafts of 24 sequences, 5 this way).
+constexpr int JOIN_FEW = 32;
+template <int HD, bool BY_TILE, int ROWS>
 __global__ __launch_bounds__(WG, 4) void paged_join_kernel(PagedAttnArgs a) {
-    constexpr int LPR = HD / 4, MS = WG / LPR, MOST = 512, KP = MOST / WG;  // lanes of a row, parts at a time
-    constexpr int NB = BY_TILE ? 2 : KP;                                    // borders of a thread
-    static_assert(TokensWork::PARTS + 2 <= MOST, "a tile's parts fit");
-    __shared__ float wt[MOST];
-    __shared__ __attribute__((aligned(16))) float red[MS][HD];
-    __shared__ float wmax[WG / WAVE], wsum[WG / WAVE];
+    constexpr int NB = JOIN_MOST / WG;  // borders of a thread
+    static_assert(TokensWork::PARTS + 2 <= JOIN_MOST && 2 * 256 <= JOIN_MOST, "a tile's parts, and all workers, fit");
+    __shared__ JoinLds<HD> lds;
     __shared__ int count[WG / WAVE], least[WG / WAVE];
-    const int r = blockIdx.y, tid = threadIdx.x, lane = tid & (WAVE - 1), wave = tid / WAVE;
+    const int r0 = blockIdx.y * ROWS, tid = threadIdx.x, lane = tid & (WAVE - 1), wave = tid / WAVE;
     const int used = a.at[a.workers].seq;
     PagedAt at;
     int w0 = blockIdx.x;  // the border looked at first is w0 + 1
@@ -602,7 +714,8 @@ __global__ __launch_bounds__(WG, 4) void paged_join_kernel(PagedAttnArgs a) {
         const PagedAt prev = a.at[w0];
         if (w0 + 1 >= used || !first_cut(at, prev)) return;
     }
-    if (r >= a.n_q * a.group - at.tile * a.tile_rows) return;
+    const int rows = min(a.n_q * a.group - at.tile * a.tile_rows, a.tile_rows);
+    if (r0 >= rows) return;
     // borders inside the tile are neighbours
     int n = 0, first = INT32_MAX;
 #pragma unroll
@@ -626,107 +739,41 @@ __global__ __launch_bounds__(WG, 4) void paged_join_kernel(PagedAttnArgs a) {
     }
     if (n == 0) return;
     n++;
-    const int w = first - 1;  // its part 1, then part 0 of those behind it
-    auto slot = [&](int k) { return ((size_t)(w + k) * 2 + (k == 0)) * a.part_rows + r; };
-    float2 ml[KP];
-    f32x4 pre[JPRE];
-    const int col = tid % LPR, k0 = tid / LPR;
-#pragma unroll
-    for (int i = 0; i < KP; i++) ml[i] = tid + i * WG < n ? a.ml[slot(tid + i * WG)] : make_float2(NEG, 0.f);
-#pragma unroll
-    for (int i = 0; i < JPRE; i++) {
-        const int k = k0 + i * MS;
-        pre[i] = k < n ? *(const f32x4 *)(a.part + slot(k) * HD + 4 * col) : f32x4{0.f, 0.f, 0.f, 0.f};
-    }
-    float m = NEG;
-#pragma unroll
-    for (int i = 0; i < KP; i++) m = fmaxf(m, ml[i].x);
-    m = wave_max_all(m);
-    if (lane == 0) wmax[wave] = m;
-    __syncthreads();
-#pragma unroll
-    for (int i = 0; i < WG / WAVE; i++) m = fmaxf(m, wmax[i]);
-    float l = 0.f;
-#pragma unroll
-    for (int i = 0; i < KP; i++) {
-        const float f = ex2(ml[i].x - m);
-        // 0 for a part that saw nothing (an empty one has no results to read)
-        if (tid + i * WG < n) wt[tid + i * WG] = ml[i].y == 0.f ? 0.f : f;
-        l += ml[i].y * f;
-    }
-    l = wave_sum(l);
-    if (lane == 0) wsum[wave] = l;
-    __syncthreads();
-    l = 0.f;
-#pragma unroll
-    for (int i = 0; i < WG / WAVE; i++) l += wsum[i];
-    f32x4 y = {0.f, 0.f, 0.f, 0.f};
-#pragma unroll
-    for (int i = 0; i < JPRE; i++) {
-        const float f = k0 + i * MS < n ? wt[k0 + i * MS] : 0.f;
-        if (f != 0.f) y += pre[i] * f;
-    }
-#pragma unroll 8
-    for (int k = k0 + JPRE * MS; k < n; k += MS) {
-        const f32x4 p = *(const f32x4 *)(a.part + slot(k) * HD + 4 * col);
-        const float f = wt[k];
-        if (f != 0.f) y += p * f;
-    }
-    *(f32x4 *)&red[k0][4 * col] = y;
-    __syncthreads();
-    if (tid < LPR) {
-#pragma unroll
-        for (int k = 1; k < MS; k++) y += *(const f32x4 *)&red[k][4 * col];
-        store_out(a.out, a.f16, row_at(a, at.seq * a.n_q, at.tile * a.tile_rows + r, at.head, a.out_stride) + 4 * col,
-                  y * inverse(l));
+    const int w = first - 1;
+    auto to = [&](int r) { return row_at(a, at.seq * a.n_q, at.tile * a.tile_rows + r, at.head, a.out_stride); };
+    if constexpr (ROWS == 1) {
+        join_row<HD>(a, w, n, r0, to(r0), lds);
+    } else if (n <= JOIN_FEW) {
+        join_rows<HD, ROWS * HD / 4 / WG>(a, w, n, r0, min(rows, r0 + ROWS), to);
+    } else {
+        for (int r = r0; r < min(rows, r0 + ROWS); r++) {
+            join_row<HD>(a, w, n, r, to(r), lds);
+            __syncthreads();  // LDS is read before the next row is written there
+        }
     }
 }
 
-// Many rows of few parts: four dimensions a thread.
-template <int HD>
+// Prompts: a workgroup per border, RT rows a thread.
+template <int HD, int RT>
 __global__ __launch_bounds__(WG) void paged_join_rows_kernel(PagedAttnArgs a) {
-    constexpr int LPR = HD / 4, RPW = WG / LPR;
-    const int w = blockIdx.x, tid = threadIdx.x, lane = tid & (WAVE - 1);
+    constexpr int R = PromptsWork::R, ROWS = WG * 4 / HD * RT;
+    const int w = blockIdx.x, lane = threadIdx.x & (WAVE - 1), r0 = blockIdx.y * ROWS;
     const int used = a.at[a.workers].seq;
     const PagedAt at = a.at[w + 1], prev = a.at[w];
     const PagedAt next = w + 1 + lane < a.workers ? a.at[w + 1 + lane] : PagedAt{-1, 0, 0, 0};
     if (w + 1 >= used || !first_cut(at, prev)) return;
-    constexpr int R = PromptsWork::R;
-    const PromptsWork sw(a, at.seq);
+    const PromptsWork sw = PromptsWork::of<true>(a, at.seq);
     const int rows = min(sw.tokens * a.group - at.tile * R, R);
-    const int r = blockIdx.y * RPW + tid / LPR, col = tid % LPR;
-    if ((int)blockIdx.y * RPW >= rows) return;
+    if (r0 >= rows) return;
     // neighbours all: 1 and those of the next 64 that begin inside the tile, and so on
     int n = 1 + __popcll(__ballot(w + 1 + lane < used && same_tile(next, at) && next.u > 0));
     for (int k = w + 1 + WAVE; n == k - w && k < used; k += WAVE) {
         const PagedAt x = k + lane < used ? a.at[k + lane] : PagedAt{-1, 0, 0, 0};
         n += __popcll(__ballot(same_tile(x, at) && x.u > 0));
     }
-    if (r >= rows) return;
-    float M = NEG, L = 0.f;
-    f32x4 y = {0.f, 0.f, 0.f, 0.f};
-    constexpr int B = 4;
-    for (int k0 = 0; k0 < n; k0 += B) {
-        float2 ml[B];
-        f32x4 p[B];
-#pragma unroll
-        for (int i = 0; i < B; i++) {
-            const int k = min(k0 + i, n - 1);
-            const size_t slot = ((size_t)(w + k) * 2 + (k == 0)) * a.part_rows + r;
-            ml[i] = a.ml[slot];
-            p[i] = *(const f32x4 *)(a.part + slot * HD + 4 * col);
-        }
-#pragma unroll
-        for (int i = 0; i < B; i++) {
-            if (k0 + i >= n || ml[i].y == 0.f) continue;  // saw nothing: an empty part has no results
-            const float m1 = fmaxf(M, ml[i].x), f0 = ex2(M - m1), f1 = ex2(ml[i].x - m1);
-            L = L * f0 + ml[i].y * f1;
-            y = y * f0 + p[i] * f1;
-            M = m1;
-        }
-    }
     const int base = min(max(a.starts[at.seq], 0), a.n_rows);
-    store_out(a.out, a.f16, row_at(a, base, at.tile * R + r, at.head, a.out_stride) + 4 * col, y * inverse(L));
+    join_rows<HD, RT>(a, w, n, r0, rows,
+                           [&](int r) { return row_at(a, base, at.tile * R + r, at.head, a.out_stride); });
 }
 
 // ---------------------------------------------------------------- prompts --
@@ -759,6 +806,7 @@ __global__ __launch_bounds__(WG, (PromptsShape<HD, F16>::PER_CU)) void paged_pro
     constexpr float PS = F16 ? 3.f : 9.f, LAZY = 15.f - PS;
     using W = PromptsWork;
     __shared__ __attribute__((aligned(16))) f16x8 kl[2][PIECES], vl[2][PIECES];
+    ask(a);
     int worker;
     PagedAt begin, end;
     const int used = share_out<W>(a, worker, begin, end);
@@ -1025,25 +1073,40 @@ __global__ __launch_bounds__(WG, (PromptsShape<HD, F16>::PER_CU)) void paged_pro
     });
 }
 
+constexpr int CUS = 256;
+
+unsigned groups_of(int n, int size) { return (unsigned)((n + size - 1) / size); }
+
 template <int HD, bool F16>
 void prompts(const PagedAttnArgs &a, hipStream_t st) {
-    constexpr int RPW = WG * 4 / HD;
     hipLaunchKernelGGL((paged_prompts_kernel<HD, F16>), dim3((unsigned)a.workers), dim3(WG), 0, st, a);
-    hipLaunchKernelGGL((paged_join_rows_kernel<HD>), dim3((unsigned)a.workers - 1, (unsigned)((a.part_rows + RPW - 1) / RPW)),
-                       dim3(WG), 0, st, a);
+    // about as many tiles as workers: two parts each, four rows a thread; few tiles: many parts
+    constexpr int RT = 4, ROWS = WG * 4 / HD;
+    const int64_t tiles = ((int64_t)a.n_rows * a.group / PR + a.n_seqs) * a.c.n_kv;
+    if (2 * tiles > a.workers)
+        hipLaunchKernelGGL((paged_join_rows_kernel<HD, RT>), dim3((unsigned)a.workers - 1, groups_of(a.part_rows, ROWS * RT)),
+                           dim3(WG), 0, st, a);
+    else
+        hipLaunchKernelGGL((paged_join_rows_kernel<HD, 1>), dim3((unsigned)a.workers - 1, groups_of(a.part_rows, ROWS)), dim3(WG),
+                           0, st, a);
+}
+template <int HD, bool BY_TILE>
+void join_tokens(const PagedAttnArgs &a, int n, hipStream_t st) {
+    constexpr int ROWS = WG * 4 / HD;
+    if ((int64_t)n * a.part_rows <= 4 * CUS)
+        hipLaunchKernelGGL((paged_join_kernel<HD, BY_TILE, 1>), dim3((unsigned)n, (unsigned)a.part_rows), dim3(WG), 0, st, a);
+    else
+        hipLaunchKernelGGL((paged_join_kernel<HD, BY_TILE, ROWS>), dim3((unsigned)n, groups_of(a.part_rows, ROWS)), dim3(WG), 0,
+                           st, a);
 }
 template <int HD, bool F16, int NT>
 void tokens(const PagedAttnArgs &a, hipStream_t st) {
     if (a.groups) hipLaunchKernelGGL((paged_tokens_kernel<HD, F16, NT, true>), dim3((unsigned)a.workers), dim3(WG), 0, st, a);
     else hipLaunchKernelGGL((paged_tokens_kernel<HD, F16, NT, false>), dim3((unsigned)a.workers), dim3(WG), 0, st, a);
     const int64_t items = (int64_t)a.n_seqs * a.c.n_kv * a.tiles;
-    if (items < a.workers)
-        hipLaunchKernelGGL((paged_join_kernel<HD, true>), dim3((unsigned)items, (unsigned)a.part_rows), dim3(WG), 0, st, a);
-    else
-        hipLaunchKernelGGL((paged_join_kernel<HD, false>), dim3((unsigned)a.workers - 1, (unsigned)a.part_rows), dim3(WG), 0, st, a);
+    if (items < a.workers) join_tokens<HD, true>(a, (int)items, st);
+    else join_tokens<HD, false>(a, a.workers - 1, st);
 }
-
-constexpr int CUS = 256;
 
 }  // namespace
 

@@ -147,9 +147,3 @@ def test_attention_refusals(which):
                  dict(ws=M + 256), dict(ws=ATTN["q"] + 1024), dict(ws=ATTN["lens"] - 16), dict(out=ATTN["ws"] + 64),
                  dict(out=ATTN["q"] + 512 * 4 * rows - 16)) + ((dict(out=ATTN["starts"]),) if which == "prompts" else ()):
         assert attn(which, **over) == E_ARG and said("overlaps"), over
-
-
-def test_more_work_than_whole_numbers_hold():
-    a = dict(ATTN, heads=4096, n=1, seqs=65536, stride=1 << 24, qs=4096 * 128, os=4096 * 128, q=1 << 50, out=1 << 52, ws=1 << 54,
-             table=1 << 56)
-    assert attn("tokens", **a) == E_RANGE and said("rows times")
