@@ -137,21 +137,19 @@ __global__ __launch_bounds__(PW) void paged_plan_kernel(PagedPlanArgs a) {
     if (tid == 0) *a.n_free = n_free - taken;  // every thread has read it before the first barrier
 }
 
-// The rows' maps from the sequences' starts, lengths and pages: sequence by
-// sequence (the last "sequence" the rows behind them), in parts.
+// The rows' maps from the sequences' starts, lengths and pages, a row a thread.
 __global__ __launch_bounds__(WG) void paged_maps_kernel(PagedPlanArgs a) {
-    const int s = blockIdx.x, step = gridDim.y * WG;
-    const bool pad = s == a.n_seqs;
-    const int r0 = a.starts[s], r1 = pad ? a.n_rows : a.starts[s + 1];
-    const int len = pad ? 0 : a.lens[s];
-    const int j0 = len - (r1 - r0);  // slots held before
-    const int32_t *row = a.table + (int64_t)s * a.stride;
-    for (int r = r0 + blockIdx.y * WG + threadIdx.x; r < r1; r += step) {
-        const int j = j0 + r - r0;
-        a.slots[r] = len > 0 ? slot_of(row[j >> a.lp], j & ((1 << a.lp) - 1), a.lp, a.n_pages) : -1;
-        if (a.pos)
-            for (int x = 0; x < 3; x++) a.pos[(int64_t)x * a.n_rows + r] = len > 0 ? j : 0;
+    const int r = blockIdx.x * WG + threadIdx.x;
+    if (r >= a.n_rows) return;
+    const int s = last_le(a.starts, a.n_seqs + 1, r);  // n_seqs: behind the last row
+    int slot = -1, j = 0;
+    if (s < a.n_seqs && a.lens[s] > 0) {
+        j = a.lens[s] - a.starts[s + 1] + r;
+        slot = slot_of(a.table[(int64_t)s * a.stride + (j >> a.lp)], j & ((1 << a.lp) - 1), a.lp, a.n_pages);
     }
+    a.slots[r] = slot;
+    if (a.pos)
+        for (int x = 0; x < 3; x++) a.pos[(int64_t)x * a.n_rows + r] = j;
 }
 
 // Pages behind the first keep slots of each sequence go back on the list, in such
@@ -333,9 +331,7 @@ hipError_t launch_paged_plan(const PagedPlanArgs &a, hipStream_t st) {
         return hipGetLastError();
     }
     hipLaunchKernelGGL(paged_plan_kernel<false>, dim3(1), dim3(PW), 0, st, a);
-    const unsigned parts = (unsigned)((a.n_rows / (a.n_seqs + 1) + 4 * WG - 1) / (4 * WG));
-    hipLaunchKernelGGL(paged_maps_kernel, dim3((unsigned)a.n_seqs + 1, parts < 1 ? 1 : parts > 256 ? 256 : parts), dim3(WG),
-                       0, st, a);
+    hipLaunchKernelGGL(paged_maps_kernel, dim3((unsigned)((a.n_rows + WG - 1) / WG)), dim3(WG), 0, st, a);
     return hipGetLastError();
 }
 

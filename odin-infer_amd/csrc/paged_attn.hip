@@ -412,17 +412,23 @@ __global__ __launch_bounds__(WG, (TokensShape<HD, F16, NT>::PER_CU)) void paged_
             k = table[min((u * TU + (kslot & ~7)) >> lp, last_page)];
             v = table[min((u * TU + 8 * g) >> lp, last_page)];
         };
+        // Read once, by one wave, K and V pass the caches by (48 sequences of 320 MB 61 -> 54 us); the
+        // groups' waves find them there (drafts of 24 sequences 21 us, 25 the other way).
+        auto once = [](const uint16_t *p) {
+            if constexpr (GROUPS) return *(const u32x4 *)p;
+            else return ldg_nt((const u32x4 *)p);
+        };
         auto load_k = [&](int u) {
             const uint16_t *p = kb + page_ok(a, kp) * page_elems + (size_t)((u * TU + kslot) & (P - 1)) * HD;
 #pragma unroll
             for (int t = 0; t < 2; t++)
 #pragma unroll
-                for (int f = 0; f < NK; f++) kr[t][f] = *(const u32x4 *)(p + 4 * t * HD + 32 * f);
+                for (int f = 0; f < NK; f++) kr[t][f] = once(p + 4 * t * HD + 32 * f);
         };
         auto load_v = [&](int u, int page) {
             const uint16_t *p = vb + page_ok(a, page) * page_elems + (size_t)((u * TU + 8 * g) & (P - 1)) * HD;
 #pragma unroll
-            for (int d = 0; d < ND; d++) vr[d] = *(const u32x4 *)(p + 16 * d * 8);
+            for (int d = 0; d < ND; d++) vr[d] = once(p + 16 * d * 8);
         };
         float m[NT], l[NT], mul[NT];
         int limit[NT];  // slots that this lane's rows see
@@ -654,7 +660,7 @@ __device__ __forceinline__ void join_row(const PagedAttnArgs &a, int w, int n, i
 // at(r): where row r goes
 template <int HD, int RT, class F>
 __device__ __forceinline__ void join_rows(const PagedAttnArgs &a, int w, int n, int r0, int rows, F at) {
-    constexpr int LPR = HD / 4, RPW = WG / LPR, B = RT == 1 ? 4 : 2;
+    constexpr int LPR = HD / 4, RPW = WG / LPR, B = RT == 1 ? 8 : 2;
     const int col = threadIdx.x % LPR, r1 = r0 + threadIdx.x / LPR;
     float M[RT], L[RT];
     f32x4 y[RT];
