@@ -61,8 +61,8 @@ __device__ __forceinline__ int slot_of(int page, int off, int lp, int n_pages) {
 // and pages; then the pages of these sequences, and (MAPS) their rows, over all
 // threads, the owner by bisection of the sums in LDS.  The n-th page taken is
 // the list's n-th from its end.  A page of a row that is new here is looked up in
-// the list, not in the table that another thread writes.  A step of 61 sequences 3.9
-// us: a chain of one load, two scans and two searches.
+// the list, not in the table that another thread writes.  A step of 61 sequences 4.4
+// us (a release of them 2.7): a chain of one load, two scans and two searches.
 template <bool MAPS>
 __global__ __launch_bounds__(PW) void paged_plan_kernel(PagedPlanArgs a) {
     __shared__ uint32_t red[PW / WAVE];
@@ -207,8 +207,8 @@ constexpr int APPEND_T = 8, APPEND_E = 512;  // packed rows and elements of a wo
 // A workgroup takes 8 packed rows and 512 of their elements.  K: a wave per row,
 // 16-byte stores.  V lies in eights of slots: rows whose slots are neighbours in one
 // eight (a run, found from the slots alone) are written together, a whole run as one
-// 16-byte piece per dimension; it belongs to the workgroup of its first row.  64 rows
-// of 8 heads of 128 (f32) 4.4 us, one chain; 8231 f16 rows 19 us: 4 TB/s, the rate of a copy.
+// 16-byte piece per dimension; it belongs to the workgroup of its first row.  8353 f16
+// rows of 8 heads of 128 17 us: 4.0 TB/s behind a launch's ramp, where a large copy makes 4.7.
 template <bool F16>
 __global__ __launch_bounds__(WG, 4) void paged_append_kernel(PagedAppendArgs a) {
     constexpr int NR = 2 * APPEND_T - 1;
@@ -321,11 +321,44 @@ __global__ __launch_bounds__(WG, 4) void paged_append_kernel(PagedAppendArgs a) 
     }
 }
 
+// Few rows: a row a workgroup, four elements a thread, V's by 2-byte stores; the slot and the
+// values are one round trip.  Rows of 8 heads of 128, one of each sequence: 64 3.2 us (by runs 6.4),
+// 300 5.1 (7.2); neighbours in one sequence: 300 4.9 (4.8), 1000 10 (6.2).
+constexpr int APPEND_FEW = 256;
+template <bool F16>
+__global__ __launch_bounds__(WG) void paged_append_row_kernel(PagedAppendArgs a) {
+    const int t = blockIdx.x, e = (blockIdx.y * WG + threadIdx.x) * 4;
+    const int row = a.c.n_kv * a.c.hd, lh = a.c.hd == 128 ? 7 : 8, P = 1 << a.c.lp;
+    if (e >= row) return;
+    const int s = a.slots[t];
+    uint32_t h[2][4];
+#pragma unroll
+    for (int w = 0; w < 2; w++) {
+        if constexpr (F16) {
+            const u32x2 x = *(const u32x2 *)((const uint16_t *)a.x[w] + (int64_t)t * a.stride[w] + e);
+#pragma unroll
+            for (int i = 0; i < 4; i++) h[w][i] = stored(h2f((i < 2 ? x.x : x.y) >> 16 * (i & 1) & 0xFFFFu));
+        } else {
+            const float4 x = *(const float4 *)((const float *)a.x[w] + (int64_t)t * a.stride[w] + e);
+            h[w][0] = stored(x.x);
+            h[w][1] = stored(x.y);
+            h[w][2] = stored(x.z);
+            h[w][3] = stored(x.w);
+        }
+    }
+    if (s < 0 || s >= (int64_t)a.c.n_pages << a.c.lp) return;
+    const size_t head = (((size_t)(s >> a.c.lp) * a.c.n_kv + (e >> lh)) << a.c.lp) * a.c.hd;
+    const int off = s & (P - 1), d = e & (a.c.hd - 1);
+    *(u32x2 *)(a.c.k + head + (size_t)off * a.c.hd + d) = u32x2{h[0][0] | h[0][1] << 16, h[0][2] | h[0][3] << 16};
+    uint16_t *v = a.c.v + head + (size_t)(off & ~7) * a.c.hd + d * 8 + (off & 7);
+#pragma unroll
+    for (int i = 0; i < 4; i++) v[8 * i] = (uint16_t)h[1][i];
+}
+
 }  // namespace
 
 hipError_t launch_paged_plan(const PagedPlanArgs &a, hipStream_t st) {
-    // one launch while the rows are few passes of the one workgroup (4 us for 1024 rows, and
-    // another 0.4 for every 1024; the second launch takes 3)
+    // one launch while the rows are few passes of the one workgroup; a second one takes 4 us
     if (a.n_rows <= 4096) {
         hipLaunchKernelGGL(paged_plan_kernel<true>, dim3(1), dim3(PW), 0, st, a);
         return hipGetLastError();
@@ -341,6 +374,12 @@ hipError_t launch_paged_release(const PagedReleaseArgs &a, hipStream_t st) {
 }
 
 hipError_t launch_paged_append(const PagedAppendArgs &a, hipStream_t st) {
+    if (a.n <= APPEND_FEW) {
+        const dim3 grid((unsigned)a.n, (unsigned)((a.c.n_kv * a.c.hd + 4 * WG - 1) / (4 * WG)));
+        if (a.f16) hipLaunchKernelGGL(paged_append_row_kernel<true>, grid, dim3(WG), 0, st, a);
+        else hipLaunchKernelGGL(paged_append_row_kernel<false>, grid, dim3(WG), 0, st, a);
+        return hipGetLastError();
+    }
     const dim3 grid((unsigned)((a.n + APPEND_T - 1) / APPEND_T), (unsigned)((a.c.n_kv * a.c.hd + APPEND_E - 1) / APPEND_E));
     if (a.f16) hipLaunchKernelGGL(paged_append_kernel<true>, grid, dim3(WG), 0, st, a);
     else hipLaunchKernelGGL(paged_append_kernel<false>, grid, dim3(WG), 0, st, a);

@@ -181,6 +181,9 @@ def rows(rng, n, n_kv, hd, t, special):
     (3, 128, 16, [100, 7, 9, 64]),
     (5, 256, 64, [33, 2]),
     (16, 128, 32, [20, 20, 1, 1, 1, 90]),
+    (8, 128, 64, [300, 5, 1, 1, 40]),  # more rows than one a workgroup
+    (2, 256, 16, [1] * 270),
+    (1, 256, 32, [9, 400, 0, 7]),
 ])
 def test_append(t, n_kv, hd, page, news):
     rng = np.random.default_rng(n_kv * hd + page + len(news) + t)
