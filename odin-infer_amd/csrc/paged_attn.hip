@@ -905,7 +905,7 @@ __global__ __launch_bounds__(WG, (PromptsShape<HD, F16>::PER_CU)) void paged_pro
         // The softmax of a half in steps: the maximum of score pairs, the rows' new maxima, weights of a
         // pair.  Rows rise together, so that one that climbs takes the others along and few halves
         // rise at all; alpha: what o is to be multiplied by then.
-        float top = 0.f, alpha = 1.f, bias = 0.f;
+        float top = 0.f, alpha = 1.f, bias = 0.f, sum = 0.f;  // sum: of the half's weights
         bool rise = false;
         auto higher = [&](const f32x16 &s, int i) {
             top = i == 0 ? fmaxf(s[0], s[1]) : fmaxf(fmaxf(top, s[2 * i]), s[2 * i + 1]);
@@ -926,12 +926,13 @@ __global__ __launch_bounds__(WG, (PromptsShape<HD, F16>::PER_CU)) void paged_pro
                 const float p = ex2(fmaf(s[2 * i + k], mul, bias));
                 hi[k] = (_Float16)p;
                 if constexpr (!F16) {
-                    l += p;
+                    sum = i + k == 0 ? p : sum + p;
                     lo[k] = (_Float16)(p - (float)hi[k]);
                 }
             }
-            if constexpr (F16) l = __builtin_amdgcn_fdot2(hi, f16x2{(_Float16)1.f, (_Float16)1.f}, l, false);
-            asm volatile("" : "+v"(hi), "+v"(l));  // here, not where it is used
+            if constexpr (F16) sum = __builtin_amdgcn_fdot2(hi, f16x2{(_Float16)1.f, (_Float16)1.f}, i == 0 ? 0.f : sum, false);
+            if (i == 7) l += sum;
+            asm volatile("" : "+v"(hi), "+v"(sum));  // here, not where it is used
             if constexpr (!F16) asm volatile("" : "+v"(lo));
 #pragma unroll
             for (int k = 0; k < 2; k++) {
