@@ -910,9 +910,11 @@ __global__ __launch_bounds__(WG, (PromptsShape<HD, F16>::PER_CU)) void paged_pro
         auto higher = [&](const f32x16 &s, int i) {
             top = i == 0 ? fmaxf(s[0], s[1]) : fmaxf(fmaxf(top, s[2 * i]), s[2 * i + 1]);
         };
+        auto highest = [&]() { top = half_reduce(top * mul, Max()); };
         auto turn = [&]() {
-            top = half_reduce(top * mul, Max());
             rise = __any(top > m + LAZY);
+            // a branch where registers allow (the f32 form at head_dim 256 takes 310 us with it, 278 without)
+            if (PromptsShape<HD, F16>::PER_CU == 2 && __builtin_expect(!rise, 1)) return;
             const float m1 = rise ? fmaxf(m, ceilf(top)) : m;
             alpha = ex2(m - m1);
             m = m1;
@@ -983,9 +985,11 @@ __global__ __launch_bounds__(WG, (PromptsShape<HD, F16>::PER_CU)) void paged_pro
 #pragma unroll
                     for (int i = 8 * j / CLIMB; i < 8 * (j + 1) / CLIMB; i++) higher(s0, i);
                 } else if (j == CLIMB) {
+                    highest();
+                } else if (j == CLIMB + 1) {
                     turn();
-                } else if ((j - CLIMB - 1) % STEP == 0 && (j - CLIMB - 1) / STEP < 8) {
-                    weigh(s0, ph1, pl1, (j - CLIMB - 1) / STEP);
+                } else if ((j - CLIMB - 2) % STEP == 0 && (j - CLIMB - 2) / STEP < 8) {
+                    weigh(s0, ph1, pl1, (j - CLIMB - 2) / STEP);
                 }
                 __builtin_amdgcn_sched_barrier(0);
             }
@@ -1040,6 +1044,7 @@ __global__ __launch_bounds__(WG, (PromptsShape<HD, F16>::PER_CU)) void paged_pro
             hide(s0, u0 * PU);
 #pragma unroll
             for (int i = 0; i < 8; i++) higher(s0, i);
+            highest();
             turn();  // o is 0
 #pragma unroll
             for (int i = 0; i < 8; i++) weigh(s0, ph0, pl0, i);
