@@ -590,7 +590,7 @@ int oi_kv8_evict_launch(const oi_kv8_dims *src_dims, const void *src, const floa
  * serve all layers: plan once a step, then append and attend in each layer's buffer.
  * Numbers there are not checked on the host: a length past the table's row counts as
  * the row's slots, a page id that the pool does not have as its last page (none in
- * slots), a negative number as 0.
+ * slots), a negative number as 0 except where said.
  * The launches allocate nothing, wait for nothing and may be captured: a replay goes
  * by the numbers that it finds.  `stream` must belong to the current device (OI_E_ARG
  * otherwise).  An output (cache, table, list, maps, rows, workspace) that shares memory
@@ -607,9 +607,9 @@ int64_t oi_paged_bytes(const oi_paged_dims *d);
 /* Room for a step's tokens: sequence i holds n_past[i] slots and gets n_new[i] more
  * (negative: 0), in pages from the end of the list free_pages[0 .. *n_free)
  * (int32 [n_pages]; at first all page ids, *n_free = n_pages), in the sequences' order.
- * A sequence is served unless its tokens do not fit its table row (table_stride
- * entries) or the n_rows rows of the step, or it needs a page and the list does not
- * hold what it and the sequences before it need.  Written: new entries of table
+ * A sequence is served unless n_past is negative, its tokens do not fit its table row
+ * (table_stride entries) or the n_rows rows of the step, or it needs a page and the list
+ * does not hold what it and the sequences before it need.  Written: new entries of table
  * [n_seqs][table_stride]; *n_free; lens [n_seqs], the slots held now, 0 where not
  * served; starts [n_seqs + 1], the packed rows' begins (sums of n_new, at most n_rows);
  * slots [n_rows], each row's slot number, -1 for rows not served or behind the last;

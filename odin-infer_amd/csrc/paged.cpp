@@ -127,7 +127,6 @@ int attention(PagedAttnArgs &a, const char *what, const oi_paged_dims *d, const 
     a.out_stride = out_stride;
     a.scale = scale2;
     a.f16 = type == OI_TYPE_F16;
-    a.n_heads = n_heads;
     a.group = (int)group;
     a.magic = group > 1 ? (uint32_t)((((uint64_t)1 << 32) + group - 1) / group) : 0u;
     a.n_seqs = n_seqs;

@@ -52,7 +52,7 @@ struct PagedAttnArgs {
     void *out;
     int64_t q_stride, out_stride;  // elements from a row (a token's heads) to the next
     float scale;                   // of q . k, times log2(e)
-    int32_t f16, n_heads, group;
+    int32_t f16, group;
     uint32_t magic;                // ceil(2^32 / group), 0 for a group of 1
     int32_t n_seqs, n_q, n_rows;   // n_q: tokens of each sequence (tokens call)
     const int32_t *starts, *lens, *table;  // starts: prompts call

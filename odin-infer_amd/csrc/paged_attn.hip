@@ -371,12 +371,12 @@ __device__ __forceinline__ float inverse(float l) { return l == 0.f ? 0.f : 1.f 
 // are done, V when its product is, pages one unit ahead of both.  The maximum is raised
 // to whole numbers, so rescaling is exact.
 // Workgroups of a CU, as registers allow.
-template <int HD, bool F16, int NT>
+template <int HD>
 struct TokensShape {
     static constexpr int PER_CU = HD == 128 ? 2 : 1;
 };
 template <int HD, bool F16, int NT, bool GROUPS>
-__global__ __launch_bounds__(WG, (TokensShape<HD, F16, NT>::PER_CU)) void paged_tokens_kernel(PagedAttnArgs a) {
+__global__ __launch_bounds__(WG, TokensShape<HD>::PER_CU) void paged_tokens_kernel(PagedAttnArgs a) {
     constexpr int NW = WG / WAVE, NK = HD / 32, ND = HD / 16, PD = HD + 4;
     using W = TokensWork;
     __shared__ __attribute__((aligned(16))) float so[NW][16][PD];
@@ -964,6 +964,7 @@ __global__ __launch_bounds__(WG, (PromptsShape<HD, F16>::PER_CU)) void paged_pro
         auto half = [&](const f16x8 *kt, const f16x8 *vt, int x, const f32x16 &s0, f32x16 &s1, const f16x8 (&ph0)[2],
                         const f16x8 (&pl0)[2], f16x8 (&ph1)[2], f16x8 (&pl1)[2]) {
             constexpr int N = NF + 2 * DT, AHEAD = 4, CLIMB = N / 4, STEP = N / 16;
+            static_assert(CLIMB + 2 + 7 * STEP < N, "all weights are formed");
             f16x8 w[N];
             auto read = [&](int j) {
                 if (j < NF) w[j] = k_piece(kt, x, j);
@@ -1133,7 +1134,7 @@ int paged_tokens_rows(int hd, int rows, bool f16) {
     return 16 * tokens_tiles(hd, rows, f16) << paged_tokens_groups(hd, rows, f16);
 }
 int paged_tokens_workers(int hd) {
-    return CUS * (hd == 128 ? TokensShape<128, true, 1>::PER_CU : TokensShape<256, true, 1>::PER_CU);
+    return CUS * (hd == 128 ? TokensShape<128>::PER_CU : TokensShape<256>::PER_CU);
 }
 int paged_prompts_workers(int hd, bool f16) {
     return CUS * (hd == 128 ? (f16 ? PromptsShape<128, true>::PER_CU : PromptsShape<128, false>::PER_CU)
