@@ -84,7 +84,8 @@ __device__ __forceinline__ int page_ok(const PagedAttnArgs &a, int id) {
 // hold to the unit moves borders by as much, alike for both workers at one).
 // Tokens: tiles alike.
 struct TokensWork {
-    static constexpr int LEAST = 4, PARTS = 256, NEAR = 2;  // a worker's least, a tile's most parts, see border()
+    // a worker's least, a tile's most parts; see border()
+    static constexpr int LEAST = 4, PARTS = 256, NEAR = 2, SHORT = 0;
     // A tile's own cost (its rows of q, the waves' results joined; 48 sequences 62 us with 1, 54
     // with 4, 57 with 8)
     static constexpr float OWN = 4.f;
@@ -111,7 +112,7 @@ struct TokensWork {
 };
 // Prompts: a tile of R rows more sees R / group slots more.
 struct PromptsWork {
-    static constexpr int R = 128, LEAST = 4, PARTS = 128, NEAR = 8;
+    static constexpr int R = 128, LEAST = 4, PARTS = 128, NEAR = 8, SHORT = 6;
     static constexpr float OWN = 4.f;  // nine short prompts 28 us with 1, 18 with 2 to 6
     int len, tokens, tiles;
     float first, step;  // of tile 0, and what each further one costs more
@@ -163,7 +164,9 @@ __device__ __forceinline__ float scan_lanes(float v) {
 // (own) and that of the lanes up to it (run); x at or behind the end of all is that end.  It
 // rises with x, as every step of it does, so workers' stretches cover each unit once, wherever
 // rounding puts the borders.  Within NEAR units of a tile's end (an eighth of a share, if that is
-// less) it moves there.
+// less) it moves there; in a tile of at most SHORT units from up to half a share, since each
+// part costs what a tile costs by itself, and the join (nine prompts of 5 to 301 tokens 26.3 ->
+// 22.3 us, a step of 12 sequences that leaves tiles of 2 to 14 units 19.7 -> 20.9).
 template <class W>
 __device__ PagedAt border(const PagedAttnArgs &a, float x, float share, float own, float run, int per) {
     const int lane = __lane_id();
@@ -197,10 +200,11 @@ __device__ PagedAt border(const PagedAttnArgs &a, float x, float share, float ow
     const float one = w.all();
     int head = min((int)min(x / one, 2e9f), a.c.n_kv - 1), u;
     int tile = w.find(a, min(max(x - (float)head * one, 0.f), one), u);
-    const int near = (int)min(share * 0.125f, (float)W::NEAR);
+    const int units = w.units(a, tile);
+    const int near = (int)min(share * (units <= W::SHORT ? 0.5f : 0.125f), (float)W::NEAR);
     if (u <= near) {
         u = 0;
-    } else if (w.units(a, tile) - u <= near) {
+    } else if (units - u <= near) {
         u = 0;
         if (++tile == w.tiles) {
             tile = 0;
@@ -370,10 +374,15 @@ __device__ __forceinline__ float inverse(float l) { return l == 0.f ? 0.f : 1.f 
 // 16 bytes a lane without LDS; K of the next unit is requested when this one's scores
 // are done, V when its product is, pages one unit ahead of both.  The maximum is raised
 // to whole numbers, so rescaling is exact.
-// Workgroups of a CU, as registers allow.
+// Memory bounds it: 48 sequences of up to 9001 slots of 8 heads of 128 (320 MB) 54.6 us, 5.9
+// TB/s; 3 of up to 120001 of 2 heads of 256 (456 MB) 74.6 us, 6.1; where a large nontemporal read
+// makes 7.0.  A sequence of 1031 slots takes 6.6 us, a chain of misses: numbers, page ids, K, V.  More
+// than 16 rows go to a wave two tiles at a time where registers allow, then to groups of waves that read
+// the same slots (24 drafts of 5 tokens, 53 MB, 20.8 us).  Three workgroups a CU spill
+// registers (131 us against 122 where two hold all); so do four tiles a wave.
 template <int HD>
 struct TokensShape {
-    static constexpr int PER_CU = HD == 128 ? 2 : 1;
+    static constexpr int PER_CU = HD == 128 ? 2 : 1;  // workgroups of a CU
 };
 template <int HD, bool F16, int NT, bool GROUPS>
 __global__ __launch_bounds__(WG, TokensShape<HD>::PER_CU) void paged_tokens_kernel(PagedAttnArgs a) {
@@ -699,7 +708,8 @@ __device__ __forceinline__ void join_rows(const PagedAttnArgs &a, int w, int n, 
 
 // Tokens.  BY_TILE: a workgroup per tile (there are few) looks for the borders in it;
 // otherwise one per border.  ROWS: 1, or those that a workgroup takes at once where their parts
-// are few (3840 workgroups of a row each took 9 us for drafts of 24 sequences, 5 this way).
+// are few (3840 workgroups of a row each took 9 us for drafts of 24 sequences, 6.7 this way).  A chain of
+// three misses: borders, (m, l) with the results, out; 3.8 us for one sequence, 4.7 for 48.
 constexpr int JOIN_FEW = 32;
 template <int HD, bool BY_TILE, int ROWS>
 __global__ __launch_bounds__(WG, 4) void paged_join_kernel(PagedAttnArgs a) {
@@ -759,7 +769,8 @@ __global__ __launch_bounds__(WG, 4) void paged_join_kernel(PagedAttnArgs a) {
     }
 }
 
-// Prompts: a workgroup per border, RT rows a thread.
+// Prompts: a workgroup per border, RT rows a thread: 14703 packed rows, two parts to a tile, 11.3
+// us with four, 16.7 with one; few tiles of many parts 20.7 and 12.1.
 template <int HD, int RT>
 __global__ __launch_bounds__(WG) void paged_join_rows_kernel(PagedAttnArgs a) {
     constexpr int R = PromptsWork::R, ROWS = WG * 4 / HD * RT;
@@ -803,6 +814,15 @@ constexpr int PR = PromptsWork::R;  // rows of a tile
 // 1's weights with V.  A row's maximum is raised only when another is more than 2^LAZY above it
 // (weights then reach 2^15 at most, from 2^PS), and o follows after the products that go by the
 // old one.
+// Packed f16 prompts of 900 to 5003 tokens, 32 heads of 128 over 8 (385 GFLOP): 490 to 515 us, 750
+// to 785 TFLOP/s; four of 8000 tokens 890; f32 rows at head_dim 256, two products for each
+// (110 GFLOP), 279 us.  Matrix and vector units are both busy in 4 of 10 cycles: a wave issues in order, and
+// two waves a SIMD do not fill each other's gaps (16 products alone 225 ns, beside their softmax
+// 433 in a loop of nothing else, 600 here).  Where pages are read once or twice, their misses add a
+// tenth to three (two times 50 tokens behind 40000 slots 118 us, 105 with pages in cache).
+// Measured and left: 64 rows a wave (700 us against 565), eight waves on 256 rows (the same, long ones 5%
+// slower), pieces of LDS read 6 or 8 ahead (the same), lines of the step after next touched ahead of
+// their fetch (10% slower), no pipeline (f16 the same, f32 slower).
 template <int HD, bool F16>
 __global__ __launch_bounds__(WG, (PromptsShape<HD, F16>::PER_CU)) void paged_prompts_kernel(PagedAttnArgs a) {
     constexpr int NW = WG / WAVE, NF = HD / 16, DT = HD / 32;
