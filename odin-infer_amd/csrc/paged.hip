@@ -138,7 +138,7 @@ __global__ __launch_bounds__(PW) void paged_plan_kernel(PagedPlanArgs a) {
 }
 
 // The rows' maps from the sequences' starts, lengths and pages, a row a thread: a bisection's
-// chain of cached loads, 4.3 us for 27000 rows of 300 sequences, with the plan's 3.9; the plan's one
+// chain of cached loads, 4.3 us for 28700 rows of 300 sequences, with the plan's 3.9; the plan's one
 // workgroup takes 29.7 for both.
 __global__ __launch_bounds__(WG) void paged_maps_kernel(PagedPlanArgs a) {
     const int r = blockIdx.x * WG + threadIdx.x;
