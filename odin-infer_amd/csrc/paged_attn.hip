@@ -828,6 +828,7 @@ __global__ __launch_bounds__(WG, (PromptsShape<HD, F16>::PER_CU)) void paged_pro
     constexpr int NW = WG / WAVE, NF = HD / 16, DT = HD / 32;
     constexpr int PIECES = PU * HD / 8;     // of K, and of V, in a step
     constexpr int CH = PIECES / WAVE / NW;  // a wave's stretches of 64 pieces, of each
+    static_assert(CH * WAVE == 2 * HD, "sixteen slots");
     constexpr int RPC = WAVE / (HD / 8);    // K rows of a stretch
     constexpr float PS = F16 ? 3.f : 9.f, LAZY = 15.f - PS;
     using W = PromptsWork;
@@ -843,15 +844,14 @@ __global__ __launch_bounds__(WG, (PromptsShape<HD, F16>::PER_CU)) void paged_pro
     const int c = lane & 31, h = lane >> 5, lp = a.c.lp, P = 1 << lp;
     const float scale = fabsf(a.scale);
     const uint32_t page_bytes = ((uint32_t)a.c.n_kv << lp) * HD * 2;
-    // a lane's place in the sixteens that its stretches come from: stretch i of a wave is number
-    // i NW + wave
+    // A wave brings the sixteen slots of its number, in CH stretches: a lane's place there.
     uint32_t ksrc[CH], vsrc[CH];
 #pragma unroll
     for (int i = 0; i < CH; i++) {
-        const int st = i * NW + wave, r = (st * RPC + lane / (HD / 8)) & 15, j = lane % (HD / 8);
+        const int r = i * RPC + lane / (HD / 8), j = lane % (HD / 8);
         const int s16 = (r & 3) | (r & 4) << 1 | (r & 8) >> 1;
         ksrc[i] = (uint32_t)(s16 * HD + 8 * (j ^ r)) * 2;
-        vsrc[i] = (uint32_t)((st * WAVE + lane) % (2 * HD)) * 16;
+        vsrc[i] = (uint32_t)(i * WAVE + lane) * 16;
     }
 
     each_piece<W>(a, begin, end, [&](const W &w, const PagedAt &at, int units, int u0, int u1) {
@@ -866,36 +866,20 @@ __global__ __launch_bounds__(WG, (PromptsShape<HD, F16>::PER_CU)) void paged_pro
         const ScalarInts table = (ScalarInts)(uintptr_t)(a.table + (int64_t)at.seq * a.stride);
         const char *kb = (const char *)(a.c.k + ((size_t)at.head << lp) * HD),
                    *vb = (const char *)(a.c.v + ((size_t)at.head << lp) * HD);
-        // A step's slots lie in sixteens, each within a page: their pages, and where they begin (K and
-        // V at the same place of their halves of the cache), in bytes.
-        struct Pages {
-            int id[4];
+        // My sixteen slots of a step lie within a page: the page, and where they begin (K and V at the
+        // same place of their halves of the cache), in bytes.
+        auto look_up = [&](int u) { return table[min((u * PU + 16 * wave) >> lp, last_page)]; };
+        auto place = [&](int u, int page) {
+            return (uint64_t)(uint32_t)page_ok(a, page) * page_bytes + (uint32_t)(((u * PU + 16 * wave) & (P - 1)) * HD * 2);
         };
-        struct Places {
-            uint64_t at[4];
-        };
-        auto look_up = [&](int u) {
-            Pages p;
+        auto fetch = [&](const char *from, uint64_t at, const uint32_t (&src)[CH], f16x8 *to) {
+            const char *x = from + at;
+            asm volatile("" : "+s"(x));  // a scalar address, the lane's 32-bit place behind it
 #pragma unroll
-            for (int j = 0; j < 4; j++) p.id[j] = table[min((u * PU + 16 * j) >> lp, last_page)];
-            return p;
-        };
-        auto place = [&](int u, const Pages &p) {
-            Places x;
-#pragma unroll
-            for (int j = 0; j < 4; j++)
-                x.at[j] = (uint64_t)(uint32_t)page_ok(a, p.id[j]) * page_bytes + (uint32_t)(((u * PU + 16 * j) & (P - 1)) * HD * 2);
-            return x;
-        };
-        auto fetch = [&](const char *from, const Places &p, const uint32_t (&src)[CH], f16x8 *to) {
-#pragma unroll
-            for (int i = 0; i < CH; i++) {
-                const char *x = from + p.at[i * NW * WAVE / (2 * HD)];
-                asm volatile("" : "+s"(x));  // a scalar address, the lane's 32-bit place behind it
+            for (int i = 0; i < CH; i++)
                 __builtin_amdgcn_global_load_lds((const __attribute__((address_space(1))) void *)(uintptr_t)(x + src[i]),
-                                                 (__attribute__((address_space(3))) void *)(to + (i * NW + wave) * WAVE), 16, 0,
+                                                 (__attribute__((address_space(3))) void *)(to + (wave * CH + i) * WAVE), 16, 0,
                                                  0);
-            }
         };
         // what this wave asked for has arrived and what it read is in registers; then all waves
         auto meet = [&]() {
@@ -903,9 +887,9 @@ __global__ __launch_bounds__(WG, (PromptsShape<HD, F16>::PER_CU)) void paged_pro
             __builtin_amdgcn_s_barrier();
             asm volatile("" ::: "memory");
         };
-        // ahead of their use: where the next steps of V and of K lie, and the pages of the one after
-        Places vp = place(u0, look_up(u0)), kp = place(u0 + 1, look_up(u0 + 1));
-        Pages ahead = look_up(u0 + 2);
+        // ahead of their use: where the next steps of V and of K lie, and the page of the one after
+        uint64_t vp = place(u0, look_up(u0)), kp = place(u0 + 1, look_up(u0 + 1));
+        int ahead = look_up(u0 + 2);
         auto go_on = [&](int u) {
             vp = kp;
             kp = place(u, ahead);
