@@ -83,7 +83,9 @@ bool tokens_fit(int32_t n_seqs, int32_t n_q) {
 }
 Workspace tokens_workspace(const oi_paged_dims *d, int32_t n_heads, int32_t n_q, bool f16) {
     const int rows = n_q * (n_heads / d->n_kv_heads);
-    return workspace(paged_tokens_workers(d->head_dim), std::min(paged_tokens_rows(d->head_dim, rows, f16), rows), d->head_dim);
+    if (rows > PAGED_TOKENS_ROWS)
+        return workspace(paged_prompts_workers(d->head_dim, f16), std::min(paged_prompts_rows(), rows), d->head_dim);
+    return workspace(paged_tokens_workers(d->head_dim), rows, d->head_dim);
 }
 bool prompts_fit(const oi_paged_dims *d, int32_t n_heads, int32_t n_seqs, int32_t n_rows) {
     const int64_t g = n_heads / d->n_kv_heads;
@@ -93,6 +95,8 @@ Workspace prompts_workspace(const oi_paged_dims *d, int32_t n_heads, int32_t n_r
     return workspace(paged_prompts_workers(d->head_dim, f16),
                      (int)std::min<int64_t>(paged_prompts_rows(), (int64_t)n_rows * (n_heads / d->n_kv_heads)), d->head_dim);
 }
+
+float tile_units(int group) { return (float)paged_prompts_rows() / (64.f * (float)group); }
 
 // What both attention calls have alike.  n_rows: tokens of q and out.
 int attention(PagedAttnArgs &a, const char *what, const oi_paged_dims *d, const void *cache, int32_t n_heads, int32_t type,
@@ -266,9 +270,11 @@ int oi_paged_tokens_launch(const oi_paged_dims *d, const void *cache, int32_t n_
         if (int rc = attention(a, W, d, cache, n_heads, type, q, q_stride, scale, n_seqs, (int64_t)n_seqs * n_q, nullptr, lens,
                                table, table_stride, out, out_stride, workspace, workspace_bytes, w, stream))
             return rc;
-        a.tile_rows = paged_tokens_rows(d->head_dim, n_q * a.group, a.f16);
+        if (n_q * a.group > PAGED_TOKENS_ROWS) {
+            a.tile_units = tile_units(a.group);
+            return launched(launch_paged_prompts(a, (hipStream_t)stream), W);
+        }
         a.groups = paged_tokens_groups(d->head_dim, n_q * a.group, a.f16);
-        a.tiles = (n_q * a.group + a.tile_rows - 1) / a.tile_rows;
         return launched(launch_paged_tokens(a, (hipStream_t)stream), W);
     });
 }
@@ -295,7 +301,7 @@ int oi_paged_prompts_launch(const oi_paged_dims *d, const void *cache, int32_t n
         if (int rc = attention(a, W, d, cache, n_heads, type, q, q_stride, scale, n_seqs, n_rows, starts, lens, table,
                                table_stride, out, out_stride, workspace, workspace_bytes, w, stream))
             return rc;
-        a.tile_units = (float)paged_prompts_rows() / (64.f * (float)a.group);
+        a.tile_units = tile_units(a.group);
         return launched(launch_paged_prompts(a, (hipStream_t)stream), W);
     });
 }

@@ -55,11 +55,10 @@ struct PagedAttnArgs {
     int32_t f16, group;
     uint32_t magic;                // ceil(2^32 / group), 0 for a group of 1
     int32_t n_seqs, n_q, n_rows;   // n_q: tokens of each sequence (tokens call)
-    const int32_t *starts, *lens, *table;  // starts: prompts call
+    const int32_t *starts, *lens, *table;  // starts: prompts call (null: n_q tokens of each)
     int32_t stride, cap;           // entries of a table row, and its slots
-    // tokens call: rows of a tile, a sequence and kv head's tiles, log2 of the groups of waves
-    int32_t tile_rows, tiles, groups;
-    float tile_units;              // prompts call: units of slots that a tile sees more than the one before
+    int32_t groups;                // tokens kernel: log2 of the groups of waves
+    float tile_units;              // prompts kernel: units of slots that a tile sees more than the one before
     // workspace
     int32_t workers, part_rows;    // part_rows: rows of a partial result
     PagedAt *at;                   // [workers + 1], the last: {used workers, 0, 0, 0}
@@ -68,8 +67,11 @@ struct PagedAttnArgs {
 };
 // the workers of a call and the bytes that they take
 int paged_tokens_workers(int hd);
-// rows of an item, given those of a sequence and kv head, and log2 of its groups of waves
-int paged_tokens_rows(int hd, int rows, bool f16);
+// Rows of a sequence and kv head that the tokens kernel takes; more go through the prompts kernel, as if packed
+// (24 sequences of 4000 slots, 32 f16 heads of 128 over 4, 16 tokens: 88 and 57 us; 8 tokens, 64 rows, at 1050
+// slots 26 either way; f32 47 and 37, 31 either way; 16 rows a fifth to a half slower there).
+constexpr int PAGED_TOKENS_ROWS = 64;
+// log2 of the groups of waves, given the rows of a sequence and kv head
 int paged_tokens_groups(int hd, int rows, bool f16);
 int paged_prompts_workers(int hd, bool f16);
 int paged_prompts_rows();  // of a tile

@@ -6,8 +6,8 @@
 //   o = sum p_s V_s,   l = sum p_s,   out = o / l  (0 where a row sees nothing)
 // m, l and o are 32-bit.  The matrix products take f16 operands: K and V are exact
 // there; an f32 q is the sum of two halves (22 bits, scaled by a power of two per
-// row), an f16 q exact.  Weights are the sum of two halves (22 bits) but for f16
-// prompts, whose outputs hold no more than 11 bits: there p is rounded once and l is
+// row), an f16 q exact.  Weights are the sum of two halves (22 bits) but for the prompts
+// kernel's f16 rows, whose outputs hold no more than 11 bits: there p is rounded once and l is
 // the sum of the rounded weights.  2^15 is where the row's largest p sits in f16:
 // another keeps all its bits down to 2^-29 of it and is lost below 2^-40.  Prompts leave
 // room above the maximum instead, so that few rises of it rescale o: from 2^3 in f16,
@@ -68,6 +68,11 @@ __device__ __forceinline__ void ask(const PagedAttnArgs &a) {
 __device__ __forceinline__ int row_token(const PagedAttnArgs &a, int r) {
     return a.magic ? (int)__umulhi((uint32_t)r, a.magic) : r;
 }
+// A sequence's first token in q and out: starts[s], or n_q of each where there are no starts.
+template <bool SCALAR>
+__device__ __forceinline__ int first_token(const PagedAttnArgs &a, int s) {
+    return a.starts ? min(max(number<SCALAR>(a.starts, s), 0), a.n_rows) : s * a.n_q;
+}
 // where row r's head lies in q or out; base: the sequence's first token
 __device__ __forceinline__ int64_t row_at(const PagedAttnArgs &a, int base, int r, int head, int64_t stride) {
     const int t = row_token(a, r);
@@ -82,32 +87,30 @@ __device__ __forceinline__ int page_ok(const PagedAttnArgs &a, int id) {
 
 // The tiles of a sequence and their costs, in units of slots (f32: a sum that f32 does not
 // hold to the unit moves borders by as much, alike for both workers at one).
-// Tokens: tiles alike.
+// Tokens: one tile.
 struct TokensWork {
     // a worker's least, a tile's most parts; see border()
     static constexpr int LEAST = 4, PARTS = 256, NEAR = 2, SHORT = 0;
     // A tile's own cost (its rows of q, the waves' results joined; 48 sequences 62 us with 1, 54
     // with 4, 57 with 8)
     static constexpr float OWN = 4.f;
-    int len, tokens, tiles;
-    float first;
+    static constexpr int tiles = 1;
+    int len;
+    float cost;
     template <bool SCALAR>
     __device__ static __forceinline__ TokensWork of(const PagedAttnArgs &a, int s) {
         TokensWork w;
         w.len = seq_len<SCALAR>(a, s);
-        w.tokens = a.n_q;
-        w.tiles = a.tiles;
-        w.first = (float)((w.len + TU - 1) / TU) + OWN;
+        w.cost = (float)((w.len + TU - 1) / TU) + OWN;
         return w;
     }
-    __device__ __forceinline__ float all() const { return (float)tiles * first; }
-    __device__ __forceinline__ float most() const { return first; }
+    __device__ __forceinline__ float all() const { return cost; }
+    __device__ __forceinline__ float most() const { return cost; }
     __device__ __forceinline__ int units(const PagedAttnArgs &, int) const { return (len + TU - 1) / TU; }
     // the tile that x falls into, and the unit there
     __device__ __forceinline__ int find(const PagedAttnArgs &a, float x, int &u) const {
-        const int t = min((int)(x / first), tiles - 1);
-        u = min((int)max(x - (float)t * first - OWN, 0.f), units(a, 0));
-        return t;
+        u = min((int)max(x - OWN, 0.f), units(a, 0));
+        return 0;
     }
 };
 // Prompts: a tile of R rows more sees R / group slots more.
@@ -119,8 +122,7 @@ struct PromptsWork {
     template <bool SCALAR>
     __device__ static __forceinline__ PromptsWork of(const PagedAttnArgs &a, int s) {
         PromptsWork w;
-        const int r0 = min(max(number<SCALAR>(a.starts, s), 0), a.n_rows);
-        const int r1 = min(max(number<SCALAR>(a.starts, s + 1), r0), a.n_rows);
+        const int r0 = first_token<SCALAR>(a, s), r1 = max(first_token<SCALAR>(a, s + 1), r0);
         w.len = seq_len<SCALAR>(a, s);
         w.tokens = r1 - r0;
         w.tiles = (int)(((uint32_t)w.tokens * (uint32_t)a.group + R - 1) / R);  // rows stay below 2^32
@@ -378,8 +380,8 @@ __device__ __forceinline__ float inverse(float l) { return l == 0.f ? 0.f : 1.f 
 // TB/s; 3 of up to 120001 of 2 heads of 256 (456 MB) 74.6 us, 6.1; where a large nontemporal read
 // makes 7.0.  A sequence of 1031 slots takes 6.6 us, a chain of misses: numbers, page ids, K, V.  More
 // than 16 rows go to a wave two tiles at a time where registers allow, then to groups of waves that read
-// the same slots (24 drafts of 5 tokens, 53 MB, 20.8 us).  Three workgroups a CU spill
-// registers (131 us against 122 where two hold all); so do four tiles a wave.
+// the same slots (24 drafts of 5 tokens, 53 MB, 20.4 us); more than 64 to the prompts' kernel.  Three
+// workgroups a CU spill registers (131 us against 122 where two hold all); so do four tiles a wave.
 template <int HD>
 struct TokensShape {
     static constexpr int PER_CU = HD == 128 ? 2 : 1;  // workgroups of a CU
@@ -408,7 +410,7 @@ __global__ __launch_bounds__(WG, TokensShape<HD>::PER_CU) void paged_tokens_kern
     const int group = wave & (ng - 1), turn = wave >> lg, step = NW >> lg;
 
     each_piece<W>(a, begin, end, [&](const W &w, const PagedAt &at, int units, int u0, int u1) {
-        const int row0 = at.tile * a.tile_rows + 16 * NT * group;
+        const int row0 = 16 * NT * group;
         const int len = w.len, seen0 = len - a.n_q + 1;  // slots that the first token sees
         const int first_limit = seen0 + row_token(a, min(row0, rows - 1));
         const int32_t *table = a.table + (int64_t)at.seq * a.stride;
@@ -546,7 +548,7 @@ __global__ __launch_bounds__(WG, TokensShape<HD>::PER_CU) void paged_tokens_kern
         const bool whole = u0 == 0 && u1 == units;
 #pragma unroll
         for (int n = 0; n < NT; n++) {
-            if (n > 0 && at.tile * a.tile_rows + 16 * n >= rows) break;
+            if (n > 0 && 16 * n >= rows) break;
             const float ls = col_reduce(l[n], Add());
 #pragma unroll
             for (int d = 0; d < ND; d++) *(f32x4 *)&so[wave][c][16 * d + 4 * g] = o[n][d];
@@ -557,8 +559,8 @@ __global__ __launch_bounds__(WG, TokensShape<HD>::PER_CU) void paged_tokens_kern
             __syncthreads();
             // a group's rows over its `step` waves, 4 step threads a row
             const int tpr = 16 >> lg, tr = tid & ((WG >> lg) - 1), r = tr >> (4 - lg), sg = tid >> (8 - lg);
-            const int row = 16 * (NT * sg + n) + r, gr = at.tile * a.tile_rows + row;
-            if (gr < rows) {
+            const int row = 16 * (NT * sg + n) + r;
+            if (row < rows) {
                 float M = NEG, wt[NW], L = 0.f;
 #pragma unroll
                 for (int k = 0; k < NW; k++)
@@ -571,7 +573,7 @@ __global__ __launch_bounds__(WG, TokensShape<HD>::PER_CU) void paged_tokens_kern
                     }
                 const size_t slot = ((size_t)worker * 2 + (u0 == 0)) * a.part_rows + row;
                 const float inv = whole ? inverse(L) : 1.f;
-                const int64_t to = row_at(a, at.seq * a.n_q, gr, at.head, a.out_stride);
+                const int64_t to = row_at(a, at.seq * a.n_q, row, at.head, a.out_stride);
                 for (int d = 4 * (tr & (tpr - 1)); d < HD; d += 4 * tpr) {
                     f32x4 y = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll
@@ -722,15 +724,15 @@ __global__ __launch_bounds__(WG, 4) void paged_join_kernel(PagedAttnArgs a) {
     PagedAt at;
     int w0 = blockIdx.x;  // the border looked at first is w0 + 1
     if constexpr (BY_TILE) {
-        const int head = (int)((uint32_t)blockIdx.x / (uint32_t)a.tiles), seq = (int)((uint32_t)head / (uint32_t)a.c.n_kv);
-        at = {seq, head - seq * a.c.n_kv, (int)blockIdx.x - head * a.tiles, 0};
+        const int seq = (int)((uint32_t)blockIdx.x / (uint32_t)a.c.n_kv);
+        at = {seq, (int)blockIdx.x - seq * a.c.n_kv, 0, 0};
         w0 = 0;
     } else {
         at = a.at[w0 + 1];
         const PagedAt prev = a.at[w0];
         if (w0 + 1 >= used || !first_cut(at, prev)) return;
     }
-    const int rows = min(a.n_q * a.group - at.tile * a.tile_rows, a.tile_rows);
+    const int rows = a.n_q * a.group;
     if (r0 >= rows) return;
     // borders inside the tile are neighbours
     int n = 0, first = INT32_MAX;
@@ -756,7 +758,7 @@ __global__ __launch_bounds__(WG, 4) void paged_join_kernel(PagedAttnArgs a) {
     if (n == 0) return;
     n++;
     const int w = first - 1;
-    auto to = [&](int r) { return row_at(a, at.seq * a.n_q, at.tile * a.tile_rows + r, at.head, a.out_stride); };
+    auto to = [&](int r) { return row_at(a, at.seq * a.n_q, r, at.head, a.out_stride); };
     if constexpr (ROWS == 1) {
         join_row<HD>(a, w, n, r0, to(r0), lds);
     } else if (n <= JOIN_FEW) {
@@ -788,7 +790,7 @@ __global__ __launch_bounds__(WG) void paged_join_rows_kernel(PagedAttnArgs a) {
         const PagedAt x = k + lane < used ? a.at[k + lane] : PagedAt{-1, 0, 0, 0};
         n += __popcll(__ballot(same_tile(x, at) && x.u > 0));
     }
-    const int base = min(max(a.starts[at.seq], 0), a.n_rows);
+    const int base = first_token<true>(a, at.seq);
     join_rows<HD, RT>(a, w, n, r0, rows,
                            [&](int r) { return row_at(a, base, at.tile * R + r, at.head, a.out_stride); });
 }
@@ -857,7 +859,7 @@ __global__ __launch_bounds__(WG, (PromptsShape<HD, F16>::PER_CU)) void paged_pro
 
     each_piece<W>(a, begin, end, [&](const W &w, const PagedAt &at, int units, int u0, int u1) {
         const int rows = w.tokens * a.group, past = w.len - w.tokens;
-        const int base = min(max(a.starts[at.seq], 0), a.n_rows);
+        const int base = first_token<true>(a, at.seq);
         const int row0 = at.tile * PR + wave * 32, r = row0 + c, rr = min(r, rows - 1);  // my rows
         const int s_end = u1 * PU;
         const int mine = row0 < rows ? past + row_token(a, min(row0 + 32, rows) - 1) + 1 : 0;  // slots my rows see
@@ -1120,24 +1122,24 @@ void join_tokens(const PagedAttnArgs &a, int n, hipStream_t st) {
 }
 template <int HD, bool F16, int NT>
 void tokens(const PagedAttnArgs &a, hipStream_t st) {
-    if (a.groups) hipLaunchKernelGGL((paged_tokens_kernel<HD, F16, NT, true>), dim3((unsigned)a.workers), dim3(WG), 0, st, a);
-    else hipLaunchKernelGGL((paged_tokens_kernel<HD, F16, NT, false>), dim3((unsigned)a.workers), dim3(WG), 0, st, a);
-    const int64_t items = (int64_t)a.n_seqs * a.c.n_kv * a.tiles;
+    constexpr bool MORE = !(HD == 128 && F16 && NT == 1);  // than 16 NT rows, as tokens_tiles has it
+    if (MORE && a.groups)
+        hipLaunchKernelGGL((paged_tokens_kernel<HD, F16, NT, MORE>), dim3((unsigned)a.workers), dim3(WG), 0, st, a);
+    else
+        hipLaunchKernelGGL((paged_tokens_kernel<HD, F16, NT, false>), dim3((unsigned)a.workers), dim3(WG), 0, st, a);
+    const int64_t items = (int64_t)a.n_seqs * a.c.n_kv;
     if (items < a.workers) join_tokens<HD, true>(a, (int)items, st);
     else join_tokens<HD, false>(a, a.workers - 1, st);
 }
 
 }  // namespace
 
-// 16-row tiles of a wave (two where registers allow) and, as a power of two, its workgroup's
-// groups of waves, which read the same slots for other rows
+// 16 rows of a wave (twice where registers allow) and, as a power of two, its workgroup's groups of
+// waves, which read the same slots for other rows
 static int tokens_tiles(int hd, int rows, bool f16) { return hd == 128 && f16 && rows > 16 ? 2 : 1; }
 int paged_tokens_groups(int hd, int rows, bool f16) {
     const int r = 16 * tokens_tiles(hd, rows, f16);
     return rows <= r ? 0 : rows <= 2 * r ? 1 : 2;
-}
-int paged_tokens_rows(int hd, int rows, bool f16) {
-    return 16 * tokens_tiles(hd, rows, f16) << paged_tokens_groups(hd, rows, f16);
 }
 int paged_tokens_workers(int hd) {
     return CUS * (hd == 128 ? TokensShape<128>::PER_CU : TokensShape<256>::PER_CU);

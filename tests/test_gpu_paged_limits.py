@@ -74,7 +74,7 @@ def test_many_heads(case, which, t):
     starts = [n_q * i for i in range(len(ends) + 1)]
     q = queries(b.rng, starts[-1], n_kv * g, 128, t)
     got = b.tokens(n_kv * g, t, n_q, q) if which == "tokens" else b.prompts(n_kv * g, t, starts, starts[-1], q)
-    b.check(got, q, starts, t, which == "prompts", 128 ** -0.5)
+    b.check(got, q, starts, t, which == "prompts" or n_q * g > 64, 128 ** -0.5)
 
 
 @pytest.mark.parametrize("t", [F32, F16])
