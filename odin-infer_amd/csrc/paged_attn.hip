@@ -41,6 +41,12 @@ typedef _Float16 f16x2 __attribute__((ext_vector_type(2)));
 typedef const __attribute__((address_space(4))) int32_t *ScalarInts;  // read through the scalar cache
 
 constexpr float NEG = -3.402823466e38f;  // the running maximum before any slot
+// A score's exponent is one multiply-add, its product with the row's factor not rounded, while a maximum is a
+// rounded product: in a row whose largest score is FAR or more in base 2 (below it they differ by 2^-3 at most)
+// they may lie powers of two apart, its weights all past f16 or all below it.  An f32 row's factor is a power of
+// two, its products exact; an f16 row weighs such scores by their distance from the largest.
+constexpr float FAR = 4194304.f;
+__device__ __forceinline__ bool is_far(float top) { return fabsf(top) >= FAR && fabsf(top) <= FLT_MAX; }
 constexpr int TU = 32;                   // slots of a unit of the tokens kernel
 constexpr int PU = 64;                   // of the prompts kernel
 
@@ -307,17 +313,17 @@ struct Add {
 };
 
 // Rows of q as the second operand of a product: the lane's NF pieces of 8 dimensions
-// of its row, PART apart.  An f32 row is two halves of q 2^-e, e the row's exponent,
-// over the lanes that hold it (reduce).  A negative scale turns q's sign, so that the
-// largest score is that of the largest product.
+// of its row, PART apart.  An f32 row is two halves of q f 2^-e, e the row's exponent,
+// over the lanes that hold it (reduce), f the scale's fraction (1/2 to 1): what is left for the scores is a
+// power of two.  A negative scale turns q's sign, so that the largest score is that of the largest product.
 template <int NF, int PART, bool F16>
 struct QPieces {
     f16x8 hi[NF], lo[F16 ? 1 : NF];
     int e = 0;
     template <class R>
-    __device__ __forceinline__ void load(const void *q, int64_t at, bool ok, bool neg, R reduce) {
+    __device__ __forceinline__ void load(const void *q, int64_t at, bool ok, float scale, R reduce) {
         if constexpr (F16) {
-            const uint32_t sign = neg ? 0x80008000u : 0u;
+            const uint32_t sign = scale < 0.f ? 0x80008000u : 0u;
 #pragma unroll
             for (int f = 0; f < NF; f++) {
                 u32x4 w = *(const u32x4 *)((const uint16_t *)q + at + PART * f);
@@ -336,8 +342,8 @@ struct QPieces {
             }
             amax = reduce(amax);
             e = ok && amax > 0.f ? (int)(__float_as_uint(amax) >> 23) - 127 - 14 : 0;
-            // 2^-e as two factors that f32 holds, the sign in one; 0 for no row
-            const float s0 = ok ? ldexpf(neg ? -1.f : 1.f, -e / 2) : 0.f, s1 = ldexpf(1.f, -e - -e / 2);
+            // f 2^-e as two factors that f32 holds; 0 for no row
+            const float s0 = ok ? ldexpf(__builtin_amdgcn_frexp_mantf(scale), -e / 2) : 0.f, s1 = ldexpf(1.f, -e - -e / 2);
 #pragma unroll
             for (int f = 0; f < NF; f++) {  // read again: the row is in cache, its registers are not free
                 const f32x4 u = *(const f32x4 *)(p + PART * f), w = *(const f32x4 *)(p + PART * f + 4);
@@ -351,6 +357,10 @@ struct QPieces {
                 }
             }
         }
+    }
+    // what its products are to be multiplied by, above 0: -inf stays -inf
+    __device__ __forceinline__ float factor(float scale) const {
+        return fmaxf(F16 ? fabsf(scale) : ldexpf(1.f, __builtin_amdgcn_frexp_expf(scale) + e), FLT_MIN);
     }
 };
 
@@ -401,8 +411,6 @@ __global__ __launch_bounds__(WG, TokensShape<HD>::PER_CU) void paged_tokens_kern
     if (worker >= used) return;
     leave_border(a, worker, begin, end);
     const int c = lane & 15, g = lane >> 4, lp = a.c.lp, P = 1 << lp;
-    const bool neg = a.scale < 0.f;
-    const float scale = fabsf(a.scale);
     const int kslot = 8 * (c >> 2) + (c & 3);  // of a product's first 16 slots; 4 more in its second
     const size_t page_elems = ((size_t)a.c.n_kv << lp) * HD;
     const int rows = a.n_q * a.group;
@@ -454,9 +462,9 @@ __global__ __launch_bounds__(WG, TokensShape<HD>::PER_CU) void paged_tokens_kern
         for (int n = 0; n < NT; n++) {
             const int row = row0 + 16 * n + c, rr = min(row, rows - 1);
             limit[n] = seen0 + row_token(a, rr);
-            q[n].load(a.q, row_at(a, at.seq * a.n_q, rr, at.head, a.q_stride) + 8 * g, row < rows, neg,
+            q[n].load(a.q, row_at(a, at.seq * a.n_q, rr, at.head, a.q_stride) + 8 * g, row < rows, a.scale,
                       [](float x) { return col_reduce(x, Max()); });
-            mul[n] = fmaxf(ldexpf(scale, q[n].e), FLT_MIN);  // above 0: -inf stays -inf
+            mul[n] = q[n].factor(a.scale);
             m[n] = NEG;
             l[n] = 0.f;
 #pragma unroll
@@ -501,14 +509,24 @@ __global__ __launch_bounds__(WG, TokensShape<HD>::PER_CU) void paged_tokens_kern
                 for (int t = 0; t < 2; t++)
 #pragma unroll
                     for (int i = 0; i < 4; i++) top = fmaxf(top, s[n][t][i]);
-                top = col_reduce(top * mul[n], Max());
+                const float most = col_reduce(top, Max());
+                top = most * mul[n];
                 const float m1 = fmaxf(m[n], ceilf(top));
+                float bias = -m1;
+                if (F16 && __builtin_expect(__any(is_far(top)), 0)) {
+                    const float from = is_far(top) ? most : 0.f;
+                    if (is_far(top)) bias = top - m1;
+#pragma unroll
+                    for (int t = 0; t < 2; t++)
+#pragma unroll
+                        for (int i = 0; i < 4; i++) s[n][t][i] -= from;
+                }
                 float sum = 0.f;
 #pragma unroll
                 for (int t = 0; t < 2; t++)
 #pragma unroll
                     for (int i = 0; i < 4; i++) {
-                        const float p = ex2(fmaf(s[n][t][i], mul[n], -m1)) * 32768.f;
+                        const float p = ex2(fmaf(s[n][t][i], mul[n], bias)) * 32768.f;
                         sum += p;
                         const _Float16 h = (_Float16)p;
                         ph[n][4 * t + i] = h;
@@ -845,7 +863,6 @@ __global__ __launch_bounds__(WG, (PromptsShape<HD, F16>::PER_CU)) void paged_pro
     if (worker >= used) return;
     leave_border(a, worker, begin, end);
     const int c = lane & 31, h = lane >> 5, lp = a.c.lp, P = 1 << lp;
-    const float scale = fabsf(a.scale);
     const uint32_t page_bytes = ((uint32_t)a.c.n_kv << lp) * HD * 2;
     // A wave brings the sixteen slots of its number, in CH stretches: a lane's place there.
     uint32_t ksrc[CH], vsrc[CH];
@@ -901,9 +918,9 @@ __global__ __launch_bounds__(WG, (PromptsShape<HD, F16>::PER_CU)) void paged_pro
         };
         if (u0 < u1) fetch(kb, vp, ksrc, kl[u0 & 1]);
         QPieces<NF, 16, F16> q;
-        q.load(a.q, row_at(a, base, rr, at.head, a.q_stride) + 8 * h, r < rows, a.scale < 0.f,
+        q.load(a.q, row_at(a, base, rr, at.head, a.q_stride) + 8 * h, r < rows, a.scale,
                [](float x) { return half_reduce(x, Max()); });
-        const float mul = fmaxf(ldexpf(scale, q.e), FLT_MIN);
+        const float mul = q.factor(a.scale);
         float m = NEG, l = 0.f;
         f32x16 o[DT];
 #pragma unroll
@@ -913,21 +930,37 @@ __global__ __launch_bounds__(WG, (PromptsShape<HD, F16>::PER_CU)) void paged_pro
         // The softmax of a half in steps: the maximum of score pairs, the rows' new maxima, weights of a
         // pair.  Rows rise together, so that one that climbs takes the others along and few halves
         // rise at all; alpha: what o is to be multiplied by then.
-        float top = 0.f, alpha = 1.f, bias = 0.f, sum = 0.f;  // sum: of the half's weights
+        // high: what a score is to pass for that; most: the row's largest score before its factor.
+        float top = 0.f, most = 0.f, alpha = 1.f, bias = 0.f, high = NEG, sum = 0.f;  // sum: of the half's weights
         bool rise = false;
         auto higher = [&](const f32x16 &s, int i) {
             top = i == 0 ? fmaxf(s[0], s[1]) : fmaxf(fmaxf(top, s[2 * i]), s[2 * i + 1]);
         };
-        auto highest = [&]() { top = half_reduce(top * mul, Max()); };
-        auto turn = [&]() {
-            rise = __any(top > m + LAZY);
-            // a branch where registers allow (the f32 form at head_dim 256 takes 310 us with it, 278 without)
-            if (PromptsShape<HD, F16>::PER_CU == 2 && __builtin_expect(!rise, 1)) return;
+        auto highest = [&]() {
+            most = half_reduce(top, Max());
+            top = most * mul;
+        };
+        auto turn = [&](f32x16 &s) {
+            rise = __any(top > high);
+            // a branch where registers allow (f32 rows at head_dim 256 take 310 us with it, 278 without; at 128 426
+            // and 429, f16 rows at 256 545 and 550)
+            if ((HD == 128 || F16) && __builtin_expect(!rise, 1)) return;
             const float m1 = rise ? fmaxf(m, ceilf(top)) : m;
             alpha = ex2(m - m1);
             m = m1;
-            bias = PS - m1;
             l *= alpha;
+            // a far maximum has no room for PS or LAZY beside it
+            const bool near = fabsf(m1) < FAR;
+            bias = (near ? PS : 0.f) - m1;
+            high = near ? m1 + LAZY : F16 ? NEG : m1;
+            if (F16 && __builtin_expect(rise, 0)) {
+                if (__any(is_far(top))) {  // every half of such a row comes by here
+                    const float from = is_far(top) ? most : 0.f;
+                    if (is_far(top)) bias = top - m1;
+#pragma unroll
+                    for (int i = 0; i < 16; i++) s[i] -= from;
+                }
+            }
         };
         auto weigh = [&](const f32x16 &s, f16x8 (&ph)[2], f16x8 (&pl)[2], int i) {
             f16x2 hi, lo;
@@ -969,7 +1002,7 @@ __global__ __launch_bounds__(WG, (PromptsShape<HD, F16>::PER_CU)) void paged_pro
         // buffer, the products of the former weights p0 with half x of the V buffer.  Pieces of K, then of
         // V come from LDS AHEAD of their use, and the vector units' work lies between their products in
         // the order written here.
-        auto half = [&](const f16x8 *kt, const f16x8 *vt, int x, const f32x16 &s0, f32x16 &s1, const f16x8 (&ph0)[2],
+        auto half = [&](const f16x8 *kt, const f16x8 *vt, int x, f32x16 &s0, f32x16 &s1, const f16x8 (&ph0)[2],
                         const f16x8 (&pl0)[2], f16x8 (&ph1)[2], f16x8 (&pl1)[2]) {
             constexpr int N = NF + 2 * DT, AHEAD = 4, CLIMB = N / 4, STEP = N / 16;
             static_assert(CLIMB + 2 + 7 * STEP < N, "all weights are formed");
@@ -996,7 +1029,7 @@ __global__ __launch_bounds__(WG, (PromptsShape<HD, F16>::PER_CU)) void paged_pro
                 } else if (j == CLIMB) {
                     highest();
                 } else if (j == CLIMB + 1) {
-                    turn();
+                    turn(s0);
                 } else if ((j - CLIMB - 2) % STEP == 0 && (j - CLIMB - 2) / STEP < 8) {
                     weigh(s0, ph1, pl1, (j - CLIMB - 2) / STEP);
                 }
@@ -1054,7 +1087,7 @@ __global__ __launch_bounds__(WG, (PromptsShape<HD, F16>::PER_CU)) void paged_pro
 #pragma unroll
             for (int i = 0; i < 8; i++) higher(s0, i);
             highest();
-            turn();  // o is 0
+            turn(s0);  // o is 0
 #pragma unroll
             for (int i = 0; i < 8; i++) weigh(s0, ph0, pl0, i);
 #pragma unroll
