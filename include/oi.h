@@ -648,8 +648,7 @@ int64_t oi_paged_prompts_workspace_bytes(const oi_paged_dims *d, int32_t n_heads
  * [n_seqs * n_q][n_heads][head_dim], q_stride and out_stride elements from a token to the
  * next, both of `type` (F32 or F16), 16-byte aligned, strides multiples of 16 bytes.
  * Query head h reads kv head h / (n_heads / n_kv_heads).  out = softmax(scale * q K) V
- * with 32-bit sums in a fixed order and weights of 22 bits (11 in F16 calls of more than 64
- * rows n_q * n_heads / n_kv_heads); scale * log2(e) must be finite in f32 (OI_E_ARG).  Cached values below the lengths must be finite (as the append
+ * with 32-bit sums in a fixed order and weights of 22 bits; scale * log2(e) must be finite in f32 (OI_E_ARG).  Cached values below the lengths must be finite (as the append
  * leaves them).  `out` may be `q` where the strides are the same. */
 int oi_paged_tokens_launch(const oi_paged_dims *d, const void *cache, int32_t n_heads, int32_t type, const void *q,
                            int64_t q_stride, float scale, int32_t n_seqs, int32_t n_q, const int32_t *lens,

@@ -68,8 +68,8 @@ struct PagedAttnArgs {
 // the workers of a call and the bytes that they take
 int paged_tokens_workers(int hd);
 // Rows of a sequence and kv head that the tokens kernel takes; more go through the prompts kernel, as if packed
-// (24 sequences of 4000 slots, 32 f16 heads of 128 over 4, 16 tokens: 88 and 57 us; 8 tokens, 64 rows, at 1050
-// slots 26 either way; f32 47 and 37, 31 either way; 16 rows a fifth to a half slower there).
+// (whole calls, 24 sequences of 32 f16 heads of 128 over 4: 16 tokens, 128 rows, at 4000 slots 90 and 77 us, at 1050
+// 38 and 37.5; 8 tokens, 64 rows, 62 and 61.5, 26 and 30; f32 77 and 85, 31 and 36).
 constexpr int PAGED_TOKENS_ROWS = 64;
 // log2 of the groups of waves, given the rows of a sequence and kv head
 int paged_tokens_groups(int hd, int rows, bool f16);

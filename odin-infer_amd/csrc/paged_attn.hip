@@ -6,9 +6,10 @@
 //   o = sum p_s V_s,   l = sum p_s,   out = o / l  (0 where a row sees nothing)
 // m, l and o are 32-bit.  The matrix products take f16 operands: K and V are exact
 // there; an f32 q is the sum of two halves (22 bits, scaled by a power of two per
-// row), an f16 q exact.  Weights are the sum of two halves (22 bits) but for the prompts
-// kernel's f16 rows, whose outputs hold no more than 11 bits: there p is rounded once and l is
-// the sum of the rounded weights.  2^15 is where the row's largest p sits in f16:
+// row), an f16 q exact.  Weights are the sum of two halves (22 bits) but for packed f16
+// prompts, whose outputs hold no more than 11 bits: there p is rounded once and l is
+// the sum of the rounded weights (with two halves 385 GFLOP of such prompts take 631 us, not 489, and are off by
+// 2.0e-4 of their size, not 2.2e-4; a caller with use for them makes an F32 call).  2^15 is where the row's largest p sits in f16:
 // another keeps all its bits down to 2^-29 of it and is lost below 2^-40.  Prompts leave
 // room above the maximum instead, so that few rises of it rescale o: from 2^3 in f16,
 // where a weight below 2^-28 is lost (2^17 of the largest such make one rounding of the
@@ -844,14 +845,15 @@ constexpr int PR = PromptsWork::R;  // rows of a tile
 // slower), pieces of LDS read 6 or 8 ahead (the same), lines of the step after next touched ahead of
 // their fetch (10% slower), a half's first pieces read before the fetches are issued (f16 at head_dim
 // 256 5% slower), waves' priorities (the same), no pipeline (f16 the same, f32 slower).
-template <int HD, bool F16>
+// TWO: weights as two halves (all but packed f16 prompts).
+template <int HD, bool F16, bool TWO>
 __global__ __launch_bounds__(WG, (PromptsShape<HD, F16>::PER_CU)) void paged_prompts_kernel(PagedAttnArgs a) {
     constexpr int NW = WG / WAVE, NF = HD / 16, DT = HD / 32;
     constexpr int PIECES = PU * HD / 8;     // of K, and of V, in a step
     constexpr int CH = PIECES / WAVE / NW;  // a wave's stretches of 64 pieces, of each
     static_assert(CH * WAVE == 2 * HD, "sixteen slots");
     constexpr int RPC = WAVE / (HD / 8);    // K rows of a stretch
-    constexpr float PS = F16 ? 3.f : 9.f, LAZY = 15.f - PS;
+    constexpr float PS = TWO ? 9.f : 3.f, LAZY = 15.f - PS;
     using W = PromptsWork;
     __shared__ __attribute__((aligned(16))) f16x8 kl[2][PIECES], vl[2][PIECES];
     ask(a);
@@ -968,19 +970,19 @@ __global__ __launch_bounds__(WG, (PromptsShape<HD, F16>::PER_CU)) void paged_pro
             for (int k = 0; k < 2; k++) {
                 const float p = ex2(fmaf(s[2 * i + k], mul, bias));
                 hi[k] = (_Float16)p;
-                if constexpr (!F16) {
+                if constexpr (TWO) {
                     sum = i + k == 0 ? p : sum + p;
                     lo[k] = (_Float16)(p - (float)hi[k]);
                 }
             }
-            if constexpr (F16) sum = __builtin_amdgcn_fdot2(hi, f16x2{(_Float16)1.f, (_Float16)1.f}, i == 0 ? 0.f : sum, false);
+            if constexpr (!TWO) sum = __builtin_amdgcn_fdot2(hi, f16x2{(_Float16)1.f, (_Float16)1.f}, i == 0 ? 0.f : sum, false);
             if (i == 7) l += sum;
             asm volatile("" : "+v"(hi), "+v"(sum));  // here, not where it is used
-            if constexpr (!F16) asm volatile("" : "+v"(lo));
+            if constexpr (TWO) asm volatile("" : "+v"(lo));
 #pragma unroll
             for (int k = 0; k < 2; k++) {
                 ph[i / 4][2 * (i % 4) + k] = hi[k];
-                if constexpr (!F16) pl[i / 4][2 * (i % 4) + k] = lo[k];
+                if constexpr (TWO) pl[i / 4][2 * (i % 4) + k] = lo[k];
             }
         };
         auto k_piece = [&](const f16x8 *kt, int x, int f) { return kt[(32 * x + c) * (HD / 8) + ((2 * f + h) ^ (c & 15))]; };
@@ -1021,7 +1023,7 @@ __global__ __launch_bounds__(WG, (PromptsShape<HD, F16>::PER_CU)) void paged_pro
                 } else {
                     const int i = (j - NF) / DT, d = (j - NF) % DT;
                     o[d] = mfma32(w[j], ph0[i], o[d]);
-                    if constexpr (!F16) o[d] = mfma32(w[j], pl0[i], o[d]);
+                    if constexpr (TWO) o[d] = mfma32(w[j], pl0[i], o[d]);
                 }
                 if (j < CLIMB) {
 #pragma unroll
@@ -1133,7 +1135,10 @@ unsigned groups_of(int n, int size) { return (unsigned)((n + size - 1) / size); 
 
 template <int HD, bool F16>
 void prompts(const PagedAttnArgs &a, hipStream_t st) {
-    hipLaunchKernelGGL((paged_prompts_kernel<HD, F16>), dim3((unsigned)a.workers), dim3(WG), 0, st, a);
+    if (F16 && a.starts)  // packed; a tokens call has none
+        hipLaunchKernelGGL((paged_prompts_kernel<HD, F16, !F16>), dim3((unsigned)a.workers), dim3(WG), 0, st, a);
+    else
+        hipLaunchKernelGGL((paged_prompts_kernel<HD, F16, true>), dim3((unsigned)a.workers), dim3(WG), 0, st, a);
     // about as many tiles as workers: two parts each, four rows a thread; few tiles: many parts
     constexpr int RT = 4, ROWS = WG * 4 / HD;
     const int64_t tiles = ((int64_t)a.n_rows * a.group / PR + a.n_seqs) * a.c.n_kv;
