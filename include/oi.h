@@ -648,7 +648,10 @@ int64_t oi_paged_prompts_workspace_bytes(const oi_paged_dims *d, int32_t n_heads
  * [n_seqs * n_q][n_heads][head_dim], q_stride and out_stride elements from a token to the
  * next, both of `type` (F32 or F16), 16-byte aligned, strides multiples of 16 bytes.
  * Query head h reads kv head h / (n_heads / n_kv_heads).  out = softmax(scale * q K) V
- * with 32-bit sums in a fixed order and weights of 22 bits; scale * log2(e) must be finite in f32 (OI_E_ARG).  Cached values below the lengths must be finite (as the append
+ * with 32-bit sums in a fixed order.  A weight is off by at most 2^-22 of itself or 2^-39 of
+ * the row's largest, whichever is more (calls of more than 64 rows n_q * n_heads /
+ * n_kv_heads: 2^-36, F16 2^-33): a smaller one may be lost.  scale * log2(e) must be
+ * finite in f32 (OI_E_ARG).  Cached values below the lengths must be finite (as the append
  * leaves them).  `out` may be `q` where the strides are the same. */
 int oi_paged_tokens_launch(const oi_paged_dims *d, const void *cache, int32_t n_heads, int32_t type, const void *q,
                            int64_t q_stride, float scale, int32_t n_seqs, int32_t n_q, const int32_t *lens,
@@ -658,8 +661,9 @@ int oi_paged_tokens_launch(const oi_paged_dims *d, const void *cache, int32_t n_
 /* The same for packed rows: sequence i's tokens are the rows starts[i] .. starts[i+1]-1
  * of n_rows (starts [n_seqs + 1], rising; numbers outside 0 .. n_rows count as the nearer
  * end), its newest; rows of no sequence stay as they are.  For whole prompts, chunks
- * behind cached slots, and drafts of differing lengths.  Weights have 22 bits, in F16
- * calls 11.  n_rows at most 2^24 and n_rows * (n_heads / n_kv_heads)^2 below 2^32. */
+ * behind cached slots, and drafts of differing lengths.  A weight is off by at most 2^-22 of
+ * itself or 2^-36 of the row's largest; in F16 calls, whose outputs hold 11 bits, 2^-11 of
+ * itself or 2^-30.  n_rows at most 2^24 and n_rows * (n_heads / n_kv_heads)^2 below 2^32. */
 int oi_paged_prompts_launch(const oi_paged_dims *d, const void *cache, int32_t n_heads, int32_t type, const void *q,
                             int64_t q_stride, float scale, int32_t n_seqs, int32_t n_rows, const int32_t *starts,
                             const int32_t *lens, const int32_t *table, int32_t table_stride, void *out,

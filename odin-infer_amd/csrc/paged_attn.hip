@@ -9,11 +9,13 @@
 // row), an f16 q exact.  Weights are the sum of two halves (22 bits) but for packed f16
 // prompts, whose outputs hold no more than 11 bits: there p is rounded once and l is
 // the sum of the rounded weights (with two halves 385 GFLOP of such prompts take 631 us, not 489, and are off by
-// 2.0e-4 of their size, not 2.2e-4; a caller with use for them makes an F32 call).  2^15 is where the row's largest p sits in f16:
-// another keeps all its bits down to 2^-29 of it and is lost below 2^-40.  Prompts leave
-// room above the maximum instead, so that few rises of it rescale o: from 2^3 in f16,
-// where a weight below 2^-28 is lost (2^17 of the largest such make one rounding of the
-// output), from 2^9 in f32 (2^-34).  Cached values are finite (the append sees to it): a slot that a
+// 2.0e-4 of their size, not 2.2e-4; a caller with use for them makes an F32 call).
+// f16 numbers end at steps of 2^-24, so a weight is off by up to 2^-25 beside its bits, and lost below that.
+// Tokens: the row's largest p is 2^14 to 2^15, so 2^-39 of it.  Prompts leave room above the maximum, so that few
+// rises of it rescale o: the largest p is from 2^(PS - 1) on, PS 6 in f16 (2^-30: 2^17 such slots make a quarter of an
+// output's rounding; 3 is 0.6% faster at head_dim 128, 3.5% at 256, and ends at 2^-27), 12 in f32 (2^-36: 2^17 make
+// 2e-6, as much as an f32 sum of them may be off by; 9 is 4% faster and ends at 2^-33), 9 for tokens of f16
+// rows (2^-33).  Cached values are finite (the append sees to it): a slot that a
 // row does not see has weight 0, and slots past a sequence's end count as zeros.
 //
 // Work is shared out on the device, since the lengths are there: every tile of rows
@@ -853,7 +855,8 @@ __global__ __launch_bounds__(WG, (PromptsShape<HD, F16>::PER_CU)) void paged_pro
     constexpr int CH = PIECES / WAVE / NW;  // a wave's stretches of 64 pieces, of each
     static_assert(CH * WAVE == 2 * HD, "sixteen slots");
     constexpr int RPC = WAVE / (HD / 8);    // K rows of a stretch
-    constexpr float PS = TWO ? 9.f : 3.f, LAZY = 15.f - PS;
+    // room for a rise of the maximum and for small weights share f16's range: see above
+    constexpr float PS = !TWO ? 6.f : F16 ? 9.f : 12.f, LAZY = 15.f - PS;
     using W = PromptsWork;
     __shared__ __attribute__((aligned(16))) f16x8 kl[2][PIECES], vl[2][PIECES];
     ask(a);
