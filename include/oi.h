@@ -607,11 +607,13 @@ int64_t oi_paged_bytes(const oi_paged_dims *d);
 /* Room for a step's tokens: sequence i holds n_past[i] slots and gets n_new[i] more
  * (negative: 0), in pages from the end of the list free_pages[0 .. *n_free)
  * (int32 [n_pages]; at first all page ids, *n_free = n_pages), in the sequences' order.
- * A sequence is served unless n_past is negative, its tokens do not fit its table row
- * (table_stride entries) or the n_rows rows of the step, or it needs a page and the list
- * does not hold what it and the sequences before it need.  Written: new entries of table
- * [n_seqs][table_stride]; *n_free; lens [n_seqs], the slots held now, 0 where not
- * served; starts [n_seqs + 1], the packed rows' begins (sums of n_new, at most n_rows);
+ * A sequence is served unless n_past is negative (a seat of none), its tokens do not fit
+ * its table row (table_stride entries), the step's n_rows rows end before its own do, or
+ * it needs a page and the list does not hold what it and the sequences before it need.
+ * Written: new entries of table [n_seqs][table_stride]; *n_free; lens [n_seqs], the slots
+ * held now, for the calls below: 0 where not served (the sequence still holds n_past[i]
+ * slots, and that is its next n_past: a loop that takes lens for it loses their pages);
+ * starts [n_seqs + 1], the packed rows' begins (sums of n_new, at most n_rows);
  * slots [n_rows], each row's slot number, -1 for rows not served or behind the last;
  * pos (NULL: none) [3][n_rows], its place in the sequence on three axes as
  * oi_rope_axes_launch takes them, 0 for such rows.  n_seqs at most 65536, n_rows at
