@@ -176,8 +176,11 @@ __device__ __forceinline__ float scan_lanes(float v) {
 // rises with x, as every step of it does, so workers' stretches cover each unit once, wherever
 // rounding puts the borders.  Within NEAR units of a tile's end (an eighth of a share, if that is
 // less) it moves there; in a tile of at most SHORT units from up to half a share, since each
-// part costs what a tile costs by itself, and the join (nine prompts of 5 to 301 tokens 26.3 ->
-// 22.3 us, a step of 12 sequences that leaves tiles of 2 to 14 units 19.7 -> 20.9).
+// part costs what a tile costs by itself, and the join.  Against an eighth throughout, 45 calls of 1 to 64 prompts
+// of 5 to 1000 tokens, some behind caches, take 0.96 of the time in the mean: 0.76 to 0.86 where a few prompts of 100
+// to 300 tokens meet, 1.13 at worst (12 prompts of 30 to 600 at head_dim 256, 47 -> 53 us; a step of 12 sequences 23.4 ->
+// 22.4, another 16.8 -> 18.4).  Fractions that fall with a tile's length in place of the step (3 to 8 units over it)
+// are the same in the mean (0.996 to 1.000 of this) and 0.82 to 1.13 of it in single calls.
 template <class W>
 __device__ PagedAt border(const PagedAttnArgs &a, float x, float share, float own, float run, int per) {
     const int lane = __lane_id();
@@ -688,7 +691,7 @@ __device__ __forceinline__ void join_row(const PagedAttnArgs &a, int w, int n, i
         store_out(a.out, a.f16, to + 4 * col, y * inverse(l));
     }
 }
-// RT rows of few parts, RT WG * 4 / HD of them apart from each other, four dimensions a thread;
+// RT rows a thread, RT WG * 4 / HD of them apart from each other, four dimensions a thread;
 // at(r): where row r goes
 template <int HD, int RT, class F>
 __device__ __forceinline__ void join_rows(const PagedAttnArgs &a, int w, int n, int r0, int rows, F at) {
@@ -730,10 +733,10 @@ __device__ __forceinline__ void join_rows(const PagedAttnArgs &a, int w, int n, 
 }
 
 // Tokens.  BY_TILE: a workgroup per tile (there are few) looks for the borders in it;
-// otherwise one per border.  ROWS: 1, or those that a workgroup takes at once where their parts
-// are few (3840 workgroups of a row each took 9 us for drafts of 24 sequences, 6.7 this way).  A chain of
+// otherwise one per border.  ROWS: 1, or those that a workgroup takes at once where there are
+// many (3840 workgroups of a row each took 9 us for drafts of 24 sequences, 6.7 this way; 64 rows of 130000
+// slots beside 63 sequences of 100: the call 72 us, 114 with tiles of many parts a row after the other).  A chain of
 // three misses: borders, (m, l) with the results, out; 3.8 us for one sequence, 4.7 for 48.
-constexpr int JOIN_FEW = 32;
 template <int HD, bool BY_TILE, int ROWS>
 __global__ __launch_bounds__(WG, 4) void paged_join_kernel(PagedAttnArgs a) {
     constexpr int NB = JOIN_MOST / WG;  // borders of a thread
@@ -780,16 +783,8 @@ __global__ __launch_bounds__(WG, 4) void paged_join_kernel(PagedAttnArgs a) {
     n++;
     const int w = first - 1;
     auto to = [&](int r) { return row_at(a, at.seq * a.n_q, r, at.head, a.out_stride); };
-    if constexpr (ROWS == 1) {
-        join_row<HD>(a, w, n, r0, to(r0), lds);
-    } else if (n <= JOIN_FEW) {
-        join_rows<HD, ROWS * HD / 4 / WG>(a, w, n, r0, min(rows, r0 + ROWS), to);
-    } else {
-        for (int r = r0; r < min(rows, r0 + ROWS); r++) {
-            join_row<HD>(a, w, n, r, to(r), lds);
-            __syncthreads();  // LDS is read before the next row is written there
-        }
-    }
+    if constexpr (ROWS == 1) join_row<HD>(a, w, n, r0, to(r0), lds);
+    else join_rows<HD, ROWS * HD / 4 / WG>(a, w, n, r0, min(rows, r0 + ROWS), to);
 }
 
 // Prompts: a workgroup per border, RT rows a thread: 14703 packed rows, two parts to a tile, 11.3

@@ -150,6 +150,9 @@ TOKENS = [  # kv heads, group, head_dim, page, tokens, lengths
     (8, 2, 128, 32, 1, [17 + 41 * i for i in range(100)]),  # a border in many tiles
     (1, 1, 128, 16, 1, [(i * 37) % 700 for i in range(1500)]),
     (4, 5, 128, 64, 16, [4000, 20000, 64, 33]),         # more than 64 rows of a kv head
+    (1, 8, 128, 64, 8, [130000] + [100] * 63),          # many rows of many parts
+    (2, 8, 256, 32, 8, [60000] + [90] * 20),
+    (1, 16, 128, 16, 2, [60000] + [40] * 600),
 ]
 
 
