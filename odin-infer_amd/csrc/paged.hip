@@ -323,10 +323,15 @@ __global__ __launch_bounds__(WG, 4) void paged_append_kernel(PagedAppendArgs a) 
     }
 }
 
-// Few rows: a row a workgroup, four elements a thread, V's by 2-byte stores; the slot and the
-// values are one round trip.  Rows of 8 heads of 128, one of each sequence: 64 3.2 us (by runs 6.4),
-// 300 5.1 (7.2); neighbours in one sequence: 300 4.9 (4.8), 1000 10 (6.2).
-constexpr int APPEND_FEW = 256;
+// Few elements: a row a workgroup, four elements a thread, V's by 2-byte stores; the slot and the
+// values are one round trip.  us (by runs), rows one of each sequence and neighbours in one, heads of 128 in f16, f32 within
+// a tenth of them:
+//   1 head    600 rows 2.8 (6.2), 2.9 (4.4)    1500 rows 3.7 (6.5), 3.7 (4.5)
+//   2 heads   600 3.5 (6.4), 3.5 (4.7)         1500 5.2 (7.2), 5.1 (4.5)
+//   8         256 4.4 (7.0), 4.1 (5.5)         300 4.8 (7.1), 4.8 (4.5)      600 7.3 (8.3), 6.9 (5.8)
+//   16        64 3.6 (6.5), 3.6 (5.5)          256 6.6 (8.3), 6.0 (5.7)      600 12.0 (11.3), 11.2 (6.8)
+//   32        64 4.1 (7.0), 4.6 (5.6)          256 11.2 (9.6), 9.8 (6.0)
+constexpr int64_t APPEND_FEW = 1 << 18;  // elements of K
 template <bool F16>
 __global__ __launch_bounds__(WG) void paged_append_row_kernel(PagedAppendArgs a) {
     const int t = blockIdx.x, e = (blockIdx.y * WG + threadIdx.x) * 4;
@@ -376,7 +381,7 @@ hipError_t launch_paged_release(const PagedReleaseArgs &a, hipStream_t st) {
 }
 
 hipError_t launch_paged_append(const PagedAppendArgs &a, hipStream_t st) {
-    if (a.n <= APPEND_FEW) {
+    if ((int64_t)a.n * a.c.n_kv * a.c.hd <= APPEND_FEW) {
         const dim3 grid((unsigned)a.n, (unsigned)((a.c.n_kv * a.c.hd + 4 * WG - 1) / (4 * WG)));
         if (a.f16) hipLaunchKernelGGL(paged_append_row_kernel<true>, grid, dim3(WG), 0, st, a);
         else hipLaunchKernelGGL(paged_append_row_kernel<false>, grid, dim3(WG), 0, st, a);
