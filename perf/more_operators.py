@@ -54,7 +54,7 @@ def listed():
         # drafts of five tokens verified for 24 requests
         dict(name="tokens-draft", op="tokens", heads=32, kv_heads=4, head_dim=128, page=32, seqs=24, n=5, lo=200,
              hi=3501, type="f16", mix=7),
-        # a gated full-attention layer: one long document beside two short requests
+        # a gated full-attention layer: two long documents (120001 and 99785 slots) beside a short request (2729)
         dict(name="tokens-long", op="tokens", heads=16, kv_heads=2, head_dim=256, page=64, seqs=3, n=1, lo=900,
              hi=120001, type="f32", mix=8),
         # short questions read together
@@ -183,6 +183,7 @@ def prepare(case, seed):
         held = [_pages(x, p) for x in past]
         want = sum(_pages(x + y, p) for x, y in zip(past, new)) - sum(held)
         room = want if case["new_hi"] <= 8 else want - want // 20
+        room = max(room, 1 - sum(held))  # a pool has a page where nothing is held and nothing asked for
         s["n_pages"] = sum(held) + room
         order = torch.randperm(s["n_pages"], generator=_gen(seed, 3), device=DEV).int()
         s["width"] = max(_pages(x + y, p) for x, y in zip(past, new)) + 3
