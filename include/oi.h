@@ -547,7 +547,9 @@ int64_t oi_kv8_attn_workspace_bytes(const oi_kv8_dims *d, int32_t n_heads, int32
  * sums; scale * log2(e) must be finite in f32 (OI_E_ARG).  Weights multiply V in 22
  * bits, in f16 calls of more than 8 rows a kv head (n * n_heads / n_kv_heads) in
  * 11; a slot whose weight times its block's step of V is below 2^-40 of the row's
- * largest such product (f16 prompts: 2^-33) counts in the sum alone.  mass
+ * largest such product (f16 prompts: 2^-33) counts in the sum alone.  Scores (times
+ * log2(e)) must stay below 2^22 in size: a row of larger ones may come out wrong or not
+ * finite.  mass
  * (NULL: none), f32 [n_kv_heads][capacity]: what each slot receives, the softmax
  * weight summed over the call's tokens and the query heads of its kv head, is
  * added to slots below n_past and stored in slots n_past .. n_past+n-1 (a new
@@ -650,10 +652,13 @@ int64_t oi_paged_prompts_workspace_bytes(const oi_paged_dims *d, int32_t n_heads
  * [n_seqs * n_q][n_heads][head_dim], q_stride and out_stride elements from a token to the
  * next, both of `type` (F32 or F16), 16-byte aligned, strides multiples of 16 bytes.
  * Query head h reads kv head h / (n_heads / n_kv_heads).  out = softmax(scale * q K) V
- * with 32-bit sums in a fixed order.  A weight is off by at most 2^-22 of itself or 2^-39 of
- * the row's largest, whichever is more (calls of more than 64 rows n_q * n_heads /
+ * with 32-bit sums.  Their order follows from the call's sizes and all its lengths: a call
+ * repeated gives the same bits, but how the work is cut, and with it a sequence's last
+ * bits, goes by the others' lengths too.  A weight is off by at most 2^-22 of itself or
+ * 2^-39 of the row's largest, whichever is more (calls of more than 64 rows n_q * n_heads /
  * n_kv_heads: 2^-36, F16 2^-33): a smaller one may be lost.  scale * log2(e) must be
- * finite in f32 (OI_E_ARG).  Cached values below the lengths must be finite (as the append
+ * finite in f32 (OI_E_ARG).  A row of q that is not finite, or whose scores times log2(e)
+ * pass f32, comes out as anything; no other row is changed by it.  Cached values below the lengths must be finite (as the append
  * leaves them).  `out` may be `q` where the strides are the same. */
 int oi_paged_tokens_launch(const oi_paged_dims *d, const void *cache, int32_t n_heads, int32_t type, const void *q,
                            int64_t q_stride, float scale, int32_t n_seqs, int32_t n_q, const int32_t *lens,
@@ -665,7 +670,7 @@ int oi_paged_tokens_launch(const oi_paged_dims *d, const void *cache, int32_t n_
  * end), its newest; rows of no sequence stay as they are.  For whole prompts, chunks
  * behind cached slots, and drafts of differing lengths.  A weight is off by at most 2^-22 of
  * itself or 2^-36 of the row's largest; in F16 calls, whose outputs hold 11 bits, 2^-11 of
- * itself or 2^-30.  n_rows at most 2^24 and n_rows * (n_heads / n_kv_heads)^2 below 2^32. */
+ * itself or 2^-30 (an F32 call over the same cache has the former).  n_rows at most 2^24 and n_rows * (n_heads / n_kv_heads)^2 below 2^32. */
 int oi_paged_prompts_launch(const oi_paged_dims *d, const void *cache, int32_t n_heads, int32_t type, const void *q,
                             int64_t q_stride, float scale, int32_t n_seqs, int32_t n_rows, const int32_t *starts,
                             const int32_t *lens, const int32_t *table, int32_t table_stride, void *out,
