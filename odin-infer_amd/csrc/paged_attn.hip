@@ -832,16 +832,17 @@ constexpr int PR = PromptsWork::R;  // rows of a tile
 // 1's weights with V.  A row's maximum is raised only when another is more than 2^LAZY above it
 // (weights then reach 2^15 at most, from 2^PS), and o follows after the products that go by the
 // old one.
-// Packed f16 prompts of 900 to 5003 tokens, 32 heads of 128 over 8 (385 GFLOP): 488 to 506 us, 760
-// to 790 TFLOP/s; four of 8000 tokens 875; f32 rows at head_dim 256, two products for each
-// (110 GFLOP), 272 us.  Matrix and vector units are both busy in 4 of 10 cycles: a wave issues in order, and
+// Packed f16 prompts of 900 to 5003 tokens, 32 heads of 128 over 8 (385 GFLOP): 478 to 505 us, 760
+// to 805 TFLOP/s; four of 8000 tokens 866; at head_dim 256 (378 GFLOP) 565 us; f32 rows there, two products for
+// each (110 GFLOP), 271 to 282 us.  Matrix and vector units are both busy in 4 of 10 cycles: a wave issues in order, and
 // two waves a SIMD do not fill each other's gaps (16 products alone 225 ns, beside their softmax
 // 433 in a loop of nothing else, 600 here).  Where pages are read once or twice, their misses add a
-// tenth to three (two times 50 tokens behind 40000 slots 118 us, 105 with pages in cache).
+// tenth to two (two times 50 tokens behind 40000 slots 121 us, 99 with pages in cache).
 // Measured and left: 64 rows a wave (700 us against 565), eight waves on 256 rows (the same, long ones 5%
 // slower), pieces of LDS read 6 or 8 ahead (the same), lines of the step after next touched ahead of
 // their fetch (10% slower), a half's first pieces read before the fetches are issued (f16 at head_dim
-// 256 5% slower), waves' priorities (the same), no pipeline (f16 the same, f32 slower).
+// 256 5% slower), waves' priorities (the same), no pipeline (f16 the same, f32 slower).  Scalar registers: 30 to 33
+// spill into lanes of a vector one; vector registers only at head_dim 256 in f32 (8), outside the products.
 // TWO: weights as two halves (all but packed f16 prompts).
 template <int HD, bool F16, bool TWO>
 __global__ __launch_bounds__(WG, (PromptsShape<HD, F16>::PER_CU)) void paged_prompts_kernel(PagedAttnArgs a) {
